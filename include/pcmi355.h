@@ -484,6 +484,67 @@ int pcm_flow_gradients(pcm_circuit* c, int32_t batch_size, float* d_grad);
 int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, float* d_m, float* d_v, float* d_leaf_params,
                        float* d_leaf_m, float* d_leaf_v, float lr, float beta1, float beta2, float eps, int32_t t);
 
+/*
+ * Rows of category scores: log-evidence [examples, variables, categories], the per-head log-likelihoods of a multi-head
+ * circuit or a forest, the logits of a network that a circuit is distilled from.  No counterpart in the reference, which
+ * does this part in its Python programs.  Element (example e, variable v, category c) of an array of scores is at
+ * x[e * stride_ex + v * stride_var + c * stride_cat]: element strides, any sign, also 0; num_vars = 1 for plain rows.
+ * A score at or below half of its type's lowest value is a mask and counts as -inf (as well -inf itself, as what adding a mask
+ * of the lowest value leaves).  With Z = sum_c exp x[c] over a row:
+ *
+ * pcm_category_scores.  d_given [examples][variables][num_given] (its own element strides; PCM_U8, PCM_I32, PCM_I64):
+ *   d_logp [rows][num_given]   x[g] - log Z; 0 where g < 0 (not observed: probability 1, as a missing value counts in a
+ *                              circuit), NaN where g >= num_cats
+ *   d_log_sum [rows]           log Z (may be NULL)
+ *   d_entropy [rows]           -sum_c p log p, p = exp(x - log Z) (may be NULL)
+ *   d_top, d_top_logp [rows][top]  the likeliest categories and their log-probabilities, equal scores by rising category; a
+ *                              category of score -inf is never among them: -1 and -inf stand where a row has no more
+ *   d_codes, d_scales          the row's checkpoint as pcm_checkpoint_rows writes it, in the same pass (both NULL: none)
+ * A row of nothing but masks: log Z = -inf, logp = -inf, entropy 0.  A row with NaN or +inf: NaN, no categories (-1).
+ * At most 64 given and 64 likeliest categories a row, 2^31 - 1 rows.  d_work: pcm_category_scores_workspace bytes of device
+ * memory (0: none) that belong to the call until its work is done; 16-byte aligned.
+ *
+ * pcm_category_scores_backward: the gradient with respect to the scores of a loss whose derivatives are d_grad_logp
+ * [rows][num_given], d_grad_top [rows][top] and d_grad_entropy [rows] (num_given = 0, top = 0, NULL: none),
+ *   sum_j gl[j] ([c = g_j] - p[c]) + sum_i gt[i] ([c = top_i] - p[c]) - gh p[c] (log p[c] + H),
+ * from the scores (d_scores) or from their checkpoint (d_codes, d_scales; d_scores NULL then) with d_log_sum and d_entropy
+ * (the latter only with d_grad_entropy) as pcm_category_scores left them.  A slot < 0 adds nothing, one >= num_cats makes its
+ * row NaN; the same category in several slots adds up; a row of log Z = -inf gets zeros.  p is as
+ * exact as d_log_sum: 2^-24 |log Z| relative.  d_grad has the type and shape of the
+ * scores and strides of its own; it may be the array of scores itself with the same strides, else the two must not overlap, and
+ * no two of its elements may be one.
+ *
+ * pcm_checkpoint_rows: rows in 8 bits, for what a forward pass keeps for its backward pass.  d_codes [rows][num_cats rounded up
+ * to 16] bytes, d_scales [rows][ceil(num_cats / 64)] words.  64 neighbours of a row with largest and smallest entries M and m
+ * share a step 2^e: e is the smallest exponent for which the range takes at most 253 steps if its mantissa is at most 253 / 256
+ * (in [1/2, 1)), at most 127 otherwise, |x| <= 2^14 steps and e >= -126.  An entry stands for (base - code) 2^e, base = rint(M /
+ * 2^e): the nearest multiple of the step.  Code 255: an entry that is masked, x <= half of the type's lowest value; it
+ * stands for -inf.  Scale word: base in bits 0..15 (two's complement), e + 127 in bits 16..23; 255 there (a block with NaN or
+ * +inf): every entry stands for NaN.  Codes behind a row's end are 255.
+ * pcm_restore_rows: the values that the codes stand for, as floats or rounded to the type the rows had.
+ *
+ * All queue their work on `stream` (of the current device), wait for nothing and allocate nothing: they can be captured.
+ */
+enum pcm_type { PCM_F32 = 0, PCM_BF16 = 1, PCM_F16 = 2, PCM_U8 = 3, PCM_I32 = 4, PCM_I64 = 5 };
+
+int64_t pcm_category_scores_workspace(int64_t num_examples, int32_t num_vars, int32_t num_cats, int32_t top);
+int pcm_category_scores(const void* d_scores, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat,
+                        int64_t num_examples, int32_t num_vars, int32_t num_cats, const void* d_given, int32_t given_type,
+                        int64_t given_stride_ex, int64_t given_stride_var, int64_t given_stride_slot, int32_t num_given,
+                        int32_t top, float* d_logp, float* d_log_sum, float* d_entropy, float* d_top_logp, int32_t* d_top,
+                        uint8_t* d_codes, int32_t* d_scales, void* d_work, int64_t work_bytes, void* stream);
+int pcm_category_scores_backward(const void* d_scores, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat,
+                                 int64_t num_examples, int32_t num_vars, int32_t num_cats, const uint8_t* d_codes,
+                                 const int32_t* d_scales, const void* d_given, int32_t given_type, int64_t given_stride_ex,
+                                 int64_t given_stride_var, int64_t given_stride_slot, int32_t num_given, const float* d_grad_logp,
+                                 int32_t top, const int32_t* d_top, const float* d_grad_top, const float* d_log_sum,
+                                 const float* d_entropy, const float* d_grad_entropy, void* d_grad, int64_t grad_stride_ex,
+                                 int64_t grad_stride_var, int64_t grad_stride_cat, void* stream);
+int pcm_checkpoint_rows(const void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat,
+                        int64_t num_examples, int32_t num_vars, int32_t num_cats, uint8_t* d_codes, int32_t* d_scales, void* stream);
+int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t num_examples, int32_t num_vars, int32_t num_cats,
+                     void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat, void* stream);
+
 /* ---- instrumentation ----------------------------------------------------------- */
 
 /* Per-kernel timing, the role of `debug = true` -> `CUDA.@time` around each launch

@@ -4,6 +4,7 @@
 #include <new>
 #include <unordered_set>
 
+#include "category_rows.hpp"
 #include "common.hpp"
 #include "hclt_engine.hpp"
 #include "sparse_engine.hpp"
@@ -367,6 +368,58 @@ int pcm_chow_liu_edges(const float* d_mi, int32_t num_vars, int32_t* d_edges, vo
 
 int pcm_chow_liu_root(const int32_t* edges, int32_t num_vars, int32_t* clt_parent) {
   return guarded([&] { pcm::chow_liu_root(edges, num_vars, clt_parent); });
+}
+
+int64_t pcm_category_scores_workspace(int64_t num_examples, int32_t num_vars, int32_t num_cats, int32_t top) {
+  return pcm::category_scores_workspace(pcm::RowsShape{num_examples, num_vars, num_cats}, top);
+}
+
+int pcm_category_scores(const void* d_scores, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat,
+                        int64_t num_examples, int32_t num_vars, int32_t num_cats, const void* d_given, int32_t given_type,
+                        int64_t given_stride_ex, int64_t given_stride_var, int64_t given_stride_slot, int32_t num_given,
+                        int32_t top, float* d_logp, float* d_log_sum, float* d_entropy, float* d_top_logp, int32_t* d_top,
+                        uint8_t* d_codes, int32_t* d_scales, void* d_work, int64_t work_bytes, void* stream) {
+  return guarded([&] {
+    pcm::category_scores(pcm::RowsRef{d_scores, type, stride_ex, stride_var, stride_cat}, pcm::RowsShape{num_examples, num_vars, num_cats},
+                         pcm::GivenRef{d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given}, top, d_logp,
+                         d_log_sum, d_entropy, d_top_logp, d_top, pcm::CkptRef{d_codes, reinterpret_cast<uint32_t*>(d_scales)}, d_work,
+                         work_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int pcm_category_scores_backward(const void* d_scores, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat,
+                                 int64_t num_examples, int32_t num_vars, int32_t num_cats, const uint8_t* d_codes,
+                                 const int32_t* d_scales, const void* d_given, int32_t given_type, int64_t given_stride_ex,
+                                 int64_t given_stride_var, int64_t given_stride_slot, int32_t num_given, const float* d_grad_logp,
+                                 int32_t top, const int32_t* d_top, const float* d_grad_top, const float* d_log_sum,
+                                 const float* d_entropy, const float* d_grad_entropy, void* d_grad, int64_t grad_stride_ex,
+                                 int64_t grad_stride_var, int64_t grad_stride_cat, void* stream) {
+  return guarded([&] {
+    const pcm::CkptRef ckpt{const_cast<uint8_t*>(d_codes), reinterpret_cast<uint32_t*>(const_cast<int32_t*>(d_scales))};
+    pcm::category_scores_backward(pcm::RowsRef{d_scores, type, stride_ex, stride_var, stride_cat}, ckpt,
+                                  pcm::RowsShape{num_examples, num_vars, num_cats},
+                                  pcm::GivenRef{d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given},
+                                  d_grad_logp, top, d_top, d_grad_top, d_log_sum, d_entropy, d_grad_entropy,
+                                  pcm::RowsRef{d_grad, type, grad_stride_ex, grad_stride_var, grad_stride_cat},
+                                  static_cast<hipStream_t>(stream));
+  });
+}
+
+int pcm_checkpoint_rows(const void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat,
+                        int64_t num_examples, int32_t num_vars, int32_t num_cats, uint8_t* d_codes, int32_t* d_scales, void* stream) {
+  return guarded([&] {
+    pcm::checkpoint_rows(pcm::RowsRef{d_rows, type, stride_ex, stride_var, stride_cat}, pcm::RowsShape{num_examples, num_vars, num_cats},
+                         pcm::CkptRef{d_codes, reinterpret_cast<uint32_t*>(d_scales)}, static_cast<hipStream_t>(stream));
+  });
+}
+
+int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t num_examples, int32_t num_vars, int32_t num_cats,
+                     void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat, void* stream) {
+  return guarded([&] {
+    pcm::restore_rows(pcm::CkptRef{const_cast<uint8_t*>(d_codes), reinterpret_cast<uint32_t*>(const_cast<int32_t*>(d_scales))},
+                      pcm::RowsShape{num_examples, num_vars, num_cats}, pcm::RowsRef{d_rows, type, stride_ex, stride_var, stride_cat},
+                      static_cast<hipStream_t>(stream));
+  });
 }
 
 int pcm_stream_probe(const void* d_src, void* d_dst, int64_t lanes, int32_t reads, int32_t writes, int32_t grid, void* stream) {

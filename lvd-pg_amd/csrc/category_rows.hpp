@@ -1,0 +1,142 @@
+// Rows of category scores: what the kernels of category_scores.hip, category_grad.hip and checkpoint_rows.hip share.
+//
+// A row is the scores x[0..C) of C categories; rows are addressed as [example][variable] with element strides.  Types:
+// float, bfloat16, half (PCM_F32, PCM_BF16, PCM_F16); every sum is held in float.
+#pragma once
+
+#include "common.hpp"
+
+namespace pcm {
+
+constexpr int kMaxSlots = 64;         // most given categories, and most likeliest ones, of a row
+constexpr int kCkptBlock = 64;        // neighbours of a row that share a scale
+constexpr int kCkptMasked = 255;      // the code of an entry of -inf
+
+struct RowsRef {                      // rows of scores (or of a gradient) in device memory
+  const void* p;
+  int dtype;
+  int64_t stride_ex, stride_var, stride_cat;
+};
+struct RowsShape {
+  int64_t examples;
+  int32_t vars, cats;
+  __host__ __device__ int64_t rows() const { return examples * vars; }
+};
+struct GivenRef {                     // categories per row, [example][variable][slot]
+  const void* p;
+  int type;                           // PCM_U8, PCM_I32, PCM_I64
+  int64_t stride_ex, stride_var, stride_slot;
+  int32_t slots;
+};
+struct CkptRef {                      // codes [rows][pitch], scales [rows][blocks]
+  uint8_t* codes;
+  uint32_t* scales;
+};
+inline int64_t ckpt_pitch(int64_t cats) { return (cats + 15) / 16 * 16; }
+inline int64_t ckpt_blocks(int64_t cats) { return (cats + kCkptBlock - 1) / kCkptBlock; }
+
+int64_t category_scores_workspace(const RowsShape& shape, int top);
+void category_scores(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, float* d_logp, float* d_log_sum,
+                     float* d_entropy, float* d_top_logp, int32_t* d_top, const CkptRef& ckpt, void* d_work, int64_t work_bytes,
+                     hipStream_t stream);
+void category_scores_backward(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, const GivenRef& given,
+                              const float* d_grad_logp, int top, const int32_t* d_top, const float* d_grad_top,
+                              const float* d_log_sum, const float* d_entropy, const float* d_grad_entropy, const RowsRef& out,
+                              hipStream_t stream);
+void checkpoint_rows(const RowsRef& x, const RowsShape& shape, const CkptRef& ckpt, hipStream_t stream);
+void restore_rows(const CkptRef& ckpt, const RowsShape& shape, const RowsRef& out, hipStream_t stream);
+// refusals that the four share
+void check_rows(const RowsRef& x, const RowsShape& shape, const char* what);
+void check_given(const GivenRef& given);
+
+#ifdef __HIPCC__
+// ---- device side ------------------------------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) { return (float)v; }
+template <typename T>
+__device__ __forceinline__ T from_float(float v) { return (T)v; }   // round to nearest, ties to even
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// Entry `slot` of a row's given categories, whatever their type; negative: not observed.
+__device__ __forceinline__ int64_t given_at(const GivenRef& g, int64_t e, int64_t v, int slot) {
+  const int64_t at = e * g.stride_ex + v * g.stride_var + slot * g.stride_slot;
+  if (g.type == PCM_U8) return static_cast<const uint8_t*>(g.p)[at];
+  if (g.type == PCM_I32) return static_cast<const int32_t*>(g.p)[at];
+  return static_cast<const int64_t*>(g.p)[at];
+}
+
+// Order of entries, likeliest first: larger value, then smaller index (the two zeros are one value).  0 is below them all.
+__device__ __forceinline__ uint64_t entry_key(float x, uint32_t index) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
+  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (uint64_t)o << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ int32_t key_index(uint64_t k) { return (int32_t) ~(uint32_t)k; }
+
+// The largest entry that counts as masked: half of the type's lowest value (what adding a mask of the lowest value leaves).
+template <typename T>
+__device__ __forceinline__ float masked_from() { return -1.7014117e38f; }
+template <>
+__device__ __forceinline__ float masked_from<bf16>() { return -1.6947657e38f; }
+template <>
+__device__ __forceinline__ float masked_from<f16>() { return -32752.f; }
+// a score with masks at -inf
+template <typename T>
+__device__ __forceinline__ float seen(T v) {
+  const float x = to_float(v);
+  return x <= masked_from<T>() ? -INFINITY : x;
+}
+template <typename T>
+__device__ __forceinline__ float type_max() { return 3.4028235e38f; }
+template <>
+__device__ __forceinline__ float type_max<bf16>() { return 3.3895314e38f; }
+template <>
+__device__ __forceinline__ float type_max<f16>() { return 65504.f; }
+
+// The scale of a block of 64: entry = (base - code) 2^e, code 0..254.  e is the smallest exponent with 253 steps (254 between
+// rounded ends) over the block's range where the range's mantissa allows, and with the largest entry within 2^14 steps, so that
+// base fits 16 bits.  A power of two makes x 2^-e, its rounding and the product back exact: an entry is off by half a step
+// at most, whoever computes it.  Word: base in bits 0..15, e + 127 in bits 16..23; 255 there: a block with NaN or +inf.
+struct BlockScale {
+  float inv, base;   // 2^-e, rint(max 2^-e)
+  uint32_t word;
+};
+__device__ __forceinline__ BlockScale block_scale(float hi, float lo, bool bad) {   // (hi < lo: no entry but masked ones)
+  if (hi < lo) hi = lo = 0.f;
+  const float r = 0.5f * hi - 0.5f * lo;   // halves: the difference itself may pass the range of float
+  const float a = fmaxf(fabsf(hi), fabsf(lo));
+  int e = -126;
+  if (r > 0.f) e = max(e, __builtin_amdgcn_frexp_expf(r) - (__builtin_amdgcn_frexp_mantf(r) > 253.f / 256.f ? 6 : 7));
+  if (a > 0.f) e = max(e, __builtin_amdgcn_frexp_expf(a) - 14);
+  BlockScale s;
+  s.inv = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+  s.base = rintf(hi * s.inv);
+  s.word = bad ? 0xff0000u : (uint32_t)(127 + e) << 16 | ((uint32_t)(int)s.base & 0xffffu);
+  return s;
+}
+// a masked entry is off: x <= masked_from<T>()
+__device__ __forceinline__ uint32_t block_code(const BlockScale& s, float x, bool off) {
+  return off ? (uint32_t)kCkptMasked : (uint32_t)__builtin_amdgcn_fmed3f(s.base - rintf(x * s.inv), 0.f, 254.f);
+}
+struct BlockUnit {
+  float step, base;
+};
+__device__ __forceinline__ BlockUnit block_unit(uint32_t word) {
+  const uint32_t e = word >> 16 & 0xffu;
+  return e == 0xffu ? BlockUnit{__builtin_nanf(""), 0.f}
+                    : BlockUnit{__builtin_bit_cast(float, e << 23), (float)(int16_t)(word & 0xffffu)};
+}
+__device__ __forceinline__ float block_entry(const BlockUnit& u, uint32_t code) {   // (the product may round up past the range)
+  const float v = (u.base - (float)code) * u.step;
+  return code == (uint32_t)kCkptMasked && u.step == u.step ? -INFINITY : v > 3.4028235e38f ? 3.4028235e38f : v;
+}
+#endif
+
+}  // namespace pcm

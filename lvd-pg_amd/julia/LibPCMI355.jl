@@ -110,6 +110,16 @@ pcm_flow_gradients(c, batch_size, d_grad) =
     ccall((:pcm_flow_gradients, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Ptr{Float32}), c, batch_size, d_grad)
 pcm_adam_flow_step(c, batch_size, d_params, d_m, d_v, d_leaf_params, d_leaf_m, d_leaf_v, lr, beta1, beta2, eps, t) =
     ccall((:pcm_adam_flow_step, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Float32, Float32, Float32, Float32, Int32), c, batch_size, d_params, d_m, d_v, d_leaf_params, d_leaf_m, d_leaf_v, lr, beta1, beta2, eps, t)
+pcm_category_scores_workspace(num_examples, num_vars, num_cats, top) =
+    ccall((:pcm_category_scores_workspace, libpcmi355), Int64, (Int64, Int32, Int32, Int32), num_examples, num_vars, num_cats, top)
+pcm_category_scores(d_scores, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, top, d_logp, d_log_sum, d_entropy, d_top_logp, d_top, d_codes, d_scales, d_work, work_bytes, stream) =
+    ccall((:pcm_category_scores, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int32, Int32, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int32, Int32, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Int32}, Ptr{UInt8}, Ptr{Int32}, Ptr{Cvoid}, Int64, Ptr{Cvoid}), d_scores, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, top, d_logp, d_log_sum, d_entropy, d_top_logp, d_top, d_codes, d_scales, d_work, work_bytes, stream)
+pcm_category_scores_backward(d_scores, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_codes, d_scales, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_grad_logp, top, d_top, d_grad_top, d_log_sum, d_entropy, d_grad_entropy, d_grad, grad_stride_ex, grad_stride_var, grad_stride_cat, stream) =
+    ccall((:pcm_category_scores_backward, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int32, Int32, Ptr{UInt8}, Ptr{Int32}, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int32, Ptr{Float32}, Int32, Ptr{Int32}, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Cvoid}, Int64, Int64, Int64, Ptr{Cvoid}), d_scores, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_codes, d_scales, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_grad_logp, top, d_top, d_grad_top, d_log_sum, d_entropy, d_grad_entropy, d_grad, grad_stride_ex, grad_stride_var, grad_stride_cat, stream)
+pcm_checkpoint_rows(d_rows, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_codes, d_scales, stream) =
+    ccall((:pcm_checkpoint_rows, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int32, Int32, Ptr{UInt8}, Ptr{Int32}, Ptr{Cvoid}), d_rows, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_codes, d_scales, stream)
+pcm_restore_rows(d_codes, d_scales, num_examples, num_vars, num_cats, d_rows, type, stride_ex, stride_var, stride_cat, stream) =
+    ccall((:pcm_restore_rows, libpcmi355), Cint, (Ptr{UInt8}, Ptr{Int32}, Int64, Int32, Int32, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Ptr{Cvoid}), d_codes, d_scales, num_examples, num_vars, num_cats, d_rows, type, stride_ex, stride_var, stride_cat, stream)
 pcm_set_timing(c, on) =
     ccall((:pcm_set_timing, libpcmi355), Cint, (Ptr{Cvoid}, Int32), c, on)
 pcm_get_timing(c, ms, n) =

@@ -17,6 +17,8 @@ from .queries import (loglikelihoods, loglikelihood, loglikelihoods_probcat, log
 from .structures import (pairwise_MI, chow_liu_tree, learn_chow_liu_tree, hclt, hclt_for_colored_images, clt_edges2parent, hclt_pc,  # noqa: F401
                          customized_hclt, joined_hclt, joined_hclt_from_clts, group_vars_by_grid, group_vars_by_cgrid)
 from .transformations import prune_pc, grow_heads_by_flows, aggregate_edge_flows, aggregate_node_flows  # noqa: F401
+from .category_rows import (CategoryScores, Checkpoint8, category_scores, category_scores_backward, checkpoint_rows,  # noqa: F401
+                            restore_rows, head_scores)
 from .jpc_io import write_jpc, read_jpc, write_mhpc, read_mhpc  # noqa: F401
 from . import nodes, prealloc  # noqa: F401
 from ._lib import PcmError, LIB_PATH  # noqa: F401

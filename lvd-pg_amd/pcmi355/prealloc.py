@@ -7,18 +7,32 @@ and check the shapes the reference asserts (:50-51, :192-193).  The parameter ma
 device once and all their rows run in one pass of the row entry points (`pcm_kld_rows`,
 `pcm_kld_backward_rows`, `pcm_gumbel_sample_rows`); the circuit only lends its structure, its own
 parameters are neither read nor changed.  Host arrays in, host arrays out, as there.
+
+Between a forward call and its reverse pass the matrices stay on the device, as there.  `checkpoint = True` at the
+preallocation keeps them in 8 bits instead (`checkpoint_rows`: 1.06 bytes a parameter, the nearest of 253 steps over the range of
+64 neighbours); the reverse pass then differentiates at the rounded parameters.  Forward results do not change.
 """
 import numpy as np
 import torch
 
+from .category_rows import Checkpoint8, checkpoint_rows
 from .queries import (kld, kld_backward, gumbel_sample_rows, gumbel_sample_backward_rows, _rows_on_device,
                       per_sample_normalized_flows, map_pc_parameters, normalize_params)
 
 _state = {}
 
 
-def kld_preallocation(mbpc, *, num_examples):
-    _state["kld"] = dict(num_examples=int(num_examples), mbpc=mbpc, rows=None)
+def _kept(rows, checkpoint):
+    """What stays of parameter rows until the reverse pass"""
+    return checkpoint_rows(rows) if checkpoint else rows
+
+
+def _rows_of(kept):
+    return kept.restore(torch.float32) if isinstance(kept, Checkpoint8) else kept
+
+
+def kld_preallocation(mbpc, *, num_examples, checkpoint=False):
+    _state["kld"] = dict(num_examples=int(num_examples), mbpc=mbpc, rows=None, checkpoint=bool(checkpoint))
 
 
 def kld_free_mem():
@@ -39,7 +53,8 @@ def kld_with_prealloc(mbpc, params1, params2, *, norm_params=False):
         raise ValueError(f"preallocated for {st['num_examples']} examples, got {p1.shape[0]}")   # :50
     if p2.shape[0] not in (1, p1.shape[0]):
         raise ValueError("params2 must have one row or as many as params1")
-    st["rows"] = (p1, p2)                      # the reference keeps both matrices on the device for the reverse pass
+    # the reference keeps both matrices on the device for the reverse pass
+    st["rows"] = _kept(p1, st["checkpoint"]), _kept(p2, st["checkpoint"])
     return kld(mbpc, p1, p2, norm_params=norm_params).cpu().numpy()
 
 
@@ -50,19 +65,19 @@ def kld_backward_with_prealloc(mbpc, *, norm_params=False, grad_wrt_logparams=Tr
     st = _state.get("kld")
     if st is None or st["mbpc"] is not mbpc or st["rows"] is None:
         raise RuntimeError("call kld_with_prealloc first")
-    p1, p2 = st["rows"]
+    p1, p2 = map(_rows_of, st["rows"])
     g1, g2 = kld_backward(mbpc, p1, p2, norm_params=norm_params, grad_wrt_logparams=grad_wrt_logparams)
     return g1.cpu().numpy(), g2.cpu().numpy()
 
 
 def gumbel_sample_preallocation(mbpc, *, num_examples, num_vars, par_buffer_size, allocate_for_grad=False,
-                                allocate_for_target=False):
+                                allocate_for_target=False, checkpoint=False):
     if allocate_for_target:
         raise NotImplementedError("gumbel_sample_target_with_prealloc (parameter targets) is not built")
     if num_vars != mbpc.size("variables") or par_buffer_size < mbpc.size("categories"):
         raise ValueError("num_vars / par_buffer_size do not fit the circuit")
     _state["sample"] = dict(num_examples=int(num_examples), num_vars=int(num_vars), width=int(par_buffer_size), mbpc=mbpc,
-                            grad=bool(allocate_for_grad), last=None)
+                            grad=bool(allocate_for_grad), checkpoint=bool(checkpoint), last=None)
 
 
 def gumbel_sample_free_mem(allocate_for_grad=False, allocate_for_target=False):
@@ -87,7 +102,7 @@ def gumbel_sample_with_prealloc(mbpc, params, *, temperature, no_gumbel=False, n
         u = torch.rand((p.shape[0], mbpc.num_inner_params()), device=p.device, generator=generator)
         noise = -torch.log(-torch.log(u * (1.0 - 1e-6) + 1e-6))
     soft = gumbel_sample_rows(mbpc, p, temperature=temperature, noise=noise, norm_params=norm_params)
-    st["last"] = (p, noise)                      # the reverse pass runs on the same parameters and draws
+    st["last"] = (_kept(p, st["checkpoint"]), noise)     # the reverse pass runs on the same parameters and draws
     C = mbpc.size("categories")
     out = np.zeros((p.shape[0], st["num_vars"], st["width"]), np.float32)
     out[:, :, :C] = soft.cpu().numpy()
@@ -104,7 +119,8 @@ def gumbel_sample_backward_with_prealloc(mbpc, input_aggr_grads, *, temperature,
         raise RuntimeError("call gumbel_sample_with_prealloc first")
     if not st["grad"]:
         raise RuntimeError("gumbel_sample_preallocation was called without allocate_for_grad")
-    p, noise = st["last"]
+    kept, noise = st["last"]
+    p = _rows_of(kept)
     og = np.asarray(input_aggr_grads, np.float32)
     if og.shape != (p.shape[0], st["num_vars"], st["width"]):
         raise ValueError(f"input_aggr_grads must be {(p.shape[0], st['num_vars'], st['width'])}, got {og.shape}")

@@ -56,18 +56,14 @@ def _ids(example_ids, device):
 _LEAN_SCORING_BATCH = 1 << 20
 
 
-def loglikelihoods(bpc, data, batch_size=None, example_ids=None):
-    """`loglikelihoods(bpc, data; batch_size)` / `loglikelihoods_probcat`
-    (src/regularization/reg_likelihood.jl:139-162): per-example log-likelihoods as a device
-    vector.  A multi-head circuit returns [num_examples, num_heads]
-    (src-jl/multi_head_pc/likelihood.jl:37-71 with head_mask = nothing).  A 3-D float32 `data`
-    [examples, variables, categories] is soft evidence (reg_likelihood.jl:51-91)."""
+def _head_values(bpc, data, batch_size=None, example_ids=None):
+    """Log-likelihoods as the forward pass writes them, [heads (1: a single-root circuit), examples]."""
     _check_data(bpc, data)
     ids = _ids(example_ids, data.device)
     n = data.shape[0] if ids is None else len(ids)
     heads = getattr(bpc, "num_heads", 0)
     if n == 0:                                  # no examples: an empty result, no launch
-        return torch.empty((0, heads) if heads else (0,), dtype=torch.float32, device=data.device)
+        return torch.empty((max(heads, 1), 0), dtype=torch.float32, device=data.device)
     batch_size = n if batch_size is None else batch_size
     if not heads and not _is_soft(data) and bpc.size("walk_kernels") == 1:
         batch_size = max(batch_size, min(n, _LEAN_SCORING_BATCH))
@@ -84,7 +80,17 @@ def loglikelihoods(bpc, data, batch_size=None, example_ids=None):
             out[:, s:s + b] = tmp
         else:
             _forward(bpc, data, d_ptr, i_ptr, b, out[0, s:s + b].data_ptr())
-    return out.t().contiguous() if heads else out[0]
+    return out
+
+
+def loglikelihoods(bpc, data, batch_size=None, example_ids=None):
+    """`loglikelihoods(bpc, data; batch_size)` / `loglikelihoods_probcat`
+    (src/regularization/reg_likelihood.jl:139-162): per-example log-likelihoods as a device
+    vector.  A multi-head circuit returns [num_examples, num_heads]
+    (src-jl/multi_head_pc/likelihood.jl:37-71 with head_mask = nothing).  A 3-D float32 `data`
+    [examples, variables, categories] is soft evidence (reg_likelihood.jl:51-91)."""
+    out = _head_values(bpc, data, batch_size, example_ids)
+    return out.t().contiguous() if getattr(bpc, "num_heads", 0) else out[0]
 
 
 def multihead_loglikelihoods(mhbpc, data, head_mask, batch_size=None, example_ids=None):

@@ -1,0 +1,156 @@
+"""Rows of category scores on the CPU: the reference against closed forms and differences, and what the entry points refuse."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import category_reference as R
+
+
+def _rows(seed, n, C, spread=3.0):
+    return np.random.default_rng(seed).normal(size=(n, C)) * spread
+
+
+def test_reference_statistics():
+    from scipy.special import logsumexp, softmax
+    from scipy.stats import entropy
+    x = _rows(1, 5, 37)
+    z, h = R.statistics(x)
+    np.testing.assert_allclose(z, logsumexp(x, 1), rtol=1e-13)
+    np.testing.assert_allclose(h, entropy(softmax(x, 1), axis=1), rtol=1e-12)
+    x[1, 3:] = -np.inf
+    x[2] = -np.inf
+    x[3, 5] = np.nan
+    x[4, 5] = np.inf
+    z, h = R.statistics(x)
+    assert z[2] == -np.inf and h[2] == 0 and np.isnan(z[3:]).all() and np.isnan(h[3:]).all() and np.isfinite(z[1])
+    i, lp = R.likeliest(np.array([[1.0, 2.0, 2.0, -np.inf]]), 5)
+    assert i.tolist() == [[1, 2, 0, -1, -1]] and lp[0, 3] == -np.inf
+
+
+def test_reference_gradient_is_the_derivative():
+    n, C = 3, 11
+    x = _rows(2, n, C)
+    rng = np.random.default_rng(3)
+    g = rng.integers(-1, C, (n, 4))
+    g[0] = [2, 2, -1, 5]
+    w, gh = rng.normal(size=(n, 4)), rng.normal(size=n)
+
+    def loss(y):
+        z, h = R.statistics(y)
+        return (R.logp_of(y, g) * w).sum() + (gh * h).sum()
+
+    z, h = R.statistics(x)
+    got, _ = R.gradient(x, z, h, [(g, w)], gh)
+    for r in range(n):
+        for c in range(C):
+            y = x.copy()
+            y[r, c] += 1e-6
+            u = x.copy()
+            u[r, c] -= 1e-6
+            # a central difference of a function with third derivatives of order one: 1e-12, and 1e-16 / 1e-6 of rounding
+            assert abs((loss(y) - loss(u)) / 2e-6 - got[r, c]) < 1e-8
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_reference_rounding_is_off_by_half_a_step(dtype):
+    x = torch.from_numpy(_rows(4, 6, 150, 9.0)).to(getattr(torch, dtype)).double().numpy()
+    x[1, 7] = -np.inf
+    x[2, 70] = R.LOWEST[dtype]
+    x[3, 130] = np.nan
+    x[4] = -5000.0 + np.arange(150) / 128.0
+    y = R.rounded(x, dtype)
+    assert y[1, 7] == -np.inf and y[2, 70] == -np.inf and np.isnan(y[3, 128:]).all() and np.isfinite(y[3, :128]).all()
+    for s in range(0, 150, 64):
+        b, c = x[[0, 4, 5], s:s + 64], y[[0, 4, 5], s:s + 64]
+        span, size = b.max(1) - b.min(1), np.abs(b).max(1)
+        assert (np.abs(c - b).max(1) <= np.maximum(span / 126.5, size * 2.0 ** -12) / 2).all()
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------------
+
+def test_python_refuses_what_it_cannot_do():
+    import pcmi355 as P
+    x = torch.zeros((4, 10))
+    for bad, what in ((torch.zeros(10), "tensor"), (torch.zeros((4, 10), dtype=torch.float64), "float"), (torch.zeros((4, 0)), "category"),
+                      (np.zeros((4, 10)), "tensor")):
+        for f in (P.category_scores, P.checkpoint_rows):
+            with pytest.raises(ValueError, match=what):
+                f(bad)
+    for given in (torch.zeros(4), torch.zeros(3, dtype=torch.int64), torch.zeros((4, 65), dtype=torch.int32),
+                  torch.zeros((4, 2, 2), dtype=torch.int32), [0, 1, 2, 3]):
+        with pytest.raises(ValueError, match="given"):
+            P.category_scores(x, given)
+    for top in (-1, 65):
+        with pytest.raises(ValueError, match="top"):
+            P.category_scores(x, top=top)
+    for f in (P.category_scores, P.checkpoint_rows):
+        with pytest.raises(ValueError, match="GPU"):
+            f(x)
+    z, g, w = torch.zeros(4), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
+    back = P.category_scores_backward
+    for call in (lambda: back(x, z, g), lambda: back(x, z, grad_logp=w), lambda: back(x, z, top=g), lambda: back(x, z, grad_entropy=w),
+                 lambda: back(x, torch.zeros(3), g, grad_logp=w), lambda: back(x, z, g, grad_logp=torch.zeros(5)),
+                 lambda: back(x, z, top=torch.zeros((4, 2)), grad_top=torch.zeros((4, 2))),
+                 lambda: back(x, z, top=torch.zeros((4, 2), dtype=torch.int32), grad_top=torch.zeros((4, 3))),
+                 lambda: back(x, z, entropy=torch.zeros(2), grad_entropy=w),
+                 lambda: P.restore_rows(x)):
+        with pytest.raises(ValueError):
+            call()
+    kept = P.Checkpoint8(torch.zeros((4, 16), dtype=torch.uint8), torch.zeros((4, 1), dtype=torch.int32), (4, 10), torch.bfloat16)
+    assert kept.nbytes == 4 * 16 + 16
+    with pytest.raises(ValueError, match="come back"):
+        kept.restore(torch.float16)
+    with pytest.raises(ValueError, match="out must be"):
+        kept.restore(out=torch.zeros((4, 9), dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="GPU"):
+        kept.restore()
+
+
+def test_where_results_may_go():
+    from pcmi355 import category_rows as M
+    t = torch.zeros((6, 8))
+    assert M._no_overlap(t) and M._no_overlap(t.t()) and M._no_overlap(t[:, ::2]) and M._no_overlap(t[2:5, 3:])
+    assert M._no_overlap(torch.zeros((2, 3, 4)).permute(2, 0, 1)) and M._no_overlap(t[:1].expand(1, 8))
+    assert not M._no_overlap(t[:1].expand(6, 8)) and not M._no_overlap(t.as_strided((4, 8), (1, 1)))
+    assert not M._no_overlap(t.as_strided((3, 3), (2, 1)))
+    assert M._apart(t[:3], t[3:]) and not M._apart(t[:4], t[3:])
+
+
+def test_entry_points_refuse_without_a_gpu():
+    from pcmi355._lib import lib
+    big = ctypes.create_string_buffer(64)
+    p = ctypes.addressof(big)
+
+    def scores(x=p, type=0, n=4, v=1, c=10, given=None, gtype=3, slots=0, top=0, logp=None, best=None, codes=None, scales=None, work=None,
+               size=0):
+        return lib.pcm_category_scores(x, type, c, 0, 1, n, v, c, given, gtype, 1, 0, 0, slots, top, logp, None, None, best, best, codes,
+                                       scales, work, size, None)
+
+    def back(x=p, type=0, n=4, v=1, c=10, codes=None, scales=None, given=None, gtype=3, slots=0, gl=None, top=0, best=None, gt=None, z=p,
+             h=None, gh=None, out=p):
+        return lib.pcm_category_scores_backward(x, type, c, 0, 1, n, v, c, codes, scales, given, gtype, 1, 0, 0, slots, gl, top, best, gt, z,
+                                                h, gh, out, c, 0, 1, None)
+
+    def keep(x=p, type=0, n=4, v=1, c=10, codes=p, scales=p):
+        return lib.pcm_checkpoint_rows(x, type, c, 0, 1, n, v, c, codes, scales, None)
+
+    def restore(codes=p, scales=p, n=4, v=1, c=10, out=p, type=0):
+        return lib.pcm_restore_rows(codes, scales, n, v, c, out, type, c, 0, 1, None)
+
+    for f in (scores, back, keep, restore):
+        assert f(type=3) == -1 and f(type=-1) == -1 and b"type" in lib.pcm_last_error()
+        assert f(c=0) == -2 and f(v=0) == -2 and f(n=-1) == -2
+        assert f(n=1 << 40) == -3 and f(n=1 << 30, v=4) == -3
+        assert f(n=0) == 0                                              # nothing to do: nothing is touched
+    for f in (scores, back):
+        assert f(slots=65, given=p) == -3 and f(top=65) == -3 and f(slots=-1) == -3 and f(top=-1) == -3
+        assert f(slots=1) == -1                                         # no categories
+        assert f(slots=1, given=p, gtype=0) == -1
+        assert f(codes=p) == -1 and f(scales=p) == -1
+    assert scores(x=None) == -1 and scores(slots=1, given=p) == -1 and scores(top=2) == -1
+    assert back(x=None) == -1 and back(codes=p, scales=p) == -1         # neither scores nor checkpoint, or both
+    assert back(slots=1, given=p) == -1 and back(top=1) == -1 and back(gh=p) == -1 and back(z=None) == -1 and back(out=None) == -1
+    assert keep(x=None) == -1 and keep(codes=None) == -1 and restore(out=None) == -1 and restore(scales=None) == -1
+    assert lib.pcm_category_scores_workspace(0, 1, 10, 3) == 0 and lib.pcm_category_scores_workspace(-1, 0, 0, 99) == 0

@@ -1,0 +1,531 @@
+"""The operators on rows of category scores on the GPU, through the public entry points, against the definitions in 64 bits.
+Bounds are those of category_reference.py: they count roundings, and were written before the first run."""
+import numpy as np
+import pytest
+
+import category_reference as R
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ("float32", "bfloat16", "float16")
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    import torch
+    assert torch.cuda.is_available(), "these tests need the GPU box"
+    import pcmi355
+    return torch, pcmi355
+
+
+def _scores(torch, dtype, shape, seed, kind="plain"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g) * 3.0 - 1.0
+    C = shape[-1]
+    if kind == "masked":                              # a third of the categories, and every fifth row altogether
+        x.masked_fill_(torch.rand(C, generator=g) < 0.33, -float("inf"))
+        x.view(-1, C)[::5] = -float("inf")
+    elif kind == "lowest":                            # masks of the type's lowest value, a row of nothing else
+        x.masked_fill_(torch.rand(C, generator=g) < 0.33, torch.finfo(getattr(torch, dtype)).min)
+        x.view(-1, C)[::5] = torch.finfo(getattr(torch, dtype)).min
+    elif kind == "ties":                              # three values, and a row of one
+        x = torch.randint(0, 3, shape, generator=g).float() * torch.tensor([0.5])
+        x.view(-1, C)[-1] = -0.0
+    elif kind == "rising":                            # every entry is the likeliest so far
+        x = torch.arange(C).float().expand(shape) * (8.0 / C) + torch.zeros(shape)
+    elif kind == "falling":
+        x = -torch.arange(C).float().expand(shape) * (8.0 / C) + torch.zeros(shape)
+    elif kind == "nan":
+        x.view(-1, C)[0, C // 2] = float("nan")
+        x.view(-1, C)[-1, C - 1] = float("inf")
+    elif kind == "peaked":
+        x.view(-1, C)[:, C // 3] += 40.0
+    elif kind == "wide":                              # far from zero, far apart
+        x = x * 100.0 - 5000.0
+    return x.to(getattr(torch, dtype))
+
+
+def _numbers(t):
+    return t.double().cpu().numpy().reshape(-1, t.shape[-1])
+
+
+def _near(got, want, bound, what):
+    got, want = got.double().cpu().numpy().reshape(want.shape), want
+    bad = np.isnan(want)
+    assert np.array_equal(np.isnan(got), bad), what
+    inf = np.isinf(want)
+    assert np.array_equal(got[inf], want[inf]), what
+    ok = ~bad & ~inf
+    off = np.abs(got[ok] - want[ok])
+    past = off - np.broadcast_to(bound, want.shape)[ok]
+    assert off.size == 0 or past.max() <= 0, (what, float(off.max()), float(past.max()))
+
+
+def _check(torch, P, x, dtype, given, top, entropy=True, checkpoint=False):
+    s = P.category_scores(x, given, top=top, entropy=entropy, checkpoint=checkpoint)
+    rows, C = x.shape[:-1], x.shape[-1]
+    raw = _numbers(x)
+    y = R.seen(raw, dtype)
+    z, h = R.statistics(y)
+    near = R.log_bound(y, z, C)
+    assert s.log_sum.shape == rows and s.log_sum.dtype == torch.float32
+    _near(s.log_sum, z, near, "log_sum")
+    if entropy:
+        _near(s.entropy, h, R.entropy_bound(y, z, C), "entropy")
+    else:
+        assert s.entropy is None
+    if given is not None:
+        g = given.cpu().numpy().astype(np.int64).reshape(len(y), -1)
+        assert s.logp.shape == given.shape
+        _near(s.logp, R.logp_of(y, g), near[:, None], "logp")
+    if top:
+        index, logp = R.likeliest(y, top)
+        assert s.top.shape == (*rows, top) and s.top.dtype == torch.int32
+        assert np.array_equal(s.top.cpu().numpy().reshape(index.shape), index), "top"
+        _near(s.top_logp, logp, near[:, None], "top_logp")
+    if checkpoint:
+        back = s.checkpoint.restore(torch.float32)
+        assert np.array_equal(_numbers(back), R.rounded(raw, dtype), equal_nan=True), "checkpoint"
+        assert (s.checkpoint.codes[:, C:] == 255).all()
+    return s
+
+
+SHAPES = [(1, 1), (3, 2), (70, 3), (5, 7), (130, 16), (9, 31), (65, 33), (4, 63), (4, 64), (7, 65), (33, 100), (8, 128), (3, 250), (21, 256),
+          (6, 257), (5, 300), (4, 511), (3, 512), (3, 513), (9, 1000), (2, 1024), (3, 1025), (5, 2047), (2, 2048), (3, 2049), (2, 4100),
+          (3, 10007), (2, 16384), (1, 50021), (2, 131072)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"{s[0]}x{s[1]}")
+def test_scores_of_every_length(gpu, dtype, shape):
+    torch, P = gpu
+    g = torch.Generator().manual_seed(shape[1])
+    x = _scores(torch, dtype, shape, 100 + shape[1]).cuda()
+    given = torch.randint(0, shape[1], (shape[0],), generator=g).cuda()
+    _check(torch, P, x, dtype, given, 0, checkpoint=True)
+    _check(torch, P, x, dtype, None, min(8, shape[1] + 1), entropy=False)
+    _check(torch, P, x, dtype, given.int()[:, None].repeat(1, 3), 20 if shape[1] > 300 else 3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["masked", "lowest", "ties", "rising", "falling", "nan", "peaked", "wide"])
+@pytest.mark.parametrize("shape", [(11, 5), (12, 30), (11, 130), (11, 256), (6, 700), (6, 3001), (6, 20000)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_scores_of_every_kind(gpu, dtype, kind, shape):
+    torch, P = gpu
+    x = _scores(torch, dtype, shape, 7, kind).cuda()
+    given = torch.randint(-2, shape[1] + 2, (shape[0], 5), generator=torch.Generator().manual_seed(8)).cuda()
+    _check(torch, P, x, dtype, given, 10, checkpoint=True)
+    _check(torch, P, x, dtype, given[:, 0], 64)
+    _check(torch, P, x, dtype, given[:, 0], 1, entropy=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [4, 17, 128, 400, 5000])
+@pytest.mark.parametrize("layout", ["examples last", "sliced", "every second", "spread", "one row for all", "offset", "variables first"])
+def test_scores_of_every_layout(gpu, dtype, C, layout):
+    torch, P = gpu
+    n, v = 70, 3
+    if layout == "examples last":                     # what a forest's forward pass leaves: [variable][category][example]
+        x = _scores(torch, dtype, (v, C, n), 1).cuda().permute(2, 0, 1)
+    elif layout == "variables first":
+        x = _scores(torch, dtype, (v, n, C), 2).cuda().transpose(0, 1)
+    elif layout == "sliced":
+        x = _scores(torch, dtype, (n, v, C + 3), 3).cuda()[:, :, 1:C + 1]
+    elif layout == "every second":
+        x = _scores(torch, dtype, (n, v, 2 * C), 4).cuda()[:, :, ::2]
+    elif layout == "spread":
+        x = _scores(torch, dtype, (C, n, v), 5).cuda().permute(1, 2, 0)
+    elif layout == "one row for all":
+        x = _scores(torch, dtype, (1, v, C), 6).cuda().expand(n, v, C)
+    else:
+        x = _scores(torch, dtype, (n * v * C + 1,), 7).cuda()[1:].view(n, v, C)
+    given = torch.randint(0, C, (v, n), generator=torch.Generator().manual_seed(9), dtype=torch.uint8 if C <= 256 else torch.int64)
+    given = given.cuda().t()                          # strides of its own
+    s = _check(torch, P, x, dtype, given, 5, checkpoint=True)
+    _check(torch, P, x[:, 1], dtype, given[:, 1], 20)
+    flat = P.category_scores(x.contiguous(), given.contiguous(), top=5, entropy=True)
+    assert torch.equal(s.top, flat.top)
+
+
+@pytest.mark.parametrize("type_", ["uint8", "int32", "int64"])
+def test_given_of_every_type_and_number(gpu, type_):
+    torch, P = gpu
+    x = _scores(torch, "float32", (40, 300), 11).cuda()
+    for slots in (1, 2, 16, 63, 64):
+        g = torch.randint(0, 250, (40, slots), generator=torch.Generator().manual_seed(slots)).to(getattr(torch, type_)).cuda()
+        _check(torch, P, x, "float32", g, 0)
+    if type_ == "int64":                              # not wrapped to 32 bits
+        g = torch.full((40,), (1 << 32) + 3, device="cuda")
+        assert torch.isnan(P.category_scores(x, g).logp).all()
+        assert (P.category_scores(x, -g).logp == 0).all()
+
+
+def test_no_rows(gpu):
+    torch, P = gpu
+    x = torch.zeros((0, 10), device="cuda")
+    s = P.category_scores(x, torch.zeros(0, dtype=torch.int64, device="cuda"), top=3, entropy=True, checkpoint=True)
+    assert s.logp.shape == (0,) and s.top.shape == (0, 3) and s.checkpoint.restore().shape == (0, 10)
+    assert P.category_scores_backward(x, s.log_sum).shape == (0, 10)
+    assert P.category_scores(torch.zeros((4, 0, 10), device="cuda"), top=2).top.shape == (4, 0, 2)
+
+
+# ---- gradients ----------------------------------------------------------------------------------------------------
+
+def _slots(torch, rows, C, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-1, C, (*rows, k), generator=g).cuda(), torch.randn((*rows, k), generator=g).cuda()
+
+
+def _check_grad(torch, P, x, dtype, k=2, top=0, gh=True, kept=False, out=None, seed=5):
+    rows, C = tuple(x.shape[:-1]), x.shape[-1]
+    s = P.category_scores(x, top=top, entropy=True, checkpoint=kept)
+    kw, slots = {}, []
+    given = None
+    if k:
+        given, kw["grad_logp"] = _slots(torch, rows, C, k, seed)
+        slots.append((given.cpu().numpy().reshape(-1, k), _numbers(kw["grad_logp"])))
+    if top:
+        kw["top"], kw["grad_top"] = s.top, _slots(torch, rows, C, top, seed + 1)[1]
+        slots.append((s.top.cpu().numpy().reshape(-1, top), _numbers(kw["grad_top"])))
+    w = None
+    if gh:
+        kw["entropy"], kw["grad_entropy"] = s.entropy, torch.randn(rows, generator=torch.Generator().manual_seed(seed + 2)).cuda()
+        w = kw["grad_entropy"].double().cpu().numpy().reshape(-1)
+    y = _numbers(x)
+    z, h = (t.double().cpu().numpy().reshape(-1) for t in (s.log_sum, s.entropy))
+    want, size = R.gradient(R.rounded(y, dtype) if kept else R.seen(y, dtype), z, h, slots, w)
+    got = P.category_scores_backward(s.checkpoint if kept else x, s.log_sum, given, out=out, **kw)
+    assert got.shape == x.shape and got.dtype == x.dtype and (out is None or got is out)
+    # the terms' sizes carry the roundings in 32 bits: a dozen operations, one addition per slot; then one to the type
+    bound = size * ((16 + k + top) * R.EPS) + np.abs(np.nan_to_num(want)) * R.HALF[dtype] + R.TINY[dtype] + 2.0 ** -126
+    _near(got, want.reshape(-1, C), bound, "gradient")
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kept", [False, True], ids=["scores", "8 bits"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"{s[0]}x{s[1]}")
+def test_gradient_of_every_length(gpu, dtype, kept, shape):
+    torch, P = gpu
+    x = _scores(torch, dtype, shape, 200 + shape[1]).cuda()
+    _check_grad(torch, P, x, dtype, k=1, gh=False, kept=kept)
+    _check_grad(torch, P, x, dtype, k=7, top=min(5, shape[1]), kept=kept)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kept", [False, True], ids=["scores", "8 bits"])
+@pytest.mark.parametrize("kind", ["masked", "lowest", "ties", "nan", "peaked", "wide"])
+@pytest.mark.parametrize("shape", [(12, 30), (11, 256), (6, 700), (6, 9000)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_gradient_of_every_kind(gpu, dtype, kept, kind, shape):
+    torch, P = gpu
+    x = _scores(torch, dtype, shape, 17, kind).cuda()
+    _check_grad(torch, P, x, dtype, k=3, top=4, kept=kept)
+    _check_grad(torch, P, x, dtype, k=0, kept=kept)
+    _check_grad(torch, P, x, dtype, k=64, top=64, gh=False, kept=kept)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kept", [False, True], ids=["scores", "8 bits"])
+@pytest.mark.parametrize("C", [4, 128, 5000])
+def test_gradient_into_every_layout(gpu, dtype, kept, C):
+    torch, P = gpu
+    n, v = 70, 3
+    t = getattr(torch, dtype)
+    heads = _scores(torch, dtype, (v, C, n), 1).cuda().permute(2, 0, 1)
+    assert _check_grad(torch, P, heads, dtype, kept=False).stride() == heads.stride()
+    for x in (heads, heads.contiguous(), _scores(torch, dtype, (n, v, C + 3), 3).cuda()[:, :, 1:C + 1]):
+        _check_grad(torch, P, x, dtype, kept=kept)
+        around = torch.full((n, v, C + 5), 7.0, dtype=t, device="cuda")
+        _check_grad(torch, P, x, dtype, kept=kept, out=around[:, :, 2:C + 2])
+        assert (around[:, :, :2] == 7).all() and (around[:, :, C + 2:] == 7).all()      # nothing beside the rows is touched
+        _check_grad(torch, P, x, dtype, kept=kept, out=torch.empty((v, C, n), dtype=t, device="cuda").permute(2, 0, 1))
+        _check_grad(torch, P, x, dtype, kept=kept, out=torch.empty((n, v, 2 * C), dtype=t, device="cuda")[:, :, 1::2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [5, 100, 256, 1001, 20000])
+def test_gradient_in_place_of_the_scores(gpu, dtype, C):
+    torch, P = gpu
+    x = _scores(torch, dtype, (9, C), 23).cuda()
+    g, w = _slots(torch, (9,), C, 6, 1)
+    s = P.category_scores(x, g, top=min(C, 8), entropy=True)
+    kw = dict(grad_logp=w, entropy=s.entropy, grad_entropy=torch.ones(9, device="cuda"), top=s.top, grad_top=torch.ones(s.top.shape, device="cuda"))
+    want = P.category_scores_backward(x, s.log_sum, g, **kw)
+    assert P.category_scores_backward(x, s.log_sum, g, out=x, **kw) is x and torch.equal(x, want)
+
+
+def test_gradient_refuses_overlapping_results(gpu):
+    torch, P = gpu
+    buf = torch.zeros(200, device="cuda")
+    x = buf[:80].view(8, 10)
+    z = P.category_scores(x).log_sum
+    for out in (buf[5:85].view(8, 10), buf[:10].expand(8, 10), torch.zeros((8, 10)), torch.zeros((8, 9), device="cuda"),
+                torch.zeros((8, 10), device="cuda", dtype=torch.float16)):
+        with pytest.raises(ValueError):
+            P.category_scores_backward(x, z, out=out)
+    with pytest.raises(ValueError):
+        P.category_scores(x, torch.zeros(8, dtype=torch.int64))                          # given on the host
+    with pytest.raises(ValueError):
+        P.category_scores_backward(x, z.cpu())
+
+
+def test_gradient_is_the_derivative(gpu):
+    """Central differences of the forward pass itself: its values are off by about 1e-6, the step is 1e-2, third derivatives
+    are of order one: 2 x 1e-6 / 2e-2 + 1e-4 / 6 for each of the four summands"""
+    torch, P = gpu
+    C = 40
+    x = _scores(torch, "float32", (1, C), 31).cuda()
+    g, w = torch.tensor([[3, 17, 3]]).cuda(), torch.tensor([[0.5, -1.0, 0.25]]).cuda()
+    s = P.category_scores(x, g, entropy=True)
+    grad = P.category_scores_backward(x, s.log_sum, g, grad_logp=w, entropy=s.entropy, grad_entropy=torch.tensor([0.7]).cuda())[0]
+    step = 1e-2
+    moved = x + torch.cat([torch.eye(C), -torch.eye(C)]).cuda() * step
+    t = P.category_scores(moved, g.expand(2 * C, 3), entropy=True)
+    loss = (t.logp.double() * w.double()).sum(1) + 0.7 * t.entropy.double()
+    diff = (loss[:C] - loss[C:]) / (2 * step)
+    assert (diff - grad.double()).abs().max() < 4 * (1e-4 + 2e-5)
+
+
+# ---- 8 bits -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["plain", "masked", "lowest", "ties", "rising", "nan", "wide"])
+@pytest.mark.parametrize("shape", [(5, 1), (3, 15), (7, 64), (4, 65), (3, 128), (9, 1000), (2, 10007), (1, 70001)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_rows_in_eight_bits(gpu, dtype, kind, shape):
+    torch, P = gpu
+    x = _scores(torch, dtype, shape, 41, kind).cuda()
+    kept = P.checkpoint_rows(x)
+    want = R.rounded(_numbers(x), dtype)
+    back = kept.restore(torch.float32)
+    assert np.array_equal(_numbers(back), want, equal_nan=True)
+    own = kept.restore()
+    top = torch.finfo(x.dtype).max
+    assert own.dtype == x.dtype and torch.equal(torch.nan_to_num(own, 1e3), torch.nan_to_num(back.clamp(max=top).to(x.dtype), 1e3))
+    assert kept.codes.shape == (shape[0], -(-shape[1] // 16) * 16) and (kept.codes[:, shape[1]:] == 255).all()
+
+
+def test_extreme_rows_in_eight_bits(gpu):
+    torch, P = gpu
+    lo, hi = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
+    rows = [[hi, -hi / 2.1, 1.0, 0.0], [lo, lo / 8, -lo, 0.0], [0.0, -0.0, 0.0, 0.0], [hi, hi, hi, hi], [-hi, -float("inf"), -hi, -hi],
+            [1e-3, 1.0, 253.0 / 256, 254.0 / 256], [5.0, 5.0 + 2.0 ** -20, 5.0, 5.0], [-1.6e38, 3.4e38, 0.0, -hi]]
+    x = torch.tensor(rows).cuda()
+    assert np.array_equal(_numbers(P.checkpoint_rows(x).restore()), R.rounded(_numbers(x), "float32"))
+    for t, name in ((torch.float16, "float16"), (torch.bfloat16, "bfloat16")):
+        m = torch.finfo(t).max
+        y = torch.tensor([[m, -m / 3, 0.5, 1.0], [m, m, m, m], [torch.finfo(t).tiny, 0.0, -torch.finfo(t).tiny, 0.0]], dtype=t).cuda()
+        kept = P.checkpoint_rows(y)
+        assert np.array_equal(_numbers(kept.restore(torch.float32)), R.rounded(_numbers(y), name))
+        assert torch.isfinite(kept.restore()).all()
+
+
+def test_eight_bits_of_every_layout(gpu):
+    torch, P = gpu
+    for dtype in TYPES:
+        for x in (_scores(torch, dtype, (300, 70), 1).cuda().t(), _scores(torch, dtype, (9, 210), 2).cuda()[:, 3:203],
+                  _scores(torch, dtype, (9, 200), 2).cuda()[:, ::2], _scores(torch, dtype, (3, 100, 5), 3).cuda().permute(2, 0, 1),
+                  _scores(torch, dtype, (1, 200), 4).cuda().expand(6, 200)):
+            kept = P.checkpoint_rows(x)
+            want = R.rounded(_numbers(x), dtype)
+            assert np.array_equal(_numbers(kept.restore(torch.float32)), want)
+            around = torch.full((*x.shape[:-1], x.shape[-1] + 4), 3.0, device="cuda")
+            out = around[..., 1:-3]
+            assert kept.restore(out=out) is out and np.array_equal(_numbers(out.contiguous()), want)
+            assert (around[..., 0] == 3).all() and (around[..., -3:] == 3).all()
+            out = torch.zeros(x.shape[::-1], device="cuda").permute(*reversed(range(x.dim())))
+            kept.restore(out=out)
+            assert np.array_equal(_numbers(out.contiguous()), want)
+
+
+# ---- as they are used ---------------------------------------------------------------------------------------------
+
+def test_same_bits_every_time(gpu):
+    torch, P = gpu
+    for shape, dtype in (((2, 131072), "bfloat16"), ((700, 256), "float32"), ((5, 20000), "float16")):
+        x = _scores(torch, dtype, shape, 51, "ties" if dtype == "bfloat16" else "plain").cuda()
+        g, w = _slots(torch, shape[:1], shape[1], 64, 1)
+        first = None
+        for _ in range(3):
+            s = P.category_scores(x, g, top=20, entropy=True)
+            d = P.category_scores_backward(x, s.log_sum, g, grad_logp=w, entropy=s.entropy, grad_entropy=w[:, 0])
+            got = (*s[:5], d)
+            if first is None:
+                first = got
+            assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_captured_and_replayed(gpu):
+    """A training step over 8-bit scores in a graph, replayed on new scores between eager calls on other streams"""
+    torch, P = gpu
+    for shape, dtype in (((3, 70001), torch.bfloat16), ((50, 256), torch.float32), ((64, 6), torch.float32)):
+        C = shape[1]
+        x = torch.randn(shape, device="cuda").to(dtype)
+        g = torch.randint(0, C, shape[:1], device="cuda")
+        w = torch.randn(shape[:1], device="cuda")
+
+        def step(x, g, w):
+            s = P.category_scores(x, g, top=4, entropy=True, checkpoint=True)
+            d = P.category_scores_backward(s.checkpoint, s.log_sum, g, grad_logp=w, entropy=s.entropy, grad_entropy=w, top=s.top,
+                                           grad_top=s.top_logp)
+            return s.logp, s.log_sum, s.entropy, s.top, s.top_logp, d, P.category_scores_backward(x, s.log_sum, g, grad_logp=w)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(x, g, w)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs = []
+        for _ in range(2):                            # two graphs of the same call, replayed one after the other
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                graphs.append((graph, None))
+                out = step(x, g, w)
+            graphs[-1] = (graph, out)
+        for k in range(4):
+            x.copy_(torch.randn(shape, device="cuda"))
+            g.copy_(torch.randint(0, C, shape[:1], device="cuda"))
+            for graph, _ in graphs:
+                graph.replay()
+            want = step(x, g, w)
+            torch.cuda.synchronize()
+            for _, out in graphs:
+                assert all(torch.equal(a, b) for a, b in zip(out, want)), (shape, k)
+
+
+def test_on_a_stream_of_its_own(gpu):
+    torch, P = gpu
+    side = torch.cuda.Stream()
+    for shape in ((4, 131072), (3000, 128)):
+        host = torch.randn(shape)
+        x = torch.empty(shape, device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)             # the scores arrive late, on the stream that the call is made on
+            x.copy_(host)
+            s = P.category_scores(x, top=3, entropy=True, checkpoint=True)
+            d = P.category_scores_backward(x, s.log_sum, entropy=s.entropy, grad_entropy=torch.ones(shape[0], device="cuda"))
+        side.synchronize()
+        t = P.category_scores(x, top=3, entropy=True, checkpoint=True)
+        assert torch.equal(s.top, t.top) and torch.equal(s.log_sum, t.log_sum) and torch.equal(s.checkpoint.codes, t.checkpoint.codes)
+        assert torch.equal(d, P.category_scores_backward(x, t.log_sum, entropy=t.entropy, grad_entropy=torch.ones(shape[0], device="cuda")))
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """Rows behind 2^31 elements and 2^32 bytes, and categories that lie further apart than that"""
+    torch, P = gpu
+    buf = torch.zeros((1 << 31) + (1 << 20), dtype=torch.float16, device="cuda")
+    far = buf[-(1 << 19):].view(4, -1)
+    far.copy_(torch.randn(far.shape, device="cuda"))
+    x = buf.as_strided((2, 1 << 17), (buf.numel() - (1 << 17), 1))
+    assert x[1].data_ptr() == far[3].data_ptr()
+    g = torch.tensor([5, 6], device="cuda")
+    w = torch.ones(2, device="cuda")
+    s = _check(torch, P, x, "float16", g, 5, checkpoint=True)
+    near = x.contiguous()
+    want = P.category_scores_backward(near, s.log_sum, g, grad_logp=w)
+    assert torch.equal(P.category_scores_backward(x, s.log_sum, g, grad_logp=w, out=x), want) and torch.equal(x, want)
+    y = buf.as_strided((1, 2), (1, buf.numel() - 1))
+    y.copy_(torch.tensor([[1.0, 2.0]]))
+    _check(torch, P, y, "float16", None, 2, checkpoint=True)
+    del buf, far, x, y
+    torch.cuda.empty_cache()
+
+
+def test_many_rows(gpu):
+    """More rows than a launch has workgroups for"""
+    torch, P = gpu
+    n = (1 << 21) + 3
+    x = torch.randn((n, 3), device="cuda")
+    g = torch.randint(0, 3, (n,), device="cuda", dtype=torch.uint8)
+    s = P.category_scores(x, g, top=1, entropy=True, checkpoint=True)
+    want = torch.log_softmax(x.double(), 1)
+    assert (s.logp - want.gather(1, g.long()[:, None])[:, 0]).abs().max() < 2e-6
+    assert torch.equal(s.top[:, 0].long(), x.argmax(1))
+    d = P.category_scores_backward(x, s.log_sum, g, grad_logp=torch.ones(n, device="cuda"))
+    assert (d - (torch.nn.functional.one_hot(g.long(), 3) - want.exp())).abs().max() < 2e-6
+    back = s.checkpoint.restore()
+    assert (back - x).abs().max() <= (x.amax(1) - x.amin(1)).max() / 126.5 / 2 + 1e-6
+
+
+def test_posterior_of_heads(gpu):
+    """A multi-head circuit and a forest: log-posterior of the examples' clusters from the per-head likelihoods"""
+    torch, P = gpu
+    from pcmi355 import workloads as W
+    rng = np.random.default_rng(3)
+    V, K, C, H, n = 24, 16, 8, 5, 37
+    data = rng.integers(0, C, (n, V)).astype(np.uint8)
+    par = W.chow_liu_parent(rng.integers(0, C, (200, V)).astype(np.uint8))
+    d = torch.from_numpy(data).cuda()
+    for forest in (False, True):
+        if forest:
+            parent = np.concatenate([par, np.where(par < 0, -1, par + V)]).astype(np.int32)
+            c = P.hclt_forest_from_clts(parent, C, K, H)
+            x = d.repeat(1, 2)
+        else:
+            c, x = P.multihead_hclt_from_clt(par, C, K, H), d
+        c.set_params(*W.init_params(np.zeros(x.shape[1]), K, C, 4, kind="dirichlet"))
+        trees = 2 if forest else 1
+        heads = np.log(rng.dirichlet(np.ones(K), (trees, H))).astype(np.float32)
+        c.set_heads(heads)
+        if forest:
+            ll = P.forest_loglikelihoods(c, x).permute(2, 0, 1)
+            given = torch.randint(0, H, (n, trees), device="cuda", dtype=torch.uint8)
+        else:
+            ll = P.loglikelihoods(c, x)
+            given = torch.randint(0, H, (n,), device="cuda", dtype=torch.uint8)
+        s = P.head_scores(c, x, given, top=2)
+        want = torch.log_softmax(ll.double(), -1)
+        pick = want.gather(-1, given.long().unsqueeze(-1)).squeeze(-1)
+        # a likelihood near -60 has steps of 4e-6; the log-sum is stored at that size, differences are not
+        assert (s.logp - pick).abs().max() < 4e-6
+        assert torch.equal(s.top.long(), torch.sort(ll, dim=-1, descending=True, stable=True).indices[..., :2])
+        assert (s.entropy + (want.exp() * want).sum(-1)).abs().max() < 4e-6
+        ids = torch.tensor([5, 0, 30], device="cuda")
+        sub = P.head_scores(c, x, given[ids], top=2, example_ids=ids)
+        assert torch.equal(sub.top, s.top[ids]) and (sub.logp - s.logp[ids]).abs().max() < 1e-5
+        if not forest:
+            mix = P.multihead_loglikelihoods(c, x, torch.ones((n, H), device="cuda"))
+            assert (s.log_sum - np.log(H) - mix).abs().max() < 2e-5
+            part = P.head_scores(c, x, given, top=2, batch_size=10)
+            assert torch.equal(part.top, s.top)
+    with pytest.raises(ValueError, match="heads"):
+        P.head_scores(P.hclt_from_clt(par, C, K), d)
+
+
+def test_variational_step_from_eight_bits(gpu):
+    """KL and relaxed samples whose parameter rows wait for the reverse pass in 8 bits: the gradients are those at the rounded
+    rows, bit for bit; forward results are untouched"""
+    torch, P = gpu
+    from pcmi355 import workloads as W
+    prealloc = P.prealloc
+    rng = np.random.default_rng(5)
+    V, K, C, rows = 12, 16, 12, 6
+    par = W.chow_liu_parent(rng.integers(0, C, (200, V)).astype(np.uint8))
+    c = P.hclt_from_clt(par, C, K)
+    n = c.num_parameters()
+    p1, p2 = (np.log(rng.uniform(0.05, 1.0, (rows, n))).astype(np.float32) for _ in range(2))
+    p2 = p2[:1]
+    r1, r2 = (P.checkpoint_rows(torch.from_numpy(p).cuda()).restore().cpu().numpy() for p in (p1, p2))
+    assert np.abs(r1 - p1).max() <= 3.0 / 126 / 2 + 1e-6 and np.abs(r1 - p1).max() > 0
+    prealloc.kld_preallocation(c, num_examples=rows)
+    want = prealloc.kld_with_prealloc(c, p1, p2)
+    prealloc.kld_with_prealloc(c, r1, r2)
+    grads = prealloc.kld_backward_with_prealloc(c)
+    prealloc.kld_preallocation(c, num_examples=rows, checkpoint=True)
+    assert np.array_equal(prealloc.kld_with_prealloc(c, p1, p2), want)
+    kept = prealloc._state["kld"]["rows"]
+    assert kept[0].nbytes < 4 * rows * n * 0.28
+    for a, b in zip(prealloc.kld_backward_with_prealloc(c), grads):
+        assert np.array_equal(a, b)
+    prealloc.kld_free_mem()
+
+    og = rng.normal(size=(rows, V, C)).astype(np.float32)
+    found = []
+    for params, checkpoint in ((r1, False), (p1, True)):
+        prealloc.gumbel_sample_preallocation(c, num_examples=rows, num_vars=V, par_buffer_size=C, allocate_for_grad=True,
+                                             checkpoint=checkpoint)
+        gen = torch.Generator(device="cuda").manual_seed(9)
+        prealloc.gumbel_sample_with_prealloc(c, params, temperature=0.8, generator=gen)
+        found.append(prealloc.gumbel_sample_backward_with_prealloc(c, og, temperature=0.8))
+        prealloc.gumbel_sample_free_mem()
+    assert np.array_equal(*found)
