@@ -52,6 +52,8 @@ void check_given(const GivenRef& given);
 #ifdef __HIPCC__
 // ---- device side ------------------------------------------------------------------------------------------------
 
+// (by value: a bit cast of a vector's element takes the vector's first one)
+__device__ __forceinline__ float as_float(uint32_t v) { return __builtin_bit_cast(float, v); }
 template <typename T>
 __device__ __forceinline__ float to_float(T v) { return (float)v; }
 template <typename T>
@@ -59,6 +61,21 @@ __device__ __forceinline__ T from_float(float v) { return (T)v; }   // round to 
 
 typedef __bf16 bf16;
 typedef _Float16 f16;
+typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of a row at an address that is aligned to its entries only
+typedef raw4 raw4_by4 __attribute__((aligned(4)));
+typedef raw4 raw4_by2 __attribute__((aligned(2)));
+template <typename T>
+__device__ __forceinline__ raw4 load16(const T* p) {
+  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const raw4_by4*>(p);
+  else return *reinterpret_cast<const raw4_by2*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, raw4 v) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<raw4_by4*>(p) = v;
+  else *reinterpret_cast<raw4_by2*>(p) = v;
+}
 
 // Entry `slot` of a row's given categories, whatever their type; negative: not observed.
 __device__ __forceinline__ int64_t given_at(const GivenRef& g, int64_t e, int64_t v, int slot) {
@@ -68,17 +85,106 @@ __device__ __forceinline__ int64_t given_at(const GivenRef& g, int64_t e, int64_
   return static_cast<const int64_t*>(g.p)[at];
 }
 
-// Order of entries, likeliest first: larger value, then smaller index (the two zeros are one value).  0 is below them all.
-__device__ __forceinline__ uint64_t entry_key(float x, uint32_t index) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
-  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (uint64_t)o << 32 | (uint32_t)~index;
+// Order of floats as whole numbers (NaN aside), and back
+__device__ __forceinline__ uint32_t float_order(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_value(uint64_t k) {
-  const uint32_t o = (uint32_t)(k >> 32);
+__device__ __forceinline__ float order_float(uint32_t o) {
   return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
+
+// Order of entries, likeliest first: larger value, then smaller index (the two zeros are one value).  0 is below them all.
+__device__ __forceinline__ uint64_t entry_key(float x, uint32_t index) {
+  return (uint64_t)float_order(x + 0.f) << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  return order_float((uint32_t)(k >> 32));
+}
 __device__ __forceinline__ int32_t key_index(uint64_t k) { return (int32_t) ~(uint32_t)k; }
+
+// ---- lanes of a wave --------------------------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, false));
+}
+// f over the lanes of groups of N (4, 8, 16 or 64) neighbours, in all of them; every lane is active
+template <int N, typename F>
+__device__ __forceinline__ float over_lanes(float v, F f) {
+  v = f(v, dpp<0xB1>(v));                       // the neighbour
+  v = f(v, dpp<0x4E>(v));                       // the next pair
+  if (N >= 8) v = f(v, dpp<0x141>(v));          // mirrored in eight
+  if (N >= 16) v = f(v, dpp<0x140>(v));         // mirrored in sixteen
+  if (N >= 64) {
+    auto h = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = f(as_float(h[0]), as_float(h[1]));
+    auto w = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = f(as_float(w[0]), as_float(w[1]));
+  }
+  return v;
+}
+struct Larger { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Smaller { __device__ float operator()(float a, float b) const { return fminf(a, b); } };
+struct LargerOrNan { __device__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); } };
+struct Sum { __device__ float operator()(float a, float b) const { return a + b; } };
+
+// the value of lane ^ J
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  const int b = (int)v;
+  if (J == 1) return __builtin_amdgcn_mov_dpp(b, 0xB1, 0xf, 0xf, false);
+  if (J == 2) return __builtin_amdgcn_mov_dpp(b, 0x4E, 0xf, 0xf, false);
+  if (J == 4)                                    // four up for the even quads, four down for the odd ones
+    return __builtin_amdgcn_update_dpp(__builtin_amdgcn_update_dpp(b, b, 0x104, 0xf, 0x5, false), b, 0x114, 0xf, 0xa, false);
+  if (J == 8) return __builtin_amdgcn_mov_dpp(b, 0x128, 0xf, 0xf, false);
+  const bool low = !((threadIdx.x & 63) & J);
+  if (J == 16) {
+    auto h = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return low ? h[1] : h[0];
+  }
+  auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return low ? h[1] : h[0];
+}
+template <int J>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  return (uint64_t)lane_xor<J>((uint32_t)(v >> 32)) << 32 | lane_xor<J>((uint32_t)v);
+}
+
+// Bitonic sorts of groups of N neighbouring lanes: the step of merge size S whose pairs lie J apart.  Which lanes keep the larger
+// value is a constant of the step, a mask that needs no comparison.
+constexpr uint64_t larger_lanes(int N, int S, int J, bool falling) {
+  uint64_t mask = 0;
+  for (int lane = 0; lane < 64; ++lane) {
+    bool f = falling;
+    for (int n = N; n > S; n /= 2) f = !(lane & (n / 2)) == f;   // the two halves of a sort run against each other
+    if (f == !(lane & J)) mask |= 1ull << lane;
+  }
+  return mask;
+}
+template <int N, int S, int J, bool kFalling, typename K>
+__device__ __forceinline__ K sort_step(K v) {
+  constexpr uint64_t larger = larger_lanes(N, S, J, kFalling);
+  const K o = lane_xor<J>(v);
+  return (v > o) == __builtin_amdgcn_inverse_ballot_w64(larger) ? v : o;
+}
+template <int N, int S, int J, bool kFalling, typename K>
+__device__ __forceinline__ K sort_merge_steps(K v) {
+  v = sort_step<N, S, J, kFalling>(v);
+  if constexpr (J > 1) v = sort_merge_steps<N, S, J / 2, kFalling>(v);
+  return v;
+}
+template <int N, int S, bool kFalling, typename K>
+__device__ __forceinline__ K sort_sizes(K v) {
+  if constexpr (S > 2) v = sort_sizes<N, S / 2, kFalling>(v);
+  return sort_merge_steps<N, S, S / 2, kFalling>(v);
+}
+template <int N, bool kFalling, typename K>
+__device__ __forceinline__ K sort_lanes(K v) { return sort_sizes<N, N, kFalling>(v); }
+// the same of lanes that rise and then fall, or fall and then rise
+template <int N, bool kFalling, typename K>
+__device__ __forceinline__ K sort_merge(K v) { return sort_merge_steps<N, N, N / 2, kFalling>(v); }
 
 // The largest entry that counts as masked: half of the type's lowest value (what adding a mask of the lowest value leaves).
 template <typename T>
@@ -92,6 +198,28 @@ template <typename T>
 __device__ __forceinline__ float seen(T v) {
   const float x = to_float(v);
   return x <= masked_from<T>() ? -INFINITY : x;
+}
+// the entries of 16 bytes, scores with masks at -inf (f16: its masks lie within the range of the exponential)
+__device__ __forceinline__ void unpack(raw4 r, float (&x)[4], float) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = as_float(r[i]);
+}
+__device__ __forceinline__ void unpack(raw4 r, float (&x)[8], bf16) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = as_float(r[i] << 16);
+    x[2 * i + 1] = as_float(r[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(raw4 r, float (&x)[8], f16) {
+  typedef f16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = r[i];
+    const pair h = __builtin_bit_cast(pair, w);
+    x[2 * i] = seen(h[0]);
+    x[2 * i + 1] = seen(h[1]);
+  }
 }
 template <typename T>
 __device__ __forceinline__ float type_max() { return 3.4028235e38f; }

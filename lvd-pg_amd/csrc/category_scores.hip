@@ -1,5 +1,6 @@
-// Log-probabilities of given categories, entropy and likeliest categories of rows of scores.
-#include "category_rows.hpp"
+// Log-probabilities of given categories, entropy and likeliest categories of rows of scores: choice of the kernel, rows of any
+// length and stride (score_stream_kernel).  Short rows and rows that lie side by side: category_scores_short.hip.
+#include "category_stats.hip.hpp"
 
 namespace pcm {
 
@@ -18,103 +19,332 @@ void check_given(const GivenRef& g) {
 }
 
 namespace {
-struct ScoreOut {
-  float *logp, *log_sum, *entropy, *top_logp;
-  int32_t* top;
+constexpr int kGroups = 4;                  // 16-byte groups that a lane requests at a time
+constexpr int kMaxWaves = 16, kMaxParts = 64;
+
+struct PartRef {                            // what parts of a row leave for the kernel that joins them
+  float4* sums;                             // [rows][parts] m, s, t
+  uint64_t* keys;                           // [rows][parts][top], falling
 };
 
-__device__ __forceinline__ float block_max(float v, float* sh) {
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-}
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+// How rows are dealt out: waves of a workgroup, and workgroups, per row
+struct Split {
+  int waves, parts, part_len;
+};
+
+// A wave's 64 likeliest entries so far, lane i holding the i-th as entry_key, and those that wait to be sorted in.  Entries at or
+// below `bar`, the value of the top-th so far, are left out; what passes waits in LDS, and 64 at a time are sorted and merged.
+// Groups of entries come by rising index, so that one that equals the bar of earlier groups loses to what is there.
+struct TopList {
+  uint64_t list = 0;
+  float bar;
+  int count = 0;
+  __device__ __forceinline__ void flush(uint64_t* wait, int top) {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_wave_barrier();
+    uint64_t k = lane < count ? wait[lane] : 0;
+    k = sort_lanes<64, false>(k);
+    list = sort_merge<64, true>(list > k ? list : k);
+    const uint64_t rest = lane + 64 < count ? wait[lane + 64] : 0;
+    __builtin_amdgcn_wave_barrier();
+    if (lane + 64 < count) wait[lane] = rest;
+    __builtin_amdgcn_wave_barrier();
+    count = max(count - 64, 0);
+    const uint32_t last = __builtin_amdgcn_readlane((uint32_t)(list >> 32), top - 1);
+    if (last) bar = fmaxf(bar, order_float(last));
+  }
+  __device__ __forceinline__ void take(float x, uint32_t index, float above, uint64_t* wait, int top) {
+    const uint64_t pass = __ballot(x > above);
+    if (!pass) return;
+    if (x > above) wait[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] = entry_key(x, index);
+    count += __popcll(pass);
+    if (count >= 64) flush(wait, top);
+  }
+};
+
+// the results of a row from its sums and sorted keys, by one wave
+template <typename T>
+__device__ __forceinline__ void write_row(const RowSums<T>& q, uint64_t key, int64_t r, int64_t e, int64_t v, const RowsRef& x, const RowsShape& shape,
+                                          const GivenRef& given, int top, const ScoreOut& out) {
+  const int lane = threadIdx.x & 63;
+  const RowResult<T> res(q);
+  const T* row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
+  if (lane < given.slots)
+    out.logp[r * given.slots + lane] = res.given(given_at(given, e, v, lane), shape.cats, [&](int64_t g) { return seen(row[g * x.stride_cat]); });
+  if (lane == 0) {
+    if (out.log_sum) out.log_sum[r] = res.log_sum();
+    if (out.entropy) out.entropy[r] = res.entropy(q);
+  }
+  if (lane < top) {
+    out.top[r * top + lane] = res.nan || !key ? -1 : key_index(key);
+    out.top_logp[r * top + lane] = res.nan ? NAN : !key ? -INFINITY : res.logp(key_value(key));
+  }
 }
 
-// One workgroup per row, three kinds of passes over it: maximum, sums, and one search per likeliest category.
-template <typename T>
-__global__ __launch_bounds__(256) void score_rows_kernel(RowsRef x, RowsShape shape, GivenRef given, int top, ScoreOut out) {
-  __shared__ float sh[4];
-  __shared__ uint64_t best_sh[4];
-  const int64_t rows = shape.rows();
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t e = r / shape.vars, v = r % shape.vars;
-    const T* row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
-    float m = -3.4028235e38f;
-    for (int c = threadIdx.x; c < shape.cats; c += 256) m = fmaxf(m, seen(row[c * x.stride_cat]));
-    m = block_max(m, sh);
-    float s = 0.f, t = 0.f;
-    for (int c = threadIdx.x; c < shape.cats; c += 256) {
-      const float d = seen(row[c * x.stride_cat]) - m, p = expf(d);
-      s += p;
-      if (p > 0.f) t += p * d;
+// One pass over a row, or a part of it, by the waves of a workgroup.  A wave takes kGroups x 16 bytes a lane at a time (one
+// entry at a time where categories are not neighbours), requests the next ones before it works on these, and keeps one maximum
+// for its lanes: a group whose largest entry lies above neither the maximum nor the list's bar goes straight into the sums.
+template <typename T, bool kUnit, bool kEnt, bool kTop, bool kCkpt>
+__global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x, RowsShape shape, GivenRef given, int top, ScoreOut out, CkptRef ckpt,
+                                                                      int parts, int part_len, PartRef part) {
+  constexpr int kVec = kUnit ? 16 / (int)sizeof(T) : 1, kLoads = kUnit ? kGroups : 16, kChunk = 64 * kVec * kLoads;
+  extern __shared__ uint64_t stream_lds[];   // per wave 128 keys that wait, and its sums
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  uint64_t* const wait = stream_lds + 128 * wave;
+  float4* const sums_lds = reinterpret_cast<float4*>(stream_lds + 128 * waves);
+  const int64_t jobs = shape.rows() * parts;
+  const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
+
+  for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const uint32_t r = parts == 1 ? (uint32_t)job : (uint32_t)job / (uint32_t)parts;   // (more than one part: fewer than 2^31 jobs)
+    const int q = parts == 1 ? 0 : (int)((uint32_t)job - r * (uint32_t)parts);
+    const int64_t e = shape.vars == 1 ? r : r / (uint32_t)shape.vars, v = shape.vars == 1 ? 0 : r % (uint32_t)shape.vars;
+    const T* const row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
+    const int first = q * part_len, end = parts == 1 ? shape.cats : min(first + part_len, shape.cats);
+
+    RowSums<T> sum;
+    TopList list;
+    list.bar = masked_from<T>();
+    bool fresh = true;
+
+    struct Chunk { typename std::conditional<kUnit, raw4, T>::type g[kLoads]; };
+    auto load = [&](Chunk& k, int at) {                       // a whole chunk
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        if constexpr (kUnit) k.g[u] = load16(row + at + (u * 64 + lane) * kVec);
+        else k.g[u] = row[(int64_t)(at + u * 64 + lane) * x.stride_cat];
+      }
+    };
+    auto load_end = [&](Chunk& k, int at) {                   // the last one: -inf behind the end
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int c = at + (u * 64 + lane) * kVec;
+        if constexpr (kUnit) {
+          if (c + kVec <= end) k.g[u] = load16(row + c);
+          else {
+            T w[kVec];
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) w[i] = c + i < end ? row[c + i] : (T)-INFINITY;
+            k.g[u] = __builtin_bit_cast(raw4, w);
+          }
+        } else k.g[u] = c < end ? row[(int64_t)c * x.stride_cat] : (T)-INFINITY;
+      }
+    };
+    auto entries = [&](const Chunk& k, int u, float (&y)[kVec]) {
+      if constexpr (kUnit) unpack(k.g[u], y, T());
+      else y[0] = seen(k.g[u]);
+    };
+    auto work = [&](const Chunk& k, int at) {
+      if (kTop && fresh) {
+        // the top-th largest of the lanes' largest entries is no larger than the top-th largest entry: a bar to start from
+        float largest = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          float y[kVec];
+          entries(k, u, y);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, y[i]);
+        }
+        const uint32_t order = sort_lanes<64, true>(float_order(largest));
+        const float top_value = order_float(__builtin_amdgcn_readlane(order, 0));
+        const uint32_t last = __builtin_amdgcn_readlane(order, top - 1);
+        if (top_value > masked_from<T>()) sum.raise(top_value);
+        list.bar = fmaxf(list.bar, order_float(last - (last == 0x80000000u ? 2 : 1)));   // (just below, both zeros being one: the entry itself has to pass)
+        fresh = false;
+      }
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        if (at + u * 64 * kVec >= end) break;
+        float y[kVec], largest = -INFINITY, gs = 0.f, gt = 0.f;
+        entries(k, u, y);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) largest = kCkpt ? __builtin_elementwise_maximum(largest, y[i]) : fmaxf(largest, y[i]);
+        if (__any(largest > (kTop ? list.bar : sum.m))) {
+          const float m1 = over_lanes<64>(largest, Larger());
+          if (m1 > sum.m) sum.raise(m1);
+          const float above = list.bar;
+          if (kTop)
+#pragma unroll 1
+            for (int i = 0; i < kVec; ++i) {
+              float yi = y[0];
+#pragma unroll
+              for (int j = 1; j < kVec; ++j) yi = i == j ? y[j] : yi;
+              list.take(yi, (uint32_t)(at + (u * 64 + lane) * kVec + i), above, wait, top);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sum.template add<kEnt>(y[i], gs, gt);
+        sum.s += gs;
+        sum.t += gt;
+        if constexpr (kCkpt) {
+          const int c = at + (u * 64 + lane) * kVec;
+          float low = INFINITY;
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) low = fminf(low, y[i] > masked_from<T>() ? y[i] : INFINITY);
+          const float hi = over_lanes<kCkptBlock / kVec>(largest, LargerOrNan()), lo = over_lanes<kCkptBlock / kVec>(low, Smaller());
+          const BlockScale scale = block_scale(hi > masked_from<T>() ? hi : -INFINITY, lo, !(hi < INFINITY));
+          uint32_t code[kVec / 4] = {};
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[i], y[i] <= masked_from<T>()) << (8 * (i % 4));
+          if (c < pitch) {
+            uint32_t* const to = reinterpret_cast<uint32_t*>(ckpt.codes + r * pitch + c);
+#pragma unroll
+            for (int i = 0; i < kVec / 4; ++i) to[i] = code[i];
+            if (c % kCkptBlock == 0 && c < shape.cats) ckpt.scales[r * blocks + c / kCkptBlock] = scale.word;
+          }
+        }
+      }
+    };
+
+    const int whole = (end - first) / kChunk, chunks = (end - first + kChunk - 1) / kChunk;
+    Chunk now, next;
+    auto request = [&](Chunk& k, int j) {
+      if (j < whole) load(k, first + j * kChunk);
+      else if (j < chunks) load_end(k, first + j * kChunk);
+    };
+    request(now, wave);
+    for (int j = wave; j < chunks; j += waves) {
+      request(next, j + waves);
+      work(now, first + j * kChunk);
+      now = next;
     }
-    s = block_sum(s, sh);
-    t = block_sum(t, sh);
-    const float ls = logf(s), z = m + ls;   // (no category at all: s = 0, z = -inf)
-    const bool nan = !(z < INFINITY), none = s == 0.f;
-    if (threadIdx.x == 0) {
-      if (out.log_sum) out.log_sum[r] = nan ? NAN : none ? -INFINITY : z;
-      if (out.entropy) out.entropy[r] = nan ? NAN : none ? 0.f : ls - t / s;
-      for (int j = 0; j < given.slots; ++j) {
-        const int64_t g = given_at(given, e, v, j);
-        float lp = NAN;
-        if (g < 0) lp = 0.f;
-        else if (g < shape.cats && !nan) lp = none ? -INFINITY : seen(row[g * x.stride_cat]) - m - ls;
-        out.logp[r * given.slots + j] = lp;
-      }
-    }
-    uint64_t last = ~0ull;
-    for (int j = 0; j < top; ++j) {
-      uint64_t best = 0;
-      for (int c = threadIdx.x; c < shape.cats; c += 256) {
-        const float y = seen(row[c * x.stride_cat]);
-        const uint64_t k = y > -INFINITY ? entry_key(y, c) : 0;
-        if (k < last && k > best) best = k;
-      }
-      for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t k = __shfl_xor((unsigned long long)best, o);
-        best = k > best ? k : best;
-      }
+    if (kTop && list.count) list.flush(wait, top);
+    sum.s = over_lanes<64>(sum.s, Sum());
+    if (kEnt) sum.t = over_lanes<64>(sum.t, Sum());
+
+    if (waves > 1) {
+      if (lane == 0) sums_lds[wave] = make_float4(sum.m, sum.s, sum.t, 0.f);
+      if (kTop) wait[lane] = list.list;
       __syncthreads();
-      if ((threadIdx.x & 63) == 0) best_sh[threadIdx.x >> 6] = best;
-      __syncthreads();
-      for (int q = 0; q < 4; ++q) best = best_sh[q] > best ? best_sh[q] : best;
-      if (threadIdx.x == 0) {
-        out.top[r * top + j] = nan || !best ? -1 : key_index(best);
-        out.top_logp[r * top + j] = nan ? NAN : !best ? -INFINITY : key_value(best) - m - ls;
-      }
-      last = best ? best : 1;
+      if (kTop)
+        for (int h = waves >> 1; h > 0; h >>= 1) {   // two lists into one, the second one turned round
+          if (wave < h) {
+            const uint64_t k = stream_lds[128 * (wave + h) + 63 - lane];
+            list.list = sort_merge<64, true>(list.list > k ? list.list : k);
+            wait[lane] = list.list;
+          }
+          __syncthreads();
+        }
+      if (wave == 0) sum.join_lanes(lane < waves ? sums_lds[lane] : make_float4(masked_from<T>(), 0.f, 0.f, 0.f));
     }
+    if (wave == 0) {
+      if (parts == 1) write_row(sum, list.list, r, e, v, x, shape, given, top, out);
+      else {
+        if (lane == 0) part.sums[job] = make_float4(sum.m, sum.s, sum.t, 0.f);
+        if (kTop && lane < top) part.keys[job * top + lane] = list.list;
+      }
+    }
+    if (waves > 1) __syncthreads();   // the next row's keys go where these are read
   }
+}
+
+// The parts of a row put together, by a workgroup of four waves
+template <typename T>
+__global__ __launch_bounds__(256) void score_join_kernel(RowsRef x, RowsShape shape, GivenRef given, int top, ScoreOut out, int parts, PartRef part) {
+  __shared__ uint64_t keys[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t r = blockIdx.x;
+  const int64_t e = r / (uint32_t)shape.vars, v = r % (uint32_t)shape.vars;
+  RowSums<T> sum;
+  const float4 own = lane < parts ? part.sums[(int64_t)r * parts + lane] : make_float4(masked_from<T>(), 0.f, 0.f, 0.f);
+  uint64_t list = 0;
+  if (top) {
+    const int from = 63 - lane;
+    uint64_t k[kMaxParts / 4];
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 4; ++i) {   // all requests first
+      const int p = wave + 4 * i;
+      k[i] = p < parts && from < top ? part.keys[((int64_t)r * parts + p) * top + from] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxParts / 4; ++i)
+      if (wave + 4 * i < parts) list = sort_merge<64, true>(list > k[i] ? list : k[i]);
+    keys[wave][lane] = list;
+    __syncthreads();
+    if (wave == 0)
+      for (int w = 1; w < 4; ++w) {
+        const uint64_t k = keys[w][from];
+        list = sort_merge<64, true>(list > k ? list : k);
+      }
+  }
+  if (wave == 0) {
+    sum.join_lanes(own);
+    write_row(sum, list, r, e, v, x, shape, given, top, out);
+  }
+}
+
+Split split_of(const RowsShape& shape) {
+  const int64_t rows = shape.rows();
+  const int chunk = 1024, wanted = 4096;   // waves that keep the memory busy
+  Split s{1, 1, shape.cats};
+  while (s.waves < kMaxWaves && rows * s.waves < wanted && s.waves * chunk < shape.cats) s.waves *= 2;
+  if (rows * s.waves < wanted / 4 && s.waves * chunk < shape.cats) {
+    const int64_t parts = std::min<int64_t>({kMaxParts, (wanted / 4 + rows * s.waves - 1) / (rows * s.waves), (shape.cats + s.waves * chunk - 1) / (s.waves * chunk)});
+    s.part_len = (int)(((shape.cats + parts - 1) / parts + 1023) / 1024 * 1024);
+    s.parts = (shape.cats + s.part_len - 1) / s.part_len;
+  }
+  return s;
+}
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+template <typename T>
+void launch_stream(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, const CkptRef& ckpt, void* work,
+                   hipStream_t stream) {
+  const Split s = split_of(shape);
+  PartRef part{};
+  if (s.parts > 1) {
+    part.sums = static_cast<float4*>(work);
+    part.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(work) + up16((size_t)shape.rows() * s.parts * sizeof(float4)));
+  }
+  const dim3 grid((unsigned)std::min<int64_t>(shape.rows() * s.parts, 1 << 20)), block(64 * s.waves);
+  const int lds = s.waves * (128 * 8 + 16);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, x, shape, given, top, out, ckpt, s.parts, s.part_len, part); };
+  const bool ent = out.entropy != nullptr;
+  if (x.stride_cat != 1) {
+    if (top) ent ? launch(score_stream_kernel<T, false, true, true, false>) : launch(score_stream_kernel<T, false, false, true, false>);
+    else ent ? launch(score_stream_kernel<T, false, true, false, false>) : launch(score_stream_kernel<T, false, false, false, false>);
+  } else if (ckpt.codes) {
+    if (top) ent ? launch(score_stream_kernel<T, true, true, true, true>) : launch(score_stream_kernel<T, true, false, true, true>);
+    else ent ? launch(score_stream_kernel<T, true, true, false, true>) : launch(score_stream_kernel<T, true, false, false, true>);
+  } else {
+    if (top) ent ? launch(score_stream_kernel<T, true, true, true, false>) : launch(score_stream_kernel<T, true, false, true, false>);
+    else ent ? launch(score_stream_kernel<T, true, true, false, false>) : launch(score_stream_kernel<T, true, false, false, false>);
+  }
+  if (s.parts > 1)
+    hipLaunchKernelGGL((score_join_kernel<T>), dim3((unsigned)shape.rows()), dim3(256), 0, stream, x, shape, given, top, out, s.parts, part);
 }
 }  // namespace
 
-int64_t category_scores_workspace(const RowsShape&, int) { return 0; }
+int64_t category_scores_workspace(const RowsShape& shape, int top) {
+  if (shape.examples < 1 || shape.vars < 1 || shape.cats < 1 || top < 0 || top > kMaxSlots || shape.examples > INT64_C(0x7fffffff) / shape.vars) return 0;
+  const Split s = split_of(shape);
+  const size_t jobs = (size_t)shape.rows() * s.parts;
+  return s.parts == 1 ? 0 : (int64_t)(up16(jobs * sizeof(float4)) + jobs * top * sizeof(uint64_t));
+}
 
-void category_scores(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, float* d_logp, float* d_log_sum,
-                     float* d_entropy, float* d_top_logp, int32_t* d_top, const CkptRef& ckpt, void*, int64_t, hipStream_t stream) {
-  check_rows(x, shape, "scores");
+void category_scores(const RowsRef& x_in, const RowsShape& shape_in, const GivenRef& given, int top, float* d_logp, float* d_log_sum,
+                     float* d_entropy, float* d_top_logp, int32_t* d_top, const CkptRef& ckpt, void* d_work, int64_t work_bytes, hipStream_t stream) {
+  check_rows(x_in, shape_in, "scores");
   check_given(given);
   if (top < 0 || top > kMaxSlots) fail(PCM_ERR_UNSUPPORTED, "0 to %d likeliest categories, got %d", kMaxSlots, top);
   if (!ckpt.codes != !ckpt.scales) fail(PCM_ERR_ARG, "a checkpoint needs both its codes and its scales");
-  if (!shape.examples) return;
-  if (!x.p || (given.slots && !d_logp) || (top && (!d_top || !d_top_logp))) fail(PCM_ERR_ARG, "scores: a pointer is null");
+  if (!shape_in.examples) return;
+  if (!x_in.p || (given.slots && !d_logp) || (top && (!d_top || !d_top_logp))) fail(PCM_ERR_ARG, "scores: a pointer is null");
+  const int64_t need = category_scores_workspace(shape_in, top);
+  if (need && (!d_work || work_bytes < need)) fail(PCM_ERR_ARG, "scores: %lld bytes of workspace, got %lld", (long long)need, (long long)work_bytes);
+  if (((uintptr_t)d_work | (uintptr_t)ckpt.codes) & 15) fail(PCM_ERR_ARG, "scores: workspace and codes must be 16-byte aligned");
+  RowsRef x = x_in;
+  const RowsShape shape = shape_in;
+  if (shape.cats == 1) x.stride_cat = 1;
   const ScoreOut out{d_logp, d_log_sum, d_entropy, d_top_logp, d_top};
-  const dim3 grid((unsigned)std::min<int64_t>(shape.rows(), 1 << 20));
-  if (x.dtype == PCM_F32) hipLaunchKernelGGL((score_rows_kernel<float>), grid, dim3(256), 0, stream, x, shape, given, top, out);
-  else if (x.dtype == PCM_BF16) hipLaunchKernelGGL((score_rows_kernel<bf16>), grid, dim3(256), 0, stream, x, shape, given, top, out);
-  else hipLaunchKernelGGL((score_rows_kernel<f16>), grid, dim3(256), 0, stream, x, shape, given, top, out);
+  const CkptRef fused = x.stride_cat == 1 ? ckpt : CkptRef{};
+  if (x.dtype == PCM_F32) launch_stream<float>(x, shape, given, top, out, fused, d_work, stream);
+  else if (x.dtype == PCM_BF16) launch_stream<bf16>(x, shape, given, top, out, fused, d_work, stream);
+  else launch_stream<f16>(x, shape, given, top, out, fused, d_work, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of category_scores failed: %s", hipGetErrorString(e));
-  if (ckpt.codes) checkpoint_rows(x, shape, ckpt, stream);
+  if (ckpt.codes && !fused.codes) checkpoint_rows(x, shape, ckpt, stream);
 }
 
 }  // namespace pcm
