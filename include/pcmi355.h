@@ -501,7 +501,7 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  *                              category of score -inf is never among them: -1 and -inf stand where a row has no more
  *   d_codes, d_scales          the row's checkpoint as pcm_checkpoint_rows writes it, in the same pass (both NULL: none)
  * A row of nothing but masks: log Z = -inf, logp = -inf, entropy 0.  A row with NaN or +inf: NaN, no categories (-1).
- * At most 64 given and 64 likeliest categories a row, 2^31 - 1 rows.  d_work: pcm_category_scores_workspace bytes of device
+ * At most 64 given and 64 likeliest categories a row, 2^30 categories, 2^31 - 1 rows.  d_work: pcm_category_scores_workspace bytes of device
  * memory (0: none) that belong to the call until its work is done; 16-byte aligned.
  *
  * pcm_category_scores_backward: the gradient with respect to the scores of a loss whose derivatives are d_grad_logp
@@ -515,7 +515,7 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  * no two of its elements may be one.
  *
  * pcm_checkpoint_rows: rows in 8 bits, for what a forward pass keeps for its backward pass.  d_codes [rows][num_cats rounded up
- * to 16] bytes, d_scales [rows][ceil(num_cats / 64)] words.  64 neighbours of a row with largest and smallest entries M and m
+ * to 16] bytes, d_scales [rows][ceil(num_cats / 64)] words, the codes 16-byte aligned.  64 neighbours of a row with largest and smallest entries M and m
  * share a step 2^e: e is the smallest exponent for which the range takes at most 253 steps if its mantissa is at most 253 / 256
  * (in [1/2, 1)), at most 127 otherwise, |x| <= 2^14 steps and e >= -126.  An entry stands for (base - code) 2^e, base = rint(M /
  * 2^e): the nearest multiple of the step.  Code 255: an entry that is masked, x <= half of the type's lowest value; it

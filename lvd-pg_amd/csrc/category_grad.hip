@@ -1,9 +1,14 @@
 // Gradient of log-probabilities, entropy and likeliest categories with respect to the rows of scores.
-#include "category_rows.hpp"
+//
+//   dx[c] = sum of the slots' gradients at c - p (G + gh (log p + H)),  p = exp(x[c] - log Z), G the sum of all slots' gradients:
+// an exponential and four products an entry, so a kernel that streams: bound by the bytes of scores (or codes) and gradient.
+#include "category_tiles.hip.hpp"
 
 namespace pcm {
 
 namespace {
+constexpr int kStaged = 2048;   // slots of all rows of a workgroup, in LDS
+
 struct GradIn {
   GivenRef given;
   const float* grad_logp;
@@ -11,50 +16,238 @@ struct GradIn {
   const int32_t* top_index;
   const float *grad_top, *log_sum, *entropy, *grad_entropy;
 };
+struct GradSlot {
+  int at;      // category; -1: adds nothing
+  float by;
+};
+__device__ __forceinline__ GradSlot grad_slot(const GradIn& in, int64_t r, int64_t e, int64_t v, int j, int cats, bool& past) {
+  const bool g = j < in.given.slots;
+  const int64_t at = g ? given_at(in.given, e, v, j) : in.top_index[r * in.top + j - in.given.slots];
+  const float by = g ? in.grad_logp[r * in.given.slots + j] : in.grad_top[r * in.top + j - in.given.slots];
+  past = at >= cats;
+  return {at < 0 || past ? -1 : (int)at, by};
+}
+struct GradRow {
+  float z, total, gh, h;
+  // total: of the slots' gradients.  A row that has no category gets p = 0 everywhere.
+  __device__ __forceinline__ GradRow(const GradIn& in, int64_t r, float sum) {
+    z = in.log_sum[r];
+    total = sum;
+    gh = in.grad_entropy ? in.grad_entropy[r] : 0.f;
+    h = in.grad_entropy ? in.entropy[r] : 0.f;
+    if (z == -INFINITY) {
+      z = INFINITY;
+      total = gh = h = 0.f;
+    }
+  }
+  __device__ __forceinline__ bool none() const { return z == INFINITY; }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float d = x - z, p = __builtin_amdgcn_exp2f(d * kLog2e);
+    return -p * fmaf(gh, fmaxf(d, -200.f) + h, total);   // (p is 0 where d is below, and may be -inf)
+  }
+};
 
-// dx[c] = sum of the slots' gradients at c - p (G + gh (log p + H)), G the sum of all slots' gradients; one workgroup per row
+// Rows of neighbouring categories in and out.  The slots of the workgroup's rows wait in LDS; of a long row only those in the
+// workgroup's segment, in their order, so that sums come out the same every time.
 template <typename T, bool kCkpt>
-__global__ __launch_bounds__(256) void grad_rows_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out) {
-  __shared__ int64_t at[2 * kMaxSlots];
-  __shared__ float by[2 * kMaxSlots];
+__global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, Tiles tiles) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  __shared__ GradSlot slot_lds[kStaged];
+  __shared__ float total_lds[kTileThreads];
+  __shared__ int near_lds;
+  const int slots = in.given.slots + in.top, per = kTileThreads >> tiles.lanes_log2, of = threadIdx.x >> tiles.lanes_log2;
   const int64_t rows = shape.rows();
+  const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
+  for (int64_t job = blockIdx.x; job < tiles.jobs; job += gridDim.x) {
+    const TileAt tile = tile_at(tiles, job);
+    const bool mine = tile.row < rows;
+    const uint32_t r = (uint32_t)(mine ? tile.row : rows - 1);
+    const int64_t e = shape.vars == 1 ? r : r / (uint32_t)shape.vars, v = shape.vars == 1 ? 0 : r % (uint32_t)shape.vars;
+    const T* const row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
+    T* const dst = static_cast<T*>(const_cast<void*>(out.p)) + e * out.stride_ex + v * out.stride_var;
+
+    raw4 raw[kCkpt ? 1 : kTileGroups];
+    Codes<kVec> code[kCkpt ? kTileGroups : 1];
+    BlockUnit unit[kCkpt ? kTileGroups : 1];
+#pragma unroll
+    for (int u = 0; u < kTileGroups; ++u) {
+      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+      if (c >= shape.cats) continue;
+      if constexpr (kCkpt) {
+        code[u] = load_codes<kVec>(ckpt.codes + r * pitch + c);
+        unit[u] = block_unit(ckpt.scales[r * blocks + c / kCkptBlock]);
+      } else raw[u] = load_group(row, c, shape.cats);
+    }
+
+    int near = slots;   // slots to look at, from near_at on
+    const GradSlot* near_at = slot_lds + of * slots;
+    float total = 0.f;
+    if (slots) {
+      if (per == 1) {
+        // wave 0: slots by the lane, twice; the others wait for what it leaves
+        if (threadIdx.x < 64) {
+          const int lane = threadIdx.x, low = (tile.first - lane) * kVec, high = low + kTileGroups * tile.step * kVec;
+          int found = 0;
+          float sum = 0.f;
+          for (int j0 = 0; j0 < slots; j0 += 64) {
+            bool past = false;
+            GradSlot s{-1, 0.f};
+            if (j0 + lane < slots) s = grad_slot(in, r, e, v, j0 + lane, shape.cats, past);
+            sum += past ? NAN : s.at >= 0 ? s.by : 0.f;
+            const bool here = s.at >= low && s.at < high;
+            const uint64_t all = __ballot(here);
+            if (here) slot_lds[found + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0))] = s;
+            found += __popcll(all);
+          }
+          sum = over_lanes<64>(sum, Sum());
+          if (lane == 0) {
+            total_lds[0] = sum;
+            near_lds = found;
+          }
+        }
+        __syncthreads();
+        total = total_lds[0];
+        near = near_lds;
+        near_at = slot_lds;
+      } else {
+        const int64_t r0 = job * per;   // (one segment a row)
+        if (threadIdx.x < per) total_lds[threadIdx.x] = 0.f;
+        for (int i = threadIdx.x; i < per * slots; i += kTileThreads) {
+          const int64_t q = r0 + i / slots;
+          GradSlot s{-1, 0.f};
+          if (q < rows) {
+            bool past;
+            const int64_t qe = shape.vars == 1 ? q : (uint32_t)q / (uint32_t)shape.vars;
+            s = grad_slot(in, q, qe, q - qe * shape.vars, i % slots, shape.cats, past);
+            if (past) s = {-2, 0.f};
+          }
+          slot_lds[i] = s;
+        }
+        __syncthreads();
+        for (int j = 0; j < slots; ++j) {
+          const GradSlot s = near_at[j];
+          total += s.at >= 0 ? s.by : s.at == -2 ? NAN : 0.f;
+        }
+      }
+    }
+    const GradRow grad(in, r, total);
+    if (grad.none()) near = 0;
+#pragma unroll
+    for (int u = 0; u < kTileGroups; ++u) {
+      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+      if (c >= shape.cats) continue;
+      float y[kVec];
+      if constexpr (kCkpt) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) y[i] = code_value(unit[u], code[u][i]);
+      } else unpack(raw[u], y, T());
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) y[i] = grad(y[i]);
+      for (int j = 0; j < near; ++j) {
+        const uint32_t i = (uint32_t)near_at[j].at - (uint32_t)c;
+        if (i < (uint32_t)kVec) {
+          const float by = near_at[j].by;
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) y[k] += i == (uint32_t)k ? by : 0.f;
+        }
+      }
+      T w[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) w[i] = from_float<T>(y[i]);
+      if (mine) store_group(dst, c, shape.cats, w);
+    }
+    if (slots) __syncthreads();   // (the next rows' slots go where these are read)
+  }
+}
+
+// Any strides, a lane per row: 64 rows that lie side by side a wave, the categories cut among waves.  Slots are looked up per entry, the
+// first four from registers.
+template <typename T, bool kCkpt>
+__global__ __launch_bounds__(256) void grad_column_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, int parts, int len,
+                                                          bool examples_first) {
+  constexpr int kNear = 4, kStep = 8;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = shape.rows(), jobs = (rows + 63) / 64 * parts;
   const int slots = in.given.slots + in.top;
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t e = r / shape.vars, v = r % shape.vars;
-    const T* row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
-    T* dst = static_cast<T*>(const_cast<void*>(out.p)) + e * out.stride_ex + v * out.stride_var;
-    __syncthreads();
-    if (threadIdx.x < slots) {
-      const int j = threadIdx.x;
-      const bool g = j < in.given.slots;
-      at[j] = g ? given_at(in.given, e, v, j) : in.top_index[r * in.top + j - in.given.slots];
-      by[j] = g ? in.grad_logp[r * in.given.slots + j] : in.grad_top[r * in.top + j - in.given.slots];
-    }
-    __syncthreads();
-    const float z = in.log_sum[r], gh = in.grad_entropy ? in.grad_entropy[r] : 0.f, h = in.grad_entropy ? in.entropy[r] : 0.f;
+  for (int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); job < jobs; job += (int64_t)gridDim.x * 4) {
+    const int64_t set = job / parts;
+    const int first = (int)(job - set * parts) * len, end = min(first + len, shape.cats);
+    const int64_t at = set * 64 + lane;
+    if (at >= rows) continue;
+    const uint32_t n = (uint32_t)at;
+    const uint32_t hi = examples_first ? n / (uint32_t)shape.examples : n / (uint32_t)shape.vars;
+    const uint32_t lo = n - hi * (examples_first ? (uint32_t)shape.examples : (uint32_t)shape.vars);
+    const int64_t e = examples_first ? lo : hi, v = examples_first ? hi : lo, r = e * shape.vars + v;
+    const T* const row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
+    T* const dst = static_cast<T*>(const_cast<void*>(out.p)) + e * out.stride_ex + v * out.stride_var;
+    GradSlot near[kNear];
     float total = 0.f;
-    for (int j = 0; j < slots; ++j)
-      if (at[j] >= 0) total += at[j] < shape.cats ? by[j] : NAN;
-    for (int c = threadIdx.x; c < shape.cats; c += 256) {
-      const float y = kCkpt ? block_entry(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c])
-                            : seen(row[c * x.stride_cat]);
-      const float d = y - z, p = expf(d);
-      float g = -p * total;
-      if (p != 0.f) g -= gh * p * (d + h);
-      for (int j = 0; j < slots; ++j)
-        if (at[j] == c) g += by[j];
-      if (z == -INFINITY) g = 0.f;
-      dst[c * out.stride_cat] = from_float<T>(g);
+#pragma unroll
+    for (int j = 0; j < kNear; ++j) near[j] = {-1, 0.f};
+    for (int j = 0; j < slots; ++j) {
+      bool past;
+      const GradSlot s = grad_slot(in, r, e, v, j, shape.cats, past);
+      total += past ? NAN : s.at >= 0 ? s.by : 0.f;
+#pragma unroll
+      for (int k = 0; k < kNear; ++k)
+        if (j == k) near[k] = s;
+    }
+    const GradRow grad(in, r, total);
+    for (int c0 = first; c0 < end; c0 += kStep) {
+      float y[kStep];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int c = c0 + i;
+        if (c >= end) y[i] = -INFINITY;
+        else if constexpr (kCkpt) y[i] = code_value(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
+        else y[i] = seen(row[(int64_t)c * x.stride_cat]);
+      }
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int c = c0 + i;
+        if (c >= end) break;
+        float g = grad(y[i]);
+        if (!grad.none()) {
+#pragma unroll
+          for (int j = 0; j < kNear; ++j) g += near[j].at == c ? near[j].by : 0.f;
+          for (int j = kNear; j < slots; ++j) {
+            bool past;
+            const GradSlot s = grad_slot(in, r, e, v, j, shape.cats, past);
+            g += s.at == c ? s.by : 0.f;
+          }
+        }
+        dst[(int64_t)c * out.stride_cat] = from_float<T>(g);
+      }
     }
   }
 }
+
+template <typename T>
+void launch_grad(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, const GradIn& in, const RowsRef& out, hipStream_t stream) {
+  const int slots = in.given.slots + in.top;
+  if (out.stride_cat == 1 && (ckpt.codes || x.stride_cat == 1)) {
+    const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), (slots * kTileThreads + kStaged - 1) / kStaged);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, tile_grid(t), dim3(kTileThreads), 0, stream, x, ckpt, shape, in, out, t); };
+    ckpt.codes ? launch(grad_tile_kernel<T, true>) : launch(grad_tile_kernel<T, false>);
+    return;
+  }
+  const int64_t sets = (shape.rows() + 63) / 64;
+  const bool examples_first = shape.vars > 1 && (out.stride_ex == 1 || out.stride_ex == -1);
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>((shape.cats + 31) / 32, (8192 + sets - 1) / sets));
+  const int len = (int)(((shape.cats + parts - 1) / parts + 7) / 8 * 8);
+  parts = (shape.cats + len - 1) / len;
+  const dim3 grid((unsigned)std::min<int64_t>((sets * parts + 3) / 4, 1 << 22));
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, ckpt, shape, in, out, (int)parts, len, examples_first); };
+  ckpt.codes ? launch(grad_column_kernel<T, true>) : launch(grad_column_kernel<T, false>);
+}
 }  // namespace
 
-void category_scores_backward(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, const GivenRef& given,
+void category_scores_backward(const RowsRef& x_in, const CkptRef& ckpt, const RowsShape& shape, const GivenRef& given,
                               const float* d_grad_logp, int top, const int32_t* d_top, const float* d_grad_top,
-                              const float* d_log_sum, const float* d_entropy, const float* d_grad_entropy, const RowsRef& out,
+                              const float* d_log_sum, const float* d_entropy, const float* d_grad_entropy, const RowsRef& out_in,
                               hipStream_t stream) {
+  RowsRef x = x_in, out = out_in;
   check_rows(out, shape, "gradient of scores");
   check_given(given);
   if (top < 0 || top > kMaxSlots) fail(PCM_ERR_UNSUPPORTED, "0 to %d likeliest categories, got %d", kMaxSlots, top);
@@ -64,13 +257,12 @@ void category_scores_backward(const RowsRef& x, const CkptRef& ckpt, const RowsS
   if (!shape.examples) return;
   if (!out.p || !d_log_sum || (given.slots && !d_grad_logp) || (top && (!d_top || !d_grad_top)) || (d_grad_entropy && !d_entropy))
     fail(PCM_ERR_ARG, "gradient of scores: a pointer is null");
+  if ((uintptr_t)ckpt.codes & 15) fail(PCM_ERR_ARG, "gradient of scores: codes must be 16-byte aligned");
+  if (shape.cats == 1) x.stride_cat = out.stride_cat = 1;
   const GradIn in{given, d_grad_logp, top, d_top, d_grad_top, d_log_sum, d_entropy, d_grad_entropy};
-  const dim3 grid((unsigned)std::min<int64_t>(shape.rows(), 1 << 20));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, ckpt, shape, in, out); };
-  const bool k = ckpt.codes != nullptr;
-  if (out.dtype == PCM_F32) k ? launch(grad_rows_kernel<float, true>) : launch(grad_rows_kernel<float, false>);
-  else if (out.dtype == PCM_BF16) k ? launch(grad_rows_kernel<bf16, true>) : launch(grad_rows_kernel<bf16, false>);
-  else k ? launch(grad_rows_kernel<f16, true>) : launch(grad_rows_kernel<f16, false>);
+  if (out.dtype == PCM_F32) launch_grad<float>(x, ckpt, shape, in, out, stream);
+  else if (out.dtype == PCM_BF16) launch_grad<bf16>(x, ckpt, shape, in, out, stream);
+  else launch_grad<f16>(x, ckpt, shape, in, out, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of category_scores_backward failed: %s", hipGetErrorString(e));
 }

@@ -8,6 +8,7 @@ void check_rows(const RowsRef& x, const RowsShape& shape, const char* what) {
   if (shape.examples < 0 || shape.vars < 1 || shape.cats < 1)
     fail(PCM_ERR_SHAPE, "%s: %lld examples, %d variables, %d categories", what, (long long)shape.examples, shape.vars, shape.cats);
   if (shape.examples > INT64_C(0x7fffffff) / shape.vars) fail(PCM_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows", what);
+  if (shape.cats > 1 << 30) fail(PCM_ERR_UNSUPPORTED, "%s: at most 2^30 categories", what);
   if (x.dtype != PCM_F32 && x.dtype != PCM_BF16 && x.dtype != PCM_F16) fail(PCM_ERR_ARG, "%s: type %d is none of PCM_F32, PCM_BF16, PCM_F16", what, x.dtype);
 }
 
@@ -291,6 +292,7 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 template <typename T>
 void launch_stream(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, const CkptRef& ckpt, void* work,
                    hipStream_t stream) {
+  if (category_scores_short<T>(x, shape, given, top, out, ckpt, stream)) return;
   const Split s = split_of(shape);
   PartRef part{};
   if (s.parts > 1) {

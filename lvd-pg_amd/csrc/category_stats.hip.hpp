@@ -17,6 +17,11 @@ struct ScoreOut {
   int32_t* top;
 };
 
+// Short rows and rows that lie side by side; false: not rows of that kind, nothing done.  `ckpt` only with stride_cat == 1.
+template <typename T>
+bool category_scores_short(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, const CkptRef& ckpt,
+                           hipStream_t stream);
+
 #ifdef __HIPCC__
 template <typename T>
 struct RowSums {

@@ -1,0 +1,85 @@
+// How the kernels that turn rows into rows, entry by entry, deal them out: G lanes a row (a power of two, up to the workgroup's 256),
+// each with up to kTileGroups groups of 16 bytes; a workgroup holds 256 / G short rows, or one of the `segments` of a long one.
+#pragma once
+
+#include "category_rows.hpp"
+
+namespace pcm {
+
+constexpr int kTileThreads = 256, kTileGroups = 4;
+
+struct Tiles {
+  int lanes_log2;      // log2 G
+  int segments;        // of a row
+  int64_t jobs;        // workgroups' worth of work
+};
+// `vec` entries a group, at least `least` lanes a row
+inline Tiles tiles_of(const RowsShape& shape, int vec, int least) {
+  const int64_t groups = ((int64_t)shape.cats + vec - 1) / vec, wanted = (groups + kTileGroups - 1) / kTileGroups;
+  Tiles t{0, 1, 0};
+  while ((1 << t.lanes_log2) < kTileThreads && (1 << t.lanes_log2) < std::max<int64_t>(wanted, least)) ++t.lanes_log2;
+  const int64_t held = (int64_t)kTileGroups << t.lanes_log2;
+  t.segments = (int)((groups + held - 1) / held);
+  const int64_t per = kTileThreads >> t.lanes_log2;
+  t.jobs = (shape.rows() + per - 1) / per * t.segments;
+  return t;
+}
+inline dim3 tile_grid(const Tiles& t) { return dim3((unsigned)std::min<int64_t>(t.jobs, 1 << 22)); }
+
+#ifdef __HIPCC__
+struct TileAt {        // of a lane in a job
+  int64_t row;         // may lie behind the last one
+  int first, step;     // group u holds the categories from (first + u * step) * vec
+};
+__device__ __forceinline__ TileAt tile_at(const Tiles& t, int64_t job) {
+  const int lanes = 1 << t.lanes_log2, in = threadIdx.x & (lanes - 1), of = threadIdx.x >> t.lanes_log2;
+  if (t.segments == 1) return {(job << (8 - t.lanes_log2)) + of, in, lanes};
+  const int64_t row = job / t.segments;   // (one row a workgroup)
+  return {row, (int)(job - row * t.segments) * kTileGroups * lanes + in, lanes};
+}
+
+// A group of 16 bytes from categories c.. of a row of `cats`; -inf behind its end
+template <typename T>
+__device__ __forceinline__ raw4 load_group(const T* row, int64_t c, int cats) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  if (c + kVec <= cats) return load16(row + c);
+  T w[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) w[i] = c + i < cats ? row[c + i] : (T)-INFINITY;
+  return __builtin_bit_cast(raw4, w);
+}
+template <typename T>
+__device__ __forceinline__ void store_group(T* row, int64_t c, int cats, const T (&w)[16 / (int)sizeof(T)]) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  if (c + kVec <= cats) {
+    store16(row + c, __builtin_bit_cast(raw4, w));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+    if (c + i < cats) row[c + i] = w[i];
+}
+// The codes of a group (c is a multiple of its size, the codes' pitch of 16)
+template <int kVec>
+struct Codes {
+  uint32_t w[kVec / 4];
+  __device__ __forceinline__ float operator[](int i) const { return (float)(w[i / 4] >> (8 * (i % 4)) & 0xffu); }
+};
+template <int kVec>
+__device__ __forceinline__ Codes<kVec> load_codes(const uint8_t* at) {
+  Codes<kVec> k;
+  if constexpr (kVec == 4) k.w[0] = *reinterpret_cast<const uint32_t*>(at);
+  else {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    k.w[0] = v.x;
+    k.w[1] = v.y;
+  }
+  return k;
+}
+__device__ __forceinline__ float code_value(const BlockUnit& u, float code) {   // (255 stands for -inf, in a block that is not NaN)
+  const float v = (u.base - code) * u.step;
+  return code == (float)kCkptMasked && u.step == u.step ? -INFINITY : v;
+}
+#endif
+
+}  // namespace pcm

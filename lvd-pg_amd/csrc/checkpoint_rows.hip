@@ -1,29 +1,101 @@
-// Checkpoints of rows in 8 bits, and the rows back from them.
-#include "category_rows.hpp"
+// Checkpoints of rows in 8 bits, and the rows back from them.  Both stream: bound by the bytes of rows and codes.
+#include "category_tiles.hip.hpp"
 
 namespace pcm {
 
 namespace {
-// one wave per block of 64 entries
+// Rows of neighbouring entries: the 64 of a block lie in 64 / kVec neighbouring lanes, which find the range with three or four steps
+template <typename T>
+__global__ __launch_bounds__(kTileThreads) void checkpoint_tile_kernel(RowsRef x, RowsShape shape, CkptRef ckpt, Tiles tiles) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  const int64_t rows = shape.rows();
+  const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
+  for (int64_t job = blockIdx.x; job < tiles.jobs; job += gridDim.x) {
+    const TileAt tile = tile_at(tiles, job);
+    const bool mine = tile.row < rows;
+    const uint32_t r = (uint32_t)(mine ? tile.row : rows - 1);
+    const int64_t e = shape.vars == 1 ? r : r / (uint32_t)shape.vars, v = shape.vars == 1 ? 0 : r % (uint32_t)shape.vars;
+    const T* const row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
+    raw4 raw[kTileGroups];
+#pragma unroll
+    for (int u = 0; u < kTileGroups; ++u) raw[u] = load_group(row, (int64_t)(tile.first + u * tile.step) * kVec, shape.cats);
+#pragma unroll
+    for (int u = 0; u < kTileGroups; ++u) {
+      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+      float y[kVec], hi = -INFINITY, lo = INFINITY;
+      unpack(raw[u], y, T());
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        hi = __builtin_elementwise_maximum(hi, y[i]);
+        lo = fminf(lo, y[i] > masked_from<T>() ? y[i] : INFINITY);
+      }
+      hi = over_lanes<kCkptBlock / kVec>(hi, LargerOrNan());
+      lo = over_lanes<kCkptBlock / kVec>(lo, Smaller());
+      const BlockScale scale = block_scale(hi > masked_from<T>() ? hi : -INFINITY, lo, !(hi < INFINITY));
+      uint32_t code[kVec / 4] = {};
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[i], y[i] <= masked_from<T>()) << (8 * (i % 4));
+      if (mine && c < pitch) {
+        uint32_t* const to = reinterpret_cast<uint32_t*>(ckpt.codes + r * pitch + c);
+#pragma unroll
+        for (int i = 0; i < kVec / 4; ++i) to[i] = code[i];
+        if (c % kCkptBlock == 0 && c < shape.cats) ckpt.scales[r * blocks + c / kCkptBlock] = scale.word;
+      }
+    }
+  }
+}
+
+// Any strides: a wave per block of 64 entries
 template <typename T>
 __global__ __launch_bounds__(256) void checkpoint_kernel(RowsRef x, RowsShape shape, CkptRef ckpt) {
   const int lane = threadIdx.x & 63;
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock, all = shape.rows() * blocks;
   for (int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); b < all; b += (int64_t)gridDim.x * 4) {
     const int64_t r = b / blocks, e = r / shape.vars, v = r % shape.vars;
-    const int c = (int)(b % blocks) * kCkptBlock + lane;
+    const int64_t c = (b % blocks) * kCkptBlock + lane;
     const T* row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
-    const bool in = c < shape.cats;
-    const float y = in ? to_float(row[c * x.stride_cat]) : -INFINITY;
+    const float y = c < shape.cats ? to_float(row[c * x.stride_cat]) : -INFINITY;
     const bool off = y <= masked_from<T>();
-    float hi = off ? -INFINITY : y, lo = off ? INFINITY : y;
-    for (int o = 32; o > 0; o >>= 1) {
-      hi = fmaxf(hi, __shfl_xor(hi, o));
-      lo = fminf(lo, __shfl_xor(lo, o));
-    }
-    const BlockScale s = block_scale(hi, lo, __any(!(y < INFINITY)));
+    const float hi = over_lanes<64>(off ? -INFINITY : y, LargerOrNan()), lo = over_lanes<64>(off ? INFINITY : y, Smaller());
+    const BlockScale s = block_scale(hi, lo, !(hi < INFINITY));
     if (c < pitch) ckpt.codes[r * pitch + c] = (uint8_t)block_code(s, y, off);
     if (lane == 0) ckpt.scales[b] = s.word;
+  }
+}
+
+// (a value may have been rounded up past the largest of the type)
+template <typename T>
+__device__ __forceinline__ T restored(float y) { return from_float<T>(y > type_max<T>() ? type_max<T>() : y); }
+
+template <typename T>
+__global__ __launch_bounds__(kTileThreads) void restore_tile_kernel(CkptRef ckpt, RowsShape shape, RowsRef out, Tiles tiles) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
+  for (int64_t job = blockIdx.x; job < tiles.jobs; job += gridDim.x) {
+    const TileAt tile = tile_at(tiles, job);
+    if (tile.row >= shape.rows()) continue;
+    const uint32_t r = (uint32_t)tile.row;
+    const int64_t e = shape.vars == 1 ? r : r / (uint32_t)shape.vars, v = shape.vars == 1 ? 0 : r % (uint32_t)shape.vars;
+    T* const dst = static_cast<T*>(const_cast<void*>(out.p)) + e * out.stride_ex + v * out.stride_var;
+    Codes<kVec> code[kTileGroups];
+    uint32_t word[kTileGroups];
+#pragma unroll
+    for (int u = 0; u < kTileGroups; ++u) {
+      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+      if (c >= shape.cats) continue;
+      code[u] = load_codes<kVec>(ckpt.codes + r * pitch + c);
+      word[u] = ckpt.scales[r * blocks + c / kCkptBlock];
+    }
+#pragma unroll
+    for (int u = 0; u < kTileGroups; ++u) {
+      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+      if (c >= shape.cats) continue;
+      const BlockUnit unit = block_unit(word[u]);
+      T w[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) w[i] = restored<T>(code_value(unit, code[u][i]));
+      store_group(dst, c, shape.cats, w);
+    }
   }
 }
 
@@ -32,35 +104,57 @@ __global__ __launch_bounds__(256) void restore_kernel(CkptRef ckpt, RowsShape sh
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock, all = shape.rows() * shape.cats;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / shape.cats, c = i % shape.cats, e = r / shape.vars, v = r % shape.vars;
-    const float y = block_entry(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
-    static_cast<T*>(const_cast<void*>(out.p))[e * out.stride_ex + v * out.stride_var + c * out.stride_cat] =
-        from_float<T>(y > type_max<T>() ? type_max<T>() : y);
+    const float y = code_value(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
+    static_cast<T*>(const_cast<void*>(out.p))[e * out.stride_ex + v * out.stride_var + c * out.stride_cat] = restored<T>(y);
+  }
+}
+
+template <typename T>
+void launch_checkpoint(const RowsRef& x, const RowsShape& shape, const CkptRef& ckpt, hipStream_t stream) {
+  if (x.stride_cat == 1) {
+    const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), kCkptBlock * (int)sizeof(T) / 16);
+    hipLaunchKernelGGL((checkpoint_tile_kernel<T>), tile_grid(t), dim3(kTileThreads), 0, stream, x, shape, ckpt, t);
+  } else {
+    const dim3 grid((unsigned)std::min<int64_t>((shape.rows() * ckpt_blocks(shape.cats) + 3) / 4, 1 << 20));
+    hipLaunchKernelGGL((checkpoint_kernel<T>), grid, dim3(256), 0, stream, x, shape, ckpt);
+  }
+}
+template <typename T>
+void launch_restore(const CkptRef& ckpt, const RowsShape& shape, const RowsRef& out, hipStream_t stream) {
+  if (out.stride_cat == 1) {
+    const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), 1);
+    hipLaunchKernelGGL((restore_tile_kernel<T>), tile_grid(t), dim3(kTileThreads), 0, stream, ckpt, shape, out, t);
+  } else {
+    const dim3 grid((unsigned)std::min<int64_t>((shape.rows() * shape.cats + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL((restore_kernel<T>), grid, dim3(256), 0, stream, ckpt, shape, out);
   }
 }
 }  // namespace
 
-void checkpoint_rows(const RowsRef& x, const RowsShape& shape, const CkptRef& ckpt, hipStream_t stream) {
+void checkpoint_rows(const RowsRef& x_in, const RowsShape& shape, const CkptRef& ckpt, hipStream_t stream) {
+  RowsRef x = x_in;
   check_rows(x, shape, "checkpoint");
   if (!shape.examples) return;
   if (!x.p || !ckpt.codes || !ckpt.scales) fail(PCM_ERR_ARG, "checkpoint: a pointer is null");
-  const dim3 grid((unsigned)std::min<int64_t>((shape.rows() * ckpt_blocks(shape.cats) + 3) / 4, 1 << 20));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, shape, ckpt); };
-  if (x.dtype == PCM_F32) launch(checkpoint_kernel<float>);
-  else if (x.dtype == PCM_BF16) launch(checkpoint_kernel<bf16>);
-  else launch(checkpoint_kernel<f16>);
+  if ((uintptr_t)ckpt.codes & 15) fail(PCM_ERR_ARG, "checkpoint: codes must be 16-byte aligned");
+  if (shape.cats == 1) x.stride_cat = 1;
+  if (x.dtype == PCM_F32) launch_checkpoint<float>(x, shape, ckpt, stream);
+  else if (x.dtype == PCM_BF16) launch_checkpoint<bf16>(x, shape, ckpt, stream);
+  else launch_checkpoint<f16>(x, shape, ckpt, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of checkpoint_rows failed: %s", hipGetErrorString(e));
 }
 
-void restore_rows(const CkptRef& ckpt, const RowsShape& shape, const RowsRef& out, hipStream_t stream) {
+void restore_rows(const CkptRef& ckpt, const RowsShape& shape, const RowsRef& out_in, hipStream_t stream) {
+  RowsRef out = out_in;
   check_rows(out, shape, "restored rows");
   if (!shape.examples) return;
   if (!out.p || !ckpt.codes || !ckpt.scales) fail(PCM_ERR_ARG, "restored rows: a pointer is null");
-  const dim3 grid((unsigned)std::min<int64_t>((shape.rows() * shape.cats + 255) / 256, 1 << 20));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, ckpt, shape, out); };
-  if (out.dtype == PCM_F32) launch(restore_kernel<float>);
-  else if (out.dtype == PCM_BF16) launch(restore_kernel<bf16>);
-  else launch(restore_kernel<f16>);
+  if ((uintptr_t)ckpt.codes & 15) fail(PCM_ERR_ARG, "restored rows: codes must be 16-byte aligned");
+  if (shape.cats == 1) out.stride_cat = 1;
+  if (out.dtype == PCM_F32) launch_restore<float>(ckpt, shape, out, stream);
+  else if (out.dtype == PCM_BF16) launch_restore<bf16>(ckpt, shape, out, stream);
+  else launch_restore<f16>(ckpt, shape, out, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of restore_rows failed: %s", hipGetErrorString(e));
 }

@@ -64,7 +64,8 @@ def likeliest(x, top):
 
 def gradient(x, z, h, slots, gh=None):
     """slots: pairs (categories [rows, k], derivatives [rows, k]); z, h as given (float64 of float32 values).  Returns the
-    gradient and the size of its terms, which roundings are relative to."""
+    gradient, the size of its terms, which roundings are relative to, and what underflow may take away: a p below 2^-126, the
+    smallest normal number of 32 bits, may count as 0, and with it its product with the rest of its term."""
     R, C = x.shape
     out = np.zeros((R, C))
     size = np.zeros((R, C))
@@ -84,12 +85,15 @@ def gradient(x, z, h, slots, gh=None):
         # p is exp of a difference that is rounded at the size of its two terms
         slack = 1.0 + np.where(np.isfinite(d), np.abs(np.where(np.isfinite(x), x, 0.0)) + np.abs(z[:, None]), 0.0)
         size += p * weight[:, None] * slack
+        under = np.broadcast_to(weight[:, None], out.shape).copy()
         if gh is not None:
             out -= np.where(p > 0, gh[:, None] * p * (d + h[:, None]), 0.0)
-            size += np.where(p > 0, np.abs(gh[:, None]) * p * (np.abs(d) + np.abs(h[:, None]) + 1.0) * slack, 0.0)
+            term = np.abs(gh[:, None]) * (np.minimum(np.abs(d), 200.0) + np.abs(h[:, None]) + 1.0)
+            size += np.where(p > 0, p * term * slack, 0.0)
+            under += term
     out[z == -np.inf] = 0.0
     size[z == -np.inf] = 0.0
-    return out, size
+    return out, size, 2.0 ** -126 * np.nan_to_num(under)
 
 
 def rounded(x, dtype):

@@ -42,7 +42,7 @@ def test_reference_gradient_is_the_derivative():
         return (R.logp_of(y, g) * w).sum() + (gh * h).sum()
 
     z, h = R.statistics(x)
-    got, _ = R.gradient(x, z, h, [(g, w)], gh)
+    got = R.gradient(x, z, h, [(g, w)], gh)[0]
     for r in range(n):
         for c in range(C):
             y = x.copy()
@@ -142,7 +142,7 @@ def test_entry_points_refuse_without_a_gpu():
     for f in (scores, back, keep, restore):
         assert f(type=3) == -1 and f(type=-1) == -1 and b"type" in lib.pcm_last_error()
         assert f(c=0) == -2 and f(v=0) == -2 and f(n=-1) == -2
-        assert f(n=1 << 40) == -3 and f(n=1 << 30, v=4) == -3
+        assert f(n=1 << 40) == -3 and f(n=1 << 30, v=4) == -3 and f(c=(1 << 30) + 1) == -3
         assert f(n=0) == 0                                              # nothing to do: nothing is touched
     for f in (scores, back):
         assert f(slots=65, given=p) == -3 and f(top=65) == -3 and f(slots=-1) == -3 and f(top=-1) == -3

@@ -193,11 +193,12 @@ def _check_grad(torch, P, x, dtype, k=2, top=0, gh=True, kept=False, out=None, s
         w = kw["grad_entropy"].double().cpu().numpy().reshape(-1)
     y = _numbers(x)
     z, h = (t.double().cpu().numpy().reshape(-1) for t in (s.log_sum, s.entropy))
-    want, size = R.gradient(R.rounded(y, dtype) if kept else R.seen(y, dtype), z, h, slots, w)
+    want, size, under = R.gradient(R.rounded(y, dtype) if kept else R.seen(y, dtype), z, h, slots, w)
     got = P.category_scores_backward(s.checkpoint if kept else x, s.log_sum, given, out=out, **kw)
     assert got.shape == x.shape and got.dtype == x.dtype and (out is None or got is out)
-    # the terms' sizes carry the roundings in 32 bits: a dozen operations, one addition per slot; then one to the type
-    bound = size * ((16 + k + top) * R.EPS) + np.abs(np.nan_to_num(want)) * R.HALF[dtype] + R.TINY[dtype] + 2.0 ** -126
+    # the terms' sizes carry the roundings in 32 bits: a dozen operations, one addition per slot; then one to the type,
+    # the smallest normal number, and underflow
+    bound = size * ((16 + k + top) * R.EPS) + np.abs(np.nan_to_num(want)) * R.HALF[dtype] + R.TINY[dtype] + 2.0 ** -126 + under
     _near(got, want.reshape(-1, C), bound, "gradient")
     return got
 
