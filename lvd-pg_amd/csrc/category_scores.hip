@@ -40,11 +40,16 @@ struct TopList {
   uint64_t list = 0;
   float bar;
   int count = 0;
+  // up to N waiting keys sorted, rising, into the last lanes
+  template <int N>
+  __device__ __forceinline__ uint64_t sorted(const uint64_t* wait) const {
+    const int i = (int)(threadIdx.x & 63) - (64 - N);
+    return sort_lanes<N, false>(i >= 0 && i < count ? wait[i] : (uint64_t)0);
+  }
   __device__ __forceinline__ void flush(uint64_t* wait, int top) {
     const int lane = threadIdx.x & 63;
     __builtin_amdgcn_wave_barrier();
-    uint64_t k = lane < count ? wait[lane] : 0;
-    k = sort_lanes<64, false>(k);
+    const uint64_t k = count <= 16 ? sorted<16>(wait) : count <= 32 ? sorted<32>(wait) : sorted<64>(wait);
     list = sort_merge<64, true>(list > k ? list : k);
     const uint64_t rest = lane + 64 < count ? wait[lane + 64] : 0;
     __builtin_amdgcn_wave_barrier();
@@ -54,12 +59,26 @@ struct TopList {
     const uint32_t last = __builtin_amdgcn_readlane((uint32_t)(list >> 32), top - 1);
     if (last) bar = fmaxf(bar, order_float(last));
   }
-  __device__ __forceinline__ void take(float x, uint32_t index, float above, uint64_t* wait, int top) {
-    const uint64_t pass = __ballot(x > above);
-    if (!pass) return;
-    if (x > above) wait[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] = entry_key(x, index);
-    count += __popcll(pass);
-    if (count >= 64) flush(wait, top);
+  // those of a lane's entries y, of categories c.., that lie above the bar
+  template <int N>
+  __device__ __forceinline__ void take(const float (&y)[N], uint32_t c, uint64_t* wait, int top) {
+    uint32_t hit = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) hit |= y[i] > bar ? 1u << i : 0u;
+    for (;;) {                                    // one entry of every lane that has some left
+      const uint64_t some = __ballot(hit != 0);
+      if (!some) break;
+      if (hit) {
+        const int i = __builtin_ctz(hit);
+        float v = y[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) v = i == j ? y[j] : v;
+        wait[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0))] = entry_key(v, c + i);
+        hit &= hit - 1;
+      }
+      count += __popcll(some);
+      if (count >= 64) flush(wait, top);
+    }
   }
 };
 
@@ -136,57 +155,55 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
       else y[0] = seen(k.g[u]);
     };
     auto work = [&](const Chunk& k, int at) {
+      float y[kLoads][kVec], largest[kLoads], lane_largest = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        entries(k, u, y[u]);
+        largest[u] = y[u][0];
+#pragma unroll
+        for (int i = 1; i < kVec; ++i) largest[u] = kCkpt ? __builtin_elementwise_maximum(largest[u], y[u][i]) : fmaxf(largest[u], y[u][i]);
+        lane_largest = fmaxf(lane_largest, largest[u]);
+      }
       if (kTop && fresh) {
         // the top-th largest of the lanes' largest entries is no larger than the top-th largest entry: a bar to start from
-        float largest = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-          float y[kVec];
-          entries(k, u, y);
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, y[i]);
-        }
-        const uint32_t order = sort_lanes<64, true>(float_order(largest));
-        const float top_value = order_float(__builtin_amdgcn_readlane(order, 0));
-        const uint32_t last = __builtin_amdgcn_readlane(order, top - 1);
-        if (top_value > masked_from<T>()) sum.raise(top_value);
+        const uint32_t last = __builtin_amdgcn_readlane(sort_lanes<64, true>(float_order(lane_largest)), top - 1);
         list.bar = fmaxf(list.bar, order_float(last - (last == 0x80000000u ? 2 : 1)));   // (just below, both zeros being one: the entry itself has to pass)
         fresh = false;
+      }
+      if (__any(lane_largest > (kTop ? list.bar : sum.m))) {
+        const float m1 = over_lanes<64>(lane_largest, Larger());
+        if (m1 > sum.m) sum.raise(m1);
+        if (kTop)
+#pragma unroll 1
+          for (int u = 0; u < kLoads; ++u) {
+            auto g = k.g[0];
+#pragma unroll
+            for (int w = 1; w < kLoads; ++w)
+              if (u == w) g = k.g[w];
+            float z[kVec];
+            if constexpr (kUnit) unpack(g, z, T());
+            else z[0] = seen(g);
+            list.take(z, (uint32_t)(at + (u * 64 + lane) * kVec), wait, top);
+          }
       }
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
         if (at + u * 64 * kVec >= end) break;
-        float y[kVec], largest = -INFINITY, gs = 0.f, gt = 0.f;
-        entries(k, u, y);
+        float gs = 0.f, gt = 0.f;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) largest = kCkpt ? __builtin_elementwise_maximum(largest, y[i]) : fmaxf(largest, y[i]);
-        if (__any(largest > (kTop ? list.bar : sum.m))) {
-          const float m1 = over_lanes<64>(largest, Larger());
-          if (m1 > sum.m) sum.raise(m1);
-          const float above = list.bar;
-          if (kTop)
-#pragma unroll 1
-            for (int i = 0; i < kVec; ++i) {
-              float yi = y[0];
-#pragma unroll
-              for (int j = 1; j < kVec; ++j) yi = i == j ? y[j] : yi;
-              list.take(yi, (uint32_t)(at + (u * 64 + lane) * kVec + i), above, wait, top);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) sum.template add<kEnt>(y[i], gs, gt);
+        for (int i = 0; i < kVec; ++i) sum.template add<kEnt>(y[u][i], gs, gt);
         sum.s += gs;
         sum.t += gt;
         if constexpr (kCkpt) {
           const int c = at + (u * 64 + lane) * kVec;
           float low = INFINITY;
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) low = fminf(low, y[i] > masked_from<T>() ? y[i] : INFINITY);
-          const float hi = over_lanes<kCkptBlock / kVec>(largest, LargerOrNan()), lo = over_lanes<kCkptBlock / kVec>(low, Smaller());
+          for (int i = 0; i < kVec; ++i) low = fminf(low, y[u][i] > masked_from<T>() ? y[u][i] : INFINITY);
+          const float hi = over_lanes<kCkptBlock / kVec>(largest[u], LargerOrNan()), lo = over_lanes<kCkptBlock / kVec>(low, Smaller());
           const BlockScale scale = block_scale(hi > masked_from<T>() ? hi : -INFINITY, lo, !(hi < INFINITY));
           uint32_t code[kVec / 4] = {};
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[i], y[i] <= masked_from<T>()) << (8 * (i % 4));
+          for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[u][i], y[u][i] <= masked_from<T>()) << (8 * (i % 4));
           if (c < pitch) {
             uint32_t* const to = reinterpret_cast<uint32_t*>(ckpt.codes + r * pitch + c);
 #pragma unroll
@@ -274,16 +291,20 @@ __global__ __launch_bounds__(256) void score_join_kernel(RowsRef x, RowsShape sh
   }
 }
 
-Split split_of(const RowsShape& shape) {
-  const int64_t rows = shape.rows();
-  const int chunk = 1024, wanted = 4096;   // waves that keep the memory busy
+// Waves that keep the memory busy: 4096.  Rows that are fewer get several, up to one for every chunk of 64 x kGroups x 16 bytes: of one
+// workgroup, which joins them in LDS, or, beyond 16, of several, with a second launch to put the parts together.
+Split split_of(const RowsShape& shape, int entry_bytes) {
+  const int64_t rows = shape.rows(), chunk = 64 * kGroups * 16 / entry_bytes, chunks = (shape.cats + chunk - 1) / chunk;
+  const int64_t wanted = std::min((4096 + rows - 1) / rows, chunks);
   Split s{1, 1, shape.cats};
-  while (s.waves < kMaxWaves && rows * s.waves < wanted && s.waves * chunk < shape.cats) s.waves *= 2;
-  if (rows * s.waves < wanted / 4 && s.waves * chunk < shape.cats) {
-    const int64_t parts = std::min<int64_t>({kMaxParts, (wanted / 4 + rows * s.waves - 1) / (rows * s.waves), (shape.cats + s.waves * chunk - 1) / (s.waves * chunk)});
-    s.part_len = (int)(((shape.cats + parts - 1) / parts + 1023) / 1024 * 1024);
-    s.parts = (shape.cats + s.part_len - 1) / s.part_len;
+  if (wanted <= kMaxWaves) {
+    while (s.waves < wanted) s.waves *= 2;
+    return s;
   }
+  s.waves = wanted > 8 * kMaxParts ? kMaxWaves : 8;
+  const int64_t parts = std::min<int64_t>(kMaxParts, (wanted + s.waves - 1) / s.waves);
+  s.part_len = (int)((chunks + parts - 1) / parts * chunk);
+  s.parts = (int)((shape.cats + s.part_len - 1) / s.part_len);
   return s;
 }
 
@@ -293,7 +314,7 @@ template <typename T>
 void launch_stream(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, const CkptRef& ckpt, void* work,
                    hipStream_t stream) {
   if (category_scores_short<T>(x, shape, given, top, out, ckpt, stream)) return;
-  const Split s = split_of(shape);
+  const Split s = split_of(shape, sizeof(T));
   PartRef part{};
   if (s.parts > 1) {
     part.sums = static_cast<float4*>(work);
@@ -318,11 +339,16 @@ void launch_stream(const RowsRef& x, const RowsShape& shape, const GivenRef& giv
 }
 }  // namespace
 
+// (whatever the type and the strides: what the entries of four bytes need, or those of two)
 int64_t category_scores_workspace(const RowsShape& shape, int top) {
   if (shape.examples < 1 || shape.vars < 1 || shape.cats < 1 || top < 0 || top > kMaxSlots || shape.examples > INT64_C(0x7fffffff) / shape.vars) return 0;
-  const Split s = split_of(shape);
-  const size_t jobs = (size_t)shape.rows() * s.parts;
-  return s.parts == 1 ? 0 : (int64_t)(up16(jobs * sizeof(float4)) + jobs * top * sizeof(uint64_t));
+  int64_t most = 0;
+  for (int bytes = 2; bytes <= 4; bytes += 2) {
+    const Split s = split_of(shape, bytes);
+    const size_t jobs = (size_t)shape.rows() * s.parts;
+    if (s.parts > 1) most = std::max(most, (int64_t)(up16(jobs * sizeof(float4)) + jobs * top * sizeof(uint64_t)));
+  }
+  return most;
 }
 
 void category_scores(const RowsRef& x_in, const RowsShape& shape_in, const GivenRef& given, int top, float* d_logp, float* d_log_sum,

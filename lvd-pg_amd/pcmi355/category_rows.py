@@ -98,7 +98,7 @@ def _check_given(given, rows):
 def _f32(t, shape, what):
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what} must be a tensor of shape {tuple(shape)}")
-    return t.to(torch.float32).contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _no_overlap(t):
@@ -128,21 +128,18 @@ def _apart(out, other):
     return b <= c or d <= a
 
 
-class _device:
-    """The device of a tensor, current for a call."""
-    __slots__ = ("guard",)
+# the stream without an object around it, where torch has it: 0.1 us instead of 2.9
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
+def _on_device_of(t, call):
+    """call(stream) with a tensor's device as the current one"""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        check(call(_raw_stream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(call(_raw_stream(index)))
 
 
 def _new_checkpoint(x, shape):
@@ -178,15 +175,14 @@ def category_scores(scores, given=None, *, top=0, entropy=False, checkpoint=Fals
     kept = _new_checkpoint(scores, shape) if checkpoint else None
     if log_sum.numel():
         n, v, c = _sizes(shape)
-        with _device(scores) as stream:
-            size = lib.pcm_category_scores_workspace(n, v, c, top)
-            work = new(size, dtype=torch.uint8, device=dev) if size else None
-            check(lib.pcm_category_scores(
-                scores.data_ptr(), _TYPES[scores.dtype], *_strides(scores), n, v, c, *where, top,
-                None if logp is None else logp.data_ptr(), log_sum.data_ptr(), None if ent is None else ent.data_ptr(),
-                None if best is None else best_logp.data_ptr(), None if best is None else best.data_ptr(),
-                None if kept is None else kept.codes.data_ptr(), None if kept is None else kept.scales.data_ptr(),
-                None if work is None else work.data_ptr(), size, stream))
+        size = lib.pcm_category_scores_workspace(n, v, c, top)
+        work = new(size, dtype=torch.uint8, device=dev) if size else None
+        _on_device_of(scores, lambda stream: lib.pcm_category_scores(
+            scores.data_ptr(), _TYPES[scores.dtype], *_strides(scores), n, v, c, *where, top,
+            None if logp is None else logp.data_ptr(), log_sum.data_ptr(), None if ent is None else ent.data_ptr(),
+            None if best is None else best_logp.data_ptr(), None if best is None else best.data_ptr(),
+            None if kept is None else kept.codes.data_ptr(), None if kept is None else kept.scales.data_ptr(),
+            None if work is None else work.data_ptr(), size, stream))
     return CategoryScores(logp, log_sum, ent, best, best_logp, kept)
 
 
@@ -234,12 +230,11 @@ def category_scores_backward(scores, log_sum, given=None, *, grad_logp=None, ent
     if log_sum.numel():
         n, v, c = _sizes(shape)
         ptr = queries._dev_ptr
-        with _device(out) as stream:
-            check(lib.pcm_category_scores_backward(
-                None if kept is not None else scores.data_ptr(), _TYPES[dtype], *((0, 0, 0) if kept is not None else _strides(scores)),
-                n, v, c, None if kept is None else kept.codes.data_ptr(), None if kept is None else kept.scales.data_ptr(), *where,
-                ptr(grad_logp), slots, ptr(top), ptr(grad_top), log_sum.data_ptr(), ptr(entropy), ptr(grad_entropy), out.data_ptr(),
-                *_strides(out), stream))
+        _on_device_of(out, lambda stream: lib.pcm_category_scores_backward(
+            None if kept is not None else scores.data_ptr(), _TYPES[dtype], *((0, 0, 0) if kept is not None else _strides(scores)),
+            n, v, c, None if kept is None else kept.codes.data_ptr(), None if kept is None else kept.scales.data_ptr(), *where,
+            ptr(grad_logp), slots, ptr(top), ptr(grad_top), log_sum.data_ptr(), ptr(entropy), ptr(grad_entropy), out.data_ptr(),
+            *_strides(out), stream))
     return out
 
 
@@ -254,9 +249,8 @@ def checkpoint_rows(rows):
     kept = _new_checkpoint(rows, tuple(rows.shape))
     if kept.codes.numel():
         n, v, c = _sizes(rows.shape)
-        with _device(rows) as stream:
-            check(lib.pcm_checkpoint_rows(rows.data_ptr(), _TYPES[rows.dtype], *_strides(rows), n, v, c, kept.codes.data_ptr(),
-                                          kept.scales.data_ptr(), stream))
+        _on_device_of(rows, lambda stream: lib.pcm_checkpoint_rows(
+            rows.data_ptr(), _TYPES[rows.dtype], *_strides(rows), n, v, c, kept.codes.data_ptr(), kept.scales.data_ptr(), stream))
     return kept
 
 
@@ -275,9 +269,8 @@ def restore_rows(checkpoint, dtype=None, out=None):
     _on_gpu(out)
     if out.numel():
         n, v, c = _sizes(checkpoint.shape)
-        with _device(out) as stream:
-            check(lib.pcm_restore_rows(checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(), n, v, c, out.data_ptr(), _TYPES[dtype],
-                                       *_strides(out), stream))
+        _on_device_of(out, lambda stream: lib.pcm_restore_rows(
+            checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(), n, v, c, out.data_ptr(), _TYPES[dtype], *_strides(out), stream))
     return out
 
 
