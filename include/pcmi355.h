@@ -520,7 +520,7 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  * (in [1/2, 1)), at most 127 otherwise, |x| <= 2^14 steps and e >= -126.  An entry stands for (base - code) 2^e, base = rint(M /
  * 2^e): the nearest multiple of the step.  Code 255: an entry that is masked, x <= half of the type's lowest value; it
  * stands for -inf.  Scale word: base in bits 0..15 (two's complement), e + 127 in bits 16..23; 255 there (a block with NaN or
- * +inf): every entry stands for NaN.  Codes behind a row's end are 255.
+ * +inf): every entry stands for NaN; bit 24: some code of the block, or behind the row's end in it, is 255.  Codes behind a row's end are 255.
  * pcm_restore_rows: the values that the codes stand for, as floats or rounded to the type the rows had.
  *
  * All queue their work on `stream` (of the current device), wait for nothing and allocate nothing: they can be captured.

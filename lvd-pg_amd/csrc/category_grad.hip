@@ -41,15 +41,16 @@ struct GradRow {
     }
   }
   __device__ __forceinline__ bool none() const { return z == INFINITY; }
-  __device__ __forceinline__ float operator()(float x) const {
+  template <bool kEnt>
+  __device__ __forceinline__ float at(float x) const {
     const float d = x - z, p = __builtin_amdgcn_exp2f(d * kLog2e);
-    return -p * fmaf(gh, fmaxf(d, -200.f) + h, total);   // (p is 0 where d is below, and may be -inf)
+    return kEnt ? -p * fmaf(gh, fmaxf(d, -200.f) + h, total) : -p * total;   // (p is 0 where d is below, and may be -inf)
   }
 };
 
 // Rows of neighbouring categories in and out.  The slots of the workgroup's rows wait in LDS; of a long row only those in the
 // workgroup's segment, in their order, so that sums come out the same every time.
-template <typename T, bool kCkpt>
+template <typename T, bool kCkpt, bool kEnt>
 __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, Tiles tiles) {
   constexpr int kVec = 16 / (int)sizeof(T);
   __shared__ GradSlot slot_lds[kStaged];
@@ -68,14 +69,14 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
 
     raw4 raw[kCkpt ? 1 : kTileGroups];
     Codes<kVec> code[kCkpt ? kTileGroups : 1];
-    BlockUnit unit[kCkpt ? kTileGroups : 1];
+    uint32_t unit[kCkpt ? kTileGroups : 1];
 #pragma unroll
     for (int u = 0; u < kTileGroups; ++u) {
       const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
       if (c >= shape.cats) continue;
       if constexpr (kCkpt) {
         code[u] = load_codes<kVec>(ckpt.codes + r * pitch + c);
-        unit[u] = block_unit(ckpt.scales[r * blocks + c / kCkptBlock]);
+        unit[u] = ckpt.scales[r * blocks + c / kCkptBlock];
       } else raw[u] = load_group(row, c, shape.cats);
     }
 
@@ -137,12 +138,10 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
       const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
       if (c >= shape.cats) continue;
       float y[kVec];
-      if constexpr (kCkpt) {
+      if constexpr (kCkpt) decode(code[u], block_unit(unit[u]), y);
+      else unpack(raw[u], y, T());
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) y[i] = code_value(unit[u], code[u][i]);
-      } else unpack(raw[u], y, T());
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) y[i] = grad(y[i]);
+      for (int i = 0; i < kVec; ++i) y[i] = grad.template at<kEnt>(y[i]);
       for (int j = 0; j < near; ++j) {
         const uint32_t i = (uint32_t)near_at[j].at - (uint32_t)c;
         if (i < (uint32_t)kVec) {
@@ -200,14 +199,14 @@ __global__ __launch_bounds__(256) void grad_column_kernel(RowsRef x, CkptRef ckp
       for (int i = 0; i < kStep; ++i) {
         const int c = c0 + i;
         if (c >= end) y[i] = -INFINITY;
-        else if constexpr (kCkpt) y[i] = code_value(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
+        else if constexpr (kCkpt) y[i] = block_entry_or_mask(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
         else y[i] = seen(row[(int64_t)c * x.stride_cat]);
       }
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
         const int c = c0 + i;
         if (c >= end) break;
-        float g = grad(y[i]);
+        float g = grad.template at<true>(y[i]);
         if (!grad.none()) {
 #pragma unroll
           for (int j = 0; j < kNear; ++j) g += near[j].at == c ? near[j].by : 0.f;
@@ -229,7 +228,9 @@ void launch_grad(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, 
   if (out.stride_cat == 1 && (ckpt.codes || x.stride_cat == 1)) {
     const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), (slots * kTileThreads + kStaged - 1) / kStaged);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, tile_grid(t), dim3(kTileThreads), 0, stream, x, ckpt, shape, in, out, t); };
-    ckpt.codes ? launch(grad_tile_kernel<T, true>) : launch(grad_tile_kernel<T, false>);
+    const bool ent = in.grad_entropy != nullptr;
+    if (ckpt.codes) ent ? launch(grad_tile_kernel<T, true, true>) : launch(grad_tile_kernel<T, true, false>);
+    else ent ? launch(grad_tile_kernel<T, false, true>) : launch(grad_tile_kernel<T, false, false>);
     return;
   }
   const int64_t sets = (shape.rows() + 63) / 64;

@@ -128,6 +128,7 @@ __device__ __forceinline__ float over_lanes(float v, F f) {
 struct Larger { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct Smaller { __device__ float operator()(float a, float b) const { return fminf(a, b); } };
 struct LargerOrNan { __device__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); } };
+struct SmallerOrNan { __device__ float operator()(float a, float b) const { return __builtin_elementwise_minimum(a, b); } };
 struct Sum { __device__ float operator()(float a, float b) const { return a + b; } };
 
 // the value of lane ^ J
@@ -231,12 +232,13 @@ __device__ __forceinline__ float type_max<f16>() { return 65504.f; }
 // The scale of a block of 64: entry = (base - code) 2^e, code 0..254.  e is the smallest exponent with 253 steps (254 between
 // rounded ends) over the block's range where the range's mantissa allows, and with the largest entry within 2^14 steps, so that
 // base fits 16 bits.  A power of two makes x 2^-e, its rounding and the product back exact: an entry is off by half a step
-// at most, whoever computes it.  Word: base in bits 0..15, e + 127 in bits 16..23; 255 there: a block with NaN or +inf.
+// at most, whoever computes it.  Word: base in bits 0..15, e + 127 in bits 16..23 (255 there: a block with NaN or +inf), bit 24: some
+// code is 255, so that a block without it can be read without looking for them.
 struct BlockScale {
   float inv, base;   // 2^-e, rint(max 2^-e)
   uint32_t word;
 };
-__device__ __forceinline__ BlockScale block_scale(float hi, float lo, bool bad) {   // (hi < lo: no entry but masked ones)
+__device__ __forceinline__ BlockScale block_scale(float hi, float lo, bool masks, bool bad) {   // (hi < lo: no entry but masked ones)
   if (hi < lo) hi = lo = 0.f;
   const float r = 0.5f * hi - 0.5f * lo;   // halves: the difference itself may pass the range of float
   const float a = fmaxf(fabsf(hi), fabsf(lo));
@@ -246,24 +248,73 @@ __device__ __forceinline__ BlockScale block_scale(float hi, float lo, bool bad) 
   BlockScale s;
   s.inv = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
   s.base = rintf(hi * s.inv);
-  s.word = bad ? 0xff0000u : (uint32_t)(127 + e) << 16 | ((uint32_t)(int)s.base & 0xffffu);
+  s.word = bad ? 0xff0000u : (uint32_t)(127 + e) << 16 | ((uint32_t)(int)s.base & 0xffffu) | (masks ? 1u << 24 : 0u);
   return s;
 }
-// a masked entry is off: x <= masked_from<T>()
-__device__ __forceinline__ uint32_t block_code(const BlockScale& s, float x, bool off) {
-  return off ? (uint32_t)kCkptMasked : (uint32_t)__builtin_amdgcn_fmed3f(s.base - rintf(x * s.inv), 0.f, 254.f);
+// base - rint(x 2^-e): adding 1.5 2^23 rounds the product, which is exact and below 2^14, to a whole number in the low bits
+__device__ __forceinline__ uint32_t block_code(const BlockScale& s, float x) {
+  return 0x4b400000u + (uint32_t)(int)s.base - __builtin_bit_cast(uint32_t, fmaf(x, s.inv, 12582912.f));
 }
+// Codes of the N entries that a lane holds of a block, which lies in 64 / N neighbouring lanes; every lane of the wave is active.
+template <int N>
+struct BlockCodes {
+  uint32_t code[N / 4], word;
+};
+template <typename T, int N>
+__device__ __forceinline__ BlockCodes<N> encode_block(const float (&y)[N]) {
+  float hi = y[0], lo = y[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    hi = __builtin_elementwise_maximum(hi, y[i]);
+    lo = __builtin_elementwise_minimum(lo, y[i]);
+  }
+  hi = over_lanes<kCkptBlock / N>(hi, LargerOrNan());
+  lo = over_lanes<kCkptBlock / N>(lo, SmallerOrNan());
+  BlockCodes<N> out;
+  if (!__any(!(lo > masked_from<T>() && hi < INFINITY))) {   // nothing masked, no NaN in any of the wave's blocks
+    const BlockScale s = block_scale(hi, lo, false, false);
+    out.word = s.word;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      out.code[i] = block_code(s, y[4 * i]) | block_code(s, y[4 * i + 1]) << 8 | block_code(s, y[4 * i + 2]) << 16 | block_code(s, y[4 * i + 3]) << 24;
+    return out;
+  }
+  float kept = INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) kept = fminf(kept, y[i] > masked_from<T>() ? y[i] : INFINITY);
+  kept = over_lanes<kCkptBlock / N>(kept, Smaller());
+  const BlockScale s = block_scale(hi > masked_from<T>() ? hi : -INFINITY, kept, lo <= masked_from<T>(), !(hi < INFINITY));
+  out.word = s.word;
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) out.code[i] = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    out.code[i / 4] |= (y[i] <= masked_from<T>() ? (uint32_t)kCkptMasked : block_code(s, y[i]) & 0xffu) << (8 * (i % 4));
+  return out;
+}
+// ... and where they go, for a lane whose entries begin at c of row r
+template <int N>
+__device__ __forceinline__ void store_codes(const CkptRef& ckpt, const BlockCodes<N>& k, int64_t r, int64_t c, int cats, int64_t pitch, int64_t blocks) {
+  if (c >= pitch) return;
+  uint8_t* const to = ckpt.codes + r * pitch + c;
+  if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = k.code[0];
+  else *reinterpret_cast<uint2*>(to) = make_uint2(k.code[0], k.code[1]);
+  if (c % kCkptBlock == 0 && c < cats) ckpt.scales[r * blocks + c / kCkptBlock] = k.word;
+}
+
 struct BlockUnit {
-  float step, base;
+  float step, base;   // an entry is (base - code) step
+  bool masks;
 };
 __device__ __forceinline__ BlockUnit block_unit(uint32_t word) {
   const uint32_t e = word >> 16 & 0xffu;
-  return e == 0xffu ? BlockUnit{__builtin_nanf(""), 0.f}
-                    : BlockUnit{__builtin_bit_cast(float, e << 23), (float)(int16_t)(word & 0xffffu)};
+  const float step = e == 0xffu ? __builtin_nanf("") : __builtin_bit_cast(float, e << 23);
+  return {step, (float)(int16_t)(word & 0xffffu), (word >> 24 & 1u) != 0};
 }
-__device__ __forceinline__ float block_entry(const BlockUnit& u, uint32_t code) {   // (the product may round up past the range)
-  const float v = (u.base - (float)code) * u.step;
-  return code == (uint32_t)kCkptMasked && u.step == u.step ? -INFINITY : v > 3.4028235e38f ? 3.4028235e38f : v;
+// (base step alone may pass the range, an entry only by rounding the largest up)
+__device__ __forceinline__ float block_entry(const BlockUnit& u, float code) { return (u.base - code) * u.step; }
+__device__ __forceinline__ float block_entry_or_mask(const BlockUnit& u, float code) {
+  return u.masks && code == (float)kCkptMasked ? -INFINITY : block_entry(u, code);
 }
 #endif
 

@@ -77,7 +77,8 @@ struct TopList {
         hit &= hit - 1;
       }
       count += __popcll(some);
-      if (count >= 64) flush(wait, top);
+      // (64 fill what is sorted at a time; fewer are sorted in at the end of a group, so that the bar rises early)
+      if (count >= 64 || (count >= max(top, 16) && !__any(hit != 0))) flush(wait, top);
     }
   }
 };
@@ -161,8 +162,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
         entries(k, u, y[u]);
         largest[u] = y[u][0];
 #pragma unroll
-        for (int i = 1; i < kVec; ++i) largest[u] = kCkpt ? __builtin_elementwise_maximum(largest[u], y[u][i]) : fmaxf(largest[u], y[u][i]);
-        lane_largest = fmaxf(lane_largest, largest[u]);
+        for (int i = 1; i < kVec; ++i) largest[u] = __builtin_elementwise_maximum(largest[u], y[u][i]);
+        lane_largest = __builtin_elementwise_maximum(lane_largest, largest[u]);
       }
       if (kTop && fresh) {
         // the top-th largest of the lanes' largest entries is no larger than the top-th largest entry: a bar to start from
@@ -171,11 +172,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
         fresh = false;
       }
       if (__any(lane_largest > (kTop ? list.bar : sum.m))) {
-        const float m1 = over_lanes<64>(lane_largest, Larger());
-        if (m1 > sum.m) sum.raise(m1);
-        if (kTop)
-#pragma unroll 1
-          for (int u = 0; u < kLoads; ++u) {
+        if (!kTop || __any(lane_largest > sum.m)) {
+          const float m1 = over_lanes<64>(lane_largest, Larger());
+          if (m1 > sum.m) sum.raise(m1);
+        }
+        if constexpr (kTop) {
+          uint32_t groups = 0;                    // that have an entry above the bar
+#pragma unroll
+          for (int u = 0; u < kLoads; ++u) groups |= __any(largest[u] > list.bar) ? 1u << u : 0u;
+          while (groups) {
+            const int u = __builtin_ctz(groups);
+            groups &= groups - 1;
             auto g = k.g[0];
 #pragma unroll
             for (int w = 1; w < kLoads; ++w)
@@ -185,6 +192,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
             else z[0] = seen(g);
             list.take(z, (uint32_t)(at + (u * 64 + lane) * kVec), wait, top);
           }
+        }
       }
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
@@ -196,20 +204,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
         sum.t += gt;
         if constexpr (kCkpt) {
           const int c = at + (u * 64 + lane) * kVec;
-          float low = INFINITY;
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) low = fminf(low, y[u][i] > masked_from<T>() ? y[u][i] : INFINITY);
-          const float hi = over_lanes<kCkptBlock / kVec>(largest[u], LargerOrNan()), lo = over_lanes<kCkptBlock / kVec>(low, Smaller());
-          const BlockScale scale = block_scale(hi > masked_from<T>() ? hi : -INFINITY, lo, !(hi < INFINITY));
-          uint32_t code[kVec / 4] = {};
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[u][i], y[u][i] <= masked_from<T>()) << (8 * (i % 4));
-          if (c < pitch) {
-            uint32_t* const to = reinterpret_cast<uint32_t*>(ckpt.codes + r * pitch + c);
-#pragma unroll
-            for (int i = 0; i < kVec / 4; ++i) to[i] = code[i];
-            if (c % kCkptBlock == 0 && c < shape.cats) ckpt.scales[r * blocks + c / kCkptBlock] = scale.word;
-          }
+          store_codes(ckpt, encode_block<T>(y[u]), r, c, shape.cats, pitch, blocks);
         }
       }
     };

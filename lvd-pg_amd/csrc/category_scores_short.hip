@@ -64,24 +64,8 @@ __global__ __launch_bounds__(256) void score_short_kernel(RowsRef x, RowsShape s
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const int c = (g * 16 + lane) * kVec;
-        float hi = -INFINITY, lo = INFINITY;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          hi = __builtin_elementwise_maximum(hi, y[g][i]);
-          lo = fminf(lo, y[g][i] > masked_from<T>() ? y[g][i] : INFINITY);
-        }
-        hi = over_lanes<kCkptBlock / kVec>(hi, LargerOrNan());
-        lo = over_lanes<kCkptBlock / kVec>(lo, Smaller());
-        const BlockScale scale = block_scale(hi > masked_from<T>() ? hi : -INFINITY, lo, !(hi < INFINITY));
-        uint32_t code[kVec / 4] = {};
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[g][i], y[g][i] <= masked_from<T>()) << (8 * (i % 4));
-        if (mine && c < pitch) {
-          uint32_t* const to = reinterpret_cast<uint32_t*>(ckpt.codes + r * pitch + c);
-#pragma unroll
-          for (int i = 0; i < kVec / 4; ++i) to[i] = code[i];
-          if (c % kCkptBlock == 0 && c < shape.cats) ckpt.scales[r * blocks + c / kCkptBlock] = scale.word;
-        }
+        const BlockCodes<kVec> k = encode_block<T>(y[g]);
+        if (mine) store_codes(ckpt, k, r, c, shape.cats, pitch, blocks);
       }
     }
     if constexpr (kTop) {

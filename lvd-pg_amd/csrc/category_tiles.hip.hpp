@@ -76,9 +76,16 @@ __device__ __forceinline__ Codes<kVec> load_codes(const uint8_t* at) {
   }
   return k;
 }
-__device__ __forceinline__ float code_value(const BlockUnit& u, float code) {   // (255 stands for -inf, in a block that is not NaN)
-  const float v = (u.base - code) * u.step;
-  return code == (float)kCkptMasked && u.step == u.step ? -INFINITY : v;
+// the entries that they stand for
+template <int kVec>
+__device__ __forceinline__ void decode(const Codes<kVec>& k, const BlockUnit& u, float (&y)[kVec]) {
+  if (__any(u.masks)) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) y[i] = block_entry_or_mask(u, k[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) y[i] = block_entry(u, k[i]);
+  }
 }
 #endif
 

@@ -22,25 +22,10 @@ __global__ __launch_bounds__(kTileThreads) void checkpoint_tile_kernel(RowsRef x
 #pragma unroll
     for (int u = 0; u < kTileGroups; ++u) {
       const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
-      float y[kVec], hi = -INFINITY, lo = INFINITY;
+      float y[kVec];
       unpack(raw[u], y, T());
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        hi = __builtin_elementwise_maximum(hi, y[i]);
-        lo = fminf(lo, y[i] > masked_from<T>() ? y[i] : INFINITY);
-      }
-      hi = over_lanes<kCkptBlock / kVec>(hi, LargerOrNan());
-      lo = over_lanes<kCkptBlock / kVec>(lo, Smaller());
-      const BlockScale scale = block_scale(hi > masked_from<T>() ? hi : -INFINITY, lo, !(hi < INFINITY));
-      uint32_t code[kVec / 4] = {};
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) code[i / 4] |= block_code(scale, y[i], y[i] <= masked_from<T>()) << (8 * (i % 4));
-      if (mine && c < pitch) {
-        uint32_t* const to = reinterpret_cast<uint32_t*>(ckpt.codes + r * pitch + c);
-#pragma unroll
-        for (int i = 0; i < kVec / 4; ++i) to[i] = code[i];
-        if (c % kCkptBlock == 0 && c < shape.cats) ckpt.scales[r * blocks + c / kCkptBlock] = scale.word;
-      }
+      const BlockCodes<kVec> k = encode_block<T>(y);
+      if (mine) store_codes(ckpt, k, r, c, shape.cats, pitch, blocks);
     }
   }
 }
@@ -57,15 +42,15 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(RowsRef x, RowsShape sh
     const float y = c < shape.cats ? to_float(row[c * x.stride_cat]) : -INFINITY;
     const bool off = y <= masked_from<T>();
     const float hi = over_lanes<64>(off ? -INFINITY : y, LargerOrNan()), lo = over_lanes<64>(off ? INFINITY : y, Smaller());
-    const BlockScale s = block_scale(hi, lo, !(hi < INFINITY));
-    if (c < pitch) ckpt.codes[r * pitch + c] = (uint8_t)block_code(s, y, off);
+    const BlockScale s = block_scale(hi, lo, __any(off), !(hi < INFINITY));
+    if (c < pitch) ckpt.codes[r * pitch + c] = off ? (uint8_t)kCkptMasked : (uint8_t)block_code(s, y);
     if (lane == 0) ckpt.scales[b] = s.word;
   }
 }
 
-// (a value may have been rounded up past the largest of the type)
+// (a value may have been rounded up past the largest of the type; NaN stays)
 template <typename T>
-__device__ __forceinline__ T restored(float y) { return from_float<T>(y > type_max<T>() ? type_max<T>() : y); }
+__device__ __forceinline__ T restored(float y) { return from_float<T>(__builtin_elementwise_minimum(y, type_max<T>())); }
 
 template <typename T>
 __global__ __launch_bounds__(kTileThreads) void restore_tile_kernel(CkptRef ckpt, RowsShape shape, RowsRef out, Tiles tiles) {
@@ -92,8 +77,10 @@ __global__ __launch_bounds__(kTileThreads) void restore_tile_kernel(CkptRef ckpt
       if (c >= shape.cats) continue;
       const BlockUnit unit = block_unit(word[u]);
       T w[kVec];
+      float y[kVec];
+      decode(code[u], unit, y);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) w[i] = restored<T>(code_value(unit, code[u][i]));
+      for (int i = 0; i < kVec; ++i) w[i] = restored<T>(y[i]);
       store_group(dst, c, shape.cats, w);
     }
   }
@@ -104,7 +91,7 @@ __global__ __launch_bounds__(256) void restore_kernel(CkptRef ckpt, RowsShape sh
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock, all = shape.rows() * shape.cats;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / shape.cats, c = i % shape.cats, e = r / shape.vars, v = r % shape.vars;
-    const float y = code_value(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
+    const float y = block_entry_or_mask(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
     static_cast<T*>(const_cast<void*>(out.p))[e * out.stride_ex + v * out.stride_var + c * out.stride_cat] = restored<T>(y);
   }
 }
