@@ -20,8 +20,11 @@ void check_given(const GivenRef& g) {
 }
 
 namespace {
-constexpr int kGroups = 4;                  // 16-byte groups that a lane requests at a time
+constexpr int kEntries = 16, kChunk = 64 * kEntries;   // of a lane, of a wave, at a time (32 entries of 2 bytes cost 20 spilled registers)
 constexpr int kMaxWaves = 16, kMaxParts = 64;
+constexpr int kRoom = 64;                   // common keys per wave of a workgroup
+constexpr int kOneListChunks = 4;           // most chunks of a wave whose entries go into one list of the workgroup's
+constexpr int kNoList = 0, kListPerWave = 1, kOneList = 2;
 
 struct PartRef {                            // what parts of a row leave for the kernel that joins them
   float4* sums;                             // [rows][parts] m, s, t
@@ -59,29 +62,16 @@ struct TopList {
     const uint32_t last = __builtin_amdgcn_readlane((uint32_t)(list >> 32), top - 1);
     if (last) bar = fmaxf(bar, order_float(last));
   }
-  // those of a lane's entries y, of categories c.., that lie above the bar
-  template <int N>
-  __device__ __forceinline__ void take(const float (&y)[N], uint32_t c, uint64_t* wait, int top) {
-    uint32_t hit = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) hit |= y[i] > bar ? 1u << i : 0u;
-    for (;;) {                                    // one entry of every lane that has some left
-      const uint64_t some = __ballot(hit != 0);
-      if (!some) break;
-      if (hit) {
-        const int i = __builtin_ctz(hit);
-        float v = y[0];
-#pragma unroll
-        for (int j = 1; j < N; ++j) v = i == j ? y[j] : v;
-        wait[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0))] = entry_key(v, c + i);
-        hit &= hit - 1;
-      }
-      count += __popcll(some);
-      // (64 fill what is sorted at a time; fewer are sorted in at the end of a group, so that the bar rises early)
-      if (count >= 64 || (count >= max(top, 16) && !__any(hit != 0))) flush(wait, top);
-    }
-  }
+  // the number just below one of float_order's (where both zeros are +0): a bar that the number itself passes
+  static __device__ __forceinline__ float below(uint32_t order) { return order_float(order - (order == 0x80000000u ? 2 : 1)); }
 };
+
+// Writes the entries x of category c of the lanes in `some` behind the first `count` keys; returns how many there are then.
+__device__ __forceinline__ int add_keys(uint64_t some, float x, uint32_t c, uint64_t* to, int count) {
+  if (some >> (threadIdx.x & 63) & 1)
+    to[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0))] = entry_key(x, c);
+  return count + __popcll(some);
+}
 
 // the results of a row from its sums and sorted keys, by one wave
 template <typename T>
@@ -102,17 +92,23 @@ __device__ __forceinline__ void write_row(const RowSums<T>& q, uint64_t key, int
   }
 }
 
-// One pass over a row, or a part of it, by the waves of a workgroup.  A wave takes kGroups x 16 bytes a lane at a time (one
-// entry at a time where categories are not neighbours), requests the next ones before it works on these, and keeps one maximum
+// One pass over a row, or a part of it, by the waves of a workgroup.  A wave takes kEntries a lane at a time (16 bytes a request, one
+// entry at a time where categories are not neighbours), requests the ones after the next as soon as these are in float, and keeps one maximum
 // for its lanes: a group whose largest entry lies above neither the maximum nor the list's bar goes straight into the sums.
-template <typename T, bool kUnit, bool kEnt, bool kTop, bool kCkpt>
+template <typename T, bool kUnit, bool kEnt, int kLists, bool kCkpt>
 __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x, RowsShape shape, GivenRef given, int top, ScoreOut out, CkptRef ckpt,
                                                                       int parts, int part_len, PartRef part) {
-  constexpr int kVec = kUnit ? 16 / (int)sizeof(T) : 1, kLoads = kUnit ? kGroups : 16, kChunk = 64 * kVec * kLoads;
-  extern __shared__ uint64_t stream_lds[];   // per wave 128 keys that wait, and its sums
+  constexpr bool kTop = kLists != kNoList, kCommon = kLists == kOneList;
+  constexpr int kVec = kUnit ? 16 / (int)sizeof(T) : 1, kLoads = kEntries / kVec;
+  extern __shared__ uint64_t stream_lds[];   // per wave 128 keys that wait, and its sums; the common keys
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   uint64_t* const wait = stream_lds + 128 * wave;
   float4* const sums_lds = reinterpret_cast<float4*>(stream_lds + 128 * waves);
+  uint64_t* const ours = reinterpret_cast<uint64_t*>(sums_lds + waves);   // the waves' common keys
+  const int room = kRoom * waves;
+  __shared__ uint32_t seed[kCommon ? 256 : 1];
+  __shared__ int ours_count, ours_full, crowds;
+  __shared__ float ours_bar;
   const int64_t jobs = shape.rows() * parts;
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
 
@@ -126,7 +122,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
     RowSums<T> sum;
     TopList list;
     list.bar = masked_from<T>();
-    bool fresh = true;
+    bool fresh = !kCommon;
 
     struct Chunk { typename std::conditional<kUnit, raw4, T>::type g[kLoads]; };
     auto load = [&](Chunk& k, int at) {                       // a whole chunk
@@ -155,7 +151,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
       if constexpr (kUnit) unpack(k.g[u], y, T());
       else y[0] = seen(k.g[u]);
     };
-    auto work = [&](const Chunk& k, int at) {
+    const int whole = (end - first) / kChunk, chunks = (end - first + kChunk - 1) / kChunk;
+    auto request = [&](Chunk& k, int j) {
+      if (j < whole) load(k, first + j * kChunk);
+      else if (j < chunks) load_end(k, first + j * kChunk);
+    };
+    auto work = [&](Chunk& k, int j) {
+      const int at = first + j * kChunk;
       float y[kLoads][kVec], largest[kLoads], lane_largest = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
@@ -165,32 +167,76 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
         for (int i = 1; i < kVec; ++i) largest[u] = __builtin_elementwise_maximum(largest[u], y[u][i]);
         lane_largest = __builtin_elementwise_maximum(lane_largest, largest[u]);
       }
+      request(k, j + 2 * waves);
       if (kTop && fresh) {
         // the top-th largest of the lanes' largest entries is no larger than the top-th largest entry: a bar to start from
         const uint32_t last = __builtin_amdgcn_readlane(sort_lanes<64, true>(float_order(lane_largest)), top - 1);
-        list.bar = fmaxf(list.bar, order_float(last - (last == 0x80000000u ? 2 : 1)));   // (just below, both zeros being one: the entry itself has to pass)
+        list.bar = fmaxf(list.bar, TopList::below(last));
         fresh = false;
       }
-      if (__any(lane_largest > (kTop ? list.bar : sum.m))) {
+      if (__any(lane_largest > (kTop ? fminf(list.bar, sum.m) : sum.m))) {   // (another wave's entries may have set the bar)
         if (!kTop || __any(lane_largest > sum.m)) {
           const float m1 = over_lanes<64>(lane_largest, Larger());
           if (m1 > sum.m) sum.raise(m1);
         }
         if constexpr (kTop) {
-          uint32_t groups = 0;                    // that have an entry above the bar
+          const float above = list.bar;           // (the bar of earlier chunks, also where it rises in between)
+          const int early = max(top, 16);         // that many waiting entries are sorted in at once, so that the bar rises
+          uint32_t crowded = 0;                   // groups with more entries above the bar than there is room for
 #pragma unroll
-          for (int u = 0; u < kLoads; ++u) groups |= __any(largest[u] > list.bar) ? 1u << u : 0u;
-          while (groups) {
-            const int u = __builtin_ctz(groups);
-            groups &= groups - 1;
-            auto g = k.g[0];
+          for (int u = 0; u < kLoads; ++u)
+            if (__any(largest[u] > above)) {
+              uint64_t some[kVec];
+              int all = 0;
 #pragma unroll
-            for (int w = 1; w < kLoads; ++w)
-              if (u == w) g = k.g[w];
-            float z[kVec];
-            if constexpr (kUnit) unpack(g, z, T());
-            else z[0] = seen(g);
-            list.take(z, (uint32_t)(at + (u * 64 + lane) * kVec), wait, top);
+              for (int i = 0; i < kVec; ++i) all += __popcll(some[i] = __ballot(y[u][i] > above));
+              // with several waves into the common keys, where there is room
+              uint64_t* to = wait;
+              int count = list.count, most = 128;
+              if (kCommon) {
+                if (lane == 0) {
+                  count = atomicAdd(&ours_count, all);
+                  if (count + all > room) atomicMin(&ours_full, count);
+                }
+                count = __builtin_amdgcn_readfirstlane(count);
+                to = ours;
+                most = room;
+              }
+              if (count + all > most) crowded |= 1u << u;
+              else {
+                if (!kCommon) list.count += all;
+#pragma unroll
+                for (int i = 0; i < kVec; ++i)
+                  if (some[i]) count = add_keys(some[i], y[u][i], (uint32_t)(at + (u * 64 + lane) * kVec + i), to, count);
+              }
+            }
+          // what is full is sorted in, then the crowded groups' entries are added, one of every lane at a time
+          uint32_t hit = 0;
+          float z[kVec];
+          int zc = 0;
+          for (;;) {
+            const uint64_t some = __ballot(hit != 0);
+            if (list.count >= (some || crowded ? 64 : early)) list.flush(wait, top);
+            else if (some) {
+              const int i = hit ? __builtin_ctz(hit) : 0;
+              float v = z[0];
+#pragma unroll
+              for (int j = 1; j < kVec; ++j) v = i == j ? z[j] : v;
+              list.count = add_keys(some, v, (uint32_t)(zc + i), wait, list.count);
+              hit &= hit - 1;
+            } else if (crowded) {
+              const int u = __builtin_ctz(crowded);
+              crowded &= crowded - 1;
+#pragma unroll
+              for (int w = 0; w < kLoads; ++w)
+                if (u == w)
+#pragma unroll
+                  for (int i = 0; i < kVec; ++i) z[i] = y[w][i];
+              zc = at + (u * 64 + lane) * kVec;
+              if (kCommon) crowds = 1;
+#pragma unroll
+              for (int i = 0; i < kVec; ++i) hit |= z[i] > above ? 1u << i : 0u;
+            } else break;
           }
         }
       }
@@ -209,27 +255,62 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
       }
     };
 
-    const int whole = (end - first) / kChunk, chunks = (end - first + kChunk - 1) / kChunk;
-    Chunk now, next;
-    auto request = [&](Chunk& k, int j) {
-      if (j < whole) load(k, first + j * kChunk);
-      else if (j < chunks) load_end(k, first + j * kChunk);
-    };
-    request(now, wave);
-    for (int j = wave; j < chunks; j += waves) {
-      request(next, j + waves);
-      work(now, first + j * kChunk);
-      now = next;
+    Chunk even, odd;
+    request(even, wave);
+    request(odd, wave + waves);
+    if constexpr (kCommon) {
+      // One bar for all waves: the top-th largest, to 16 bits, of the largest entries of up to 256 sets of lanes.  The row's likeliest
+      // entries lie above it, and not many more: the waves collect them together, and one of them sorts them in the end.
+      const int sets = waves <= 4 ? 64 : 256 / waves, each = 64 / sets, words = sets * waves / 64;
+      float largest = -INFINITY;
+      if (wave < chunks) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          float y[kVec];
+          entries(even, u, y);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) largest = __builtin_elementwise_maximum(largest, y[i]);
+        }
+      }
+      if (each > 1) largest = fmaxf(largest, dpp<0xB1>(largest));
+      if (each > 2) largest = fmaxf(largest, dpp<0x4E>(largest));
+      if (lane % each == 0) seed[wave * sets + lane / each] = float_order(largest);
+      __syncthreads();
+      if (wave == 0) {
+        uint32_t v[4], bar = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < words ? seed[i * 64 + lane] : 0;
+        for (int b = 31; b >= 16; --b) {
+          const uint32_t higher = bar | 1u << b;
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) n += __popcll(__ballot(v[i] >= higher));
+          if (n >= top) bar = higher;
+        }
+        if (lane == 0) {
+          ours_bar = TopList::below(bar);
+          ours_count = 0;
+          ours_full = room;
+          crowds = 0;
+        }
+      }
+      __syncthreads();
+      list.bar = fmaxf(list.bar, ours_bar);
     }
-    if (kTop && list.count) list.flush(wait, top);
+    for (int j = wave; j < chunks; j += 2 * waves) {
+      work(even, j);
+      if (j + waves < chunks) work(odd, j + waves);
+    }
+    if (kTop && list.count) list.flush(wait, top);   // (fewer than 64)
     sum.s = over_lanes<64>(sum.s, Sum());
     if (kEnt) sum.t = over_lanes<64>(sum.t, Sum());
 
     if (waves > 1) {
       if (lane == 0) sums_lds[wave] = make_float4(sum.m, sum.s, sum.t, 0.f);
-      if (kTop) wait[lane] = list.list;
       __syncthreads();
-      if (kTop)
+      if (kTop && (!kCommon || crowds)) {          // (one list: only of rows whose entries rise and rise)
+        wait[lane] = list.list;
+        __syncthreads();
         for (int h = waves >> 1; h > 0; h >>= 1) {   // two lists into one, the second one turned round
           if (wave < h) {
             const uint64_t k = stream_lds[128 * (wave + h) + 63 - lane];
@@ -238,6 +319,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
           }
           __syncthreads();
         }
+      }
+      if (kCommon && wave == 0) {
+        const int all = min(ours_count, ours_full);
+        for (int n = 0; n < all; n += 64) {
+          list.count = min(all - n, 64);
+          list.flush(ours + n, top);
+        }
+      }
       if (wave == 0) sum.join_lanes(lane < waves ? sums_lds[lane] : make_float4(masked_from<T>(), 0.f, 0.f, 0.f));
     }
     if (wave == 0) {
@@ -286,19 +375,22 @@ __global__ __launch_bounds__(256) void score_join_kernel(RowsRef x, RowsShape sh
   }
 }
 
-// Waves that keep the memory busy: 4096.  Rows that are fewer get several, up to one for every chunk of 64 x kGroups x 16 bytes: of one
-// workgroup, which joins them in LDS, or, beyond 16, of several, with a second launch to put the parts together.
-Split split_of(const RowsShape& shape, int entry_bytes) {
-  const int64_t rows = shape.rows(), chunk = 64 * kGroups * 16 / entry_bytes, chunks = (shape.cats + chunk - 1) / chunk;
-  const int64_t wanted = std::min((4096 + rows - 1) / rows, chunks);
+// Rows that are fewer than keep the memory busy get several waves, up to one for every chunk: of one workgroup, which joins them in
+// LDS, or of several, with a second launch to put the parts together.  Waves cost little where there are only sums (4096 rows of
+// 131072 bf16 scores: 203 us with one wave a row, 184 with four, 230 with sixteen); a list of the likeliest costs each of them its start
+// (8 likeliest: 206, 245 with two waves a row; 1000 rows of 50021 with 20: 71 with four, 90 with eight).
+Split split_of(const RowsShape& shape, bool top) {
+  const int64_t rows = shape.rows(), chunks = (shape.cats + kChunk - 1) / kChunk;
+  const int64_t wanted = std::min(((top ? 2560 : 16384) + rows - 1) / rows, chunks);
+  const int most = top ? kMaxWaves / 2 : kMaxWaves;
   Split s{1, 1, shape.cats};
-  if (wanted <= kMaxWaves) {
-    while (s.waves < wanted) s.waves *= 2;
+  if (wanted <= 2 * most) {
+    while (s.waves < std::min<int64_t>(wanted, most)) s.waves *= 2;
     return s;
   }
   s.waves = wanted > 8 * kMaxParts ? kMaxWaves : 8;
   const int64_t parts = std::min<int64_t>(kMaxParts, (wanted + s.waves - 1) / s.waves);
-  s.part_len = (int)((chunks + parts - 1) / parts * chunk);
+  s.part_len = (int)((chunks + parts - 1) / parts * kChunk);
   s.parts = (int)((shape.cats + s.part_len - 1) / s.part_len);
   return s;
 }
@@ -309,41 +401,37 @@ template <typename T>
 void launch_stream(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, const CkptRef& ckpt, void* work,
                    hipStream_t stream) {
   if (category_scores_short<T>(x, shape, given, top, out, ckpt, stream)) return;
-  const Split s = split_of(shape, sizeof(T));
+  const Split s = split_of(shape, top > 0);
   PartRef part{};
   if (s.parts > 1) {
     part.sums = static_cast<float4*>(work);
     part.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(work) + up16((size_t)shape.rows() * s.parts * sizeof(float4)));
   }
   const dim3 grid((unsigned)std::min<int64_t>(shape.rows() * s.parts, 1 << 20)), block(64 * s.waves);
-  const int lds = s.waves * (128 * 8 + 16);
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, x, shape, given, top, out, ckpt, s.parts, s.part_len, part); };
   const bool ent = out.entropy != nullptr;
-  if (x.stride_cat != 1) {
-    if (top) ent ? launch(score_stream_kernel<T, false, true, true, false>) : launch(score_stream_kernel<T, false, false, true, false>);
-    else ent ? launch(score_stream_kernel<T, false, true, false, false>) : launch(score_stream_kernel<T, false, false, false, false>);
-  } else if (ckpt.codes) {
-    if (top) ent ? launch(score_stream_kernel<T, true, true, true, true>) : launch(score_stream_kernel<T, true, false, true, true>);
-    else ent ? launch(score_stream_kernel<T, true, true, false, true>) : launch(score_stream_kernel<T, true, false, false, true>);
-  } else {
-    if (top) ent ? launch(score_stream_kernel<T, true, true, true, false>) : launch(score_stream_kernel<T, true, false, true, false>);
-    else ent ? launch(score_stream_kernel<T, true, true, false, false>) : launch(score_stream_kernel<T, true, false, false, false>);
-  }
+  // A list of the likeliest per wave pays over many chunks, as its bar rises; one of all waves costs each of them little
+  const int lists = !top ? kNoList : s.waves > 1 && s.part_len <= (int64_t)kOneListChunks * s.waves * kChunk ? kOneList : kListPerWave;
+  const int lds = s.waves * (128 * 8 + 16 + (lists == kOneList ? kRoom * 8 : 0));
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, x, shape, given, top, out, ckpt, s.parts, s.part_len, part); };
+  auto choose = [&](auto unit, auto keep) {
+    constexpr bool kUnit = decltype(unit)::value, kCkpt = decltype(keep)::value;
+    if (lists == kNoList) ent ? launch(score_stream_kernel<T, kUnit, true, kNoList, kCkpt>) : launch(score_stream_kernel<T, kUnit, false, kNoList, kCkpt>);
+    else if (lists == kListPerWave) ent ? launch(score_stream_kernel<T, kUnit, true, kListPerWave, kCkpt>) : launch(score_stream_kernel<T, kUnit, false, kListPerWave, kCkpt>);
+    else ent ? launch(score_stream_kernel<T, kUnit, true, kOneList, kCkpt>) : launch(score_stream_kernel<T, kUnit, false, kOneList, kCkpt>);
+  };
+  if (x.stride_cat != 1) choose(std::false_type(), std::false_type());
+  else if (ckpt.codes) choose(std::true_type(), std::true_type());
+  else choose(std::true_type(), std::false_type());
   if (s.parts > 1)
     hipLaunchKernelGGL((score_join_kernel<T>), dim3((unsigned)shape.rows()), dim3(256), 0, stream, x, shape, given, top, out, s.parts, part);
 }
 }  // namespace
 
-// (whatever the type and the strides: what the entries of four bytes need, or those of two)
 int64_t category_scores_workspace(const RowsShape& shape, int top) {
   if (shape.examples < 1 || shape.vars < 1 || shape.cats < 1 || top < 0 || top > kMaxSlots || shape.examples > INT64_C(0x7fffffff) / shape.vars) return 0;
-  int64_t most = 0;
-  for (int bytes = 2; bytes <= 4; bytes += 2) {
-    const Split s = split_of(shape, bytes);
-    const size_t jobs = (size_t)shape.rows() * s.parts;
-    if (s.parts > 1) most = std::max(most, (int64_t)(up16(jobs * sizeof(float4)) + jobs * top * sizeof(uint64_t)));
-  }
-  return most;
+  const Split s = split_of(shape, top > 0);
+  const size_t jobs = (size_t)shape.rows() * s.parts;
+  return s.parts == 1 ? 0 : (int64_t)(up16(jobs * sizeof(float4)) + jobs * top * sizeof(uint64_t));
 }
 
 void category_scores(const RowsRef& x_in, const RowsShape& shape_in, const GivenRef& given, int top, float* d_logp, float* d_log_sum,
