@@ -27,6 +27,7 @@ struct GivenRef {                     // categories per row, [example][variable]
   int type;                           // PCM_U8, PCM_I32, PCM_I64
   int64_t stride_ex, stride_var, stride_slot;
   int32_t slots;
+  int32_t vars = 1;                   // for a kernel that takes examples and variables as one axis: the latter's number
 };
 struct CkptRef {                      // codes [rows][pitch], scales [rows][blocks]
   uint8_t* codes;

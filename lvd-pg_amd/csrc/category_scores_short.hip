@@ -1,9 +1,16 @@
-// Short rows of scores, and rows that lie side by side (stride 1 from row to row, as a forest's forward pass leaves them).
+// Short rows of scores, many rows, and rows that lie side by side (stride 1 from row to row, as a forest's forward pass leaves them).
 #include "category_stats.hip.hpp"
 
 namespace pcm {
 
 namespace {
+// Rows of neighbouring categories that go a lane each: as many as fill the device with 64 a wave.  Times in us, a lane a row / 16 lanes a
+// row (up to 256 categories) or a wave a row: 65536 rows of 128 (f32, 4 likeliest) 17 / 17, 262144 37 / 59, 524288 66 / 113; 32768 rows of
+// 512 24 / 56, 65536 of 1000 68 / 118, 65536 of 2000 (bf16) 85 / 144, 8192 of 2000 43 / 24.
+constexpr int kShortCats = 256;
+constexpr int64_t kLaneRowsShort = 65536, kLaneRows = 32768;   // fewest rows, up to and beyond kShortCats categories
+constexpr int kLaneCats = 2048;                                // most categories
+
 // Rows of up to 256 neighbouring categories: 16 lanes a row, all of it in registers, four rows a wave.  A lane holds kGroups
 // times 16 bytes; the sums need no running maximum.  The likeliest are found one after the other: the largest entry of 16 lanes
 // (four steps), the lowest index that has it (four), and out it goes.
@@ -107,18 +114,22 @@ __global__ __launch_bounds__(256) void score_short_kernel(RowsRef x, RowsShape s
   }
 }
 
-// A lane per row: rows that lie side by side, and rows of a few categories.  `parts` waves share the categories of 64 rows and
-// meet in LDS; each lane keeps its sums and, sorted in, its kList likeliest.
-template <typename T, int kList>
-__global__ __launch_bounds__(1024) void score_column_kernel(RowsRef x, RowsShape shape, GivenRef given, int top, ScoreOut out, int parts,
-                                                            bool examples_first) {
-  constexpr int kStep = 8, kWords = 3 + 2 * kList;
-  extern __shared__ float column_lds[];   // [waves][kWords][64]
+// A lane per row: no step across lanes, and what a row costs once is shared by 64.  Rows that lie side by side are read as they are;
+// rows of neighbouring categories go through LDS, 128 bytes of each of the wave's 64 rows at a time (kStaged).  A lane takes kStep
+// entries: their maximum, their sums, and which of them lie above the last of its kList likeliest, kept sorted.  Those, a few once the
+// list has filled, are sorted in one of every lane at a time, a median and a comparison per place.  `parts` waves share the categories
+// of 64 rows and meet in LDS.
+template <typename T, int kList, bool kStaged>
+__global__ __launch_bounds__(kStaged ? 256 : 1024, kStaged ? kList > 4 ? 3 : 4 : 1) void score_lane_kernel(RowsRef x, RowsShape shape, GivenRef given, int top, ScoreOut out, int parts,
+                                                                         bool examples_first) {
+  constexpr int kStep = 16, kWords = 3 + 2 * kList, kVec = 16 / (int)sizeof(T), kTile = 8 * kVec, kPitch = 36;   // (words of a row in LDS)
+  extern __shared__ float lane_lds[];   // per wave a tile [64][kPitch] (kStaged); then, of several parts, [waves][kWords][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sets = (blockDim.x >> 6) / parts, set = wave / parts, q = wave % parts;
   const int64_t rows = shape.rows();
-  const int len = ((shape.cats + parts - 1) / parts + kStep - 1) / kStep * kStep;
+  const int len = ((shape.cats + parts - 1) / parts + kTile - 1) / kTile * kTile;
   const int first = min(q * len, shape.cats), end = min(first + len, shape.cats);
+  float* const tile = lane_lds + (size_t)wave * 64 * kPitch;
   for (int64_t n0 = (int64_t)blockIdx.x * sets * 64; n0 < rows; n0 += (int64_t)gridDim.x * sets * 64) {
     const int64_t at = n0 + set * 64 + lane;
     const bool mine = at < rows;
@@ -140,34 +151,113 @@ __global__ __launch_bounds__(1024) void score_column_kernel(RowsRef x, RowsShape
       value[j] = masked_from<T>();
       index[j] = -1;
     }
-    // behind those that are as large: they have lower indices
+    // behind those that are as large: they have lower indices (w lies above the last)
     auto sort_in = [&](float w, int32_t i) {
 #pragma unroll
-      for (int j = kList - 1; j >= 0; --j) {
-        const bool here = w > value[j], above = j > 0 && w > value[j ? j - 1 : 0];
-        value[j] = above ? value[j ? j - 1 : 0] : here ? w : value[j];
-        index[j] = above ? index[j ? j - 1 : 0] : here ? i : index[j];
+      for (int j = kList - 1; j > 0; --j) {
+        index[j] = w > value[j - 1] ? index[j - 1] : w > value[j] ? i : index[j];
+        value[j] = __builtin_amdgcn_fmed3f(w, value[j - 1], value[j]);
       }
+      index[0] = w > value[0] ? i : index[0];
+      value[0] = fmaxf(w, value[0]);
     };
-    for (int c0 = first; c0 < end; c0 += kStep) {
-      float y[kStep], largest = -INFINITY, s = 0.f, t = 0.f;
+    // the entries of a step, and one of them by its place
+    auto work = [&](const float (&y)[kStep], int c0, auto&& entry) {
+      float largest = y[0], s = 0.f, t = 0.f;
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) y[i] = c0 + i < end ? seen(row[(int64_t)(c0 + i) * x.stride_cat]) : -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) largest = fmaxf(largest, y[i]);
+      for (int i = 1; i < kStep; ++i) largest = __builtin_elementwise_maximum(largest, y[i]);
       if (largest > sum.m) sum.raise(largest);
+      if constexpr (kList > 0) {
+        uint32_t hit = 0;
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) hit |= y[i] > value[kList - 1] ? 1u << i : 0u;
+        if (__any(__popc(hit) > kStep / 2)) {        // (a list that fills, entries that rise)
+#pragma unroll
+          for (int i = 0; i < kStep; ++i)
+            if (y[i] > value[kList - 1]) sort_in(y[i], c0 + i);
+          hit = 0;
+        }
+        while (hit) {
+          const int i = __builtin_ctz(hit);
+          hit &= hit - 1;
+          const float w = entry(i);
+          if (w > value[kList - 1]) sort_in(w, c0 + i);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kStep; ++i) sum.template add<true>(y[i], s, t);
       sum.s += s;
       sum.t += t;
-      if constexpr (kList > 0)
-        if (largest > value[kList - 1])
+    };
+    if constexpr (kStaged) {
+      // rows lie stride_ex apart (one variable); eight lanes hold 128 bytes of a row, a request eight rows
+      const int64_t r0 = n0 + set * 64;
+      const int in = (lane & 7) * kVec;
+      raw4 raw[8];
+      auto request = [&](int c0) {
 #pragma unroll
-          for (int i = 0; i < kStep; ++i)
-            if (y[i] > value[kList - 1]) sort_in(y[i], c0 + i);
+        for (int i = 0; i < 8; ++i) {
+          const int64_t r = min(r0 + i * 8 + (lane >> 3), rows - 1);
+          const T* const from = static_cast<const T*>(x.p) + r * x.stride_ex;
+          if (c0 + in + kVec <= end) raw[i] = load16(from + c0 + in);
+          else {
+            T w[kVec];
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) w[k] = c0 + in + k < end ? from[c0 + in + k] : (T)-INFINITY;
+            raw[i] = __builtin_bit_cast(raw4, w);
+          }
+        }
+      };
+      if (first < end) request(first);
+      for (int c0 = first; c0 < end; c0 += kTile) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<raw4*>(tile + (i * 8 + (lane >> 3)) * kPitch + (lane & 7) * 4) = raw[i];
+        __builtin_amdgcn_wave_barrier();
+        if (c0 + kTile < end) request(c0 + kTile);
+        const float* const own = tile + lane * kPitch;
+#pragma unroll 1
+        for (int h = 0; h < kTile && c0 + h < end; h += kStep) {
+          const float* const half = own + h * (int)sizeof(T) / 4;
+          float y[kStep];
+#pragma unroll
+          for (int i = 0; i < kStep / kVec; ++i) {
+            float z[kVec];
+            unpack(*reinterpret_cast<const raw4*>(half + 4 * i), z, T());
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) y[i * kVec + k] = z[k];
+          }
+          work(y, c0 + h, [&](int i) { return seen(reinterpret_cast<const T*>(half)[i]); });
+        }
+      }
+    } else {
+      float y[kStep];
+      T next[kStep];
+      auto request = [&](int c0) {
+        const T* const from = row + (int64_t)c0 * x.stride_cat;
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) next[i] = c0 + i < end ? from[(int64_t)i * x.stride_cat] : (T)-INFINITY;
+      };
+      request(first);
+      for (int c0 = first; c0 < end; c0 += kStep) {
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) y[i] = seen(next[i]);
+        request(c0 + kStep);
+        work(y, c0, [&](int i) {
+          float a[kStep];
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) a[k] = y[k];
+#pragma unroll
+          for (int w = kStep / 2; w > 0; w /= 2)
+#pragma unroll
+            for (int k = 0; k < w; ++k) a[k] = i & w ? a[k + w] : a[k];
+          return a[0];
+        });
+      }
     }
     if (parts > 1) {
-      float* const own = column_lds + (size_t)wave * kWords * 64 + lane;
+      __syncthreads();                      // (tiles are done with)
+      float* const own = lane_lds + (size_t)wave * kWords * 64 + lane;
       if (q > 0) {
         own[0] = sum.m;
         own[64] = sum.s;
@@ -193,21 +283,23 @@ __global__ __launch_bounds__(1024) void score_column_kernel(RowsRef x, RowsShape
           if (m > other.m) other.raise(m);
           sum.s += other.s;
           sum.t += other.t;
+          if constexpr (kList > 0)
 #pragma unroll 1
-          for (int j = 0; j < kList; ++j) {
-            const float w = o[(3 + j) * 64];
-            if (w > value[kList ? kList - 1 : 0]) sort_in(w, __builtin_bit_cast(int32_t, o[(3 + kList + j) * 64]));
-          }
+            for (int j = 0; j < kList; ++j) {
+              const float w = o[(3 + j) * 64];
+              if (w > value[kList - 1]) sort_in(w, __builtin_bit_cast(int32_t, o[(3 + kList + j) * 64]));
+            }
         }
       }
-      __syncthreads();   // (the next rows' sums go where these were read)
+      __syncthreads();   // (the next rows' tiles and sums go where these were read)
     }
     if (q == 0 && mine) {
       const RowResult<T> res(sum);
       const int64_t r = (int64_t)e * shape.vars + v;
+      const int64_t ge = kStaged && given.vars > 1 ? r / given.vars : e, gv = kStaged && given.vars > 1 ? r - ge * given.vars : v;
       for (int j = 0; j < given.slots; ++j)
         out.logp[r * given.slots + j] =
-            res.given(given_at(given, e, v, j), shape.cats, [&](int64_t g) { return seen(row[g * x.stride_cat]); });
+            res.given(given_at(given, ge, gv, j), shape.cats, [&](int64_t g) { return seen(row[g * x.stride_cat]); });
       if (out.log_sum) out.log_sum[r] = res.log_sum();
       if (out.entropy) out.entropy[r] = res.entropy(sum);
 #pragma unroll
@@ -230,33 +322,46 @@ void launch_short(const RowsRef& x, const RowsShape& shape, const GivenRef& give
 }
 
 template <typename T, int kList>
-void launch_column(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, hipStream_t stream) {
+void launch_lane(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, bool staged, hipStream_t stream) {
   const int64_t sets = (shape.rows() + 63) / 64;
-  const int most = kList > 8 ? 4 : kList > 4 ? 8 : 16;   // (LDS)
+  const int most = staged || kList > 8 ? 4 : kList > 4 ? 8 : 16;   // (LDS)
   int parts = 1;
-  while (parts < most && sets * parts < 4096 && shape.cats / parts >= 32) parts *= 2;
+  while (parts < most && sets * parts < 4096 && shape.cats / parts >= 64) parts *= 2;
   const int waves = std::max(4, parts), per = waves / parts;
-  const int lds = parts > 1 ? waves * (3 + 2 * kList) * 64 * 4 : 0;
+  const int lds = std::max(staged ? waves * 64 * 36 * 4 : 0, parts > 1 ? waves * (3 + 2 * kList) * 64 * 4 : 0);
   const bool examples_first = shape.vars > 1 && (x.stride_ex == 1 || x.stride_ex == -1);
-  hipLaunchKernelGGL((score_column_kernel<T, kList>), dim3((unsigned)std::min<int64_t>((sets + per - 1) / per, 1 << 20)), dim3(64 * waves), lds,
-                     stream, x, shape, given, top, out, parts, examples_first);
+  const dim3 grid((unsigned)std::min<int64_t>((sets + per - 1) / per, 1 << 20)), block(64 * waves);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, x, shape, given, top, out, parts, examples_first); };
+  staged ? launch(score_lane_kernel<T, kList, true>) : launch(score_lane_kernel<T, kList, false>);
 }
 }  // namespace
 
 template <typename T>
 bool category_scores_short(const RowsRef& x, const RowsShape& shape, const GivenRef& given, int top, const ScoreOut& out, const CkptRef& ckpt,
                            hipStream_t stream) {
+  if (top > 16) return false;
   const bool neighbours = x.stride_cat == 1;
   const bool side_by_side = !neighbours && ((shape.examples > 1 && std::abs(x.stride_ex) == 1) || (shape.vars > 1 && std::abs(x.stride_var) == 1));
-  if (top > 16) return false;
-  if (side_by_side || (shape.cats <= 16 && !ckpt.codes)) {
-    if (top == 0) launch_column<T, 0>(x, shape, given, top, out, stream);
-    else if (top <= 4) launch_column<T, 4>(x, shape, given, top, out, stream);
-    else if (top <= 8) launch_column<T, 8>(x, shape, given, top, out, stream);
-    else launch_column<T, 16>(x, shape, given, top, out, stream);
+  // rows of neighbouring categories one stride apart: their examples and variables are one axis
+  const bool even = shape.vars == 1 || x.stride_ex == (int64_t)shape.vars * x.stride_var;
+  const bool staged = neighbours && even && shape.cats > 16 && shape.cats <= kLaneCats &&
+                      shape.rows() >= (shape.cats <= kShortCats ? kLaneRowsShort : kLaneRows) && !ckpt.codes;
+  if (side_by_side || staged || (shape.cats <= 16 && !ckpt.codes)) {
+    RowsRef y = x;
+    RowsShape one = shape;
+    GivenRef g = given;
+    if (staged) {
+      g.vars = shape.vars;
+      y.stride_ex = shape.vars == 1 ? x.stride_ex : x.stride_var;
+      one = {shape.rows(), 1, shape.cats};
+    }
+    if (top == 0) launch_lane<T, 0>(y, one, g, top, out, staged, stream);
+    else if (top <= 4) launch_lane<T, 4>(y, one, g, top, out, staged, stream);
+    else if (top <= 8) launch_lane<T, 8>(y, one, g, top, out, staged, stream);
+    else launch_lane<T, 16>(y, one, g, top, out, staged, stream);
     return true;
   }
-  if (!neighbours || shape.cats > 256) return false;
+  if (!neighbours || shape.cats > kShortCats) return false;
   constexpr int kGroup = 256 / (int)sizeof(T);   // categories of 16 lanes times 16 bytes
   if (shape.cats <= kGroup) launch_short<T, 1>(x, shape, given, top, out, ckpt, stream);
   else if (shape.cats <= 2 * kGroup) launch_short<T, 2>(x, shape, given, top, out, ckpt, stream);

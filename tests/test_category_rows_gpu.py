@@ -160,6 +160,37 @@ def test_given_of_every_type_and_number(gpu, type_):
         assert (P.category_scores(x, -g).logp == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(65537, 17), (65600, 33), (65536, 130), (32769, 257), (32800, 511), (32768, 1100)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_scores_of_many_short_rows(gpu, dtype, shape):
+    """A lane a row: the last rows of a wave, of a workgroup, and rows whose list keeps changing"""
+    torch, P = gpu
+    n, C = shape
+    kinds = ("plain", "masked", "ties", "rising", "falling", "nan", "lowest")
+    x = torch.cat([_scores(torch, dtype, (n // 7 + 1, C), 61 + k, kind) for k, kind in enumerate(kinds)])[:n].cuda()
+    x = x[torch.randperm(n, generator=torch.Generator().manual_seed(1)).cuda()]      # kinds side by side
+    given = torch.randint(0, C, (n,), generator=torch.Generator().manual_seed(2)).cuda()
+    for top in (0, 1, 4, 7, 16):
+        s = P.category_scores(x, given, top=top, entropy=True)
+        few = slice(None) if top == 4 else slice(n - 300, n)                          # all of them once, the last ones always
+        t = P.category_scores(x[few][:300], given[few][:300], top=top, entropy=True)
+        _check(torch, P, x[few][-300:], dtype, given[few][-300:], top)
+        for a, b in zip(s[:5], t[:5]):
+            if a is not None:
+                a = a[few][:300]
+                if a.dtype == torch.int32:
+                    assert torch.equal(a, b)
+                else:                                                                 # another order of the same sums
+                    assert torch.equal(torch.isfinite(a), torch.isfinite(b))
+                    assert (torch.nan_to_num(a, 0, 0, 0) - torch.nan_to_num(b, 0, 0, 0)).abs().max() < 5e-5
+    if C == 130:
+        v = x.view(256, 256, C)
+        g = given.view(256, 256).t().contiguous().t()                                # given of other strides than the rows
+        s = P.category_scores(v, g, top=3)
+        t = P.category_scores(x, given, top=3)
+        assert torch.equal(s.top.view(-1, 3), t.top) and torch.equal(torch.nan_to_num(s.logp.reshape(-1), 7), torch.nan_to_num(t.logp, 7))
+
+
 def test_no_rows(gpu):
     torch, P = gpu
     x = torch.zeros((0, 10), device="cuda")
