@@ -489,8 +489,8 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  * circuit or a forest, the logits of a network that a circuit is distilled from.  No counterpart in the reference, which
  * does this part in its Python programs.  Element (example e, variable v, category c) of an array of scores is at
  * x[e * stride_ex + v * stride_var + c * stride_cat]: element strides, any sign, also 0; num_vars = 1 for plain rows.
- * A score at or below half of its type's lowest value is a mask and counts as -inf (as well -inf itself, as what adding a mask
- * of the lowest value leaves).  With Z = sum_c exp x[c] over a row:
+ * A score at or below half of its type's lowest value is a mask and counts as -inf: -inf itself, and what adding a
+ * mask of the lowest value leaves.  With Z = sum_c exp x[c] over a row:
  *
  * pcm_category_scores.  d_given [examples][variables][num_given] (its own element strides; PCM_U8, PCM_I32, PCM_I64):
  *   d_logp [rows][num_given]   x[g] - log Z; 0 where g < 0 (not observed: probability 1, as a missing value counts in a
@@ -500,7 +500,8 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  *   d_top, d_top_logp [rows][top]  the likeliest categories and their log-probabilities, equal scores by rising category; a
  *                              category of score -inf is never among them: -1 and -inf stand where a row has no more
  *   d_codes, d_scales          the row's checkpoint as pcm_checkpoint_rows writes it, in the same pass (both NULL: none)
- * A row of nothing but masks: log Z = -inf, logp = -inf, entropy 0.  A row with NaN or +inf: NaN, no categories (-1).
+ * A row of nothing but masks: log Z = -inf, logp = -inf, no categories (-1) and, being no distribution, entropy NaN.  A row with NaN,
+ * +inf or a score beyond 2^127: NaN, no categories (-1).
  * At most 64 given and 64 likeliest categories a row, 2^30 categories, 2^31 - 1 rows.  d_work: pcm_category_scores_workspace bytes of device
  * memory (0: none) that belong to the call until its work is done; 16-byte aligned.
  *

@@ -62,7 +62,7 @@ struct RowResult {
     z = q.m + fmaf(fmaf(-q.m, kLog2e, q.c), kLn2, ls);
   }
   __device__ __forceinline__ float log_sum() const { return nan ? NAN : none ? -INFINITY : z; }
-  __device__ __forceinline__ float entropy(const RowSums<T>& q) const { return nan ? NAN : none ? 0.f : fmaf(-q.t / q.s, kLn2, ls); }
+  __device__ __forceinline__ float entropy(const RowSums<T>& q) const { return nan || none ? NAN : fmaf(-q.t / q.s, kLn2, ls); }
   __device__ __forceinline__ float logp(float x) const {   // of an entry of the row that is seen as x
     return nan ? NAN : none || x <= masked_from<T>() ? -INFINITY : fmaf(fmaf(x, kLog2e, -c), kLn2, -ls);
   }

@@ -29,7 +29,7 @@ def statistics(x):
         p = np.exp(lp)
         h = -np.where(p > 0, p * lp, 0.0).sum(1)
         z = safe + ls
-        h[ls == -np.inf] = 0.0
+        h[ls == -np.inf] = np.nan                    # no distribution
         z[bad] = np.nan
         h[bad] = np.nan
     return z, h
@@ -87,6 +87,7 @@ def gradient(x, z, h, slots, gh=None):
         size += p * weight[:, None] * slack
         under = np.broadcast_to(weight[:, None], out.shape).copy()
         if gh is not None:
+            h = np.nan_to_num(h)
             out -= np.where(p > 0, gh[:, None] * p * (d + h[:, None]), 0.0)
             term = np.abs(gh[:, None]) * (np.minimum(np.abs(d), 200.0) + np.abs(h[:, None]) + 1.0)
             size += np.where(p > 0, p * term * slack, 0.0)
