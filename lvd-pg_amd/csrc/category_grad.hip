@@ -48,19 +48,18 @@ struct GradRow {
   }
 };
 
-// Rows of neighbouring categories in and out.  The slots of the workgroup's rows wait in LDS; of a long row only those in the
-// workgroup's segment, in their order, so that sums come out the same every time.
+// Rows of neighbouring categories in and out.  Where a wave holds one row (64 lanes a row or more), its slots wait in the wave's lanes, and a
+// group of the row asks once which of them it holds: none, mostly.  Slots of shorter rows wait in LDS.  Either way they are added in
+// their order, so that sums come out the same every time.
 template <typename T, bool kCkpt, bool kEnt>
 __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, Tiles tiles) {
   constexpr int kVec = 16 / (int)sizeof(T);
   __shared__ GradSlot slot_lds[kStaged];
-  __shared__ float total_lds[kTileThreads];
-  __shared__ int near_lds;
-  const int slots = in.given.slots + in.top, per = kTileThreads >> tiles.lanes_log2, of = threadIdx.x >> tiles.lanes_log2;
+  const int slots = in.given.slots + in.top, per = kTileThreads >> tiles.lanes_log2, of = threadIdx.x >> tiles.lanes_log2, lane = threadIdx.x & 63;
   const int64_t rows = shape.rows();
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
   for (int64_t job = blockIdx.x; job < tiles.jobs; job += gridDim.x) {
-    const TileAt tile = tile_at(tiles, job);
+    TileAt tile = tile_at(tiles, job);
     const bool mine = tile.row < rows;
     const uint32_t r = (uint32_t)(mine ? tile.row : rows - 1);
     const int64_t e = shape.vars == 1 ? r : r / (uint32_t)shape.vars, v = shape.vars == 1 ? 0 : r % (uint32_t)shape.vars;
@@ -70,92 +69,93 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
     raw4 raw[kCkpt ? 1 : kTileGroups];
     Codes<kVec> code[kCkpt ? kTileGroups : 1];
     uint32_t unit[kCkpt ? kTileGroups : 1];
+    auto request = [&] {
 #pragma unroll
-    for (int u = 0; u < kTileGroups; ++u) {
-      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
-      if (c >= shape.cats) continue;
-      if constexpr (kCkpt) {
-        code[u] = load_codes<kVec>(ckpt.codes + r * pitch + c);
-        unit[u] = ckpt.scales[r * blocks + c / kCkptBlock];
-      } else raw[u] = load_group(row, c, shape.cats);
-    }
+      for (int u = 0; u < kTileGroups; ++u) {
+        const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+        if (c >= shape.cats) continue;
+        if constexpr (kCkpt) {
+          code[u] = load_codes<kVec>(ckpt.codes + r * pitch + c);
+          unit[u] = ckpt.scales[r * blocks + c / kCkptBlock];
+        } else raw[u] = load_group(row, c, shape.cats);
+      }
+    };
+    request();
 
-    int near = slots;   // slots to look at, from near_at on
-    const GradSlot* near_at = slot_lds + of * slots;
     float total = 0.f;
-    if (slots) {
-      if (per == 1) {
-        // wave 0: slots by the lane, twice; the others wait for what it leaves
-        if (threadIdx.x < 64) {
-          const int lane = threadIdx.x, low = (tile.first - lane) * kVec, high = low + kTileGroups * tile.step * kVec;
-          int found = 0;
-          float sum = 0.f;
-          for (int j0 = 0; j0 < slots; j0 += 64) {
-            bool past = false;
-            GradSlot s{-1, 0.f};
-            if (j0 + lane < slots) s = grad_slot(in, r, e, v, j0 + lane, shape.cats, past);
-            sum += past ? NAN : s.at >= 0 ? s.by : 0.f;
-            const bool here = s.at >= low && s.at < high;
-            const uint64_t all = __ballot(here);
-            if (here) slot_lds[found + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0))] = s;
-            found += __popcll(all);
-          }
-          sum = over_lanes<64>(sum, Sum());
-          if (lane == 0) {
-            total_lds[0] = sum;
-            near_lds = found;
-          }
+    GradSlot own[2] = {{-1, 0.f}, {-1, 0.f}};   // slots lane and 64 + lane
+    if (slots && per <= 4) {
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (64 * h + lane < slots) {
+          bool past;
+          own[h] = grad_slot(in, r, e, v, 64 * h + lane, shape.cats, past);
+          sum += past ? NAN : own[h].at >= 0 ? own[h].by : 0.f;
         }
-        __syncthreads();
-        total = total_lds[0];
-        near = near_lds;
-        near_at = slot_lds;
-      } else {
-        const int64_t r0 = job * per;   // (one segment a row)
-        if (threadIdx.x < per) total_lds[threadIdx.x] = 0.f;
-        for (int i = threadIdx.x; i < per * slots; i += kTileThreads) {
-          const int64_t q = r0 + i / slots;
-          GradSlot s{-1, 0.f};
-          if (q < rows) {
-            bool past;
-            const int64_t qe = shape.vars == 1 ? q : (uint32_t)q / (uint32_t)shape.vars;
-            s = grad_slot(in, q, qe, q - qe * shape.vars, i % slots, shape.cats, past);
-            if (past) s = {-2, 0.f};
-          }
-          slot_lds[i] = s;
+      total = over_lanes<64>(sum, Sum());
+    } else if (slots) {
+      const int64_t r0 = job * per;   // (one segment a row)
+      for (int i = threadIdx.x; i < per * slots; i += kTileThreads) {
+        const int64_t q = r0 + i / slots;
+        GradSlot s{-1, 0.f};
+        if (q < rows) {
+          bool past;
+          const int64_t qe = shape.vars == 1 ? q : (uint32_t)q / (uint32_t)shape.vars;
+          s = grad_slot(in, q, qe, q - qe * shape.vars, i % slots, shape.cats, past);
+          if (past) s = {-2, 0.f};
         }
-        __syncthreads();
-        for (int j = 0; j < slots; ++j) {
-          const GradSlot s = near_at[j];
-          total += s.at >= 0 ? s.by : s.at == -2 ? NAN : 0.f;
-        }
+        slot_lds[i] = s;
+      }
+      __syncthreads();
+      for (int j = 0; j < slots; ++j) {
+        const GradSlot s = slot_lds[of * slots + j];
+        total += s.at >= 0 ? s.by : s.at == -2 ? NAN : 0.f;
       }
     }
     const GradRow grad(in, r, total);
-    if (grad.none()) near = 0;
+    const bool add = slots && !grad.none();
+    for (int turn = 0;; ++turn) {
 #pragma unroll
-    for (int u = 0; u < kTileGroups; ++u) {
-      const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
-      if (c >= shape.cats) continue;
-      float y[kVec];
-      if constexpr (kCkpt) decode(code[u], block_unit(unit[u]), y);
-      else unpack(raw[u], y, T());
+      for (int u = 0; u < kTileGroups; ++u) {
+        const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+        uint64_t here[2] = {0, 0};     // slots in the wave's part of the row (asked by all of its lanes)
+        if (add && per <= 4) {
+          const uint32_t c0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)c);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) y[i] = grad.template at<kEnt>(y[i]);
-      for (int j = 0; j < near; ++j) {
-        const uint32_t i = (uint32_t)near_at[j].at - (uint32_t)c;
-        if (i < (uint32_t)kVec) {
-          const float by = near_at[j].by;
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) y[k] += i == (uint32_t)k ? by : 0.f;
+          for (int h = 0; h < 2; ++h) here[h] = __ballot((uint32_t)own[h].at - c0 < (uint32_t)(64 * kVec));
         }
-      }
-      T w[kVec];
+        if (c >= shape.cats) continue;
+        float y[kVec];
+        if constexpr (kCkpt) decode(code[u], block_unit(unit[u]), y);
+        else unpack(raw[u], y, T());
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) w[i] = from_float<T>(y[i]);
-      if (mine) store_group(dst, c, shape.cats, w);
+        for (int i = 0; i < kVec; ++i) y[i] = grad.template at<kEnt>(y[i]);
+        auto add_slot = [&](int at, float by) {
+          const uint32_t i = (uint32_t)at - (uint32_t)c;
+          if (i < (uint32_t)kVec)
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) y[k] += i == (uint32_t)k ? by : 0.f;
+        };
+        if (per <= 4) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            for (uint64_t left = here[h]; left; left &= left - 1) {
+              const int j = __builtin_ctzll(left);
+              add_slot(__builtin_amdgcn_readlane(own[h].at, j), as_float(__builtin_amdgcn_readlane(__builtin_bit_cast(int, own[h].by), j)));
+            }
+        } else if (add)
+          for (int j = 0; j < slots; ++j) add_slot(slot_lds[of * slots + j].at, slot_lds[of * slots + j].by);
+        T w[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) w[i] = from_float<T>(y[i]);
+        if (mine) store_group(dst, c, shape.cats, w);
+      }
+      if (turn + 1 == tiles.turns) break;
+      tile.first += kTileGroups * tile.step;
+      request();
     }
-    if (slots) __syncthreads();   // (the next rows' slots go where these are read)
+    if (slots && per > 4) __syncthreads();   // (the next rows' slots go where these are read)
   }
 }
 
@@ -226,7 +226,7 @@ template <typename T>
 void launch_grad(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, const GradIn& in, const RowsRef& out, hipStream_t stream) {
   const int slots = in.given.slots + in.top;
   if (out.stride_cat == 1 && (ckpt.codes || x.stride_cat == 1)) {
-    const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), (slots * kTileThreads + kStaged - 1) / kStaged);
+    const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), (slots * kTileThreads + kStaged - 1) / kStaged, 8192);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, tile_grid(t), dim3(kTileThreads), 0, stream, x, ckpt, shape, in, out, t); };
     const bool ent = in.grad_entropy != nullptr;
     if (ckpt.codes) ent ? launch(grad_tile_kernel<T, true, true>) : launch(grad_tile_kernel<T, true, false>);

@@ -1,5 +1,6 @@
 // How the kernels that turn rows into rows, entry by entry, deal them out: G lanes a row (a power of two, up to the workgroup's 256),
-// each with up to kTileGroups groups of 16 bytes; a workgroup holds 256 / G short rows, or one of the `segments` of a long one.
+// each with up to kTileGroups groups of 16 bytes at a time; a workgroup holds 256 / G short rows, or one of the `segments` of a long
+// one, in `turns`.
 #pragma once
 
 #include "category_rows.hpp"
@@ -11,15 +12,18 @@ constexpr int kTileThreads = 256, kTileGroups = 4;
 struct Tiles {
   int lanes_log2;      // log2 G
   int segments;        // of a row
+  int turns;           // of a segment
   int64_t jobs;        // workgroups' worth of work
 };
-// `vec` entries a group, at least `least` lanes a row
-inline Tiles tiles_of(const RowsShape& shape, int vec, int least) {
+// `vec` entries a group, at least `least` lanes a row; a segment takes several turns where there are more than `wanted_jobs` jobs without
+inline Tiles tiles_of(const RowsShape& shape, int vec, int least, int64_t wanted_jobs = INT64_MAX) {
   const int64_t groups = ((int64_t)shape.cats + vec - 1) / vec, wanted = (groups + kTileGroups - 1) / kTileGroups;
-  Tiles t{0, 1, 0};
+  Tiles t{0, 1, 1, 0};
   while ((1 << t.lanes_log2) < kTileThreads && (1 << t.lanes_log2) < std::max<int64_t>(wanted, least)) ++t.lanes_log2;
   const int64_t held = (int64_t)kTileGroups << t.lanes_log2;
-  t.segments = (int)((groups + held - 1) / held);
+  const int64_t all = (groups + held - 1) / held, rows = std::max<int64_t>(shape.rows(), 1);
+  t.turns = (int)std::max<int64_t>(1, all / std::max<int64_t>(1, (std::min(wanted_jobs, rows * all) + rows - 1) / rows));
+  t.segments = (int)((all + t.turns - 1) / t.turns);
   const int64_t per = kTileThreads >> t.lanes_log2;
   t.jobs = (shape.rows() + per - 1) / per * t.segments;
   return t;
@@ -35,7 +39,7 @@ __device__ __forceinline__ TileAt tile_at(const Tiles& t, int64_t job) {
   const int lanes = 1 << t.lanes_log2, in = threadIdx.x & (lanes - 1), of = threadIdx.x >> t.lanes_log2;
   if (t.segments == 1) return {(job << (8 - t.lanes_log2)) + of, in, lanes};
   const int64_t row = job / t.segments;   // (one row a workgroup)
-  return {row, (int)(job - row * t.segments) * kTileGroups * lanes + in, lanes};
+  return {row, (int)(job - row * t.segments) * t.turns * kTileGroups * lanes + in, lanes};
 }
 
 // A group of 16 bytes from categories c.. of a row of `cats`; -inf behind its end
