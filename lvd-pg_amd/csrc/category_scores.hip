@@ -132,16 +132,16 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
         else k.g[u] = row[(int64_t)(at + u * 64 + lane) * x.stride_cat];
       }
     };
-    auto load_end = [&](Chunk& k, int at) {                   // the last one: -inf behind the end
+    auto load_end = [&](Chunk& k, int at) {                   // the first or the last one: -inf before the start and behind the end
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
         const int c = at + (u * 64 + lane) * kVec;
         if constexpr (kUnit) {
-          if (c + kVec <= end) k.g[u] = load16(row + c);
+          if (c >= first && c + kVec <= end) k.g[u] = load16(row + c);
           else {
             T w[kVec];
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) w[i] = c + i < end ? row[c + i] : (T)-INFINITY;
+            for (int i = 0; i < kVec; ++i) w[i] = c + i >= first && c + i < end ? row[c + i] : (T)-INFINITY;
             k.g[u] = __builtin_bit_cast(raw4, w);
           }
         } else k.g[u] = c < end ? row[(int64_t)c * x.stride_cat] : (T)-INFINITY;
@@ -151,13 +151,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void score_stream_kernel(RowsRef x,
       if constexpr (kUnit) unpack(k.g[u], y, T());
       else y[0] = seen(k.g[u]);
     };
-    const int whole = (end - first) / kChunk, chunks = (end - first + kChunk - 1) / kChunk;
+    // Entries of two bytes: requests at multiples of 16 bytes, so that none straddles two lines (4096 rows of 50303: 97 us without, 75 of 50304).
+    // A checkpoint's blocks begin with the row.
+    const int start = kUnit && !kCkpt && sizeof(T) == 2 ? first - (int)((uintptr_t)(row + first) % 16 / sizeof(T)) : first;
+    const int chunks = (end - start + kChunk - 1) / kChunk;
     auto request = [&](Chunk& k, int j) {
-      if (j < whole) load(k, first + j * kChunk);
-      else if (j < chunks) load_end(k, first + j * kChunk);
+      const int at = start + j * kChunk;
+      if (at >= first && at + kChunk <= end) load(k, at);
+      else if (j < chunks) load_end(k, at);
     };
     auto work = [&](Chunk& k, int j) {
-      const int at = first + j * kChunk;
+      const int at = start + j * kChunk;
       float y[kLoads][kVec], largest[kLoads], lane_largest = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
