@@ -501,7 +501,7 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  *                              category of score -inf is never among them: -1 and -inf stand where a row has no more
  *   d_codes, d_scales          the row's checkpoint as pcm_checkpoint_rows writes it, in the same pass (both NULL: none)
  * A row of nothing but masks: log Z = -inf, logp = -inf, no categories (-1) and, being no distribution, entropy NaN.  A row with NaN,
- * +inf or a score beyond 2^127: NaN, no categories (-1).
+ * +inf: NaN, no categories (-1).
  * At most 64 given and 64 likeliest categories a row, 2^30 categories, 2^31 - 1 rows.  d_work: pcm_category_scores_workspace bytes of device
  * memory (0: none) that belong to the call until its work is done; 16-byte aligned.
  *

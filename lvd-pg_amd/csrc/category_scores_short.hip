@@ -47,10 +47,7 @@ __global__ __launch_bounds__(256) void score_short_kernel(RowsRef x, RowsShape s
 #pragma unroll
       for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, y[g][i]);
     largest = over_lanes<16>(largest, Larger());
-    if (largest > masked_from<T>()) {
-      sum.m = largest;
-      sum.c = largest * kLog2e;
-    }
+    if (largest > masked_from<T>()) sum.set(largest);
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g)
@@ -276,8 +273,7 @@ __global__ __launch_bounds__(kStaged ? 256 : 1024, kStaged ? kList > 4 ? 3 : 4 :
         for (int p = 1; p < parts; ++p) {
           const float* const o = own + (size_t)p * kWords * 64;
           RowSums<T> other;
-          other.m = o[0];
-          other.c = o[0] > masked_from<T>() ? o[0] * kLog2e : 0.f;
+          if (o[0] > masked_from<T>()) other.set(o[0]);
           other.s = o[64];
           other.t = o[128];
           if (m > other.m) other.raise(m);

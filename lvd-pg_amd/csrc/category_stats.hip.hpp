@@ -1,10 +1,12 @@
 // What the forward kernels on rows of scores share: sums of exponentials above a moving maximum, and results of a row.
 //
-// A row's sums are held relative to the running maximum m, in base 2: with c = m log2 e,
-//   s = sum 2^(x log2 e - c),   t = sum 2^(d) d, d = x log2 e - c,
+// A row's sums are held relative to the running maximum m, in base 2: with k = log2 e and c = m k,
+//   s = sum 2^(x k - c),   t = sum 2^(d) d, d = x k - c,
 // so that an entry costs one fused multiply-add, one exponential and two or three additions.  c is rounded, but it is the same
-// c in every term, and r = c - m log2 e is found exactly by one fused multiply-add at the end:
-//   log Z = m + r ln 2 + log s,   log p[g] = (x[g] log2 e - c) ln 2 - log s,   H = log s - t ln 2 / s.
+// c in every term, and r = c - m k is found exactly by one fused multiply-add at the end (u = ln 2):
+//   log Z = m + r u + log s,   log p[g] = (x[g] k - c) u - log s,   H = log s - t u / s.
+// From |m| = 2^30 on r could pass the range of the exponential.  There entries that are not m lie 64 or more below it and
+// count for nothing; k = u = 1 takes the differences exactly, and s becomes the number of entries that are m.
 // Entries that count as masks never move m off its start, masked_from<T>(), where c = 0 and their terms underflow to 0.
 #pragma once
 
@@ -23,27 +25,39 @@ bool category_scores_short(const RowsRef& x, const RowsShape& shape, const Given
                            hipStream_t stream);
 
 #ifdef __HIPCC__
+// (in every step below c is the product as rounded, never fused into what it is subtracted from)
 template <typename T>
 struct RowSums {
-  float m = masked_from<T>(), c = 0.f, s = 0.f, t = 0.f;
+  float m = masked_from<T>(), c = 0.f, k = kLog2e, s = 0.f, t = 0.f;
+  static __device__ __forceinline__ bool far(float m) { return masked_from<T>() < -1e30f && fabsf(m) >= 1073741824.f; }
+  __device__ __forceinline__ void set(float to) {     // m, where nothing is summed yet
+#pragma clang fp contract(off)
+    m = to;
+    k = far(to) ? 1.f : kLog2e;
+    c = to * k;
+  }
   __device__ __forceinline__ void raise(float to) {   // m and c to a larger maximum, the sums with them
-    const float c1 = to * kLog2e, dc = m > masked_from<T>() ? fmaxf(c - c1, -200.f) : -200.f, al = __builtin_amdgcn_exp2f(dc);
+#pragma clang fp contract(off)
+    const bool near = m > masked_from<T>() && !far(m) && !far(to);
+    const float c0 = c;
+    set(to);
+    const float dc = near ? fmaxf(c0 - c, -200.f) : -200.f, al = __builtin_amdgcn_exp2f(dc);
     t = al * (t + s * dc);
     s *= al;
-    m = to;
-    c = c1;
   }
   template <bool kEnt>
   __device__ __forceinline__ void add(float x, float& gs, float& gt) const {   // to a group's own sums
-    const float d = fmaf(x, kLog2e, -c), e = __builtin_amdgcn_exp2f(d);
+    const float d = fmaf(x, k, -c), e = __builtin_amdgcn_exp2f(d);
     gs += e;
     if (kEnt) gt = fmaf(e, fmaxf(d, -200.f), gt);   // (0 where e is: d may be -inf)
   }
   // the sums of a row from those that every lane of the wave holds (m, s, t) of other entries
   __device__ __forceinline__ void join_lanes(float4 o) {
+#pragma clang fp contract(off)
     m = over_lanes<64>(o.x, Larger());
-    c = m > masked_from<T>() ? m * kLog2e : 0.f;
-    const float d = o.x > masked_from<T>() ? fmaxf(o.x * kLog2e - c, -200.f) : -200.f, al = __builtin_amdgcn_exp2f(d);
+    if (m > masked_from<T>()) set(m);
+    const float d0 = o.x * kLog2e - c;
+    const float d = o.x == m ? 0.f : o.x > masked_from<T>() && !far(o.x) && !far(m) ? fmaxf(d0, -200.f) : -200.f, al = __builtin_amdgcn_exp2f(d);
     t = over_lanes<64>(al * (o.z + o.y * d), Sum());
     s = over_lanes<64>(o.y * al, Sum());
   }
@@ -52,19 +66,20 @@ struct RowSums {
 template <typename T>
 struct RowResult {
   bool nan, none;
-  float c, ls, z;
+  float c, k, u, ls, z;
   __device__ __forceinline__ explicit RowResult(const RowSums<T>& q) {
-    // (beyond 2^127 c would pass the range of float)
-    nan = !(q.s < INFINITY) || q.m > 1.7014118e38f;
+    nan = !(q.s < INFINITY);
     none = !nan && !(q.m > masked_from<T>());
     c = q.c;
+    k = q.k;
+    u = RowSums<T>::far(q.m) ? 1.f : kLn2;
     ls = logf(q.s);
-    z = q.m + fmaf(fmaf(-q.m, kLog2e, q.c), kLn2, ls);
+    z = q.m + fmaf(fmaf(-q.m, k, c), u, ls);
   }
   __device__ __forceinline__ float log_sum() const { return nan ? NAN : none ? -INFINITY : z; }
-  __device__ __forceinline__ float entropy(const RowSums<T>& q) const { return nan || none ? NAN : fmaf(-q.t / q.s, kLn2, ls); }
+  __device__ __forceinline__ float entropy(const RowSums<T>& q) const { return nan || none ? NAN : fmaf(-q.t / q.s, u, ls); }
   __device__ __forceinline__ float logp(float x) const {   // of an entry of the row that is seen as x
-    return nan ? NAN : none || x <= masked_from<T>() ? -INFINITY : fmaf(fmaf(x, kLog2e, -c), kLn2, -ls);
+    return nan ? NAN : none || x <= masked_from<T>() ? -INFINITY : fmaf(fmaf(x, k, -c), u, -ls);
   }
   template <typename Load>
   __device__ __forceinline__ float given(int64_t g, int32_t cats, Load&& load) const {

@@ -147,6 +147,37 @@ def test_scores_of_every_layout(gpu, dtype, C, layout):
     assert torch.equal(s.top, flat.top)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(24, 5), (24, 30), (24, 200), (24, 700), (24, 20000), (65544, 40)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_scores_far_from_zero(gpu, dtype, shape):
+    """Rows of any level up to the largest number of the type: their log-probabilities and entropies depend on differences only"""
+    torch, P = gpu
+    n, C = shape
+    levels = [0.0, -5000.0, 3e4, -3e4] if dtype == "float16" else \
+        [5e3, -5e3, 1e6, -1e6, 2e9, -2e9, 2.0 ** 30, -2.0 ** 30, 2.0 ** 30 - 64, 64 - 2.0 ** 30, 7e12, -7e12, 1e20, -1e20, 1.5e38, -1.5e38, 3.3e38]
+    g = torch.Generator().manual_seed(C)
+    x = torch.randint(-3, 3, shape, generator=g).double() * 0.75 + torch.tensor(levels).double()[torch.arange(n) % len(levels), None]
+    x[:, C // 2:] -= x[:, C // 2:].abs() * 2.0 ** -6    # some far below, at the end
+    x[-1, C - 1] = x[-1, 0] + 40.0                      # and a largest one late
+    x = x.to(getattr(torch, dtype)).cuda()
+    given = torch.randint(0, C, (n, 3), generator=g).cuda()
+    few = slice(-24, None)
+    raw = _numbers(x[few])
+    want, (index, best) = R.logp_of(raw, given[few].cpu().numpy()), R.likeliest(raw, 9)
+    # as R.sum_bound, whose arguments are now off by the rounding of up to 64 more, and the roundings of a difference and of two logarithms
+    slack = R.sum_bound(C) + 128 * R.EPS
+    bound = lambda lp: slack + 8 * R.EPS * (np.abs(np.where(np.isfinite(lp), lp, 0.0)) + 84.0)
+    for entropy, top in ((True, 9), (False, 0), (True, 1)):
+        s = P.category_scores(x, given, top=top, entropy=entropy)
+        _near(s.log_sum[few], R.statistics(raw)[0], R.log_bound(raw, R.statistics(raw)[0], C), "log_sum")
+        _near(s.logp[few], want, bound(want), "logp")
+        if entropy:
+            _near(s.entropy[few], R.statistics(raw)[1], R.entropy_bound(raw, 0.0, C) + 256 * R.EPS * (2.0 + np.log(C)), "entropy")
+        if top:
+            assert np.array_equal(s.top[few].cpu().numpy(), index[:, :top])
+            _near(s.top_logp[few], best[:, :top], bound(best[:, :top]), "top_logp")
+
+
 @pytest.mark.parametrize("type_", ["uint8", "int32", "int64"])
 def test_given_of_every_type_and_number(gpu, type_):
     torch, P = gpu
