@@ -10,6 +10,10 @@ namespace {
 constexpr int kShortCats = 256;
 constexpr int64_t kLaneRowsShort = 65536, kLaneRows = 32768;   // fewest rows, up to and beyond kShortCats categories
 constexpr int kLaneCats = 2048;                                // most categories
+// Rows that lie side by side: as many as fill the device with 64 a wave, too; fewer go a wave or more each, which read the same lines at
+// the same time.  A lane a row / waves a row, us, f32, entropy, no list: 1024 rows of 128 6.2 / 4.3, 4096 6.4 / 5.8; 1024 of 1000 14 / 8,
+// 4096 14 / 30; 1024 of 5000 38 / 34, 4096 40 / 172; 64 of 50000 295 / 25, 1024 298 / 283.
+constexpr int64_t kSideRowsShort = 6144, kSideRows = 2048;
 
 // Rows of up to 256 neighbouring categories: 16 lanes a row, all of it in registers, four rows a wave.  A lane holds kGroups
 // times 16 bytes; the sums need no running maximum.  The likeliest are found one after the other: the largest entry of 16 lanes
@@ -337,7 +341,8 @@ bool category_scores_short(const RowsRef& x, const RowsShape& shape, const Given
                            hipStream_t stream) {
   if (top > 16) return false;
   const bool neighbours = x.stride_cat == 1;
-  const bool side_by_side = !neighbours && ((shape.examples > 1 && std::abs(x.stride_ex) == 1) || (shape.vars > 1 && std::abs(x.stride_var) == 1));
+  const bool side_by_side = !neighbours && shape.rows() >= (shape.cats <= kShortCats ? kSideRowsShort : kSideRows) &&
+                            ((shape.examples > 1 && std::abs(x.stride_ex) == 1) || (shape.vars > 1 && std::abs(x.stride_var) == 1));
   // rows of neighbouring categories one stride apart: their examples and variables are one axis
   const bool even = shape.vars == 1 || x.stride_ex == (int64_t)shape.vars * x.stride_var;
   const bool staged = neighbours && even && shape.cats > 16 && shape.cats <= kLaneCats &&

@@ -222,6 +222,35 @@ def test_scores_of_many_short_rows(gpu, dtype, shape):
         assert torch.equal(s.top.view(-1, 3), t.top) and torch.equal(torch.nan_to_num(s.logp.reshape(-1), 7), torch.nan_to_num(t.logp, 7))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [3, 20, 128, 256, 300, 2100])
+@pytest.mark.parametrize("last", ["examples", "variables"])
+def test_scores_of_many_rows_side_by_side(gpu, dtype, C, last):
+    """As many as go a lane each, and a few less"""
+    torch, P = gpu
+    kinds = ("plain", "masked", "ties", "rising", "falling", "nan", "lowest")
+    for rows in ((6147, 6141) if C <= 256 else (2049, 2046)):
+        v = 3
+        n = rows // v
+        y = torch.cat([_scores(torch, dtype, (rows // 7 + 1, C), 81 + k, kind) for k, kind in enumerate(kinds)])[:rows].cuda()
+        y = y[torch.randperm(rows, generator=torch.Generator().manual_seed(1)).cuda()].view(n, v, C)
+        x = y.permute(1, 2, 0).contiguous().permute(2, 0, 1) if last == "examples" else y.transpose(1, 2).contiguous().transpose(1, 2)
+        given = torch.randint(-1, C + 1, (n, v), generator=torch.Generator().manual_seed(2)).cuda()
+        for top in (0, 2, 8, 15):
+            s = P.category_scores(x, given, top=top, entropy=True)
+            t = P.category_scores(y, given, top=top, entropy=True)
+            if top:
+                assert torch.equal(s.top, t.top)
+            few = slice(n - 60, n)
+            _check(torch, P, x[few], dtype, given[few], top)
+            raw = _numbers(x[few])
+            z, h = R.statistics(R.seen(raw, dtype))
+            _near(s.log_sum[few], z, R.log_bound(R.seen(raw, dtype), z, C), "log_sum")
+            _near(s.entropy[few], h, R.entropy_bound(R.seen(raw, dtype), z, C), "entropy")
+            want = R.logp_of(R.seen(raw, dtype), given[few].cpu().numpy().reshape(-1, 1))
+            _near(s.logp[few].reshape(-1, 1), want, R.log_bound(R.seen(raw, dtype), z, C)[:, None], "logp")
+
+
 def test_no_rows(gpu):
     torch, P = gpu
     x = torch.zeros((0, 10), device="cuda")
