@@ -432,7 +432,9 @@ void launch_stream(const RowsRef& x, const RowsShape& shape, const GivenRef& giv
 }  // namespace
 
 int64_t category_scores_workspace(const RowsShape& shape, int top) {
-  if (shape.examples < 1 || shape.vars < 1 || shape.cats < 1 || top < 0 || top > kMaxSlots || shape.examples > INT64_C(0x7fffffff) / shape.vars) return 0;
+  if (shape.examples < 1 || shape.vars < 1 || shape.cats < 1 || shape.cats > 1 << 30 || top < 0 || top > kMaxSlots ||
+      shape.examples > INT64_C(0x7fffffff) / shape.vars)
+    return 0;
   const Split s = split_of(shape, top > 0);
   const size_t jobs = (size_t)shape.rows() * s.parts;
   return s.parts == 1 ? 0 : (int64_t)(up16(jobs * sizeof(float4)) + jobs * top * sizeof(uint64_t));

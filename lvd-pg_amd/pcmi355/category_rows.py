@@ -27,6 +27,12 @@ class Checkpoint8:
     __slots__ = ("codes", "scales", "shape", "dtype")
 
     def __init__(self, codes, scales, shape, dtype):
+        n, v, c = _sizes(shape)
+        if codes.dtype != torch.uint8 or codes.shape != (n * v, -(-c // 16) * 16) or not codes.is_contiguous() \
+                or scales.dtype != torch.int32 or scales.shape != (n * v, -(-c // _BLOCK)) or not scales.is_contiguous() \
+                or scales.device != codes.device or dtype not in _TYPES:
+            raise ValueError(f"no checkpoint of rows {tuple(shape)} of {dtype}: codes {codes.dtype} {tuple(codes.shape)}, scales "
+                             f"{scales.dtype} {tuple(scales.shape)}")
         self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
 
     @property
@@ -122,10 +128,10 @@ def _check_out(out, shape, dtype, device):
         raise ValueError("out has elements that share memory")
 
 
-def _apart(out, other):
-    """out and another tensor share no memory"""
-    (a, b), (c, d) = _extent(out), _extent(other)
-    return b <= c or d <= a
+def _apart(out, *others):
+    """out shares no memory with other tensors"""
+    (a, b), rest = _extent(out), (_extent(t) for t in others if t is not None and t.numel())
+    return not out.numel() or all(b <= c or d <= a for c, d in rest)
 
 
 # the stream without an object around it, where torch has it: 0.1 us instead of 2.9
@@ -224,9 +230,10 @@ def category_scores_backward(scores, log_sum, given=None, *, grad_logp=None, ent
         out = torch.empty(shape, dtype=dtype, device=dev) if kept is not None else torch.empty_like(scores)
     else:
         _check_out(out, shape, dtype, dev)
-        if out.numel() and kept is None and not (out.data_ptr() == scores.data_ptr() and out.stride() == scores.stride()) \
-                and not _apart(out, scores):
+        if kept is None and not (out.data_ptr() == scores.data_ptr() and out.stride() == scores.stride()) and not _apart(out, scores):
             raise ValueError("out overlaps the scores without being them")
+        if not _apart(out, log_sum, given, grad_logp, entropy, grad_entropy, top, grad_top, *((kept.codes, kept.scales) if kept else ())):
+            raise ValueError("out overlaps another argument")
     if log_sum.numel():
         n, v, c = _sizes(shape)
         ptr = queries._dev_ptr
@@ -266,6 +273,8 @@ def restore_rows(checkpoint, dtype=None, out=None):
         out = torch.empty(checkpoint.shape, dtype=dtype, device=checkpoint.device)
     else:
         _check_out(out, checkpoint.shape, dtype, checkpoint.device)
+        if not _apart(out, checkpoint.codes, checkpoint.scales):
+            raise ValueError("out overlaps the checkpoint")
     _on_gpu(out)
     if out.numel():
         n, v, c = _sizes(checkpoint.shape)

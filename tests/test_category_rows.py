@@ -108,6 +108,33 @@ def test_python_refuses_what_it_cannot_do():
         kept.restore()
 
 
+def test_a_checkpoint_is_of_its_shape():
+    import pcmi355 as P
+    codes, scales = torch.zeros((6, 80), dtype=torch.uint8), torch.zeros((6, 2), dtype=torch.int32)
+    P.Checkpoint8(codes, scales, (2, 3, 70), torch.float32)
+    for c, s, shape, dtype in ((codes, scales, (6, 64), torch.float32), (codes, scales, (5, 70), torch.float32), (codes.int(), scales, (6, 70), torch.float32),
+                               (codes, scales.long(), (6, 70), torch.float32), (codes, scales[:, :1], (6, 70), torch.float32),
+                               (codes[:, :79], scales, (6, 70), torch.float32), (torch.zeros((80, 6), dtype=torch.uint8).t(), scales, (6, 70), torch.float32),
+                               (codes, torch.zeros((2, 6), dtype=torch.int32).t(), (6, 70), torch.float32), (codes, scales, (6, 70), torch.float64),
+                               (codes, scales.to("meta"), (6, 70), torch.float32), (codes, scales, (420,), torch.float32)):
+        with pytest.raises(ValueError):
+            P.Checkpoint8(c, s, shape, dtype)
+
+
+def test_workspaces_are_asked_for_and_checked():
+    from pcmi355._lib import lib
+    big = ctypes.create_string_buffer(64)
+    p = (ctypes.addressof(big) + 15) & ~15
+    need = lib.pcm_category_scores_workspace(1, 1, 131072, 8)
+    assert need > 0 and lib.pcm_category_scores_workspace(100000, 1, 131072, 8) == 0
+    call = lambda work, size: lib.pcm_category_scores(p, 0, 131072, 0, 1, 1, 1, 131072, None, 3, 0, 0, 0, 0, 8, None, None, None, p, p, None, None,
+                                                      work, size, None)
+    assert call(None, need) == -1 and call(p, need - 1) == -1 and b"workspace" in lib.pcm_last_error()
+    assert call(p + 8, need) == -1 and b"aligned" in lib.pcm_last_error()
+    for n, v, c in ((1, 1, (1 << 31) - 1), (1 << 40, 1, 10), (1 << 30, 4, 10)):
+        assert lib.pcm_category_scores_workspace(n, v, c, 8) == 0      # such rows are refused
+
+
 def test_where_results_may_go():
     from pcmi355 import category_rows as M
     t = torch.zeros((6, 8))
@@ -116,6 +143,7 @@ def test_where_results_may_go():
     assert not M._no_overlap(t[:1].expand(6, 8)) and not M._no_overlap(t.as_strided((4, 8), (1, 1)))
     assert not M._no_overlap(t.as_strided((3, 3), (2, 1)))
     assert M._apart(t[:3], t[3:]) and not M._apart(t[:4], t[3:])
+    assert M._apart(t[:3], None, t[3:4], t[:0], t[4:]) and not M._apart(t[:3], None, t[4:], t[2]) and M._apart(t[:0], t)
 
 
 def test_entry_points_refuse_without_a_gpu():

@@ -346,6 +346,28 @@ def test_gradient_in_place_of_the_scores(gpu, dtype, C):
     assert P.category_scores_backward(x, s.log_sum, g, out=x, **kw) is x and torch.equal(x, want)
 
 
+def test_results_refuse_to_overlap_what_is_read(gpu):
+    torch, P = gpu
+    x = torch.randn((8, 64), device="cuda")
+    g = torch.zeros(8, dtype=torch.int64, device="cuda")
+    s = P.category_scores(x, g, checkpoint=True)
+    buf = torch.zeros(8 * 64 + 8, device="cuda")
+    for k in (0, 500):
+        w = buf[k:k + 8]
+        with pytest.raises(ValueError, match="overlaps"):
+            P.category_scores_backward(x, s.log_sum, g, grad_logp=w, out=buf[:512].view(8, 64))
+        with pytest.raises(ValueError, match="overlaps"):
+            P.category_scores_backward(x, w, out=buf[:512].view(8, 64))
+    P.category_scores_backward(x, s.log_sum, g, grad_logp=buf[512:], out=buf[:512].view(8, 64))
+    bytes_ = torch.zeros(8 * 64 * 5, dtype=torch.uint8, device="cuda")
+    kept = P.Checkpoint8(bytes_[:512].view(8, 64), s.checkpoint.scales, (8, 64), torch.float32)
+    out = bytes_[496:496 + 2048].view(torch.float32).view(8, 64)
+    with pytest.raises(ValueError, match="overlaps"):
+        kept.restore(out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        P.category_scores_backward(kept, s.log_sum, out=out)
+
+
 def test_gradient_refuses_overlapping_results(gpu):
     torch, P = gpu
     buf = torch.zeros(200, device="cuda")
