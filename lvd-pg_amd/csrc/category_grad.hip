@@ -48,10 +48,11 @@ struct GradRow {
   }
 };
 
-// Rows of neighbouring categories in and out.  Where a wave holds one row (64 lanes a row or more), its slots wait in the wave's lanes, and a
+// Rows of neighbouring categories in and out (kUnit), or of any others, entry by entry.  Where a wave holds one row (64 lanes a row or more), its slots wait in the wave's lanes, and a
 // group of the row asks once which of them it holds: none, mostly.  Slots of shorter rows wait in LDS.  Either way they are added in
-// their order, so that sums come out the same every time.
-template <typename T, bool kCkpt, bool kEnt>
+// their order, so that sums come out the same every time.  512 x 784 rows of 256 f16 (kUnit): 92 to 102 us, 4.2 TB/s of scores and
+// gradient; 65536 rows of 256 f32 of every second category, entry by entry: 71 us, 265 with a lane per row.
+template <typename T, bool kCkpt, bool kEnt, bool kUnit>
 __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, Tiles tiles) {
   constexpr int kVec = 16 / (int)sizeof(T);
   __shared__ GradSlot slot_lds[kStaged];
@@ -77,7 +78,8 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
         if constexpr (kCkpt) {
           code[u] = load_codes<kVec>(ckpt.codes + r * pitch + c);
           unit[u] = ckpt.scales[r * blocks + c / kCkptBlock];
-        } else raw[u] = load_group(row, c, shape.cats);
+        } else if constexpr (kUnit) raw[u] = load_group(row, c, shape.cats);
+        else raw[u] = gather_group(row, c, shape.cats, x.stride_cat);
       }
     };
     request();
@@ -149,7 +151,10 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
         T w[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) w[i] = from_float<T>(y[i]);
-        if (mine) store_group(dst, c, shape.cats, w);
+        if (mine) {
+          if constexpr (kUnit) store_group(dst, c, shape.cats, w);
+          else scatter_group(dst, c, shape.cats, out.stride_cat, w);
+        }
       }
       if (turn + 1 == tiles.turns) break;
       tile.first += kTileGroups * tile.step;
@@ -159,8 +164,8 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
   }
 }
 
-// Any strides, a lane per row: 64 rows that lie side by side a wave, the categories cut among waves.  Slots are looked up per entry, the
-// first four from registers.
+// Rows that lie side by side, in or out, a lane per row: 64 of them a wave, the categories cut among waves.  Slots are looked up per entry,
+// the first four from registers.  65536 rows of 256 f32: 33 us from scores, 22 from codes (26 and 21 as rows of neighbours).
 template <typename T, bool kCkpt>
 __global__ __launch_bounds__(256) void grad_column_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, int parts, int len,
                                                           bool examples_first) {
@@ -174,10 +179,8 @@ __global__ __launch_bounds__(256) void grad_column_kernel(RowsRef x, CkptRef ckp
     const int first = (int)(job - set * parts) * len, end = min(first + len, shape.cats);
     const int64_t at = set * 64 + lane;
     if (at >= rows) continue;
-    const uint32_t n = (uint32_t)at;
-    const uint32_t hi = examples_first ? n / (uint32_t)shape.examples : n / (uint32_t)shape.vars;
-    const uint32_t lo = n - hi * (examples_first ? (uint32_t)shape.examples : (uint32_t)shape.vars);
-    const int64_t e = examples_first ? lo : hi, v = examples_first ? hi : lo, r = e * shape.vars + v;
+    const RowAt n = row_at(shape, (uint32_t)at, examples_first);
+    const int64_t e = n.e, v = n.v, r = n.r;
     const T* const row = static_cast<const T*>(x.p) + e * x.stride_ex + v * x.stride_var;
     T* const dst = static_cast<T*>(const_cast<void*>(out.p)) + e * out.stride_ex + v * out.stride_var;
     GradSlot near[kNear];
@@ -195,12 +198,14 @@ __global__ __launch_bounds__(256) void grad_column_kernel(RowsRef x, CkptRef ckp
     const GradRow grad(in, r, total);
     for (int c0 = first; c0 < end; c0 += kStep) {
       float y[kStep];
+      if constexpr (kCkpt) {             // (c0 is a multiple of 8, the codes' pitch of 16)
+        const Codes<kStep> code = load_codes<kStep>(ckpt.codes + r * pitch + c0);
+        const BlockUnit unit = block_unit(ckpt.scales[r * blocks + c0 / kCkptBlock]);
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int c = c0 + i;
-        if (c >= end) y[i] = -INFINITY;
-        else if constexpr (kCkpt) y[i] = block_entry_or_mask(block_unit(ckpt.scales[r * blocks + c / kCkptBlock]), ckpt.codes[r * pitch + c]);
-        else y[i] = seen(row[(int64_t)c * x.stride_cat]);
+        for (int i = 0; i < kStep; ++i) y[i] = block_entry_or_mask(unit, code[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) y[i] = c0 + i < end ? seen(row[(int64_t)(c0 + i) * x.stride_cat]) : -INFINITY;
       }
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
@@ -225,16 +230,18 @@ __global__ __launch_bounds__(256) void grad_column_kernel(RowsRef x, CkptRef ckp
 template <typename T>
 void launch_grad(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, const GradIn& in, const RowsRef& out, hipStream_t stream) {
   const int slots = in.given.slots + in.top;
-  if (out.stride_cat == 1 && (ckpt.codes || x.stride_cat == 1)) {
+  const bool unit = out.stride_cat == 1 && (ckpt.codes || x.stride_cat == 1);
+  if (unit || !(side_by_side(out, shape) || (!ckpt.codes && side_by_side(x, shape)))) {
     const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), (slots * kTileThreads + kStaged - 1) / kStaged, 8192);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, tile_grid(t), dim3(kTileThreads), 0, stream, x, ckpt, shape, in, out, t); };
     const bool ent = in.grad_entropy != nullptr;
-    if (ckpt.codes) ent ? launch(grad_tile_kernel<T, true, true>) : launch(grad_tile_kernel<T, true, false>);
-    else ent ? launch(grad_tile_kernel<T, false, true>) : launch(grad_tile_kernel<T, false, false>);
+    if (!unit) ckpt.codes ? launch(grad_tile_kernel<T, true, true, false>) : launch(grad_tile_kernel<T, false, true, false>);
+    else if (ckpt.codes) ent ? launch(grad_tile_kernel<T, true, true, true>) : launch(grad_tile_kernel<T, true, false, true>);
+    else ent ? launch(grad_tile_kernel<T, false, true, true>) : launch(grad_tile_kernel<T, false, false, true>);
     return;
   }
   const int64_t sets = (shape.rows() + 63) / 64;
-  const bool examples_first = shape.vars > 1 && (out.stride_ex == 1 || out.stride_ex == -1);
+  const bool examples_first = examples_side_by_side(out, shape);
   int64_t parts = std::max<int64_t>(1, std::min<int64_t>((shape.cats + 31) / 32, (8192 + sets - 1) / sets));
   const int len = (int)(((shape.cats + parts - 1) / parts + 7) / 8 * 8);
   parts = (shape.cats + len - 1) / len;

@@ -329,7 +329,7 @@ void launch_lane(const RowsRef& x, const RowsShape& shape, const GivenRef& given
   while (parts < most && sets * parts < 4096 && shape.cats / parts >= 64) parts *= 2;
   const int waves = std::max(4, parts), per = waves / parts;
   const int lds = std::max(staged ? waves * 64 * 36 * 4 : 0, parts > 1 ? waves * (3 + 2 * kList) * 64 * 4 : 0);
-  const bool examples_first = shape.vars > 1 && (x.stride_ex == 1 || x.stride_ex == -1);
+  const bool examples_first = examples_side_by_side(x, shape);
   const dim3 grid((unsigned)std::min<int64_t>((sets + per - 1) / per, 1 << 20)), block(64 * waves);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, x, shape, given, top, out, parts, examples_first); };
   staged ? launch(score_lane_kernel<T, kList, true>) : launch(score_lane_kernel<T, kList, false>);
@@ -341,13 +341,12 @@ bool category_scores_short(const RowsRef& x, const RowsShape& shape, const Given
                            hipStream_t stream) {
   if (top > 16) return false;
   const bool neighbours = x.stride_cat == 1;
-  const bool side_by_side = !neighbours && shape.rows() >= (shape.cats <= kShortCats ? kSideRowsShort : kSideRows) &&
-                            ((shape.examples > 1 && std::abs(x.stride_ex) == 1) || (shape.vars > 1 && std::abs(x.stride_var) == 1));
+  const bool side = !neighbours && side_by_side(x, shape) && shape.rows() >= (shape.cats <= kShortCats ? kSideRowsShort : kSideRows);
   // rows of neighbouring categories one stride apart: their examples and variables are one axis
   const bool even = shape.vars == 1 || x.stride_ex == (int64_t)shape.vars * x.stride_var;
   const bool staged = neighbours && even && shape.cats > 16 && shape.cats <= kLaneCats &&
                       shape.rows() >= (shape.cats <= kShortCats ? kLaneRowsShort : kLaneRows) && !ckpt.codes;
-  if (side_by_side || staged || (shape.cats <= 16 && !ckpt.codes)) {
+  if (side || staged || (shape.cats <= 16 && !ckpt.codes)) {
     RowsRef y = x;
     RowsShape one = shape;
     GivenRef g = given;

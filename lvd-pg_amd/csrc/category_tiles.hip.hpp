@@ -31,6 +31,16 @@ inline Tiles tiles_of(const RowsShape& shape, int vec, int least, int64_t wanted
 inline dim3 tile_grid(const Tiles& t) { return dim3((unsigned)std::min<int64_t>(t.jobs, 1 << 22)); }
 
 #ifdef __HIPCC__
+// The n-th row, counted examples first or variables first
+struct RowAt {
+  int64_t e, v, r;
+};
+__device__ __forceinline__ RowAt row_at(const RowsShape& shape, uint32_t n, bool examples_first) {
+  const uint32_t by = examples_first ? (uint32_t)shape.examples : (uint32_t)shape.vars, hi = n / by, lo = n - hi * by;
+  const int64_t e = examples_first ? lo : hi, v = examples_first ? hi : lo;
+  return {e, v, e * shape.vars + v};
+}
+
 struct TileAt {        // of a lane in a job
   int64_t row;         // may lie behind the last one
   int first, step;     // group u holds the categories from (first + u * step) * vec
@@ -51,6 +61,21 @@ __device__ __forceinline__ raw4 load_group(const T* row, int64_t c, int cats) {
 #pragma unroll
   for (int i = 0; i < kVec; ++i) w[i] = c + i < cats ? row[c + i] : (T)-INFINITY;
   return __builtin_bit_cast(raw4, w);
+}
+// ... of a row whose categories are not neighbours
+template <typename T>
+__device__ __forceinline__ raw4 gather_group(const T* row, int64_t c, int cats, int64_t stride) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  T w[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) w[i] = c + i < cats ? row[(c + i) * stride] : (T)-INFINITY;
+  return __builtin_bit_cast(raw4, w);
+}
+template <typename T>
+__device__ __forceinline__ void scatter_group(T* row, int64_t c, int cats, int64_t stride, const T (&w)[16 / (int)sizeof(T)]) {
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i)
+    if (c + i < cats) row[(c + i) * stride] = w[i];
 }
 template <typename T>
 __device__ __forceinline__ void store_group(T* row, int64_t c, int cats, const T (&w)[16 / (int)sizeof(T)]) {

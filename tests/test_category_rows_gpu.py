@@ -451,6 +451,40 @@ def test_eight_bits_of_every_layout(gpu):
             assert np.array_equal(_numbers(out.contiguous()), want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [1, 15, 17, 64, 70, 128, 200, 321])
+def test_eight_bits_of_many_rows_of_any_strides(gpu, dtype, C):
+    """The same codes whatever the strides, rows back into any strides, and gradients from codes and in place"""
+    torch, P = gpu
+    n, v = 47, 3
+    kinds = ("plain", "masked", "lowest", "ties", "rising", "nan", "wide")
+    rows = n * v
+    y = torch.cat([_scores(torch, dtype, (rows // 7 + 1, C), 91 + k, kind) for k, kind in enumerate(kinds)])[:rows].cuda()
+    y = y[torch.randperm(rows, generator=torch.Generator().manual_seed(1)).cuda()].view(n, v, C)
+    want = P.checkpoint_rows(y)
+    plain, wide = want.restore(), want.restore(torch.float32)
+    g, w = _slots(torch, (n, v), C, 6, 3)
+    s = P.category_scores(y, g, entropy=True)
+    kw = dict(grad_logp=w, entropy=s.entropy, grad_entropy=w[..., 0].contiguous())
+    from_codes, from_scores = P.category_scores_backward(want, s.log_sum, g, **kw), P.category_scores_backward(y, s.log_sum, g, **kw)
+    same = lambda a, b: torch.equal(torch.nan_to_num(a.double(), 1e300), torch.nan_to_num(b.double(), 1e300))
+    layouts = ((lambda t: torch.empty((v, C, n), dtype=t, device="cuda").permute(2, 0, 1)), (lambda t: torch.empty((n, C, v), dtype=t, device="cuda").transpose(1, 2)),
+               (lambda t: torch.empty((C, n, v), dtype=t, device="cuda").permute(1, 2, 0)), (lambda t: torch.empty((n, v, 3 * C), dtype=t, device="cuda")[..., 1::3]),
+               (lambda t: torch.empty((n, v, C + 1), dtype=t, device="cuda")[..., 1:]))
+    for layout in layouts:
+        x = layout(y.dtype)
+        x.copy_(y)
+        kept = P.checkpoint_rows(x)
+        assert torch.equal(kept.codes, want.codes) and torch.equal(kept.scales, want.scales)
+        kept = P.category_scores(x, checkpoint=True).checkpoint
+        assert torch.equal(kept.codes, want.codes) and torch.equal(kept.scales, want.scales)
+        assert same(want.restore(out=layout(y.dtype)), plain) and same(want.restore(out=layout(torch.float32)), wide)
+        assert same(P.category_scores_backward(want, s.log_sum, g, out=layout(y.dtype), **kw), from_codes)
+        assert same(P.category_scores_backward(x, s.log_sum, g, out=layout(y.dtype), **kw), from_scores)
+        assert same(P.category_scores_backward(y, s.log_sum, g, out=layout(y.dtype), **kw), from_scores)
+        assert same(P.category_scores_backward(x, s.log_sum, g, out=x, **kw), from_scores)
+
+
 # ---- as they are used ---------------------------------------------------------------------------------------------
 
 def test_same_bits_every_time(gpu):
