@@ -3,9 +3,10 @@
 // A row's sums are held relative to the running maximum m, in base 2: with k = log2 e and c = m k,
 //   s = sum 2^(x k - c),   t = sum 2^(d) d, d = x k - c,
 // so that an entry costs one fused multiply-add, one exponential and two or three additions.  c is rounded, but it is the same
-// c in every term, and r = c - m k is found exactly by one fused multiply-add at the end (u = ln 2):
-//   log Z = m + r u + log s,   log p[g] = (x[g] k - c) u - log s,   H = log s - t u / s.
-// From |m| = 2^30 on r could pass the range of the exponential.  There entries that are not m lie 64 or more below it and
+// c in every term.  In the end all is taken relative to m itself, by the term of m (u = ln 2):
+//   dm = m k - c,   q = log(s / 2^dm),   log Z = m + q,   log p[g] = (x[g] k - c - dm) u - q,   H = q - u (t - s dm) / s,
+// where a row of one category comes out as 0, 0 exactly.
+// From |m| = 2^30 on dm could pass the range of the exponential.  There entries that are not m lie 64 or more below it and
 // count for nothing; k = u = 1 takes the differences exactly, and s becomes the number of entries that are m.
 // Entries that count as masks never move m off its start, masked_from<T>(), where c = 0 and their terms underflow to 0.
 #pragma once
@@ -66,20 +67,25 @@ struct RowSums {
 template <typename T>
 struct RowResult {
   bool nan, none;
-  float c, k, u, ls, z;
-  __device__ __forceinline__ explicit RowResult(const RowSums<T>& q) {
-    nan = !(q.s < INFINITY);
-    none = !nan && !(q.m > masked_from<T>());
-    c = q.c;
-    k = q.k;
-    u = RowSums<T>::far(q.m) ? 1.f : kLn2;
-    ls = logf(q.s);
-    z = q.m + fmaf(fmaf(-q.m, k, c), u, ls);
+  float c, k, u, dm, q, z;
+  __device__ __forceinline__ explicit RowResult(const RowSums<T>& sum) {
+    nan = !(sum.s < INFINITY);
+    none = !nan && !(sum.m > masked_from<T>());
+    c = sum.c;
+    k = sum.k;
+    u = RowSums<T>::far(sum.m) ? 1.f : kLn2;
+    dm = fmaf(sum.m, k, -c);
+    q = logf(sum.s / __builtin_amdgcn_exp2f(dm));
+    z = sum.m + q;
   }
   __device__ __forceinline__ float log_sum() const { return nan ? NAN : none ? -INFINITY : z; }
-  __device__ __forceinline__ float entropy(const RowSums<T>& q) const { return nan || none ? NAN : fmaf(-q.t / q.s, u, ls); }
+  __device__ __forceinline__ float entropy(const RowSums<T>& sum) const {
+    const float one = __builtin_amdgcn_exp2f(dm);   // (of one category alone: its term, in both sums)
+    const float t = sum.s == one && sum.t == one * dm ? 0.f : fmaf(-sum.s, dm, sum.t);
+    return nan || none ? NAN : fmaf(-t / sum.s, u, q);
+  }
   __device__ __forceinline__ float logp(float x) const {   // of an entry of the row that is seen as x
-    return nan ? NAN : none || x <= masked_from<T>() ? -INFINITY : fmaf(fmaf(x, k, -c), u, -ls);
+    return nan ? NAN : none || x <= masked_from<T>() ? -INFINITY : fmaf(fmaf(x, k, -c) - dm, u, -q);
   }
   template <typename Load>
   __device__ __forceinline__ float given(int64_t g, int32_t cats, Load&& load) const {

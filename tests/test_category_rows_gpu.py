@@ -178,6 +178,27 @@ def test_scores_far_from_zero(gpu, dtype, shape):
             _near(s.top_logp[few], best[:, :top], bound(best[:, :top]), "top_logp")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(40, 2), (40, 30), (40, 250), (40, 900), (3, 90000), (65600, 20), (6200, 50)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_rows_of_one_category_are_certain(gpu, dtype, shape):
+    """All but one category masked: its log-probability and the entropy are 0, not nearly, and the gradient vanishes"""
+    torch, P = gpu
+    n, C = shape
+    g = torch.randint(0, C, (n,), generator=torch.Generator().manual_seed(C))
+    x = torch.full(shape, -float("inf"))
+    x[torch.arange(n), g] = torch.randn(n) * 9.0 - 2.0
+    x = x.to(getattr(torch, dtype)).cuda()
+    for y in (x, x.t().contiguous().t()):
+        for top in (0, 1, 3):
+            s = P.category_scores(y, g.cuda(), top=top, entropy=True)
+            assert (s.logp == 0).all() and (s.entropy == 0).all()
+            assert torch.equal(s.log_sum, x.float().amax(1))
+            if top:
+                assert torch.equal(s.top[:, 0].cpu().long(), g) and (s.top_logp[:, 0] == 0).all() and (s.top[:, 1:] == -1).all()
+        d = P.category_scores_backward(y, s.log_sum, g.cuda(), grad_logp=torch.ones(n, device="cuda"), entropy=s.entropy, grad_entropy=torch.ones(n, device="cuda"))
+        assert (d == 0).all()
+
+
 @pytest.mark.parametrize("type_", ["uint8", "int32", "int64"])
 def test_given_of_every_type_and_number(gpu, type_):
     torch, P = gpu
