@@ -8,6 +8,10 @@ namespace pcm {
 
 namespace {
 constexpr int kStaged = 2048;   // slots of all rows of a workgroup, in LDS
+// Most slots that every lane of a row of several per workgroup looks through; more are added in LDS by one lane of the row, where the row
+// has more than kLdsCats f32 entries.  Looked through / in LDS, us: 65536 rows of 128 with 8 slots 21.8 / 19.3, 24 40 / 28, 64 95 / 58; 16384 of
+// 500 with 24 31 / 23; 347990 of 22 with 24 69 / 78, 64 201 / 253; 16384 of 900 f16 with 24 36 / 36.
+constexpr int kFewSlots = 6, kLdsCats = 64;
 
 struct GradIn {
   GivenRef given;
@@ -52,11 +56,13 @@ struct GradRow {
 // group of the row asks once which of them it holds: none, mostly.  Slots of shorter rows wait in LDS.  Either way they are added in
 // their order, so that sums come out the same every time.  512 x 784 rows of 256 f16 (kUnit): 92 to 102 us, 4.2 TB/s of scores and
 // gradient; 65536 rows of 256 f32 of every second category, entry by entry: 71 us, 265 with a lane per row.
-template <typename T, bool kCkpt, bool kEnt, bool kUnit>
+template <typename T, bool kCkpt, bool kEnt, bool kUnit, bool kInLds>
 __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, Tiles tiles) {
   constexpr int kVec = 16 / (int)sizeof(T);
   __shared__ GradSlot slot_lds[kStaged];
+  extern __shared__ float grad_lds[];   // kInLds (one turn): the rows' gradients, [per][width]
   const int slots = in.given.slots + in.top, per = kTileThreads >> tiles.lanes_log2, of = threadIdx.x >> tiles.lanes_log2, lane = threadIdx.x & 63;
+  const int width = (kTileGroups * kVec) << tiles.lanes_log2;
   const int64_t rows = shape.rows();
   const int64_t pitch = (shape.cats + 15) / 16 * 16, blocks = (shape.cats + kCkptBlock - 1) / kCkptBlock;
   for (int64_t job = blockIdx.x; job < tiles.jobs; job += gridDim.x) {
@@ -139,6 +145,11 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
 #pragma unroll
             for (int k = 0; k < kVec; ++k) y[k] += i == (uint32_t)k ? by : 0.f;
         };
+        if constexpr (kInLds) {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) grad_lds[of * width + (int)c + i] = y[i];
+          continue;
+        }
         if (per <= 4) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -152,6 +163,25 @@ __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, Ckpt
 #pragma unroll
         for (int i = 0; i < kVec; ++i) w[i] = from_float<T>(y[i]);
         if (mine) {
+          if constexpr (kUnit) store_group(dst, c, shape.cats, w);
+          else scatter_group(dst, c, shape.cats, out.stride_cat, w);
+        }
+      }
+      if constexpr (kInLds) {
+        __syncthreads();
+        if (add && (threadIdx.x & ((1 << tiles.lanes_log2) - 1)) == 0)
+          for (int j = 0; j < slots; ++j) {
+            const GradSlot s = slot_lds[of * slots + j];
+            if (s.at >= 0) grad_lds[of * width + s.at] += s.by;
+          }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kTileGroups; ++u) {
+          const int64_t c = (int64_t)(tile.first + u * tile.step) * kVec;
+          if (c >= shape.cats || !mine) continue;
+          T w[kVec];
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) w[i] = from_float<T>(grad_lds[of * width + (int)c + i]);
           if constexpr (kUnit) store_group(dst, c, shape.cats, w);
           else scatter_group(dst, c, shape.cats, out.stride_cat, w);
         }
@@ -233,11 +263,17 @@ void launch_grad(const RowsRef& x, const CkptRef& ckpt, const RowsShape& shape, 
   const bool unit = out.stride_cat == 1 && (ckpt.codes || x.stride_cat == 1);
   if (unit || !(side_by_side(out, shape) || (!ckpt.codes && side_by_side(x, shape)))) {
     const Tiles t = tiles_of(shape, 16 / (int)sizeof(T), (slots * kTileThreads + kStaged - 1) / kStaged, 8192);
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, tile_grid(t), dim3(kTileThreads), 0, stream, x, ckpt, shape, in, out, t); };
-    const bool ent = in.grad_entropy != nullptr;
-    if (!unit) ckpt.codes ? launch(grad_tile_kernel<T, true, true, false>) : launch(grad_tile_kernel<T, false, true, false>);
-    else if (ckpt.codes) ent ? launch(grad_tile_kernel<T, true, true, true>) : launch(grad_tile_kernel<T, true, false, true>);
-    else ent ? launch(grad_tile_kernel<T, false, true, true>) : launch(grad_tile_kernel<T, false, false, true>);
+    const bool in_lds = sizeof(T) == 4 && t.lanes_log2 < 6 && shape.cats > kLdsCats && slots > kFewSlots, ent = in.grad_entropy != nullptr;
+    const int lds = in_lds ? kTileThreads * kTileGroups * (16 / (int)sizeof(T)) * 4 : 0;
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, tile_grid(t), dim3(kTileThreads), lds, stream, x, ckpt, shape, in, out, t); };
+    auto choose = [&](auto keep) {
+      constexpr bool kCkpt = decltype(keep)::value;
+      if constexpr (sizeof(T) == 4)
+        if (in_lds) return unit ? launch(grad_tile_kernel<T, kCkpt, true, true, true>) : launch(grad_tile_kernel<T, kCkpt, true, false, true>);
+      if (!unit) launch(grad_tile_kernel<T, kCkpt, true, false, false>);
+      else ent ? launch(grad_tile_kernel<T, kCkpt, true, true, false>) : launch(grad_tile_kernel<T, kCkpt, false, true, false>);
+    };
+    ckpt.codes ? choose(std::true_type()) : choose(std::false_type());
     return;
   }
   const int64_t sets = (shape.rows() + 63) / 64;

@@ -367,6 +367,36 @@ def test_gradient_in_place_of_the_scores(gpu, dtype, C):
     assert P.category_scores_backward(x, s.log_sum, g, out=x, **kw) is x and torch.equal(x, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [40, 128, 300, 500, 900])
+@pytest.mark.parametrize("kept", [False, True], ids=["scores", "8 bits"])
+def test_gradient_of_many_slots_in_few_categories(gpu, dtype, kept, C):
+    """Slots that share categories, in every layout of the gradient: the same bits every time (the order of a row's total differs
+    between layouts)"""
+    torch, P = gpu
+    n, k = 301, 20
+    x = _scores(torch, dtype, (n, C), 27, "masked").cuda()
+    gen = torch.Generator().manual_seed(C)
+    g, w = torch.randint(-1, 4, (n, k), generator=gen).cuda() * (C // 4), torch.randn((n, k), generator=gen).cuda()
+    g[7, 3] = C
+    s = P.category_scores(x, g, entropy=True, checkpoint=True)
+    source = s.checkpoint if kept else x
+    for kw in (dict(), dict(entropy=s.entropy, grad_entropy=w[:, 0].contiguous())):
+        want = P.category_scores_backward(source, s.log_sum, g, grad_logp=w, **kw)
+        raw = _numbers(x)
+        z, h = s.log_sum.double().cpu().numpy(), s.entropy.double().cpu().numpy()
+        exact, size, under = R.gradient(R.rounded(raw, dtype) if kept else R.seen(raw, dtype), z, h, [(g.cpu().numpy(), _numbers(w))],
+                                        _numbers(w)[:, 0] if kw else None)
+        bound = size * ((16 + k) * R.EPS) + np.abs(np.nan_to_num(exact)) * R.HALF[dtype] + R.TINY[dtype] + 2.0 ** -126 + under
+        _near(want, exact, bound, "gradient")
+        for out in (torch.empty((C, n), dtype=x.dtype, device="cuda").t(), torch.empty((n, 2 * C), dtype=x.dtype, device="cuda")[:, ::2], torch.empty_like(x)):
+            got = P.category_scores_backward(source, s.log_sum, g, grad_logp=w, out=out, **kw)
+            _near(got, exact, bound, "gradient")
+            first = torch.nan_to_num(got.double(), 1e300)
+            again = P.category_scores_backward(source, s.log_sum, g, grad_logp=w, out=out.zero_(), **kw)
+            assert torch.equal(torch.nan_to_num(again.double(), 1e300), first)
+
+
 def test_results_refuse_to_overlap_what_is_read(gpu):
     torch, P = gpu
     x = torch.randn((8, 64), device="cuda")
