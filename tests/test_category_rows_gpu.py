@@ -13,7 +13,7 @@ TYPES = ("float32", "bfloat16", "float16")
 @pytest.fixture(scope="module")
 def gpu():
     import torch
-    assert torch.cuda.is_available(), "these tests need the GPU box"
+    assert torch.cuda.is_available(), "these tests need a GPU"
     import pcmi355
     return torch, pcmi355
 
