@@ -7,6 +7,7 @@ from, matrices of parameter rows.  The reference leaves this to its Python progr
 
 Everything runs on torch's current stream of the tensors' device, waits for nothing, and can be captured into a graph; nothing
 here records for torch.autograd: a backward pass is a call, as `kld_backward` is."""
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -19,6 +20,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INDEX_TYPES = {torch.uint8: 3, torch.int32: 4, torch.int64: 5}
 _MAX_SLOTS = 64      # most given, and most likeliest, categories of a row
 _BLOCK = 64          # neighbours of a row that share a scale
+_MAX_CATS, _MAX_ROWS = 1 << 30, (1 << 31) - 1
 
 
 class Checkpoint8:
@@ -28,6 +30,7 @@ class Checkpoint8:
 
     def __init__(self, codes, scales, shape, dtype):
         n, v, c = _sizes(shape)
+        _check_sizes(shape, "a checkpoint of rows")
         if codes.dtype != torch.uint8 or codes.shape != (n * v, -(-c // 16) * 16) or not codes.is_contiguous() \
                 or scales.dtype != torch.int32 or scales.shape != (n * v, -(-c // _BLOCK)) or not scales.is_contiguous() \
                 or scales.device != codes.device or dtype not in _TYPES:
@@ -64,6 +67,14 @@ def _check_rows(x, what):
                          "[examples, variables, categories]")
     if x.shape[-1] < 1:
         raise ValueError(f"{what} need at least one category")
+    if x.numel() >> 30:                                      # (fewer entries: none of the sizes is past its limit)
+        _check_sizes(x.shape, what)
+
+
+def _check_sizes(shape, what):
+    """The entry points take sizes in 32 bits: what does not fit is refused here, it would arrive cut off"""
+    if shape[-1] > _MAX_CATS or math.prod(shape[:-1]) > _MAX_ROWS:
+        raise ValueError(f"{what} of shape {tuple(shape)}: at most 2^30 categories and 2^31 - 1 rows")
 
 
 def _on_gpu(*tensors):

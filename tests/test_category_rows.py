@@ -108,6 +108,23 @@ def test_python_refuses_what_it_cannot_do():
         kept.restore()
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    """Sizes reach the library in 32 bits: 2^32 + 5 categories are not 5, 2^32 + 1 rows not one"""
+    import pcmi355 as P
+    one = torch.zeros(1, dtype=torch.float16)
+    for shape in ((1, (1 << 32) + 5), (2, 3, (1 << 31) + 7), (1, (1 << 30) + 1), ((1 << 32) + 1, 4), (1, (1 << 32) + 1, 4), (1 << 16, 1 << 15, 2)):
+        x = one.expand(shape)
+        for f in (P.category_scores, P.checkpoint_rows, lambda y: P.category_scores_backward(y, one)):
+            with pytest.raises(ValueError, match="at most 2.30 categories"):
+                f(x)
+        rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
+        codes = torch.zeros(1, dtype=torch.uint8, device="meta").expand(rows, -(-shape[-1] // 16) * 16)
+        with pytest.raises(ValueError, match="at most 2.30 categories"):
+            P.Checkpoint8(codes, torch.zeros(1, dtype=torch.int32, device="meta").expand(rows, -(-shape[-1] // 64)), shape, torch.float16)
+    with pytest.raises(ValueError, match="GPU"):                        # the largest that the library takes
+        P.checkpoint_rows(one.expand(1, 1 << 30))
+
+
 def test_a_checkpoint_is_of_its_shape():
     import pcmi355 as P
     codes, scales = torch.zeros((6, 80), dtype=torch.uint8), torch.zeros((6, 2), dtype=torch.int32)
