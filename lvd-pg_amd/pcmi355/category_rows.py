@@ -140,10 +140,28 @@ def _check_out(out, shape, dtype, device):
         raise ValueError("out has elements that share memory")
 
 
+def _may_meet(ahead, a, b):
+    """Whether two sets of bytes may share one (False: they do not).  A set is (bytes of an element, [(stride, number), ...]), the
+    second one's first byte lies `ahead` of the first one's.  Strides that are multiples of a period drop out modulo that
+    period, and what is left of the sets can only meet as it lies or one period back."""
+    if ahead >= a[0] + sum(s * (n - 1) for s, n in a[1]) or -ahead >= b[0] + sum(s * (n - 1) for s, n in b[1]):
+        return False
+    for period in {s for s, _ in a[1] + b[1]}:
+        rest = [(e, [(s, n) for s, n in parts if s % period]) for e, parts in (a, b)]
+        if all(e + sum(s * (n - 1) for s, n in parts) <= period for e, parts in rest) \
+                and not any(_may_meet(ahead % period - back, *rest) for back in (0, period)):
+            return False
+    return True
+
+
+def _bytes(t):
+    return t.element_size(), [(s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if s and n > 1]
+
+
 def _apart(out, *others):
     """out shares no memory with other tensors"""
-    (a, b), rest = _extent(out), (_extent(t) for t in others if t is not None and t.numel())
-    return not out.numel() or all(b <= c or d <= a for c, d in rest)
+    (a, b), rest = _extent(out), ((t, *_extent(t)) for t in others if t is not None and t.numel())
+    return not out.numel() or all(b <= c or d <= a or not _may_meet(c - a, _bytes(out), _bytes(t)) for t, c, d in rest)
 
 
 # the stream without an object around it, where torch has it: 0.1 us instead of 2.9

@@ -163,6 +163,43 @@ def test_where_results_may_go():
     assert M._apart(t[:3], None, t[3:4], t[:0], t[4:]) and not M._apart(t[:3], None, t[4:], t[2]) and M._apart(t[:0], t)
 
 
+def test_results_may_lie_between_what_is_read():
+    """Tensors whose extents cross are refused only where an element may be shared: counted byte by byte"""
+    from pcmi355 import category_rows as M
+    t = torch.zeros((6, 20))
+    for a, b in ((t[:, :10], t[:, 10:]), (t[:, ::2], t[:, 1::2]), (t[:, 4:9], t[:, 12:13]), (t[::2], t[1::2]), (t[:, :10].t(), t[:, 10:]),
+                 (t[:, 3], t[:, 5:9]), (t[:, :18:2], t[:, 1:18:2]), (t.view(-1)[:114].view(6, 19)[:, :18:2], t.view(-1)[:114].view(6, 19)[:, 1:18:2]),
+                 (t.view(6, 4, 5)[:, :2], t.view(6, 4, 5)[:, 2:]), (t.view(6, 4, 5)[..., :3], t.view(6, 4, 5)[..., 3:])):
+        assert M._apart(a, b) and M._apart(b, a)
+    for a, b in ((t[:, :10], t[:, 9:]), (t[:, ::2], t[:, ::2]), (t[:, ::2], t[:, 1::3]), (t[::2], t[::3]), (t[:, :10].t(), t), (t[:, 3], t[:, 3:9]),
+                 (t.view(6, 4, 5)[:, :2], t.view(6, 4, 5)[:, 1]), (t.view(6, 4, 5)[..., :3], t.view(6, 4, 5)[:, 2, 2:])):
+        assert not M._apart(a, b) and not M._apart(b, a)
+    # any two views of a buffer: never called apart where a byte is shared
+    rng = np.random.default_rng(1)
+    buf = torch.zeros(400, dtype=torch.uint8)
+
+    def view():
+        dtype = (torch.uint8, torch.float16, torch.float32)[rng.integers(3)]
+        whole = buf.view(dtype)
+        size, stride = rng.integers(1, 5, 3).tolist(), rng.integers(0, 12, 3).tolist()
+        reach = sum(s * (n - 1) for s, n in zip(stride, size))
+        return whole.as_strided(size, stride, int(rng.integers(0, max(1, len(whole) - reach)))) if reach < len(whole) else whole[:3]
+
+    def bytes_of(v):
+        at = torch.zeros(v.shape, dtype=torch.int64) + (v.data_ptr() - buf.data_ptr())
+        for d, (s, n) in enumerate(zip(v.stride(), v.shape)):
+            at = at + (torch.arange(n) * s * v.element_size()).view([-1 if i == d else 1 for i in range(v.dim())])
+        return {int(x) + k for x in at.reshape(-1) for k in range(v.element_size())}
+
+    between = 0
+    for _ in range(3000):
+        a, b = view(), view()
+        shared = bool(bytes_of(a) & bytes_of(b))
+        assert not (shared and M._apart(a, b))
+        between += M._apart(a, b) and not (M._extent(a)[1] <= M._extent(b)[0] or M._extent(b)[1] <= M._extent(a)[0])
+    assert between                                    # (some of them lie between each other)
+
+
 def test_entry_points_refuse_without_a_gpu():
     from pcmi355._lib import lib
     big = ctypes.create_string_buffer(64)

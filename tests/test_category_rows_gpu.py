@@ -419,6 +419,24 @@ def test_results_refuse_to_overlap_what_is_read(gpu):
         P.category_scores_backward(kept, s.log_sum, out=out)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [20, 129, 1000])
+def test_results_beside_what_is_read(gpu, dtype, C):
+    """A gradient into the other columns, or the other rows, of the buffer that holds the scores; rows back beside their source"""
+    torch, P = gpu
+    n, t = 150, getattr(torch, dtype)
+    buf, side = torch.empty((2 * n, 2 * C + 3), dtype=t, device="cuda"), torch.empty((2 * C, n), dtype=t, device="cuda")
+    for x, out in ((buf[:n, :C], buf[:n, C + 3:]), (buf[::2, :C], buf[1::2, :C]), (buf[:n, :2 * C:2], buf[:n, 1:2 * C:2]),
+                   (side[::2].t(), side[1::2].t())):
+        x.copy_(_scores(torch, dtype, (n, C), 71).cuda())
+        before = x.clone()
+        kept = P.checkpoint_rows(x)
+        _check_grad(torch, P, x, dtype, k=3, out=out)
+        assert torch.equal(x, before)
+        _check_grad(torch, P, x, dtype, k=3, kept=True, out=out)
+        assert kept.restore(out=out) is out and torch.equal(out, kept.restore()) and torch.equal(x, before)
+
+
 def test_gradient_refuses_overlapping_results(gpu):
     torch, P = gpu
     buf = torch.zeros(200, device="cuda")
