@@ -518,8 +518,11 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  * pcm_checkpoint_rows: rows in 8 bits, for what a forward pass keeps for its backward pass.  d_codes [rows][num_cats rounded up
  * to 16] bytes, d_scales [rows][ceil(num_cats / 64)] words, the codes 16-byte aligned.  64 neighbours of a row with largest and smallest entries M and m
  * share a step 2^e: e is the smallest exponent for which the range takes at most 253 steps if its mantissa is at most 253 / 256
- * (in [1/2, 1)), at most 127 otherwise, |x| <= 2^14 steps and e >= -126.  An entry stands for (base - code) 2^e, base = rint(M /
- * 2^e): the nearest multiple of the step.  Code 255: an entry that is masked, x <= half of the type's lowest value; it
+ * (in [1/2, 1)), fewer than 128 otherwise, |x| <= 2^14 steps and e >= -126.  An entry stands for (base - code) 2^e, base = rint(M /
+ * 2^e): the nearest multiple of the step, off by half a step at most, that is by (M - m) / 253 or, where it is more, by 2^-14 of
+ * the largest |x|.  Far from zero the latter is what counts, and p in a backward pass from codes is off by a factor of up to its
+ * exponential (1.3 at |x| = 8000, e at 20000); scores less their log Z, whose gradient is the same, do not pay for their level.
+ * Code 255: an entry that is masked, x <= half of the type's lowest value; it
  * stands for -inf.  Scale word: base in bits 0..15 (two's complement), e + 127 in bits 16..23; 255 there (a block with NaN or
  * +inf): every entry stands for NaN; bit 24: some code of the block, or behind the row's end in it, is 255.  Codes behind a row's end are 255.
  * pcm_restore_rows: the values that the codes stand for, as floats or rounded to the type the rows had.

@@ -197,7 +197,7 @@ def category_scores(scores, given=None, *, top=0, entropy=False, checkpoint=Fals
     never among them (-1 and -inf where a row has no more).  A score at or below half of the type's lowest value is a mask and
     counts as -inf; a row of nothing else has log-sum and log-probabilities -inf and, being no distribution, entropy NaN; a
     row with NaN or +inf has NaN and -1.  checkpoint: also the scores in 8 bits (`checkpoint_rows`), for
-    `category_scores_backward`.  Returns `CategoryScores`, numbers in float32."""
+    `category_scores_backward`, which see for scores far from zero.  Returns `CategoryScores`, numbers in float32."""
     _check_rows(scores, "scores")
     shape = tuple(scores.shape)
     rows = shape[:-1]
@@ -232,7 +232,11 @@ def category_scores_backward(scores, log_sum, given=None, *, grad_logp=None, ent
     `grad_top` by those of the `top` categories and `grad_entropy` by the entropy (each may be left out); `log_sum`,
     `entropy` and `top` as `category_scores` returned them.
 
-    `scores`: the scores, or their `Checkpoint8`: the backward pass then reads a byte per score.  Returns a tensor of the scores'
+    `scores`: the scores, or their `Checkpoint8`: the backward pass then reads a byte per score,
+    and its probabilities are off by a factor of exp(half a step) at most, 1 + 1/253 of the range of 64 neighbours for small ones.
+    Steps grow with the level of a row, |x| / 2^13 at most: the factor may be 1.13 for scores near -3000, 1.3 near -8000, e near
+    -20000.  Nothing but differences within a row counts here, so keep such scores less their `log_sum` (`category_scores` of
+    `scores - s.log_sum[..., None]`): the level is gone, and steps follow the range alone.  Returns a tensor of the scores'
     shape and type; `out`: where it goes, also the scores themselves, which are then overwritten.  The same category in several
     slots adds up, a negative one adds nothing, one past the categories makes its row NaN."""
     kept = scores if isinstance(scores, Checkpoint8) else None
@@ -281,8 +285,9 @@ def category_scores_backward(scores, log_sum, given=None, *, grad_logp=None, ent
 
 def checkpoint_rows(rows):
     """Rows (float32, bfloat16 or float16, [rows, n] or [examples, variables, n], any strides) in 8 bits, for what a forward pass
-    keeps for its backward pass: 64 neighbours of a row share a power-of-two step that covers their range in at most 253
-    steps, and every entry becomes the nearest multiple of it, off by half a step (1/253 to 1/508 of the range) at most.  Entries
+    keeps for its backward pass: 64 neighbours of a row share a power-of-two step, the smallest that covers their range in at
+    most 253 steps and the largest |x| among them in 2^14, and every entry becomes the nearest multiple of it.  It is off by half a
+    step at most: 1/253 of the range, or |x| / 2^14 where that is more, as in rows that lie far from zero.  Entries
     at or below half of the type's lowest value (masks) come back as -inf, a block with NaN or +inf as NaN.  Returns a
     `Checkpoint8`, 1.06 bytes an entry."""
     _check_rows(rows, "rows")

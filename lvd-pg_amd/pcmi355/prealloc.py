@@ -9,8 +9,8 @@ device once and all their rows run in one pass of the row entry points (`pcm_kld
 parameters are neither read nor changed.  Host arrays in, host arrays out, as there.
 
 Between a forward call and its reverse pass the matrices stay on the device, as there.  `checkpoint = True` at the
-preallocation keeps them in 8 bits instead (`checkpoint_rows`: 1.06 bytes a parameter, the nearest of 253 steps over the range of
-64 neighbours); the reverse pass then differentiates at the rounded parameters.  Forward results do not change.
+preallocation keeps them in 8 bits instead (`checkpoint_rows`: 1.06 bytes a parameter, off by 1/253 of the range of 64
+neighbours, or by 2^-14 of the largest of them where that is more); the reverse pass then differentiates at the rounded parameters.  Forward results do not change.
 """
 import numpy as np
 import torch

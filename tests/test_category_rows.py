@@ -68,6 +68,18 @@ def test_reference_rounding_is_off_by_half_a_step(dtype):
         assert (np.abs(c - b).max(1) <= np.maximum(span / 126.5, size * 2.0 ** -12) / 2).all()
 
 
+def test_reference_rounding_follows_the_level():
+    """Half a step is at most 1/253 of the range of 64 neighbours or 2^-14 of the largest |x|, whichever is more; far from zero it is
+    the latter, and the former alone would not hold"""
+    for level in (0.0, -600.0, -3000.0, -8000.0, -20000.0):
+        x = (level + _rows(6, 500, 64, 2.5)).astype(np.float32).astype(np.float64)
+        off, span, size = np.abs(R.rounded(x, "float32") - x).max(1), np.ptp(x, axis=1), np.abs(x).max(1)
+        assert (off <= np.maximum(span / 253, size / 2.0 ** 14)).all()
+        assert (off > span / 253).any() == (level <= -3000.0)
+        shifted = (x - R.statistics(x)[0][:, None]).astype(np.float32).astype(np.float64)
+        assert (np.abs(R.rounded(shifted, "float32") - shifted).max(1) <= np.ptp(shifted, axis=1) / 253).all()
+
+
 # ---- refusals -----------------------------------------------------------------------------------------------------
 
 def test_python_refuses_what_it_cannot_do():

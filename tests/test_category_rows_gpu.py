@@ -487,6 +487,34 @@ def test_rows_in_eight_bits(gpu, dtype, kind, shape):
     assert kept.codes.shape == (shape[0], -(-shape[1] // 16) * 16) and (kept.codes[:, shape[1]:] == 255).all()
 
 
+@pytest.mark.parametrize("C", [64, 200, 1000])
+def test_gradient_from_eight_bits_far_from_zero(gpu, C):
+    """Likelihoods of whole images lie thousands below zero: what 8 bits may cost their probabilities there, and that scores less
+    their log-sum pay for their range alone"""
+    torch, P = gpu
+    n = 300
+    g, w = _slots(torch, (n,), C, 1, 3)
+    slots = [(g.cpu().numpy(), _numbers(w))]
+    for level in (0.0, -600.0, -3000.0, -8000.0, -20000.0):
+        x = (torch.randn((n, C), generator=torch.Generator().manual_seed(C)) * 2.5 + level).cuda()
+        z = P.category_scores(x).log_sum
+        for y, far in ((x, True), (x - z[:, None], False)):
+            s = P.category_scores(y, checkpoint=True)
+            raw = _numbers(y)
+            half = np.zeros(n)
+            for b in range(0, C, 64):
+                part = raw[:, b:b + 64]
+                # a block of few entries may span less than the level alone asks for: of a row less its log-sum |x| is below 64
+                half = np.maximum(half, np.maximum(np.ptp(part, axis=1) / 253, np.abs(part).max(1) / 2.0 ** 14))
+            assert far or half.max() <= max(np.ptp(raw, axis=1).max() / 253, 64 / 2.0 ** 14)
+            want, size, under = R.gradient(raw, s.log_sum.double().cpu().numpy(), None, slots)
+            got = P.category_scores_backward(s.checkpoint, s.log_sum, g, grad_logp=w)
+            # p |w| times what half a step makes of p, and roundings in 32 bits of the larger p
+            p = np.exp(raw - s.log_sum.double().cpu().numpy()[:, None]) * np.abs(_numbers(w)) * (g.cpu().numpy() >= 0)
+            bound = p * np.expm1(half)[:, None] + size * np.exp(half)[:, None] * 17 * R.EPS + 2.0 ** -126 + under
+            _near(got, want, bound, "gradient")
+
+
 def test_extreme_rows_in_eight_bits(gpu):
     torch, P = gpu
     lo, hi = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
