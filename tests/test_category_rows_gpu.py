@@ -243,6 +243,56 @@ def test_scores_of_many_short_rows(gpu, dtype, shape):
         assert torch.equal(s.top.view(-1, 3), t.top) and torch.equal(torch.nan_to_num(s.logp.reshape(-1), 7), torch.nan_to_num(t.logp, 7))
 
 
+def _within(torch, got, want, bound, what):
+    """_near on the device: NaN where NaN is wanted, the same infinities, the rest within the bound"""
+    got = got.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf]), what
+    past = torch.where(torch.isfinite(want), (got - want).abs() - bound, 0.0)
+    assert past.max() <= 0, (what, float(past.max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(65537, 17), (65600, 33), (65536, 130), (32769, 257), (32800, 511), (32768, 1100)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_every_one_of_many_short_rows(gpu, dtype, shape):
+    """A lane a row: each row of every kind against its definition in 64 bits, here on the device"""
+    torch, P = gpu
+    n, C = shape
+    kinds = ("plain", "masked", "ties", "rising", "falling", "nan", "lowest")
+    x = torch.cat([_scores(torch, dtype, (n // 7 + 1, C), 101 + k, kind) for k, kind in enumerate(kinds)])[:n].cuda()
+    x = x[torch.randperm(n, generator=torch.Generator().manual_seed(1)).cuda()]
+    given = torch.randint(-1, C + 1, (n, 2), generator=torch.Generator().manual_seed(2)).cuda()
+    y = x.double()
+    y = torch.where(y <= R.LOWEST[dtype] / 2, -np.inf, y)
+    bad = (torch.isnan(y) | (y == np.inf)).any(1)
+    none = ~bad & (y == -np.inf).all(1)
+    nan, inf = torch.full((), np.nan, dtype=torch.float64, device="cuda"), torch.full((), np.inf, dtype=torch.float64, device="cuda")
+    m = torch.where(bad | none, 0.0, y.amax(1))
+    d = y - m[:, None]
+    q = torch.log(d.exp().sum(1))
+    lp = d - q[:, None]
+    z = torch.where(bad, nan, torch.where(none, -inf, m + q))
+    h = torch.where(bad | none, nan, -torch.where(lp > -np.inf, lp.exp() * lp, 0.0).sum(1))
+    lp = torch.where(bad[:, None], nan, torch.where(none[:, None], -inf, lp))
+    want = lp.gather(1, given.clamp(0, C - 1))
+    want = torch.where(given < 0, 0.0, torch.where(given >= C, nan, want))
+    value, index = torch.sort(torch.where(bad[:, None], -inf, y), dim=1, descending=True, stable=True)
+    index = torch.where(value > -np.inf, index, -1)[:, :16]
+    best = torch.where(bad[:, None], nan, torch.where(index >= 0, lp.gather(1, index.clamp(min=0)), -inf))
+    # the sums of R.sum_bound, but added up by one lane: 16 entries one after the other, then C / 16 groups, then up to four parts
+    chain = (2 * 104 + 4 + C / 16 + 16 + 4) * R.EPS
+    near = chain + 4 * R.EPS * (torch.where(torch.isfinite(y), y.abs(), 0.0).amax(1) + torch.nan_to_num(z.abs(), 0.0, 0.0) + 20.0)
+    for top in (0, 1, 4, 7, 16):
+        s = P.category_scores(x, given, top=top, entropy=True)
+        _within(torch, s.log_sum, z, near, "log_sum")
+        _within(torch, s.entropy, h, (chain + 8 * R.EPS) * (2.0 + 2.0 * np.log(C + 1.0)), "entropy")
+        _within(torch, s.logp, want, near[:, None], "logp")
+        if top:
+            assert torch.equal(s.top.long(), index[:, :top])
+            _within(torch, s.top_logp, best[:, :top], near[:, None], "top_logp")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("C", [3, 20, 128, 256, 300, 2100])
 @pytest.mark.parametrize("last", ["examples", "variables"])
