@@ -742,6 +742,112 @@ def test_many_rows(gpu):
     assert (back - x).abs().max() <= (x.amax(1) - x.amin(1)).max() / 126.5 / 2 + 1e-6
 
 
+# A launch has at most 2^22 workgroups (gradients, tiles of checkpoints and of rows back) or 2^20 (all others); rows
+# beyond go to the same workgroups in further turns, which use the LDS and the registers of the turns before.  Rows that overlap in
+# memory keep the scores small.  All rows at once, and in parts that a launch takes in one turn: the same bits.
+
+def _whole_and_in_parts(torch, n, parts, call):
+    """call(first, end) gives the results of those rows, tensors with a row axis at 0"""
+    whole, step = call(0, n), n // parts + 1
+    for a in range(0, n, step):
+        for w, p in zip(whole, call(a, min(a + step, n))):
+            w = w[a:a + step]
+            assert w.shape == p.shape and (torch.equal(w, p) if w.dtype in (torch.int32, torch.uint8) else bool((w == p).all()))
+
+
+@pytest.mark.parametrize("kind, C, per, top, checkpoint, strides", [
+    ("a lane a row", 2, 256, 0, False, (1, 1)),
+    ("a lane a row by way of LDS", 17, 256, 0, False, (1, 1)),
+    ("a lane a row, side by side", 17, 256, 1, False, (1, 3)),
+    ("sixteen lanes a row", 40, 16, 3, True, (1, 1)),
+    ("a wave a row with a list", 300, 1, 20, False, (1, 1)),
+    ("a wave a row with a checkpoint", 300, 1, 0, True, (1, 1)),
+    ("a wave a row of any strides", 300, 1, 20, False, (2, 2)),
+], ids=lambda v: v.replace(" ", "_") if isinstance(v, str) else None)
+def test_scores_of_more_rows_than_workgroups(gpu, kind, C, per, top, checkpoint, strides):
+    torch, P = gpu
+    most = (1 << 20) * per
+    n = most + 5 * per + 3
+    buf = torch.randn(strides[0] * n + strides[1] * C, device="cuda").to(torch.float16)
+    x = buf.as_strided((n, C), strides)
+    given = torch.randint(-1, C, (n,), device="cuda", dtype=torch.int32)
+
+    def call(a, b):
+        s = P.category_scores(x[a:b], given[a:b], top=top, entropy=not checkpoint, checkpoint=checkpoint)
+        return [t for t in s[:5] if t is not None] + ([s.checkpoint.codes, s.checkpoint.scales] if checkpoint else [])
+
+    _whole_and_in_parts(torch, n, 2, call)
+    z = P.category_scores(x, None).log_sum[-300:]
+    y = _numbers(x[-300:])
+    _near(z, R.statistics(y)[0], R.log_bound(y, R.statistics(y)[0], C), "log_sum")
+    del buf, x, given
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind, dtype, C, per, slots, side", [
+    ("slots of short rows in LDS", "float16", 2, 256, 1, False),
+    ("gradients of short rows in LDS", "float32", 65, 32, 7, False),
+    ("side by side", "float16", 2, 256, 1, True),
+], ids=lambda v: v.replace(" ", "_") if isinstance(v, str) and " " in v else None)
+def test_gradient_of_more_rows_than_workgroups(gpu, kind, dtype, C, per, slots, side):
+    torch, P = gpu
+    most = (1 << 22) * per
+    n, t = most + 5 * per + 3, getattr(torch, dtype)
+    x = torch.randn(n + 3 * C, device="cuda", dtype=t).as_strided((n, C), (1, 3) if side else (1, 1))
+    z = P.category_scores(x).log_sum
+    given = torch.randint(0, C, (n, slots), device="cuda", dtype=torch.uint8)
+    w = torch.randn((n, slots), device="cuda")
+
+    def call(a, b):
+        out = torch.empty((C, b - a), dtype=t, device="cuda").t() if side else torch.empty((b - a, C), dtype=t, device="cuda")
+        return (P.category_scores_backward(x[a:b], z[a:b], given[a:b], grad_logp=w[a:b], out=out),)
+
+    _whole_and_in_parts(torch, n, 4, call)
+    want, size, under = R.gradient(_numbers(x[-300:]), z[-300:].double().cpu().numpy(), None, [(given[-300:].cpu().numpy(), _numbers(w[-300:]))])
+    got = call(n - 300, n)[0]
+    _near(got, want, size * ((16 + slots) * R.EPS) + np.abs(want) * R.HALF[dtype] + R.TINY[dtype] + 2.0 ** -126 + under, "gradient")
+    del x, z, given, w, got
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind, dtype, C, log2_rows, strides", [
+    ("tiles", "float32", 2, 26, (1, 1)),
+    ("side by side", "float16", 2, 28, (1, 3)),
+    ("any strides", "float16", 2, 22, (2, 3)),
+], ids=lambda v: v.replace(" ", "_") if isinstance(v, str) and v != "float32" and v != "float16" else None)
+def test_checkpoints_of_more_rows_than_workgroups(gpu, kind, dtype, C, log2_rows, strides):
+    torch, P = gpu
+    n = (1 << log2_rows) + 700
+    x = torch.randn(strides[0] * n + strides[1] * C, device="cuda").to(getattr(torch, dtype)).as_strided((n, C), strides)
+
+    def call(a, b):
+        kept = P.checkpoint_rows(x[a:b])
+        return kept.codes, kept.scales
+
+    _whole_and_in_parts(torch, n, 2, call)
+    assert np.array_equal(_numbers(P.checkpoint_rows(x[-300:]).restore(torch.float32)), R.rounded(_numbers(x[-300:]), dtype))
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind, log2_rows", [("tiles", 30), ("side by side", 28), ("any strides", 27)], ids=lambda v: v.replace(" ", "_") if isinstance(v, str) else None)
+def test_rows_back_of_more_rows_than_workgroups(gpu, kind, log2_rows):
+    torch, P = gpu
+    n, C = (1 << log2_rows) + 700, 2
+    few = P.checkpoint_rows(torch.randn((1 << 16, C), device="cuda").to(torch.float16))
+    turns = n // (1 << 16) + 1
+    codes, scales = few.codes.repeat(turns, 1)[:n].contiguous(), few.scales.repeat(turns, 1)[:n].contiguous()
+    out = torch.empty((C, n), dtype=torch.float16, device="cuda").t() if kind == "side by side" else torch.empty((n, 2 * C), dtype=torch.float16, device="cuda")[:, ::2] \
+        if kind == "any strides" else torch.empty((n, C), dtype=torch.float16, device="cuda")
+    want = few.restore()
+    P.Checkpoint8(codes, scales, (n, C), torch.float16).restore(out=out)
+    for a in range(0, n, 1 << 26):
+        part = out[a:a + (1 << 26)]
+        assert bool((part == want.repeat(-(-len(part) // (1 << 16)), 1)[:len(part)]).all())
+    del codes, scales, out
+    torch.cuda.empty_cache()
+
+
 def test_posterior_of_heads(gpu):
     """A multi-head circuit and a forest: log-posterior of the examples' clusters from the per-head likelihoods"""
     torch, P = gpu
