@@ -39,7 +39,6 @@ inline bool side_by_side(const RowsRef& x, const RowsShape& shape) {
   return examples_side_by_side(x, shape) || (shape.examples > 1 && (x.stride_ex == 1 || x.stride_ex == -1)) ||
          (shape.vars > 1 && (x.stride_var == 1 || x.stride_var == -1));
 }
-inline int64_t ckpt_pitch(int64_t cats) { return (cats + 15) / 16 * 16; }
 inline int64_t ckpt_blocks(int64_t cats) { return (cats + kCkptBlock - 1) / kCkptBlock; }
 
 int64_t category_scores_workspace(const RowsShape& shape, int top);
