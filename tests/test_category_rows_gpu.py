@@ -418,6 +418,28 @@ def test_gradient_in_place_of_the_scores(gpu, dtype, C):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [3, 70, 300, 5000])
+@pytest.mark.parametrize("slots", [1, 9])
+def test_gradient_of_rows_of_nothing_but_masks(gpu, dtype, C, slots):
+    """Zeros, whatever their slots: missing, within the row or past it; a row beside them with a slot past its end is NaN"""
+    torch, P = gpu
+    n = 70
+    for mask in (-float("inf"), R.LOWEST[dtype]):
+        x = _scores(torch, dtype, (n, C), 29)
+        x[::2] = mask
+        g = torch.full((n, slots), C, dtype=torch.int64)
+        g[::4] = C - 1
+        g[2::8, 0] = -1
+        x, g, one = x.cuda(), g.cuda(), torch.ones(n, device="cuda")
+        s = P.category_scores(x, entropy=True, checkpoint=True)
+        for source in (x, s.checkpoint):
+            for kw in (dict(), dict(entropy=s.entropy, grad_entropy=one)):
+                for out in (torch.empty((n, C), dtype=x.dtype, device="cuda"), torch.empty((C, n), dtype=x.dtype, device="cuda").t()):
+                    d = P.category_scores_backward(source, s.log_sum, g, grad_logp=one[:, None].expand(n, slots), out=out, **kw)
+                    assert (d[::2] == 0).all() and torch.isnan(d[1::2]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("C", [40, 128, 300, 500, 900])
 @pytest.mark.parametrize("kept", [False, True], ids=["scores", "8 bits"])
 def test_gradient_of_many_slots_in_few_categories(gpu, dtype, kept, C):
