@@ -499,7 +499,8 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  *   d_entropy [rows]           -sum_c p log p, p = exp(x - log Z) (may be NULL)
  *   d_top, d_top_logp [rows][top]  the likeliest categories and their log-probabilities, equal scores by rising category; a
  *                              category of score -inf is never among them: -1 and -inf stand where a row has no more
- *   d_codes, d_scales          the row's checkpoint as pcm_checkpoint_rows writes it, in the same pass (both NULL: none)
+ *   d_codes, d_scales          the row's checkpoint as pcm_checkpoint_rows writes it (both NULL: none): in the same pass if stride_cat
+ *                              is 1 or num_cats is, otherwise by a second launch, which reads the scores again
  * A row of nothing but masks: log Z = -inf, logp = -inf, no categories (-1) and, being no distribution, entropy NaN.  A row with NaN or
  * +inf: NaN, no categories (-1).
  * At most 64 given and 64 likeliest categories a row, 2^30 categories, 2^31 - 1 rows.  d_work: pcm_category_scores_workspace bytes of device
@@ -510,7 +511,7 @@ int pcm_adam_flow_step(pcm_circuit* c, int32_t batch_size, float* d_params, floa
  *   sum_j gl[j] ([c = g_j] - p[c]) + sum_i gt[i] ([c = top_i] - p[c]) - gh p[c] (log p[c] + H),
  * from the scores (d_scores) or from their checkpoint (d_codes, d_scales; d_scores NULL then) with d_log_sum and d_entropy
  * (the latter only with d_grad_entropy) as pcm_category_scores left them.  A slot < 0 adds nothing, one >= num_cats makes its
- * row NaN; the same category in several slots adds up; a row of log Z = -inf gets zeros.  p is as
+ * row NaN; the same category in several slots adds up; a row of log Z = -inf gets zeros, whatever its slots.  p is as
  * exact as d_log_sum: 2^-24 |log Z| relative.  d_grad has the type and shape of the
  * scores and strides of its own; it may be the array of scores itself with the same strides, else the two must not overlap, and
  * no two of its elements may be one.

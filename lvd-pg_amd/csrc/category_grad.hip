@@ -54,7 +54,7 @@ struct GradRow {
 
 // Rows of neighbouring categories in and out (kUnit), or of any others, entry by entry.  Where a wave holds one row (64 lanes a row or more), its slots wait in the wave's lanes, and a
 // group of the row asks once which of them it holds: none, mostly.  Slots of shorter rows wait in LDS.  Either way they are added in
-// their order, so that sums come out the same every time.  512 x 784 rows of 256 f16 (kUnit): 92 to 102 us, 4.2 TB/s of scores and
+// their order, so that sums come out the same every time.  512 x 784 rows of 256 f16 (kUnit): 98 us, 4.2 TB/s of scores and
 // gradient; 65536 rows of 256 f32 of every second category, entry by entry: 71 us, 265 with a lane per row.
 template <typename T, bool kCkpt, bool kEnt, bool kUnit, bool kInLds>
 __global__ __launch_bounds__(kTileThreads) void grad_tile_kernel(RowsRef x, CkptRef ckpt, RowsShape shape, GradIn in, RowsRef out, Tiles tiles) {

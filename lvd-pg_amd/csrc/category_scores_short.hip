@@ -12,7 +12,8 @@ constexpr int64_t kLaneRowsShort = 65536, kLaneRows = 32768;   // fewest rows, u
 constexpr int kLaneCats = 2048;                                // most categories
 // Rows that lie side by side: as many as fill the device with 64 a wave, too; fewer go a wave or more each, which read the same lines at
 // the same time.  A lane a row / waves a row, us, f32, entropy, no list: 1024 rows of 128 6.2 / 4.3, 4096 6.4 / 5.8; 1024 of 1000 14 / 8,
-// 4096 14 / 30; 1024 of 5000 38 / 34, 4096 40 / 172; 64 of 50000 295 / 25, 1024 298 / 283.
+// 4096 14 / 30; 1024 of 5000 38 / 34, 4096 40 / 172; 64 of 50000 295 / 25, 1024 298 / 283.  The lines are drawn for rows without a list: with
+// 8 likeliest some 4096 rows of 300 take 21 / 16, of 1000 33 / 33, of 5000 92 / 151, of 50000 645 / 2144.
 constexpr int64_t kSideRowsShort = 6144, kSideRows = 2048;
 
 // Rows of up to 256 neighbouring categories: 16 lanes a row, all of it in registers, four rows a wave.  A lane holds kGroups

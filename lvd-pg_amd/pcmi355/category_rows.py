@@ -189,14 +189,14 @@ def _new_checkpoint(x, shape):
 
 def category_scores(scores, given=None, *, top=0, entropy=False, checkpoint=False):
     """Log-probabilities of `given` categories under rows of scores, with the rows' log-sum, entropy and `top` likeliest
-    categories, in one pass over the scores.
+    categories, in one pass over the scores (a checkpoint of rows whose categories are not neighbours takes a second one).
 
     scores: float32, bfloat16 or float16 GPU tensor [rows, categories] or [examples, variables, categories], any strides.
     given: uint8, int32 or int64, one category per row or [rows..., slots] with up to 64; a negative one was not observed and has
     log-probability 0, one past the categories NaN.  top: 0 to 64; equal scores by rising category, masked categories
     never among them (-1 and -inf where a row has no more).  A score at or below half of the type's lowest value is a mask and
-    counts as -inf; a row of nothing else has log-sum and log-probabilities -inf and, being no distribution, entropy NaN; a
-    row with NaN or +inf has NaN and -1.  checkpoint: also the scores in 8 bits (`checkpoint_rows`), for
+    counts as -inf; a row of nothing else has log-sum and log-probabilities -inf and, being no distribution, entropy NaN
+    (leave such rows out of a mean over a padded batch); a row with NaN or +inf has NaN and -1.  checkpoint: also the scores in 8 bits (`checkpoint_rows`), for
     `category_scores_backward`, which see for scores far from zero.  Returns `CategoryScores`, numbers in float32."""
     _check_rows(scores, "scores")
     shape = tuple(scores.shape)
