@@ -550,6 +550,69 @@ int pcm_checkpoint_rows(const void* d_rows, int32_t type, int64_t stride_ex, int
 int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t num_examples, int32_t num_vars, int32_t num_cats,
                      void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride_cat, void* stream);
 
+/*
+ * Scores of categories that are products of features and weights, without keeping them.  Features f [examples][variables][length] (element
+ * strides, any sign, also 0; num_vars = 1 for plain rows) and weights w [num_cats][length] (element strides) are of one type, PCM_F32,
+ * PCM_BF16 or PCM_F16; the bias b [num_cats] (neighbours; NULL: zeros) is of any of them.  With
+ *   x[n][c] = f[n] . w[c] + b[c],  Z[n] = log sum_c exp x[n][c]:
+ * pcm_linear_scores: d_logp [rows][num_given]  x[n][g] - Z[n]; 0 where g < 0 (not observed), NaN where g >= num_cats;
+ *   d_log_sum [rows] Z (may be NULL).  Given categories as for pcm_category_scores, at most 64 a row.
+ * pcm_linear_scores_backward: the gradients of a loss whose derivatives are d_grad_logp [rows][num_given] by the log-probabilities and
+ *   d_grad_log_sum [rows] by the log-sums (NULL: none), from dx[n][c] = sum_j gl[n][j] [c = g_j] - (sum_j gl[n][j] - gz[n]) p[n][c],
+ *   p = exp(x - Z): d_grad_features [rows][length] dx w, d_grad_weight [num_cats][length] dx^T f, both of the features' type,
+ *   d_grad_bias [num_cats] sum_n dx, of the bias's type (bias_type, also where d_bias is NULL); NULL: not wanted.  d_log_sum as
+ *   pcm_linear_scores left it.  The scores are computed once more, in pieces of the categories.  A slot < 0 adds nothing, one >=
+ *   num_cats makes its row's dx NaN; a category in several slots adds up.  A row whose derivatives are all 0 (all its slots < 0: the
+ *   padding of a batch) has no part in any gradient, whatever its features hold; so has one of log Z = -inf.
+ * A bias at or below half of its type's lowest value masks its category: x = -inf, whatever f and w hold; the weights of such a category
+ *   have no part in the features' gradients.  A row of nothing but masks: log Z and logp -inf.  NaN in a row's features or in an
+ *   unmasked category's weights, and scores of +inf: NaN.
+ * Products of 16-bit types are exact and summed in 32 bits; float is taken as three bfloat16 parts whose six largest products are summed
+ *   (what is left out lies 2^-26 below a product).  dx is rounded to the features' type, relative to a power of two a row (float:
+ *   three parts again).  Sums have a fixed order: the same bits every time.
+ * At most 2^22 rows, 2^30 categories, length 2^20.  d_work: so many bytes of device memory as the _workspace function of the same arguments says, 16-byte
+ * aligned, which belong to the call until its work is done; `of`: 1 features, 2 weight, 4 bias, added.
+ *
+ * Rows in 8-bit integers, for products of them (pcm_rows8): d_codes [rows][length rounded up to 128], zeros behind a row's end, 16-byte
+ * aligned, and d_scales [rows].  Code rint(x (127 / a)) and scale a / 127, a the row's largest |x|, in 32 bits; a row whose a lies
+ * below 2^-119 has codes and scale 0, one with NaN or an infinity scale NaN.  At most 2^31 - 1 rows, length 131071.
+ * pcm_product8: d_out[r][c] = (sum_k rows[r][k] channels[c][k]) row_scale[r] channel_scale[c] + b[c], the sum in whole numbers, which are exact
+ *   (lengths up to 131071), rounded to `type` once at the end; rows of d_out are out_stride >= num_channels entries apart.
+ * pcm_linear_scores8: pcm_linear_scores of x = such a product.
+ *
+ * All queue their work on `stream` (of the current device), wait for nothing and allocate nothing: they can be captured.
+ */
+int64_t pcm_linear_scores_workspace(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var,
+                                    int64_t stride, int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars,
+                                    int32_t length, int32_t num_cats);
+int pcm_linear_scores(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride,
+                      int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars, int32_t length,
+                      int32_t num_cats, const void* d_bias, int32_t bias_type, const void* d_given, int32_t given_type,
+                      int64_t given_stride_ex, int64_t given_stride_var, int64_t given_stride_slot, int32_t num_given, float* d_logp,
+                      float* d_log_sum, void* d_work, int64_t work_bytes, void* stream);
+int64_t pcm_linear_scores_backward_workspace(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex,
+                                             int64_t stride_var, int64_t stride, int64_t weight_stride_cat, int64_t weight_stride,
+                                             int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats, int32_t of);
+int pcm_linear_scores_backward(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var,
+                               int64_t stride, int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars,
+                               int32_t length, int32_t num_cats, const void* d_bias, int32_t bias_type, const void* d_given,
+                               int32_t given_type, int64_t given_stride_ex, int64_t given_stride_var, int64_t given_stride_slot,
+                               int32_t num_given, const float* d_grad_logp, const float* d_grad_log_sum, const float* d_log_sum,
+                               void* d_grad_features, void* d_grad_weight, void* d_grad_bias, void* d_work, int64_t work_bytes,
+                               void* stream);
+int pcm_rows8(const void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride, int64_t num_examples,
+              int32_t num_vars, int32_t length, int8_t* d_codes, float* d_scales, void* stream);
+int64_t pcm_product8_workspace(int64_t num_rows, int64_t num_channels, int32_t length);
+int pcm_product8(const int8_t* d_rows, const float* d_row_scales, int64_t num_rows, const int8_t* d_channels, const float* d_channel_scales,
+                 int64_t num_channels, int32_t length, const void* d_bias, int32_t bias_type, void* d_out, int32_t type, int64_t out_stride,
+                 void* d_work, int64_t work_bytes, void* stream);
+int64_t pcm_linear_scores8_workspace(int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats);
+int pcm_linear_scores8(const int8_t* d_features, const float* d_feature_scales, const int8_t* d_weight, const float* d_weight_scales,
+                       int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats, const void* d_bias, int32_t bias_type,
+                       const void* d_given, int32_t given_type, int64_t given_stride_ex, int64_t given_stride_var,
+                       int64_t given_stride_slot, int32_t num_given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
+                       void* stream);
+
 /* ---- instrumentation ----------------------------------------------------------- */
 
 /* Per-kernel timing, the role of `debug = true` -> `CUDA.@time` around each launch

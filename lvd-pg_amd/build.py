@@ -10,7 +10,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.hip", "hclt_engine.hip", "hclt_queries.hip", "hclt_kld.hip", "hclt_wide.hip", "chow_liu.hip",
            "pairwise_mi_static.hip", "chow_liu_edges.hip", "sparse_engine.hip", "param_rows.hip", "flow_rows.hip", "stream_probe.hip",
-           "host_stage.hip", "category_scores.hip", "category_scores_short.hip", "category_grad.hip", "checkpoint_rows.hip"]
+           "host_stage.hip", "category_scores.hip", "category_scores_short.hip", "category_grad.hip", "checkpoint_rows.hip",
+           "lay_out.hip", "linear_scores.hip", "linear_gradient.hip", "product_out.hip", "product8.hip"]
 OUT = os.path.join(HERE, "libpcmi355.so")
 OBJ_DIR = os.path.join(HERE, "build")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

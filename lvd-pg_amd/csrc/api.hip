@@ -7,6 +7,7 @@
 #include "category_rows.hpp"
 #include "common.hpp"
 #include "hclt_engine.hpp"
+#include "linear_scores.hpp"
 #include "sparse_engine.hpp"
 
 namespace {
@@ -419,6 +420,104 @@ int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t nu
     pcm::restore_rows(pcm::CkptRef{const_cast<uint8_t*>(d_codes), reinterpret_cast<uint32_t*>(const_cast<int32_t*>(d_scales))},
                       pcm::RowsShape{num_examples, num_vars, num_cats}, pcm::RowsRef{d_rows, type, stride_ex, stride_var, stride_cat},
                       static_cast<hipStream_t>(stream));
+  });
+}
+
+namespace {
+pcm::Matrix2 features_of(const void* p, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride, int64_t n, int32_t v, int32_t length) {
+  return {p, type, stride_ex, stride_var, stride, n, v, length};
+}
+pcm::Matrix2 weights_of(const void* p, int32_t type, int64_t stride_cat, int64_t stride, int32_t cats, int32_t length) {
+  return {p, type, stride_cat, 0, stride, cats, 1, length};
+}
+bool linear_sizes(int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats) {   // sizes that an entry point takes
+  return num_examples >= 1 && num_vars >= 1 && length >= 1 && num_cats >= 1 && num_examples <= pcm::kMaxLinearRows &&
+         num_examples * num_vars <= pcm::kMaxLinearRows && length <= pcm::kMaxLength && num_cats <= 1 << 30;
+}
+}  // namespace
+
+int64_t pcm_linear_scores_workspace(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var,
+                                    int64_t stride, int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars,
+                                    int32_t length, int32_t num_cats) {
+  if (!linear_sizes(num_examples, num_vars, length, num_cats)) return 0;
+  return pcm::linear_scores_workspace(features_of(d_features, type, stride_ex, stride_var, stride, num_examples, num_vars, length),
+                                      weights_of(d_weight, type, weight_stride_cat, weight_stride, num_cats, length));
+}
+
+int pcm_linear_scores(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride,
+                      int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars, int32_t length,
+                      int32_t num_cats, const void* d_bias, int32_t bias_type, const void* d_given, int32_t given_type,
+                      int64_t given_stride_ex, int64_t given_stride_var, int64_t given_stride_slot, int32_t num_given, float* d_logp,
+                      float* d_log_sum, void* d_work, int64_t work_bytes, void* stream) {
+  return guarded([&] {
+    pcm::linear_scores(features_of(d_features, type, stride_ex, stride_var, stride, num_examples, num_vars, length),
+                       weights_of(d_weight, type, weight_stride_cat, weight_stride, num_cats, length), pcm::BiasRef{d_bias, bias_type},
+                       pcm::GivenRef{d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given}, d_logp, d_log_sum,
+                       d_work, work_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t pcm_linear_scores_backward_workspace(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex,
+                                             int64_t stride_var, int64_t stride, int64_t weight_stride_cat, int64_t weight_stride,
+                                             int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats, int32_t of) {
+  if (!linear_sizes(num_examples, num_vars, length, num_cats)) return 0;
+  return pcm::linear_scores_backward_workspace(features_of(d_features, type, stride_ex, stride_var, stride, num_examples, num_vars, length),
+                                               weights_of(d_weight, type, weight_stride_cat, weight_stride, num_cats, length), of & 1,
+                                               of >> 1 & 1, of >> 2 & 1);
+}
+
+int pcm_linear_scores_backward(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var,
+                               int64_t stride, int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars,
+                               int32_t length, int32_t num_cats, const void* d_bias, int32_t bias_type, const void* d_given,
+                               int32_t given_type, int64_t given_stride_ex, int64_t given_stride_var, int64_t given_stride_slot,
+                               int32_t num_given, const float* d_grad_logp, const float* d_grad_log_sum, const float* d_log_sum,
+                               void* d_grad_features, void* d_grad_weight, void* d_grad_bias, void* d_work, int64_t work_bytes,
+                               void* stream) {
+  return guarded([&] {
+    pcm::linear_scores_backward(features_of(d_features, type, stride_ex, stride_var, stride, num_examples, num_vars, length),
+                                weights_of(d_weight, type, weight_stride_cat, weight_stride, num_cats, length),
+                                pcm::BiasRef{d_bias, bias_type},
+                                pcm::GivenRef{d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given},
+                                d_grad_logp, d_grad_log_sum, d_log_sum, pcm::LinearGradients{d_grad_features, d_grad_weight, d_grad_bias},
+                                d_work, work_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int pcm_rows8(const void* d_rows, int32_t type, int64_t stride_ex, int64_t stride_var, int64_t stride, int64_t num_examples,
+              int32_t num_vars, int32_t length, int8_t* d_codes, float* d_scales, void* stream) {
+  return guarded([&] {
+    pcm::rows8(features_of(d_rows, type, stride_ex, stride_var, stride, num_examples, num_vars, length), d_codes, d_scales,
+               static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t pcm_product8_workspace(int64_t num_rows, int64_t num_channels, int32_t length) {
+  return pcm::product8_workspace(num_rows, num_channels, length);
+}
+
+int pcm_product8(const int8_t* d_rows, const float* d_row_scales, int64_t num_rows, const int8_t* d_channels, const float* d_channel_scales,
+                 int64_t num_channels, int32_t length, const void* d_bias, int32_t bias_type, void* d_out, int32_t type, int64_t out_stride,
+                 void* d_work, int64_t work_bytes, void* stream) {
+  return guarded([&] {
+    pcm::product8(d_rows, d_row_scales, num_rows, d_channels, d_channel_scales, num_channels, length, pcm::BiasRef{d_bias, bias_type}, d_out,
+                  type, out_stride, d_work, work_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t pcm_linear_scores8_workspace(int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats) {
+  return linear_sizes(num_examples, num_vars, length, num_cats) ? pcm::linear_scores8_workspace(num_examples * num_vars, num_cats) : 0;
+}
+
+int pcm_linear_scores8(const int8_t* d_features, const float* d_feature_scales, const int8_t* d_weight, const float* d_weight_scales,
+                       int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats, const void* d_bias, int32_t bias_type,
+                       const void* d_given, int32_t given_type, int64_t given_stride_ex, int64_t given_stride_var,
+                       int64_t given_stride_slot, int32_t num_given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
+                       void* stream) {
+  return guarded([&] {
+    pcm::linear_scores8(d_features, d_feature_scales, num_examples, num_vars, d_weight, d_weight_scales, num_cats, length,
+                        pcm::BiasRef{d_bias, bias_type},
+                        pcm::GivenRef{d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given}, d_logp,
+                        d_log_sum, d_work, work_bytes, static_cast<hipStream_t>(stream));
   });
 }
 

@@ -1,0 +1,359 @@
+// Gradients of log-probabilities and log-sums of scores that are products of features and weights, without keeping the scores.
+//
+//   dx[n][c] = sum_j gl[n][j] [c = g_j] - (sum_j gl[n][j] - gz[n]) p[n][c],  p = exp(x - Z)
+//   features: dx w, weights: dx^T f, bias: sum_n dx
+// The categories are taken in pieces: the scores of a piece once more (gradient_kernel), whose dx goes into the workspace in both
+// orders, rounded to the operands' 16 bits (float: three planes), then the piece's two products.  dx is held as dx 2^(15 - e[n]),
+// 2^e[n] the next power of two above what |dx| of the row can be, so that half's range holds it whatever the loss's scale; features are
+// turned with 2^(e[n] - largest e), which is exact, for the sum over rows.
+#include "product_out.hip.hpp"
+
+namespace pcm {
+
+namespace {
+constexpr int kMostBlocks = 256;     // candidates of the largest exponent
+
+// Per row: the weight of p, and the exponent
+__global__ __launch_bounds__(256) void row_terms_kernel(GivenRef given, const float* grad_logp, const float* grad_log_sum, const float* log_sum,
+                                                        int64_t rows, int64_t cats, float* of_p, int* expo, int* most) {
+  __shared__ int sub[256];
+  int best = kDeadRow;
+  for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < rows; n += kMostBlocks * 256) {
+    float total = 0.f, size = 0.f;
+    bool past = false;
+    for (int s = 0; s < given.slots; ++s) {
+      const int64_t g = given_at(given, n / given.vars, n % given.vars, s);
+      if (g < 0) continue;
+      past |= g >= cats;
+      const float by = grad_logp[n * given.slots + s];
+      total += by;
+      size += fabsf(by);
+    }
+    if (grad_log_sum) total -= grad_log_sum[n];
+    size += fabsf(total);
+    int e = kDeadRow;
+    if (past) total = size = __builtin_nanf("");
+    if (log_sum[n] == -INFINITY) size = 0.f;                        // no category: no gradient
+    if (size != 0.f) e = size < INFINITY ? min(max(ilogbf(size) + 1, -100), 127) : 0;   // (NaN, inf: as they are)
+    of_p[n] = total;
+    expo[n] = e;
+    best = max(best, e);
+  }
+  sub[threadIdx.x] = best;
+  __syncthreads();
+  for (int s = 128; s; s /= 2) {
+    if (threadIdx.x < s) sub[threadIdx.x] = max(sub[threadIdx.x], sub[threadIdx.x + s]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) most[blockIdx.x] = sub[0];
+}
+
+struct GradientTask : ScoreInputs {
+  int64_t first;                     // the piece's first category, which is row 0 of w; cats is the piece's size
+  const float *grad_logp, *log_sum, *of_p;
+  const int* expo;
+  uint16_t* by_row;                  // dx [plane][row][pitch_row]; null: not needed
+  uint16_t* by_cat;                  // dx [plane][category of the piece][pitch_cat]
+  int64_t pitch_row, pitch_cat, plane_row, plane_cat;
+  float* bias_parts;                 // [tile of rows][category of the piece]; null: none
+};
+
+template <typename T, bool kPlanes>
+struct Coded {                       // a number as the operands hold it
+  uint16_t p[kPlanes ? 3 : 1];
+  __device__ __forceinline__ explicit Coded(float v) {
+    if constexpr (kPlanes) {
+      const Planes q = planes(v);
+      p[0] = __builtin_bit_cast(uint16_t, q.h);
+      p[1] = __builtin_bit_cast(uint16_t, q.m);
+      p[2] = __builtin_bit_cast(uint16_t, q.l);
+    } else {
+      p[0] = __builtin_bit_cast(uint16_t, (T)v);
+    }
+  }
+};
+
+template <typename T, typename S, bool kPlanes>
+__device__ __forceinline__ void gradient_tile(const GradientTask& t) {
+  product_tile<T, S>(t.w, t.f, t.cats, t.rows, t.steps, [&](auto& sums, int64_t m, int64_t n, char* lds) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x / 64, wm = wave % S::waves_m * S::WM;
+    float* const bias = reinterpret_cast<float*>(lds);                      // [BM]
+    float* const scale = bias + S::BM;                                      // [BM]
+    float* const of_bias = scale + S::BM;                                   // [waves_n][BM]
+    tile_constants<S>(t, m - wm, bias, scale);
+    constexpr int kPl = kPlanes ? 3 : 1;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int64_t row = n + 32 * j + (lane & 31);
+      const bool valid = row < t.rows;
+      const int64_t at = valid ? row : t.rows - 1;
+      scores_of<S>(t, sums, j, 1.f, bias + wm, scale + wm, half);
+      const float z = t.log_sum[at], of_p = t.of_p[at];
+      const int e = valid ? t.expo[at] : kDeadRow;
+      const float by = e == kDeadRow ? 0.f : ldexpf(1.f, 15 - e);
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = __builtin_amdgcn_exp2f((sums[i][j][r] - z) * kLog2e);
+          sums[i][j][r] = by == 0.f ? 0.f : -of_p * p;
+        }
+      if (t.given.slots && by != 0.f) {
+        const int64_t ex = row / t.given.vars, v = row % t.given.vars;
+        for (int s = 0; s < t.given.slots; ++s) {
+          const int64_t g = given_at(t.given, ex, v, s) - t.first - m;
+          if (g < 0 || g >= S::WM || (g >> 2 & 1) != half) continue;
+          const float add = t.grad_logp[row * t.given.slots + s];
+#pragma unroll
+          for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (g == 32 * i + 8 * (r / 4) + 4 * half + r % 4) sums[i][j][r] += add;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t c = m + 32 * i + 8 * q + 4 * half;
+          uint16_t code[kPl][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const Coded<T, kPlanes> one(sums[i][j][4 * q + k] * by);
+#pragma unroll
+            for (int pl = 0; pl < kPl; ++pl) code[pl][k] = one.p[pl];
+          }
+#pragma unroll
+          for (int pl = 0; pl < kPl; ++pl) {
+            if (t.by_row && valid && c < t.pitch_row)
+              *reinterpret_cast<uint2*>(t.by_row + pl * t.plane_row + row * t.pitch_row + c) =
+                  make_uint2(code[pl][0] | (uint32_t)code[pl][1] << 16, code[pl][2] | (uint32_t)code[pl][3] << 16);
+            if (t.by_cat && row < t.pitch_cat) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (c + k < t.cats) {
+                  uint16_t* const to = t.by_cat + pl * t.plane_cat + (c + k) * t.pitch_cat + row;
+                  to[0] = code[pl][k];
+                  if (S::BN < kKBytes / 2 && row + S::BN < t.pitch_cat) to[S::BN] = 0;   // (one tile of rows, shorter than a step)
+                }
+            }
+          }
+        }
+    }
+    if (t.bias_parts) {
+      // over the wave's rows: its j, then the 32 lanes of a half
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float s = 0.f;
+#pragma unroll
+          for (int j = 0; j < S::FN; ++j) s += sums[i][j][r];
+          s = over_lanes<16>(s, Sum());
+          s += __shfl_xor(s, 16);
+          if ((lane & 31) == 0) of_bias[wave / S::waves_m * S::BM + wm + 32 * i + 8 * (r / 4) + 4 * half + r % 4] = s;
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < S::BM; i += S::threads) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < S::waves / S::waves_m; ++w) s += of_bias[w * S::BM + i];
+        if (m - wm + i < t.cats) t.bias_parts[n / S::BN * t.cats + m - wm + i] = s;
+      }
+    }
+  });
+}
+template <typename T, typename S, bool kPlanes>
+__global__ __launch_bounds__(S::threads) void gradient_kernel(GradientTask t) {
+  gradient_tile<T, S, kPlanes>(t);
+}
+
+__global__ __launch_bounds__(256) void join_bias_kernel(const float* parts, int64_t count, int64_t cats, void* out, int type,
+                                                        int64_t first) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= cats) return;
+  float s = 0.f;
+  for (int64_t i = 0; i < count; ++i) s += parts[i * cats + c];
+  store_as(out, type, first + c, s);
+}
+
+typedef TileSizes<256, 256, 128, 64> Wide;
+typedef TileSizes<128, 128, 64, 64> Middle;
+typedef TileSizes<128, 32, 32, 32> Narrow;
+int tile_rows(int64_t cats, int64_t rows) { return rows <= 32 ? 32 : ((cats + 255) / 256) * ((rows + 255) / 256) >= 192 ? 256 : 128; }
+
+template <typename T, typename S, bool kPlanes>
+void launch(const GradientTask& t, hipStream_t stream) {
+  const int64_t tiles = ((t.cats + S::BM - 1) / S::BM) * ((t.rows + S::BN - 1) / S::BN);
+  hipLaunchKernelGGL((gradient_kernel<T, S, kPlanes>), dim3((unsigned)tiles), dim3(S::threads), 0, stream, t);
+}
+template <typename T, bool kPlanes>
+void launch(const GradientTask& t, hipStream_t stream) {
+  const int size = tile_rows(t.cats, t.rows);
+  if (size == 256) launch<T, Wide, kPlanes>(t, stream);
+  else if (size == 128) launch<T, Middle, kPlanes>(t, stream);
+  else launch<T, Narrow, kPlanes>(t, stream);
+}
+
+// What the workspace holds, and how the categories are cut into pieces
+struct Plan {
+  int planes;
+  bool lay_f, lay_w;
+  int64_t rows, cats, length, piece, pieces;
+  int features_parts, weight_parts;
+  int64_t of_p, expo, most, f, f_turned, w, w_turned, by_row, by_cat, features, weight, bias, bytes;   // offsets
+
+  Plan(const Matrix2& fm, const Matrix2& wm, bool of_features, bool of_weight, bool of_bias) {
+    planes = planes_of(fm.type);
+    rows = fm.rows();
+    cats = wm.examples;
+    length = fm.length;
+    lay_f = !readable(fm);
+    lay_w = !readable(wm);
+    // a piece's dx takes 2^26 entries or so, 4096 categories at least and 2^20 at most, in tiles of 256
+    const int64_t most_cats = std::min<int64_t>(kMaxLength, std::max<int64_t>(4096, ((int64_t)1 << 26) / std::max<int64_t>(rows, 1) / 256 * 256));
+    pieces = (cats + most_cats - 1) / most_cats;
+    piece = pieces == 1 ? cats : round_up((cats + pieces - 1) / pieces, 256);
+    pieces = (cats + piece - 1) / piece;
+    const int products = planes == 3 ? 6 : 1;
+    features_parts = parts_for(length, rows, laid_length(piece) * 2 / kKBytes * products);
+    features_parts = (int)std::min<int64_t>(features_parts, std::max<int64_t>(1, laid_length(piece) * 2 / kKBytes));
+    weight_parts = parts_for(length, piece, laid_length(rows) * 2 / kKBytes * products);
+    weight_parts = (int)std::min<int64_t>(weight_parts, std::max<int64_t>(1, laid_length(rows) * 2 / kKBytes));
+    int64_t at = 0;
+    auto take = [&](bool needed, int64_t n) {
+      const int64_t here = at;
+      if (needed) at += round_up(n, 256);
+      return here;
+    };
+    of_p = take(true, rows * 4);
+    expo = take(true, rows * 4);
+    most = take(true, kMostBlocks * 4);
+    f = take(lay_f, laid_bytes(rows, length, planes));
+    f_turned = take(of_weight, laid_bytes(length, rows, planes));
+    w = take(lay_w, laid_bytes(piece, length, planes));
+    w_turned = take(of_features, laid_bytes(length, piece, planes));
+    by_row = take(of_features, laid_bytes(rows, piece, planes));
+    by_cat = take(of_weight, laid_bytes(piece, rows, planes));
+    features = take(of_features && (features_parts > 1 || pieces > 1), features_parts * rows * length * 4);
+    weight = take(of_weight && weight_parts > 1, weight_parts * piece * length * 4);
+    bias = take(of_bias, (rows + 31) / 32 * piece * 4);
+    bytes = at;
+  }
+};
+}  // namespace
+
+int64_t linear_scores_backward_workspace(const Matrix2& f, const Matrix2& w, bool of_features, bool of_weight, bool of_bias) {
+  return Plan(f, w, of_features, of_weight, of_bias).bytes;
+}
+
+void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const GivenRef& given_in, const float* d_grad_logp,
+                            const float* d_grad_log_sum, const float* d_log_sum, const LinearGradients& out, void* d_work, int64_t work_bytes,
+                            hipStream_t stream) {
+  check_linear(f, w, bias, given_in, "gradient of linear scores");
+  const int64_t rows = f.rows(), cats = w.examples;
+  if (given_in.slots && (!given_in.p || !d_grad_logp)) fail(PCM_ERR_ARG, "gradient of linear scores: given categories and their derivatives go together");
+  if (!w.p || (rows && (!f.p || !d_log_sum))) fail(PCM_ERR_ARG, "gradient of linear scores: a pointer is null");
+  const Plan plan(f, w, out.features, out.weight, out.bias);
+  check_workspace(d_work, work_bytes, plan.bytes, "gradient of linear scores");
+  char* const work = static_cast<char*>(d_work);
+  GivenRef given = given_in;
+  given.vars = f.vars;
+  float* const of_p = reinterpret_cast<float*>(work + plan.of_p);
+  int *const expo = reinterpret_cast<int*>(work + plan.expo), *const most = reinterpret_cast<int*>(work + plan.most);
+  if (!rows) {   // sums of nothing
+    if (out.weight) join_parts(nullptr, 0, false, f.length, cats, Finish(), out.weight, f.type, f.length, stream);
+    if (out.bias) join_parts(nullptr, 0, false, cats, 1, Finish(), out.bias, bias.type, cats, stream);
+    return;
+  }
+  hipLaunchKernelGGL(row_terms_kernel, dim3(kMostBlocks), dim3(256), 0, stream, given, d_grad_logp, d_grad_log_sum, d_log_sum, rows, cats, of_p, expo, most);
+  const int planes = plan.planes, products = planes == 3 ? 6 : 1, size = f.type == PCM_F32 ? 4 : 2, operands = f.type == PCM_F16 ? PCM_F16 : PCM_BF16;
+  const int64_t turned_f = laid_length(rows);
+  char* at = work + plan.f;
+  const Operand features = operand_of(f, at, stream);
+  LayOut scaled;
+  scaled.expo = expo;
+  scaled.most = most;
+  if (out.weight) lay_out(f, 0, rows, true, scaled, work + plan.f_turned, stream);
+  LayOut masked;
+  masked.mask = bias;
+  const bool features_direct = plan.pieces == 1 && plan.features_parts == 1;
+  for (int64_t first = 0; first < cats; first += plan.piece) {
+    const int64_t count = std::min(plan.piece, cats - first), laid = laid_length(count);
+    GradientTask t{};
+    if (plan.lay_w) {
+      lay_out(w, first, count, false, LayOut(), work + plan.w, stream);
+      t.w = {work + plan.w, laid_length(w.length) * 2, count * laid_length(w.length) * 2};
+    } else {
+      t.w = {static_cast<const char*>(w.p) + first * w.stride_ex * 2, w.stride_ex * 2, 0};
+    }
+    t.f = features;
+    t.cats = count;
+    t.rows = rows;
+    t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), products, 1};
+    t.bias = bias;
+    if (t.bias.p) t.bias.p = static_cast<const char*>(bias.p) + first * (bias.type == PCM_F32 ? 4 : 2);
+    t.given = given;
+    t.first = first;
+    t.grad_logp = d_grad_logp;
+    t.log_sum = d_log_sum;
+    t.of_p = of_p;
+    t.expo = expo;
+    t.pitch_row = laid;
+    t.pitch_cat = turned_f;
+    t.plane_row = rows * laid;
+    t.plane_cat = count * turned_f;
+    t.by_row = out.features ? reinterpret_cast<uint16_t*>(work + plan.by_row) : nullptr;
+    t.by_cat = out.weight ? reinterpret_cast<uint16_t*>(work + plan.by_cat) : nullptr;
+    t.bias_parts = out.bias ? reinterpret_cast<float*>(work + plan.bias) : nullptr;
+    if (f.type == PCM_F32) launch<bf16, true>(t, stream);
+    else if (f.type == PCM_BF16) launch<bf16, false>(t, stream);
+    else launch<f16, false>(t, stream);
+    if (out.bias) {
+      const int64_t each = tile_rows(count, rows);
+      hipLaunchKernelGGL(join_bias_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, stream, t.bias_parts, (rows + each - 1) / each, count,
+                         out.bias, bias.type, first);
+    }
+    if (out.features) {
+      lay_out(w, first, count, true, masked, work + plan.w_turned, stream);
+      OutTask o{};
+      o.a = {work + plan.w_turned, laid * 2, f.length * laid * 2};
+      o.b = {t.by_row, laid * 2, t.plane_row * 2};
+      o.m = f.length;
+      o.n = rows;
+      o.steps = {(int)(laid * 2 / kKBytes), products, (int)std::min<int64_t>(plan.features_parts, laid * 2 / kKBytes)};
+      o.out = features_direct ? out.features : work + plan.features;
+      o.type = features_direct ? f.type : kRawSums;
+      o.pitch = f.length;
+      o.add = first > 0;
+      o.finish.expo = expo;
+      product_out(operands, o, stream);
+    }
+    if (out.weight) {
+      OutTask o{};
+      o.a = {work + plan.f_turned, turned_f * 2, f.length * turned_f * 2};
+      o.b = {t.by_cat, turned_f * 2, t.plane_cat * 2};
+      o.m = f.length;
+      o.n = count;
+      o.steps = {(int)(turned_f * 2 / kKBytes), products, plan.weight_parts};
+      o.pitch = f.length;
+      o.finish.most = most;
+      char* const to = static_cast<char*>(out.weight) + first * f.length * size;
+      o.out = plan.weight_parts > 1 ? work + plan.weight : to;
+      o.type = plan.weight_parts > 1 ? kRawSums : f.type;
+      product_out(operands, o, stream);
+      if (plan.weight_parts > 1) join_parts(o.out, plan.weight_parts, false, o.m, o.n, o.finish, to, f.type, f.length, stream);
+    }
+  }
+  if (out.features && !features_direct) {
+    Finish finish;
+    finish.expo = expo;
+    // (a last piece of fewer steps than parts leaves some of them as the pieces before it did)
+    join_parts(work + plan.features, plan.features_parts, false, f.length, rows, finish, out.features, f.type, f.length, stream);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of linear_scores_backward failed: %s", hipGetErrorString(e));
+}
+
+}  // namespace pcm

@@ -1,0 +1,120 @@
+// Scores of categories that are products of features and weights, x[n][c] = f[n] . w[c] + b[c]: what the kernels of linear_scores.hip,
+// linear_gradient.hip, product8.hip and lay_out.hip share.
+//
+// All products run over rows that are neighbours along the summed axis, in pieces of 128 bytes (product_tiles.hip.hpp): 16-bit
+// types as they are, 8-bit codes as whole numbers, and float as three bfloat16 planes h + m + l, whose six largest products
+// (hl lh mm hm mh hh, in this order) leave out what lies 2^-26 below the product.  Rows that do not lie so (odd lengths, other
+// strides, float, or summed along the other axis) are laid out in the workspace first (lay_out.hip).
+#pragma once
+
+#include "category_rows.hpp"
+
+namespace pcm {
+
+constexpr int64_t kMaxLength = 1 << 20;      // entries of a row of features or weights
+constexpr int64_t kMaxLinearRows = 1 << 22;  // rows of features (tokens)
+constexpr int64_t kMaxLength8 = 131071;      // of 8-bit rows: so many products of -128 and -128 stay within 32 bits
+constexpr int kKBytes = 128;                 // bytes of a row that a step of a product takes
+constexpr int kDeadRow = -100000;            // the exponent of a row whose gradient is nothing
+
+struct Matrix2 {                             // rows of a matrix in device memory, [example][variable][entry] (weights: vars = 1)
+  const void* p;
+  int type;                                  // PCM_F32, PCM_BF16, PCM_F16
+  int64_t stride_ex, stride_var, stride;
+  int64_t examples;
+  int32_t vars, length;
+  __host__ __device__ int64_t rows() const { return examples * vars; }
+};
+struct Operand {                             // rows that a product can read: 16-byte aligned, multiples of 128 bytes, zeros behind the end
+  const void* p;
+  int64_t pitch, plane;                      // bytes from row to row, and from plane to plane (float)
+};
+struct BiasRef {                             // a number per category; null: zeros
+  const void* p;
+  int type;
+};
+struct ScaleRef {                            // of 8-bit rows: scales of b's rows (n) and of a's rows (m); null: none
+  const float *n, *m;
+};
+
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+inline int planes_of(int type) { return type == PCM_F32 ? 3 : 1; }
+// entries of a laid out row: a multiple of 128 bytes of 16-bit entries
+inline int64_t laid_length(int64_t length) { return round_up(length, kKBytes / 2); }
+inline int64_t laid_bytes(int64_t rows, int64_t length, int planes) { return round_up(rows * laid_length(length) * 2 * planes, 256); }
+
+// What laying out changes on the way: rows are scaled by powers of two (float exponents `expo` relative to the largest of `most`,
+// nothing of a row at kDeadRow), categories that the bias masks become zeros.
+struct LayOut {
+  const int* expo = nullptr;
+  const int* most = nullptr;                 // 256 candidates of the largest exponent
+  BiasRef mask{nullptr, 0};
+};
+// x, rows [first, first + count) of it, as 16-bit planes: [plane][row][laid_length(length)], or with `turned`
+// [plane][entry][laid_length(count)]
+void lay_out(const Matrix2& x, int64_t first, int64_t count, bool turned, const LayOut& with, void* d_to, hipStream_t stream);
+// whether a product can read the rows where they are
+bool readable(const Matrix2& x);
+
+// what the entry points share
+void check_linear(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const GivenRef& given, const char* what);
+void check_workspace(const void* d_work, int64_t work_bytes, int64_t need, const char* what);
+Operand operand_of(const Matrix2& x, char*& work, hipStream_t stream);
+
+int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w);
+void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum,
+                   void* d_work, int64_t work_bytes, hipStream_t stream);
+int64_t linear_scores8_workspace(int64_t rows, int64_t cats);
+void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
+                    int32_t length, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
+                    hipStream_t stream);
+struct LinearGradients {                     // results, each may be null
+  void *features, *weight;                   // [rows][length], [cats][length], of the features' type
+  void* bias;                                // [cats], of the bias's type
+};
+int64_t linear_scores_backward_workspace(const Matrix2& f, const Matrix2& w, bool of_features, bool of_weight, bool of_bias);
+void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const GivenRef& given, const float* d_grad_logp,
+                            const float* d_grad_log_sum, const float* d_log_sum, const LinearGradients& out, void* d_work, int64_t work_bytes,
+                            hipStream_t stream);
+void rows8(const Matrix2& x, int8_t* d_codes, float* d_scales, hipStream_t stream);
+int64_t product8_workspace(int64_t rows, int64_t cats, int32_t length);
+void product8(const int8_t* a, const float* a_scales, int64_t rows, const int8_t* b, const float* b_scales, int64_t cats, int32_t length,
+              const BiasRef& bias, void* d_out, int type, int64_t pitch, void* d_work, int64_t work_bytes, hipStream_t stream);
+
+#ifdef __HIPCC__
+// The bias of category m with what masks it at -inf, and everything behind the last category
+__device__ __forceinline__ float bias_at(const BiasRef& b, int64_t m, int64_t cats) {
+  if (m >= cats) return -INFINITY;
+  if (!b.p) return 0.f;
+  if (b.type == PCM_F32) return seen(static_cast<const float*>(b.p)[m]);
+  if (b.type == PCM_BF16) return seen(static_cast<const bf16*>(b.p)[m]);
+  return seen(static_cast<const f16*>(b.p)[m]);
+}
+// a score: the product and the bias, -inf where the bias masks the category, whatever the product
+__device__ __forceinline__ float score_of(float product, float bias) {
+  return bias == -INFINITY ? -INFINITY : product + bias;
+}
+__device__ __forceinline__ int largest_exponent(const int* most) {   // by every lane of a wave
+  const int lane = threadIdx.x & 63;
+  int e = max(max(most[lane], most[lane + 64]), max(most[lane + 128], most[lane + 192]));
+#pragma unroll
+  for (int s = 32; s; s /= 2) e = max(e, __shfl_xor(e, s));
+  return e;
+}
+// A float as three bfloat16: the nearest one, the nearest one to what is left, and once more; the sum is within 2^-26 of it.
+// (what would round up beyond the type's range is cut off instead)
+struct Planes {
+  bf16 h, m, l;
+};
+__device__ __forceinline__ Planes planes(float x) {
+  Planes p;
+  p.h = (bf16)x;
+  if (__builtin_isinf((float)p.h) && !__builtin_isinf(x)) p.h = __builtin_bit_cast(bf16, (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16));
+  const float r = x - (float)p.h;
+  p.m = (bf16)r;
+  p.l = (bf16)(r - (float)p.m);
+  return p;
+}
+#endif
+
+}  // namespace pcm

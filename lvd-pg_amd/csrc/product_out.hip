@@ -1,0 +1,129 @@
+// Products that are written out: gradients of features and weights, and products of 8-bit rows.
+#include "product_out.hip.hpp"
+
+namespace pcm {
+
+namespace {
+template <typename T, typename S>
+__device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
+  product_tile<T, S>(t.a, t.b, t.m, t.n, t.steps, [&](auto& sums, int64_t m, int64_t n, char* lds) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, wm = threadIdx.x / 64 % S::waves_m * S::WM;
+    const bool raw = t.type == kRawSums;
+    const int most = t.finish.most ? largest_exponent(t.finish.most) : 0;
+    float* const bias = reinterpret_cast<float*>(lds);   // [BM]
+    float* const scale = bias + S::BM;                   // [BM]
+    const int64_t m0 = m - wm;
+    __syncthreads();
+    for (int i = threadIdx.x; i < S::BM; i += S::threads) {
+      bias[i] = m0 + i < t.m ? bias_of(t.finish.bias, m0 + i) : 0.f;
+      scale[i] = t.finish.scale.m && m0 + i < t.m ? t.finish.scale.m[m0 + i] : 1.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int64_t row = n + 32 * j + (lane & 31);
+      if (row >= t.n) continue;
+      const FinishAt finish(t.finish, row, most);
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int in = 32 * i + 8 * q + 4 * half;
+          const int64_t col = m + in;
+          if (col >= t.m) continue;
+          if (raw) {
+            uint32_t* const to = static_cast<uint32_t*>(t.out) + ((int64_t)blockIdx.y * t.n + row) * t.pitch + col;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < t.m) {
+                auto v = sums[i][j][4 * q + e];
+                if constexpr (!__is_same(T, int8_t)) {
+                  if (t.add) v += __builtin_bit_cast(float, to[e]);
+                }
+                to[e] = __builtin_bit_cast(uint32_t, v);
+              }
+            continue;
+          }
+          const float4 b = *reinterpret_cast<const float4*>(bias + wm + in), s = *reinterpret_cast<const float4*>(scale + wm + in);
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = finish((float)sums[i][j][4 * q + e], (&s.x)[e], (&b.x)[e]);
+          const int64_t at = row * t.pitch + col;
+          if (fours && col + 4 <= t.m) store_four(t.out, t.type, at, v);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < t.m) store_as(t.out, t.type, at + e, v[e]);
+        }
+    }
+  });
+}
+template <typename T, typename S>
+__global__ __launch_bounds__(S::threads) void out_kernel(OutTask t, bool fours) {
+  out_tile<T, S>(t, fours);
+}
+
+__global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, int count, bool whole, int64_t m, int64_t n, Finish finish, void* out,
+                                                         int type, int64_t pitch) {
+  const int most = finish.most ? largest_exponent(finish.most) : 0;
+  const int64_t all = n * m;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / m, col = i % m;
+    float sum = 0.f;
+    if (whole) {
+      int s = 0;
+      for (int p = 0; p < count; ++p) s += (int)parts[p * all + i];
+      sum = (float)s;
+    } else {
+      for (int p = 0; p < count; ++p) sum += __builtin_bit_cast(float, parts[p * all + i]);
+    }
+    const FinishAt f(finish, row, most);
+    store_as(out, type, row * pitch + col, f(sum, finish.scale.m ? finish.scale.m[col] : 1.f, bias_of(finish.bias, col)));
+  }
+}
+
+typedef TileSizes<256, 256, 128, 64> Wide;
+typedef TileSizes<128, 128, 64, 64> Middle;
+typedef TileSizes<128, 32, 32, 32> Narrow;
+
+template <typename T, typename S>
+void launch(const OutTask& t, hipStream_t stream) {
+  const int64_t tiles = ((t.m + S::BM - 1) / S::BM) * ((t.n + S::BN - 1) / S::BN);
+  if (tiles > 0x7fffffff) fail(PCM_ERR_UNSUPPORTED, "product: %lld tiles", (long long)tiles);
+  const int size = t.type == PCM_F32 ? 4 : 2;
+  const bool fours = t.type != kRawSums && t.pitch % 4 == 0 && (uintptr_t)t.out % (4 * size) == 0;
+  hipLaunchKernelGGL((out_kernel<T, S>), dim3((unsigned)tiles, (unsigned)t.steps.parts), dim3(S::threads), 0, stream, t, fours);
+}
+bool wide(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
+template <typename T>
+void launch(const OutTask& t, hipStream_t stream) {
+  if (t.n <= 32) launch<T, Narrow>(t, stream);
+  else if (wide(t.m, t.n)) launch<T, Wide>(t, stream);
+  else launch<T, Middle>(t, stream);
+}
+}  // namespace
+
+int parts_for(int64_t m, int64_t n, int64_t steps) {
+  if (wide(m, n) && n > 32) return 1;
+  const int64_t tiles = ((m + 127) / 128) * ((n + (n <= 32 ? 31 : 127)) / (n <= 32 ? 32 : 128));
+  // as many parts as fill the device twice over, each of eight steps or more
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 8, 64}));
+}
+
+void product_out(int operands, const OutTask& t, hipStream_t stream) {
+  if (operands == PCM_BF16) launch<bf16>(t, stream);
+  else if (operands == PCM_F16) launch<f16>(t, stream);
+  else launch<int8_t>(t, stream);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of a product failed: %s", hipGetErrorString(e));
+}
+
+void join_parts(const void* parts, int count, bool whole, int64_t m, int64_t n, const Finish& finish, void* out, int type, int64_t pitch, hipStream_t stream) {
+  hipLaunchKernelGGL(join_parts_kernel, dim3((unsigned)std::min<int64_t>((n * m + 255) / 256, 1 << 14)), dim3(256), 0, stream,
+                     static_cast<const uint32_t*>(parts), count, whole, m, n, finish, out, type, pitch);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of join_parts failed: %s", hipGetErrorString(e));
+}
+
+}  // namespace pcm

@@ -1,0 +1,241 @@
+// Products of two matrices whose rows are both neighbours along the summed axis, sum_k a[m][k] b[n][k], on the matrix cores: the tile
+// loop that the kernels of linear_scores.hip, linear_gradient.hip and product8.hip share, each with what it does with the sums.
+#pragma once
+
+#include <algorithm>
+
+#include "linear_scores.hpp"
+
+namespace pcm {
+
+// What a product sums over: steps [first, first + count) of 128 bytes, of one pair of planes or of the six of float.  With parts > 1
+// part blockIdx.y takes its share of the steps.
+struct Steps {
+  int count, products, parts;
+};
+
+#ifdef __HIPCC__
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// 32 x 32 sums over 32 bytes of both operands' rows: lane l gives 16 bytes of row l % 32, of its half; it gets of the sums, as entry i,
+// row 8 (i / 4) + 4 (l / 32) + i % 4 of a and row l % 32 of b.
+template <typename T>
+struct Cores;
+template <>
+struct Cores<bf16> {
+  typedef v16f Sums;
+  static __device__ __forceinline__ v16f mma(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Cores<f16> {
+  typedef v16f Sums;
+  static __device__ __forceinline__ v16f mma(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Cores<int8_t> {
+  typedef v16i Sums;
+  static __device__ __forceinline__ v16i mma(v4i a, v4i b, v16i c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+};
+
+typedef __attribute__((address_space(3))) void LdsVoid;
+
+template <int kBM, int kBN, int kWM, int kWN>
+struct TileSizes {
+  static constexpr int BM = kBM, BN = kBN, WM = kWM, WN = kWN;   // rows of a and of b, of a workgroup and of a wave
+  static constexpr int waves_m = kBM / kWM, waves = waves_m * (kBN / kWN), threads = 64 * waves;
+  static constexpr int FM = kWM / 32, FN = kWN / 32;
+  static constexpr int stage = (kBM + kBN) * kKBytes;            // bytes in LDS
+};
+
+// A wave's share of a stage: requests of 1 KB, eight rows of 128 bytes, straight into LDS.  There chunk c (16 bytes) of row r lies at
+// c ^ (r / 2) % 8 of the row, so that sixteen lanes reading one chunk of neighbouring rows meet all banks once.  Rows past the
+// end are read from the last row; what they give is not used.
+template <typename S>
+struct TileLoader {
+  static constexpr int each = S::stage / 1024 / S::waves;
+  static_assert(each * 1024 * S::waves == S::stage && S::BM % 8 == 0 && S::BN % 8 == 0);
+  const char *a0, *b0;
+  int64_t plane_a, plane_b;
+  __amdgpu_buffer_rsrc_t a, b;
+  uint32_t at[each];
+  uint32_t k, begin, end;      // the bytes of a row that come next, and between which
+  int wave, product;
+
+  // the six products of planes h m l (0 1 2), smallest first: hl lh mm hm mh hh, two bits each
+  __device__ __forceinline__ void choose_planes() {
+    const int64_t pa = 0x118 >> 2 * product & 3, pb = 0x52 >> 2 * product & 3;
+    a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a0 + pa * plane_a), 0, 0xffffffffu, 0x00020000);
+    b = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b0 + pb * plane_b), 0, 0xffffffffu, 0x00020000);
+  }
+  __device__ __forceinline__ TileLoader(const Operand& oa, const Operand& ob, int64_t m0, int64_t n0, int64_t m, int64_t n, int first, int count,
+                                        int products) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    a0 = static_cast<const char*>(oa.p) + m0 * oa.pitch;
+    b0 = static_cast<const char*>(ob.p) + n0 * ob.pitch;
+    plane_a = oa.plane;
+    plane_b = ob.plane;
+    product = 6 - products;
+    k = begin = (uint32_t)first * kKBytes;
+    end = begin + (uint32_t)count * kKBytes;
+    choose_planes();
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < each; ++i) {
+      const int q = i * S::waves + wave;
+      const bool of_a = q < S::BM / 8;
+      const int row = (of_a ? q : q - S::BM / 8) * 8 + lane / 8;
+      const int64_t last = (of_a ? m - m0 : n - n0) - 1;
+      at[i] = (uint32_t)((row < last ? row : last) * (of_a ? oa.pitch : ob.pitch)) + ((lane & 7) ^ (row >> 1 & 7)) * 16;
+    }
+  }
+  __device__ __forceinline__ void load(char* lds) {
+#pragma unroll
+    for (int i = 0; i < each; ++i) {
+      const int q = i * S::waves + wave;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(q < S::BM / 8 ? a : b, (LdsVoid*)(lds + q * 1024), 16, at[i], k, 0, 0);
+    }
+    k += kKBytes;
+    if (k == end && product < 5) {
+      k = begin;
+      ++product;
+      choose_planes();
+    }
+  }
+};
+
+// The tile of workgroup blockIdx.x: each of the eight dies takes a run of tiles, four rows of b's tiles at a time, so that what its
+// workgroups read at one time meets in its cache
+struct TileAt {
+  int64_t m0, n0;
+};
+template <typename S>
+__device__ __forceinline__ TileAt tile_at(int64_t m, int64_t n) {
+  const int tiles_m = (int)((m + S::BM - 1) / S::BM), tiles_n = (int)((n + S::BN - 1) / S::BN);
+  const int all = gridDim.x, die = blockIdx.x % 8;
+  const int id = die * (all / 8) + min(die, all % 8) + blockIdx.x / 8;
+  constexpr int kRows = 4;
+  const int group = id / (kRows * tiles_m), in = id % (kRows * tiles_m);
+  const int rows = min(kRows, tiles_n - group * kRows);
+  return {(int64_t)(in / rows) * S::BM, (int64_t)(group * kRows + in % rows) * S::BN};
+}
+
+// Sums of the tile at (m0, n0), handed to done(sums, m, n, lds): sums[i][j] of the wave's rows m + 32 i of a and n + 32 j of b, and the
+// first stage's LDS for its own use (after a barrier).
+//
+// Two stages of 128 bytes in LDS.  Fragments are read from LDS one step of 32 bytes ahead of their products, and the barrier at a stage's
+// end stands before its last products: they run while the next stage's first fragments are on their way.  A stage's memory
+// requests go out as soon as that barrier has freed its LDS, one stage ahead of their use.
+template <typename T, typename S, typename Done>
+__device__ __forceinline__ void product_tile(const Operand& a, const Operand& b, int64_t m, int64_t n, const Steps& steps, Done done) {
+  __shared__ __attribute__((aligned(1024))) char s0[S::stage];
+  __shared__ __attribute__((aligned(1024))) char s1[S::stage];
+  const TileAt tile = tile_at<S>(m, n);
+  const int part = blockIdx.y, first = (int)((int64_t)steps.count * part / steps.parts);
+  const int count = (int)((int64_t)steps.count * (part + 1) / steps.parts) - first;
+  TileLoader<S> from(a, b, tile.m0, tile.n0, m, n, first, count, steps.products);
+  const int stages = count * steps.products;
+  const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5, swap = row >> 1 & 7;
+  const int wm = from.wave % S::waves_m * S::WM, wn = from.wave / S::waves_m * S::WN;
+  const int at_a = (wm + row) * kKBytes, at_b = (S::BM + wn + row) * kKBytes;
+  typename Cores<T>::Sums sums[S::FM][S::FN] = {};
+  v4i fa[2][S::FM], fb[2][S::FN];
+  auto read = [&](const char* s, int step, int w) {
+    const int c = ((2 * step + half) ^ swap) * 16;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) fb[w][j] = *reinterpret_cast<const v4i*>(s + at_b + j * 32 * kKBytes + c);
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) fa[w][i] = *reinterpret_cast<const v4i*>(s + at_a + i * 32 * kKBytes + c);
+  };
+  auto multiply = [&](int w) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) sums[i][j] = Cores<T>::mma(fa[w][i], fb[w][j], sums[i][j]);
+  };
+  auto mix = [] {   // a fragment's read between two products
+#pragma unroll
+    for (int i = 0; i < S::FM * S::FN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i < S::FM + S::FN) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+  };
+  auto stage = [&](char* mine, const char* next, int t) {
+#pragma unroll
+    for (int step = 1; step < 4; ++step) {
+      read(mine, step, step & 1);
+      multiply(~step & 1);
+      mix();
+    }
+    __syncthreads();
+    if (t + 1 < stages) read(next, 0, 0);
+    if (t + 2 < stages) from.load(mine);
+    multiply(1);
+  };
+  if (stages > 0) {
+    from.load(s0);
+    __syncthreads();
+    if (stages > 1) from.load(s1);
+    read(s0, 0, 0);
+    for (int t = 0; t < stages; t += 2) {
+      stage(s0, s1, t);
+      if (t + 1 < stages) stage(s1, s0, t + 1);
+    }
+  }
+  done(sums, tile.m0 + wm, tile.n0 + wn, s0);
+}
+
+// ---- scores of categories (a) under rows of features (b) -------------------------------------------------------
+struct ScoreInputs {
+  Operand w, f;
+  int64_t cats, rows;
+  Steps steps;
+  BiasRef bias;
+  ScaleRef scale;
+  GivenRef given;
+};
+__device__ __forceinline__ float bits_float(float v) { return v; }
+__device__ __forceinline__ float bits_float(int v) { return __builtin_bit_cast(float, v); }
+// bias and scales of a tile's categories into LDS; barriers before and after
+template <typename S>
+__device__ __forceinline__ void tile_constants(const ScoreInputs& t, int64_t m0, float* bias, float* scale) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < S::BM; i += S::threads) {
+    bias[i] = bias_at(t.bias, m0 + i, t.cats);
+    scale[i] = t.scale.m && m0 + i < t.cats ? t.scale.m[m0 + i] : 1.f;
+  }
+  __syncthreads();
+}
+// The wave's sums of its j-th rows of features become scores, in place (as their bits, where sums are whole numbers)
+template <typename S, typename Sums>
+__device__ __forceinline__ void scores_of(const ScoreInputs& t, Sums (&sums)[S::FM][S::FN], int j, float scale_n, const float* bias,
+                                          const float* scale, int half) {
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = 32 * i + 8 * q + 4 * half;
+      const float4 b = *reinterpret_cast<const float4*>(bias + at);
+      float4 s = make_float4(1.f, 1.f, 1.f, 1.f);
+      if constexpr (__is_same(Sums, v16i)) s = *reinterpret_cast<const float4*>(scale + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float be = (&b.x)[e];
+        if constexpr (__is_same(Sums, v16i)) {
+          sums[i][j][4 * q + e] = __builtin_bit_cast(int, score_of((float)sums[i][j][4 * q + e] * scale_n * (&s.x)[e], be));
+        } else {
+          sums[i][j][4 * q + e] = score_of(sums[i][j][4 * q + e], be);
+        }
+      }
+    }
+}
+#endif
+
+}  // namespace pcm

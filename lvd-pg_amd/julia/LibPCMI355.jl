@@ -120,6 +120,24 @@ pcm_checkpoint_rows(d_rows, type, stride_ex, stride_var, stride_cat, num_example
     ccall((:pcm_checkpoint_rows, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int32, Int32, Ptr{UInt8}, Ptr{Int32}, Ptr{Cvoid}), d_rows, type, stride_ex, stride_var, stride_cat, num_examples, num_vars, num_cats, d_codes, d_scales, stream)
 pcm_restore_rows(d_codes, d_scales, num_examples, num_vars, num_cats, d_rows, type, stride_ex, stride_var, stride_cat, stream) =
     ccall((:pcm_restore_rows, libpcmi355), Cint, (Ptr{UInt8}, Ptr{Int32}, Int64, Int32, Int32, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Ptr{Cvoid}), d_codes, d_scales, num_examples, num_vars, num_cats, d_rows, type, stride_ex, stride_var, stride_cat, stream)
+pcm_linear_scores_workspace(d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats) =
+    ccall((:pcm_linear_scores_workspace, libpcmi355), Int64, (Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32, Int32, Int32), d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats)
+pcm_linear_scores(d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats, d_bias, bias_type, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_logp, d_log_sum, d_work, work_bytes, stream) =
+    ccall((:pcm_linear_scores, libpcmi355), Cint, (Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32, Int32, Int32, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int32, Ptr{Float32}, Ptr{Float32}, Ptr{Cvoid}, Int64, Ptr{Cvoid}), d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats, d_bias, bias_type, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_logp, d_log_sum, d_work, work_bytes, stream)
+pcm_linear_scores_backward_workspace(d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats, of) =
+    ccall((:pcm_linear_scores_backward_workspace, libpcmi355), Int64, (Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32, Int32, Int32, Int32), d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats, of)
+pcm_linear_scores_backward(d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats, d_bias, bias_type, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_grad_logp, d_grad_log_sum, d_log_sum, d_grad_features, d_grad_weight, d_grad_bias, d_work, work_bytes, stream) =
+    ccall((:pcm_linear_scores_backward, libpcmi355), Cint, (Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int64, Int64, Int32, Int32, Int32, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int32, Ptr{Float32}, Ptr{Float32}, Ptr{Float32}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Ptr{Cvoid}), d_features, d_weight, type, stride_ex, stride_var, stride, weight_stride_cat, weight_stride, num_examples, num_vars, length, num_cats, d_bias, bias_type, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_grad_logp, d_grad_log_sum, d_log_sum, d_grad_features, d_grad_weight, d_grad_bias, d_work, work_bytes, stream)
+pcm_rows8(d_rows, type, stride_ex, stride_var, stride, num_examples, num_vars, length, d_codes, d_scales, stream) =
+    ccall((:pcm_rows8, libpcmi355), Cint, (Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int64, Int32, Int32, Ptr{Int8}, Ptr{Float32}, Ptr{Cvoid}), d_rows, type, stride_ex, stride_var, stride, num_examples, num_vars, length, d_codes, d_scales, stream)
+pcm_product8_workspace(num_rows, num_channels, length) =
+    ccall((:pcm_product8_workspace, libpcmi355), Int64, (Int64, Int64, Int32), num_rows, num_channels, length)
+pcm_product8(d_rows, d_row_scales, num_rows, d_channels, d_channel_scales, num_channels, length, d_bias, bias_type, d_out, type, out_stride, d_work, work_bytes, stream) =
+    ccall((:pcm_product8, libpcmi355), Cint, (Ptr{Int8}, Ptr{Float32}, Int64, Ptr{Int8}, Ptr{Float32}, Int64, Int32, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Int32, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}), d_rows, d_row_scales, num_rows, d_channels, d_channel_scales, num_channels, length, d_bias, bias_type, d_out, type, out_stride, d_work, work_bytes, stream)
+pcm_linear_scores8_workspace(num_examples, num_vars, length, num_cats) =
+    ccall((:pcm_linear_scores8_workspace, libpcmi355), Int64, (Int64, Int32, Int32, Int32), num_examples, num_vars, length, num_cats)
+pcm_linear_scores8(d_features, d_feature_scales, d_weight, d_weight_scales, num_examples, num_vars, length, num_cats, d_bias, bias_type, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_logp, d_log_sum, d_work, work_bytes, stream) =
+    ccall((:pcm_linear_scores8, libpcmi355), Cint, (Ptr{Int8}, Ptr{Float32}, Ptr{Int8}, Ptr{Float32}, Int64, Int32, Int32, Int32, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Int32, Int64, Int64, Int64, Int32, Ptr{Float32}, Ptr{Float32}, Ptr{Cvoid}, Int64, Ptr{Cvoid}), d_features, d_feature_scales, d_weight, d_weight_scales, num_examples, num_vars, length, num_cats, d_bias, bias_type, d_given, given_type, given_stride_ex, given_stride_var, given_stride_slot, num_given, d_logp, d_log_sum, d_work, work_bytes, stream)
 pcm_set_timing(c, on) =
     ccall((:pcm_set_timing, libpcmi355), Cint, (Ptr{Cvoid}, Int32), c, on)
 pcm_get_timing(c, ms, n) =

@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(HERE, "..", "..", "include", "pcmi355.h")
 OUT = os.path.join(HERE, "LibPCMI355.jl")
 
-_SCALARS = {"int32_t": "Int32", "int64_t": "Int64", "float": "Float32", "int": "Cint", "uint8_t": "UInt8"}
+_SCALARS = {"int32_t": "Int32", "int64_t": "Int64", "float": "Float32", "int": "Cint", "uint8_t": "UInt8", "int8_t": "Int8"}
 _RETURNS = {"int": "Cint", "int64_t": "Int64", "const char*": "Cstring"}
 
 

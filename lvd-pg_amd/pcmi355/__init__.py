@@ -19,6 +19,7 @@ from .structures import (pairwise_MI, chow_liu_tree, learn_chow_liu_tree, hclt, 
 from .transformations import prune_pc, grow_heads_by_flows, aggregate_edge_flows, aggregate_node_flows  # noqa: F401
 from .category_rows import (CategoryScores, Checkpoint8, category_scores, category_scores_backward, checkpoint_rows,  # noqa: F401
                             restore_rows, head_scores)
+from .linear_rows import (LinearGradients, LinearScores, Rows8, linear_scores, linear_scores_backward, product8, rows8)  # noqa: F401
 from .jpc_io import write_jpc, read_jpc, write_mhpc, read_mhpc  # noqa: F401
 from . import nodes, prealloc  # noqa: F401
 from ._lib import PcmError, LIB_PATH  # noqa: F401

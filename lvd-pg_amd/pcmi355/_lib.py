@@ -22,6 +22,14 @@ lib.pcm_version.restype = ctypes.c_int
 lib.pcm_size.restype = c_i64
 lib.pcm_category_scores_workspace.restype = c_i64
 lib.pcm_category_scores_workspace.argtypes = [c_i64, c_i32, c_i32, c_i32]
+lib.pcm_linear_scores_workspace.restype = c_i64
+lib.pcm_linear_scores_workspace.argtypes = [vp, vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32]
+lib.pcm_linear_scores_backward_workspace.restype = c_i64
+lib.pcm_linear_scores_backward_workspace.argtypes = [vp, vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32]
+lib.pcm_product8_workspace.restype = c_i64
+lib.pcm_product8_workspace.argtypes = [c_i64, c_i64, c_i32]
+lib.pcm_linear_scores8_workspace.restype = c_i64
+lib.pcm_linear_scores8_workspace.argtypes = [c_i64, c_i32, c_i32, c_i32]
 lib.pcm_chow_liu_edges_workspace.restype = c_i64
 lib.pcm_chow_liu_edges_workspace.argtypes = [c_i32]
 lib.pcm_size.argtypes = [H, c_i32]
@@ -82,6 +90,14 @@ _SIGS = {
                                      vp, c_i32, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, vp],
     "pcm_checkpoint_rows": [vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, vp, vp, vp],
     "pcm_restore_rows": [vp, vp, c_i64, c_i32, c_i32, vp, c_i32, c_i64, c_i64, c_i64, vp],
+    "pcm_linear_scores": [vp, vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, vp, c_i32, vp, c_i32,
+                          c_i64, c_i64, c_i64, c_i32, vp, vp, vp, c_i64, vp],
+    "pcm_linear_scores_backward": [vp, vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, vp, c_i32, vp,
+                                   c_i32, c_i64, c_i64, c_i64, c_i32, vp, vp, vp, vp, vp, vp, vp, c_i64, vp],
+    "pcm_rows8": [vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32, vp, vp, vp],
+    "pcm_product8": [vp, vp, c_i64, vp, vp, c_i64, c_i32, vp, c_i32, vp, c_i32, c_i64, vp, c_i64, vp],
+    "pcm_linear_scores8": [vp, vp, vp, vp, c_i64, c_i32, c_i32, c_i32, vp, c_i32, vp, c_i32, c_i64, c_i64, c_i64, c_i32, vp, vp,
+                           vp, c_i64, vp],
     "pcm_set_timing": [H, c_i32],
     "pcm_get_timing": [H, vp, c_i32],
 }
