@@ -37,19 +37,20 @@ __device__ __forceinline__ void score_tile(const ScoreTask& t) {
       __builtin_amdgcn_sched_barrier(0);   // one j at a time: registers are full
       const int64_t row = n + 32 * j + (lane & 31);
       const bool valid = row < t.rows;
-      scores_of<S>(t, sums, j, t.scale.n ? t.scale.n[valid ? row : t.rows - 1] : 1.f, bias + wm, scale + wm, half);
+      float x[S::FM][16];
+      scores_of<S>(sums, j, t.scale.n ? t.scale.n[valid ? row : t.rows - 1] : 1.f, bias + wm, scale + wm, half, x);
       float largest = -INFINITY;
 #pragma unroll
       for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) largest = fmaxf(largest, bits_float(sums[i][j][r]));
+        for (int r = 0; r < 16; ++r) largest = fmaxf(largest, x[i][r]);
       const float base = largest == -INFINITY ? 0.f : largest;
       float sum = 0.f;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((bits_float(sums[i][j][r]) - base) * kLog2e);
+        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((x[i][r] - base) * kLog2e);
       // (NaN beside no other category: the sum has it, with base 0)
       Part p{sum == 0.f ? largest : base, sum};
       p = join(p, {__shfl_xor(p.base, 32), __shfl_xor(p.sum, 32)});
@@ -64,7 +65,7 @@ __device__ __forceinline__ void score_tile(const ScoreTask& t) {
           for (int i = 0; i < S::FM; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (g == 32 * i + 8 * (r / 4) + 4 * half + r % 4) found = bits_float(sums[i][j][r]);
+              found = (int)g == 32 * i + 8 * (r / 4) + 4 * half + r % 4 ? x[i][r] : found;
           t.logp[row * t.given.slots + s] = found;
         }
       }
@@ -199,7 +200,7 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   t.w = operand_of(w, work, stream);
   t.cats = w.examples;
   t.rows = f.rows();
-  t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), f.type == PCM_F32 ? 6 : 1, 1};
+  t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), f.type == PCM_F32 ? kSixOfThree : kOnePlane, 1};
   t.bias = bias;
   t.given = given;
   t.given.vars = f.vars;
@@ -228,7 +229,7 @@ void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, in
   t.w = {w, pitch, 0};
   t.cats = cats;
   t.rows = shape.rows();
-  t.steps = {(int)(pitch / kKBytes), 1, 1};
+  t.steps = {(int)(pitch / kKBytes), kOnePlane, 1};
   t.bias = bias;
   t.scale = {f_scales, w_scales};
   t.given = given;

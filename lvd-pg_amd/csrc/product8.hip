@@ -79,7 +79,7 @@ void product8(const int8_t* a, const float* a_scales, int64_t rows, const int8_t
   t.b = {a, codes, 0};
   t.m = cats;
   t.n = rows;
-  t.steps = {steps, 1, parts};
+  t.steps = {steps, kOnePlane, parts};
   t.finish.scale = {a_scales, b_scales};
   t.finish.bias = bias;
   if (parts == 1) {

@@ -8,10 +8,18 @@
 
 namespace pcm {
 
-// What a product sums over: steps [first, first + count) of 128 bytes, of one pair of planes or of the six of float.  With parts > 1
-// part blockIdx.y takes its share of the steps.
+// Which planes of a and of b are multiplied, one after the other: two bits each, the first product lowest
+struct PlanePairs {
+  int count;
+  uint32_t a, b;
+};
+constexpr PlanePairs kOnePlane{1, 0, 0}, kTwoOfB{2, 0, 0x1};   // b in two parts: the smaller one first
+constexpr PlanePairs kSixOfThree{6, 0x118, 0x52};              // h m l (0 1 2): hl lh mm hm mh hh
+// What a product sums over: `count` steps of 128 bytes for each pair of planes.  With parts > 1 part blockIdx.y takes its share of the steps.
 struct Steps {
-  int count, products, parts;
+  int count;
+  PlanePairs pairs;
+  int parts;
 };
 
 #ifdef __HIPCC__
@@ -67,22 +75,21 @@ struct TileLoader {
   __amdgpu_buffer_rsrc_t a, b;
   uint32_t at[each];
   uint32_t k, begin, end;      // the bytes of a row that come next, and between which
-  int wave, product;
+  PlanePairs pairs;
+  int wave, product = 0;
 
-  // the six products of planes h m l (0 1 2), smallest first: hl lh mm hm mh hh, two bits each
   __device__ __forceinline__ void choose_planes() {
-    const int64_t pa = 0x118 >> 2 * product & 3, pb = 0x52 >> 2 * product & 3;
+    const int64_t pa = pairs.a >> 2 * product & 3, pb = pairs.b >> 2 * product & 3;
     a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a0 + pa * plane_a), 0, 0xffffffffu, 0x00020000);
     b = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b0 + pb * plane_b), 0, 0xffffffffu, 0x00020000);
   }
   __device__ __forceinline__ TileLoader(const Operand& oa, const Operand& ob, int64_t m0, int64_t n0, int64_t m, int64_t n, int first, int count,
-                                        int products) {
+                                        const PlanePairs& of) : pairs(of) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     a0 = static_cast<const char*>(oa.p) + m0 * oa.pitch;
     b0 = static_cast<const char*>(ob.p) + n0 * ob.pitch;
     plane_a = oa.plane;
     plane_b = ob.plane;
-    product = 6 - products;
     k = begin = (uint32_t)first * kKBytes;
     end = begin + (uint32_t)count * kKBytes;
     choose_planes();
@@ -103,7 +110,7 @@ struct TileLoader {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(q < S::BM / 8 ? a : b, (LdsVoid*)(lds + q * 1024), 16, at[i], k, 0, 0);
     }
     k += kKBytes;
-    if (k == end && product < 5) {
+    if (k == end && product + 1 < pairs.count) {
       k = begin;
       ++product;
       choose_planes();
@@ -140,8 +147,8 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
   const TileAt tile = tile_at<S>(m, n);
   const int part = blockIdx.y, first = (int)((int64_t)steps.count * part / steps.parts);
   const int count = (int)((int64_t)steps.count * (part + 1) / steps.parts) - first;
-  TileLoader<S> from(a, b, tile.m0, tile.n0, m, n, first, count, steps.products);
-  const int stages = count * steps.products;
+  TileLoader<S> from(a, b, tile.m0, tile.n0, m, n, first, count, steps.pairs);
+  const int stages = count * steps.pairs.count;
   const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5, swap = row >> 1 & 7;
   const int wm = from.wave % S::waves_m * S::WM, wn = from.wave / S::waves_m * S::WN;
   const int at_a = (wm + row) * kKBytes, at_b = (S::BM + wn + row) * kKBytes;
@@ -201,8 +208,6 @@ struct ScoreInputs {
   ScaleRef scale;
   GivenRef given;
 };
-__device__ __forceinline__ float bits_float(float v) { return v; }
-__device__ __forceinline__ float bits_float(int v) { return __builtin_bit_cast(float, v); }
 // bias and scales of a tile's categories into LDS; barriers before and after
 template <typename S>
 __device__ __forceinline__ void tile_constants(const ScoreInputs& t, int64_t m0, float* bias, float* scale) {
@@ -213,26 +218,23 @@ __device__ __forceinline__ void tile_constants(const ScoreInputs& t, int64_t m0,
   }
   __syncthreads();
 }
-// The wave's sums of its j-th rows of features become scores, in place (as their bits, where sums are whole numbers)
+// The scores of the wave's j-th rows of features
 template <typename S, typename Sums>
-__device__ __forceinline__ void scores_of(const ScoreInputs& t, Sums (&sums)[S::FM][S::FN], int j, float scale_n, const float* bias,
-                                          const float* scale, int half) {
+__device__ __forceinline__ void scores_of(const Sums (&sums)[S::FM][S::FN], int j, float scale_n, const float* bias, const float* scale, int half,
+                                          float (&x)[S::FM][16]) {
 #pragma unroll
   for (int i = 0; i < S::FM; ++i)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int at = 32 * i + 8 * q + 4 * half;
       const float4 b = *reinterpret_cast<const float4*>(bias + at);
-      float4 s = make_float4(1.f, 1.f, 1.f, 1.f);
-      if constexpr (__is_same(Sums, v16i)) s = *reinterpret_cast<const float4*>(scale + at);
+      if constexpr (__is_same(Sums, v16i)) {
+        const float4 s = *reinterpret_cast<const float4*>(scale + at);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float be = (&b.x)[e];
-        if constexpr (__is_same(Sums, v16i)) {
-          sums[i][j][4 * q + e] = __builtin_bit_cast(int, score_of((float)sums[i][j][4 * q + e] * scale_n * (&s.x)[e], be));
-        } else {
-          sums[i][j][4 * q + e] = score_of(sums[i][j][4 * q + e], be);
-        }
+        for (int e = 0; e < 4; ++e) x[i][4 * q + e] = score_of((float)sums[i][j][4 * q + e] * scale_n * (&s.x)[e], (&b.x)[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][4 * q + e] = score_of(sums[i][j][4 * q + e], (&b.x)[e]);
       }
     }
 }
