@@ -3,7 +3,7 @@
 //   dx[n][c] = sum_j gl[n][j] [c = g_j] - (sum_j gl[n][j] - gz[n]) p[n][c],  p = exp(x - Z)
 //   features: dx w, weights: dx^T f, bias: sum_n dx
 // The categories are taken in pieces: the scores of a piece once more (gradient_kernel), whose dx goes into the workspace in both
-// orders, rounded to the operands' 16 bits (float: three planes; fewer than 1024 rows: two), then the piece's two products.  dx is held as dx 2^(15 - e[n]),
+// orders, rounded to the operands' 16 bits (fewer than 1024 rows: in two parts; float: as it is, in one order), then the piece's two products.  dx is held as dx 2^(15 - e[n]),
 // 2^e[n] the next power of two above what |dx| of the row can be, so that half's range holds it whatever the loss's scale; features are
 // turned with 2^(e[n] - largest e), which is exact, for the sum over rows.
 #include "product_out.hip.hpp"
@@ -53,6 +53,7 @@ struct GradientTask : ScoreInputs {
   int64_t first;                     // the piece's first category, which is row 0 of w; cats is the piece's size
   const float *grad_logp, *log_sum, *of_p;
   const int* expo;
+  float* dx;                         // float: dx [row][pitch_row]
   uint16_t* by_row;                  // dx [plane][row][pitch_row]; null: not needed
   uint16_t* by_cat;                  // dx [plane][category of the piece][pitch_cat]
   int64_t pitch_row, pitch_cat, plane_row, plane_cat;
@@ -90,7 +91,7 @@ __device__ __forceinline__ void turn(uint32_t& a, uint32_t& b) {
 
 template <typename T, typename S, int kParts>
 __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
-  product_tile<T, S>(t.w, t.f, t.cats, t.rows, t.steps, [&](auto& sums, int64_t m, int64_t n, char* lds) {
+  score_sums<T, S>(t, [&](auto& sums, int64_t m, int64_t n, char* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x / 64, wm = wave % S::waves_m * S::WM;
     float* const bias = reinterpret_cast<float*>(lds);                      // [BM]
     float* const scale = bias + S::BM;                                      // [BM]
@@ -106,7 +107,7 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
       scores_of<S>(sums, j, 1.f, bias + wm, scale + wm, half, dx);
       const float z = t.log_sum[at], of_p = t.of_p[at];
       const int e = valid ? t.expo[at] : kDeadRow;
-      const float by = e == kDeadRow ? 0.f : ldexpf(1.f, 15 - e);
+      const float by = e == kDeadRow ? 0.f : __is_same(T, float) ? 1.f : ldexpf(1.f, 15 - e);
 #pragma unroll
       for (int i = 0; i < S::FM; ++i)
 #pragma unroll
@@ -138,6 +139,17 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
           }
       }
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (__is_same(T, float)) {
+        if (t.dx && valid) {
+          float* const to = t.dx + row * t.pitch_row + m + 4 * half;
+#pragma unroll
+          for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (m + 32 * i + 8 * q + 4 * half < t.pitch_row)
+                *reinterpret_cast<float4*>(to + 32 * i + 8 * q) = make_float4(dx[i][4 * q], dx[i][4 * q + 1], dx[i][4 * q + 2], dx[i][4 * q + 3]);
+        }
+      } else {
       // by row: eight neighbouring categories a lane, from both halves' four; by category: four neighbouring rows, of a quad of lanes
       uint16_t* by_row = t.by_row + row * t.pitch_row + m + 8 * half;
       const int64_t row4 = row - (lane & 3);
@@ -181,6 +193,7 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
             }
           }
         }
+      }
     }
     if (t.bias_parts) {
       __syncthreads();
@@ -196,6 +209,12 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
 template <typename T, typename S, int kParts>
 __global__ __launch_bounds__(S::threads) void gradient_kernel(GradientTask t) {
   gradient_tile<T, S, kParts>(t);
+}
+
+// float: categories that the bias masks, whose weights have no part in the features' gradients
+__global__ __launch_bounds__(256) void masked_kernel(BiasRef bias, int64_t cats, int* skip) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c < cats) skip[c] = bias_at(bias, c, cats) == -INFINITY ? kDeadRow : 0;
 }
 
 // 32 categories a workgroup, eight lanes to each
@@ -216,7 +235,7 @@ __global__ __launch_bounds__(256) void join_bias_kernel(const float* parts, int6
 typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
 typedef TileSizes<128, 32, 32, 32> Narrow;
-int tile_rows(int64_t cats, int64_t rows) { return rows <= 32 ? 32 : ((cats + 255) / 256) * ((rows + 255) / 256) >= 192 ? 256 : 128; }
+int tile_rows(int64_t cats, int64_t rows, bool of_float) { return of_float ? 128 : rows <= 32 ? 32 : ((cats + 255) / 256) * ((rows + 255) / 256) >= 192 ? 256 : 128; }
 
 template <typename T, typename S, int kParts>
 void launch(const GradientTask& t, hipStream_t stream) {
@@ -225,7 +244,7 @@ void launch(const GradientTask& t, hipStream_t stream) {
 }
 template <typename T, int kParts>
 void launch(const GradientTask& t, hipStream_t stream) {
-  const int size = tile_rows(t.cats, t.rows);
+  const int size = tile_rows(t.cats, t.rows, false);
   if (size == 256) launch<T, Wide, kParts>(t, stream);
   else if (size == 128) launch<T, Middle, kParts>(t, stream);
   else launch<T, Narrow, kParts>(t, stream);
@@ -233,35 +252,33 @@ void launch(const GradientTask& t, hipStream_t stream) {
 
 // What the workspace holds, and how the categories are cut into pieces
 struct Plan {
-  int planes, dx_planes;
-  PlanePairs pairs, dx_pairs;
-  bool lay_f, lay_w;
+  bool of_float, lay_f, lay_w;
+  int dx_planes;
+  PlanePairs dx_pairs;
   int64_t rows, cats, length, piece, pieces;
   int features_parts, weight_parts;
-  int64_t of_p, expo, most, f, f_turned, w, w_turned, by_row, by_cat, features, weight, bias, bytes;   // offsets
+  int64_t of_p, expo, most, skip, f, f_turned, w, w_turned, by_row, by_cat, features, weight, bias, bytes;   // offsets
 
   Plan(const Matrix2& fm, const Matrix2& wm, bool of_features, bool of_weight, bool of_bias) {
-    planes = planes_of(fm.type);
+    of_float = fm.type == PCM_F32;
     rows = fm.rows();
-    // The rounding of dx is the larger part of the error where sums have few terms that count, as the gradient of a given category's weights
-    // has with few rows; over many rows it is what rounding the results costs.  In two parts: 20 rows of 64 bf16, 25000
-    // categories, 2.3e-3 -> 1.6e-3 of the result (as rounding alone); the two products take twice the steps.
-    dx_planes = planes == 3 ? 3 : rows < kFewRows ? 2 : 1;
-    pairs = planes == 3 ? kSixOfThree : kOnePlane;
-    dx_pairs = planes == 3 ? kSixOfThree : dx_planes == 2 ? kTwoOfB : kOnePlane;
     cats = wm.examples;
     length = fm.length;
     lay_f = !readable(fm);
     lay_w = !readable(wm);
+    // The rounding of dx is the larger part of the error where sums have few terms that count, as the gradient of a given category's weights
+    // has with few rows; over many rows it is what rounding the results costs.  In two parts: 20 rows of 64 bf16, 25000
+    // categories, 2.3e-3 -> 1.6e-3 of the result (as rounding alone); the two products take twice the steps.
+    dx_planes = !of_float && rows < kFewRows ? 2 : 1;
+    dx_pairs = dx_planes == 2 ? kTwoOfB : kOnePlane;
     // a piece's dx takes 2^26 entries or so, 4096 categories at least and 2^20 at most, in tiles of 256
     const int64_t most_cats = std::min<int64_t>(kMaxLength, std::max<int64_t>(4096, ((int64_t)1 << 26) / std::max<int64_t>(rows, 1) / 256 * 256));
     pieces = (cats + most_cats - 1) / most_cats;
     piece = pieces == 1 ? cats : round_up((cats + pieces - 1) / pieces, 256);
     pieces = (cats + piece - 1) / piece;
-    features_parts = parts_for(length, rows, laid_length(piece) * 2 / kKBytes * dx_pairs.count);
-    features_parts = (int)std::min<int64_t>(features_parts, std::max<int64_t>(1, laid_length(piece) * 2 / kKBytes));
-    weight_parts = parts_for(length, piece, laid_length(rows) * 2 / kKBytes * dx_pairs.count);
-    weight_parts = (int)std::min<int64_t>(weight_parts, std::max<int64_t>(1, laid_length(rows) * 2 / kKBytes));
+    const int64_t cat_steps = steps_of(piece), row_steps = steps_of(rows);
+    features_parts = (int)std::min<int64_t>(parts_for(length, rows, cat_steps * dx_pairs.count, of_float), cat_steps);
+    weight_parts = (int)std::min<int64_t>(parts_for(length, piece, row_steps * dx_pairs.count, of_float), std::max<int64_t>(1, row_steps));
     int64_t at = 0;
     auto take = [&](bool needed, int64_t n) {
       const int64_t here = at;
@@ -271,17 +288,20 @@ struct Plan {
     of_p = take(true, rows * 4);
     expo = take(true, rows * 4);
     most = take(true, kMostBlocks * 4);
-    f = take(lay_f, laid_bytes(rows, length, planes));
-    f_turned = take(of_weight, laid_bytes(length, rows, planes));
-    w = take(lay_w, laid_bytes(piece, length, planes));
-    w_turned = take(of_features, laid_bytes(length, piece, planes));
-    by_row = take(of_features, laid_bytes(rows, piece, dx_planes));
-    by_cat = take(of_weight, laid_bytes(piece, rows, dx_planes));
+    skip = take(of_float && of_features, cats * 4);
+    f = take(lay_f, laid_bytes(rows, length, 1));
+    f_turned = take(of_weight && !of_float, laid_bytes(length, rows, 1));
+    w = take(lay_w, laid_bytes(piece, length, 1));
+    w_turned = take(of_features && !of_float, laid_bytes(length, piece, 1));
+    by_row = take(of_float ? of_features || of_weight : of_features, of_float ? rows * round_up(piece, 4) * 4 : laid_bytes(rows, piece, dx_planes));
+    by_cat = take(of_weight && !of_float, laid_bytes(piece, rows, dx_planes));
     features = take(of_features && (features_parts > 1 || pieces > 1), features_parts * rows * length * 4);
     weight = take(of_weight && weight_parts > 1, weight_parts * piece * length * 4);
     bias = take(of_bias, (rows + 31) / 32 * piece * 4);
     bytes = at;
   }
+  // steps of a sum over n entries
+  int64_t steps_of(int64_t n) const { return of_float ? (n + kFloatSteps - 1) / kFloatSteps : laid_length(n) * 2 / kKBytes; }
 };
 }  // namespace
 
@@ -309,30 +329,40 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     return;
   }
   hipLaunchKernelGGL(row_terms_kernel, dim3(kMostBlocks), dim3(256), 0, stream, given, d_grad_logp, d_grad_log_sum, d_log_sum, rows, cats, of_p, expo, most);
-  const int size = f.type == PCM_F32 ? 4 : 2, operands = f.type == PCM_F16 ? PCM_F16 : PCM_BF16;
-  const int64_t turned_f = laid_length(rows);
+  const bool of_float = plan.of_float;
+  const int size = of_float ? 4 : 2;
+  int* const skip = of_float && out.features && bias.p ? reinterpret_cast<int*>(work + plan.skip) : nullptr;
+  if (skip) hipLaunchKernelGGL(masked_kernel, dim3((unsigned)((cats + 255) / 256)), dim3(256), 0, stream, bias, cats, skip);
   char* at = work + plan.f;
-  const Operand features = operand_of(f, at, stream);
+  const Operand features = of_float ? Operand{} : operand_of(f, at, stream);
   LayOut scaled;
   scaled.expo = expo;
   scaled.most = most;
-  if (out.weight) lay_out(f, 0, rows, true, scaled, work + plan.f_turned, stream);
+  if (out.weight && !of_float) lay_out(f, 0, rows, true, scaled, work + plan.f_turned, stream);
   LayOut masked;
   masked.mask = bias;
+  const int64_t turned_f = laid_length(rows);
   const bool features_direct = plan.pieces == 1 && plan.features_parts == 1;
   for (int64_t first = 0; first < cats; first += plan.piece) {
-    const int64_t count = std::min(plan.piece, cats - first), laid = laid_length(count);
+    const int64_t count = std::min(plan.piece, cats - first), laid = laid_length(count), pitch = of_float ? round_up(count, 4) : laid;
+    Matrix2 of_piece = w;
+    of_piece.p = static_cast<const char*>(w.p) + first * w.stride_ex * size;
+    of_piece.examples = count;
     GradientTask t{};
-    if (plan.lay_w) {
+    if (of_float) {
+      t.fw = float_operand(of_piece, false);
+      t.ff = float_operand(f, false);
+      t.fk = f.length;
+    } else if (plan.lay_w) {
       lay_out(w, first, count, false, LayOut(), work + plan.w, stream);
-      t.w = {work + plan.w, laid_length(w.length) * 2, count * laid_length(w.length) * 2};
+      t.w = {work + plan.w, laid_length(w.length) * 2, 0};
     } else {
-      t.w = {static_cast<const char*>(w.p) + first * w.stride_ex * 2, w.stride_ex * 2, 0};
+      t.w = {of_piece.p, w.stride_ex * 2, 0};
     }
     t.f = features;
     t.cats = count;
     t.rows = rows;
-    t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), plan.pairs, 1};
+    t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), kOnePlane, 1};
     t.bias = bias;
     if (t.bias.p) t.bias.p = static_cast<const char*>(bias.p) + first * (bias.type == PCM_F32 ? 4 : 2);
     t.given = given;
@@ -341,55 +371,71 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     t.log_sum = d_log_sum;
     t.of_p = of_p;
     t.expo = expo;
-    t.pitch_row = laid;
+    t.pitch_row = pitch;
     t.pitch_cat = turned_f;
     t.plane_row = rows * laid;
     t.plane_cat = count * turned_f;
-    t.by_row = out.features ? reinterpret_cast<uint16_t*>(work + plan.by_row) : nullptr;
-    t.by_cat = out.weight ? reinterpret_cast<uint16_t*>(work + plan.by_cat) : nullptr;
+    if (of_float) t.dx = out.features || out.weight ? reinterpret_cast<float*>(work + plan.by_row) : nullptr;
+    else t.by_row = out.features ? reinterpret_cast<uint16_t*>(work + plan.by_row) : nullptr;
+    t.by_cat = out.weight && !of_float ? reinterpret_cast<uint16_t*>(work + plan.by_cat) : nullptr;
     t.bias_parts = out.bias ? reinterpret_cast<float*>(work + plan.bias) : nullptr;
-    if (f.type == PCM_F32) launch<bf16, 3>(t, stream);
+    if (of_float) launch<float, FloatTile, 1>(t, stream);
     else if (f.type == PCM_BF16) plan.dx_planes == 2 ? launch<bf16, 2>(t, stream) : launch<bf16, 1>(t, stream);
     else plan.dx_planes == 2 ? launch<f16, 2>(t, stream) : launch<f16, 1>(t, stream);
     if (out.bias) {
-      const int64_t each = tile_rows(count, rows);
+      const int64_t each = tile_rows(count, rows, of_float);
       hipLaunchKernelGGL(join_bias_kernel, dim3((unsigned)((count + 31) / 32)), dim3(256), 0, stream, t.bias_parts, (rows + each - 1) / each, count,
                          out.bias, bias.type, first);
     }
+    const Matrix2 dx{t.dx, PCM_F32, pitch, 0, 1, rows, 1, (int32_t)count};
     if (out.features) {
-      lay_out(w, first, count, true, masked, work + plan.w_turned, stream);
       OutTask o{};
-      o.a = {work + plan.w_turned, laid * 2, f.length * laid * 2};
-      o.b = {t.by_row, laid * 2, t.plane_row * 2};
+      if (of_float) {
+        o.fa = float_operand(of_piece, true, skip ? skip + first : nullptr);
+        o.fb = float_operand(dx, false);
+        o.fk = count;
+      } else {
+        lay_out(w, first, count, true, masked, work + plan.w_turned, stream);
+        o.a = {work + plan.w_turned, laid * 2, 0};
+        o.b = {t.by_row, laid * 2, t.plane_row * 2};
+        o.finish.expo = expo;
+      }
       o.m = f.length;
       o.n = rows;
-      o.steps = {(int)(laid * 2 / kKBytes), plan.dx_pairs, (int)std::min<int64_t>(plan.features_parts, laid * 2 / kKBytes)};
+      o.steps = {(int)(laid * 2 / kKBytes), plan.dx_pairs, (int)std::min(plan.steps_of(count), (int64_t)plan.features_parts)};
       o.out = features_direct ? out.features : work + plan.features;
       o.type = features_direct ? f.type : kRawSums;
       o.pitch = f.length;
       o.add = first > 0;
-      o.finish.expo = expo;
-      product_out(operands, o, stream);
+      o.finish.dead = expo;
+      product_out(f.type, o, stream);
     }
     if (out.weight) {
       OutTask o{};
-      o.a = {work + plan.f_turned, turned_f * 2, f.length * turned_f * 2};
-      o.b = {t.by_cat, turned_f * 2, t.plane_cat * 2};
+      if (of_float) {
+        o.fa = float_operand(f, true, expo);
+        o.fb = float_operand(dx, true);
+        o.fk = rows;
+      } else {
+        o.a = {work + plan.f_turned, turned_f * 2, 0};
+        o.b = {t.by_cat, turned_f * 2, t.plane_cat * 2};
+        o.finish.most = most;
+      }
       o.m = f.length;
       o.n = count;
       o.steps = {(int)(turned_f * 2 / kKBytes), plan.dx_pairs, plan.weight_parts};
       o.pitch = f.length;
-      o.finish.most = most;
       char* const to = static_cast<char*>(out.weight) + first * f.length * size;
       o.out = plan.weight_parts > 1 ? work + plan.weight : to;
       o.type = plan.weight_parts > 1 ? kRawSums : f.type;
-      product_out(operands, o, stream);
+      product_out(f.type, o, stream);
       if (plan.weight_parts > 1) join_parts(o.out, plan.weight_parts, false, o.m, o.n, o.finish, to, f.type, f.length, stream);
     }
   }
   if (out.features && !features_direct) {
     Finish finish;
-    finish.expo = expo;
+    finish.dead = expo;
+    if (!of_float) finish.expo = expo;
     // (a last piece of fewer steps than parts leaves some of them as the pieces before it did)
     join_parts(work + plan.features, plan.features_parts, false, f.length, rows, finish, out.features, f.type, f.length, stream);
   }

@@ -4,7 +4,7 @@
 // Categories are the rows of a, so that a lane's sums are of one row of features: it takes their maximum and the sum of
 // exponentials in registers, the tile's waves join theirs in LDS, and a pair of numbers per row and tile of categories is all that
 // is written; a second launch joins those.  The score of a given category is written by the lane that has it.
-#include "product_tiles.hip.hpp"
+#include "float_tiles.hip.hpp"
 
 namespace pcm {
 
@@ -25,7 +25,7 @@ struct ScoreTask : ScoreInputs {
 
 template <typename T, typename S>
 __device__ __forceinline__ void score_tile(const ScoreTask& t) {
-  product_tile<T, S>(t.w, t.f, t.cats, t.rows, t.steps, [&](auto& sums, int64_t m, int64_t n, char* lds) {
+  score_sums<T, S>(t, [&](auto& sums, int64_t m, int64_t n, char* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x / 64, wm = wave % S::waves_m * S::WM;
     float* const bias = reinterpret_cast<float*>(lds);                      // [BM]
     float* const scale = bias + S::BM;                                      // [BM]
@@ -125,7 +125,8 @@ typedef TileSizes<128, 128, 64, 64> Middle;
 typedef TileSizes<128, 32, 32, 32> Narrow;
 enum { kWide, kMiddle, kNarrow };
 
-int tiles_for(int64_t m, int64_t n) {
+int tiles_for(int64_t m, int64_t n, bool of_float) {
+  if (of_float) return kMiddle;
   if (n <= 32) return kNarrow;
   const int64_t wide = ((m + 255) / 256) * ((n + 255) / 256);
   return wide >= 192 ? kWide : kMiddle;
@@ -138,22 +139,22 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch(const ScoreTask& t, hipStream_t stream) {
-  const int size = tiles_for(t.cats, t.rows);
+  const int size = tiles_for(t.cats, t.rows, false);
   if (size == kWide) launch<T, Wide>(t, stream);
   else if (size == kMiddle) launch<T, Middle>(t, stream);
   else launch<T, Narrow>(t, stream);
 }
-int64_t tiles_of_cats(int64_t cats, int64_t rows) {
-  const int64_t each = tiles_for(cats, rows) == kWide ? 256 : 128;
+int64_t tiles_of_cats(int64_t cats, int64_t rows, bool of_float) {
+  const int64_t each = tiles_for(cats, rows, of_float) == kWide ? 256 : 128;
   return (cats + each - 1) / each;
 }
-int64_t parts_bytes(int64_t cats, int64_t rows) { return round_up(tiles_of_cats(cats, rows) * rows * (int64_t)sizeof(Part), 256); }
+int64_t parts_bytes(int64_t cats, int64_t rows, bool of_float) { return round_up(tiles_of_cats(cats, rows, of_float) * rows * (int64_t)sizeof(Part), 256); }
 
 void join_launch(const ScoreTask& t, float* d_log_sum, hipStream_t stream) {
   // few rows: all lanes of a workgroup to one, many: neighbouring rows side by side
   const int per = t.rows >= 4096 ? 16 : t.rows >= 512 ? 4 : 1;
-  hipLaunchKernelGGL(join_scores_kernel, dim3((unsigned)((t.rows + per - 1) / per)), dim3(256), 0, stream, t.parts, tiles_of_cats(t.cats, t.rows),
-                     t.rows, per, t.given, t.cats, t.logp, d_log_sum);
+  hipLaunchKernelGGL(join_scores_kernel, dim3((unsigned)((t.rows + per - 1) / per)), dim3(256), 0, stream, t.parts,
+                     tiles_of_cats(t.cats, t.rows, t.fw.p),                     t.rows, per, t.given, t.cats, t.logp, d_log_sum);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of linear_scores failed: %s", hipGetErrorString(e));
 }
@@ -170,8 +171,8 @@ void check_linear(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const
 }
 
 int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w) {
-  return (readable(f) ? 0 : laid_bytes(f.rows(), f.length, planes_of(f.type))) + (readable(w) ? 0 : laid_bytes(w.rows(), w.length, planes_of(w.type))) +
-         parts_bytes(w.examples, f.rows());
+  return (readable(f) ? 0 : laid_bytes(f.rows(), f.length, 1)) + (readable(w) ? 0 : laid_bytes(w.rows(), w.length, 1)) +
+         parts_bytes(w.examples, f.rows(), f.type == PCM_F32);
 }
 
 void check_workspace(const void* d_work, int64_t work_bytes, int64_t need, const char* what) {
@@ -179,12 +180,25 @@ void check_workspace(const void* d_work, int64_t work_bytes, int64_t need, const
   if ((uintptr_t)d_work & 15) fail(PCM_ERR_ARG, "%s: the workspace must be 16-byte aligned", what);
 }
 
-// a matrix as a product reads it: where it is, or laid out at `work`, which then moves on
+FloatOperand float_operand(const Matrix2& x, bool turned, const int* skip) {
+  FloatOperand o{static_cast<const float*>(x.p), x.stride_ex, x.stride_var, x.stride, x.vars, turned, skip};
+  if (x.vars > 1 && (x.examples == 1 || x.stride_ex == x.vars * x.stride_var)) {   // one axis of rows
+    o.stride_ex = x.stride_var;
+    o.vars = 1;
+  }
+  if (o.vars == 1 && o.stride != 1 && o.stride_ex == 1 && !skip) {                 // neighbours along the other axis
+    std::swap(o.stride, o.stride_ex);
+    o.turned = !turned;
+  }
+  return o;
+}
+
+// a matrix of 16-bit entries as a product reads it: where it is, or laid out at `work`, which then moves on
 Operand operand_of(const Matrix2& x, char*& work, hipStream_t stream) {
   if (readable(x)) return {x.p, (x.vars == 1 ? x.stride_ex : x.stride_var) * 2, 0};
   lay_out(x, 0, x.rows(), false, LayOut(), work, stream);
-  const Operand o{work, laid_length(x.length) * 2, x.rows() * laid_length(x.length) * 2};
-  work += laid_bytes(x.rows(), x.length, planes_of(x.type));
+  const Operand o{work, laid_length(x.length) * 2, 0};
+  work += laid_bytes(x.rows(), x.length, 1);
   return o;
 }
 
@@ -196,22 +210,29 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   check_workspace(d_work, work_bytes, linear_scores_workspace(f, w), "linear scores");
   ScoreTask t{};
   char* work = static_cast<char*>(d_work);
-  t.f = operand_of(f, work, stream);
-  t.w = operand_of(w, work, stream);
+  if (f.type == PCM_F32) {
+    t.ff = float_operand(f, false);
+    t.fw = float_operand(w, false);
+    t.fk = f.length;
+  } else {
+    t.f = operand_of(f, work, stream);
+    t.w = operand_of(w, work, stream);
+  }
   t.cats = w.examples;
   t.rows = f.rows();
-  t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), f.type == PCM_F32 ? kSixOfThree : kOnePlane, 1};
+  t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), kOnePlane, 1};
   t.bias = bias;
   t.given = given;
   t.given.vars = f.vars;
   t.logp = d_logp;
   t.parts = reinterpret_cast<Part*>(work);
-  if (f.type == PCM_F16) launch<f16>(t, stream);
+  if (f.type == PCM_F32) launch<float, FloatTile>(t, stream);
+  else if (f.type == PCM_F16) launch<f16>(t, stream);
   else launch<bf16>(t, stream);
   join_launch(t, d_log_sum, stream);
 }
 
-int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows); }
+int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, false); }
 
 void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
                     int32_t length, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,

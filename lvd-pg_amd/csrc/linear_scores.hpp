@@ -1,10 +1,9 @@
 // Scores of categories that are products of features and weights, x[n][c] = f[n] . w[c] + b[c]: what the kernels of linear_scores.hip,
 // linear_gradient.hip, product8.hip and lay_out.hip share.
 //
-// All products run over rows that are neighbours along the summed axis, in pieces of 128 bytes (product_tiles.hip.hpp): 16-bit
-// types as they are, 8-bit codes as whole numbers, and float as three bfloat16 planes h + m + l, whose six largest products
-// (hl lh mm hm mh hh, in this order) leave out what lies 2^-26 below the product.  Rows that do not lie so (odd lengths, other
-// strides, float, or summed along the other axis) are laid out in the workspace first (lay_out.hip).
+// Products of 16-bit types and of 8-bit codes run over rows that are neighbours along the summed axis, in pieces of 128 bytes
+// (product_tiles.hip.hpp); rows that do not lie so (odd lengths, other strides, or summed along the other axis) are laid out in the
+// workspace first (lay_out.hip).  Float is read where it is, as three bfloat16 parts (float_tiles.hip.hpp).
 #pragma once
 
 #include "category_rows.hpp"
@@ -27,7 +26,7 @@ struct Matrix2 {                             // rows of a matrix in device memor
 };
 struct Operand {                             // rows that a product can read: 16-byte aligned, multiples of 128 bytes, zeros behind the end
   const void* p;
-  int64_t pitch, plane;                      // bytes from row to row, and from plane to plane (float)
+  int64_t pitch, plane;                      // bytes from row to row, and from plane to plane (numbers in two parts)
 };
 struct BiasRef {                             // a number per category; null: zeros
   const void* p;
@@ -38,7 +37,6 @@ struct ScaleRef {                            // of 8-bit rows: scales of b's row
 };
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-inline int planes_of(int type) { return type == PCM_F32 ? 3 : 1; }
 // entries of a laid out row: a multiple of 128 bytes of 16-bit entries
 inline int64_t laid_length(int64_t length) { return round_up(length, kKBytes / 2); }
 inline int64_t laid_bytes(int64_t rows, int64_t length, int planes) { return round_up(rows * laid_length(length) * 2 * planes, 256); }
@@ -50,8 +48,7 @@ struct LayOut {
   const int* most = nullptr;                 // 256 candidates of the largest exponent
   BiasRef mask{nullptr, 0};
 };
-// x, rows [first, first + count) of it, as 16-bit planes: [plane][row][laid_length(length)], or with `turned`
-// [plane][entry][laid_length(count)]
+// rows [first, first + count) of x, of a 16-bit type, as [row][laid_length(length)], or with `turned` as [entry][laid_length(count)]
 void lay_out(const Matrix2& x, int64_t first, int64_t count, bool turned, const LayOut& with, void* d_to, hipStream_t stream);
 // whether a product can read the rows where they are
 bool readable(const Matrix2& x);
@@ -101,19 +98,9 @@ __device__ __forceinline__ int largest_exponent(const int* most) {   // by every
   for (int s = 32; s; s /= 2) e = max(e, __shfl_xor(e, s));
   return e;
 }
-// A float as three bfloat16: the nearest one, the nearest one to what is left, and once more; the sum is within 2^-26 of it.
-// (what would round up beyond the type's range is cut off instead)
-struct Planes {
-  bf16 h, m, l;
-};
-__device__ __forceinline__ Planes planes(float x) {
-  Planes p;
-  p.h = (bf16)x;
-  if (__builtin_isinf((float)p.h) && !__builtin_isinf(x)) p.h = __builtin_bit_cast(bf16, (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16));
-  const float r = x - (float)p.h;
-  p.m = (bf16)r;
-  p.l = (bf16)(r - (float)p.m);
-  return p;
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {   // two of 16 bits
+  return (uint32_t)__builtin_bit_cast(uint16_t, (T)a) | (uint32_t)__builtin_bit_cast(uint16_t, (T)b) << 16;
 }
 #endif
 

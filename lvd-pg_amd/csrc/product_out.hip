@@ -6,7 +6,7 @@ namespace pcm {
 namespace {
 template <typename T, typename S>
 __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
-  product_tile<T, S>(t.a, t.b, t.m, t.n, t.steps, [&](auto& sums, int64_t m, int64_t n, char* lds) {
+  auto done = [&](auto& sums, int64_t m, int64_t n, char* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = threadIdx.x / 64 % S::waves_m * S::WM;
     const bool raw = t.type == kRawSums;
     const int most = t.finish.most ? largest_exponent(t.finish.most) : 0;
@@ -57,7 +57,9 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
               if (col + e < t.m) store_as(t.out, t.type, at + e, v[e]);
         }
     }
-  });
+  };
+  if constexpr (__is_same(T, float)) float_tile(t.fa, t.fb, t.m, t.n, t.fk, t.steps.parts, done);
+  else product_tile<T, S>(t.a, t.b, t.m, t.n, t.steps, done);
 }
 template <typename T, typename S>
 __global__ __launch_bounds__(S::threads) void out_kernel(OutTask t, bool fours) {
@@ -104,15 +106,17 @@ void launch(const OutTask& t, hipStream_t stream) {
 }
 }  // namespace
 
-int parts_for(int64_t m, int64_t n, int64_t steps) {
-  if (wide(m, n) && n > 32) return 1;
+int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
+  if (of_float) n = std::max<int64_t>(n, 33);          // (one size of tiles)
+  else if (wide(m, n) && n > 32) return 1;
   const int64_t tiles = ((m + 127) / 128) * ((n + (n <= 32 ? 31 : 127)) / (n <= 32 ? 32 : 128));
   // as many parts as fill the device twice over, each of eight steps or more
   return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 8, 64}));
 }
 
 void product_out(int operands, const OutTask& t, hipStream_t stream) {
-  if (operands == PCM_BF16) launch<bf16>(t, stream);
+  if (operands == PCM_F32) launch<float, FloatTile>(t, stream);
+  else if (operands == PCM_BF16) launch<bf16>(t, stream);
   else if (operands == PCM_F16) launch<f16>(t, stream);
   else launch<int8_t>(t, stream);
   const hipError_t e = hipGetLastError();

@@ -2,7 +2,7 @@
 // second launch joins.
 #pragma once
 
-#include "product_tiles.hip.hpp"
+#include "float_tiles.hip.hpp"
 
 namespace pcm {
 
@@ -10,13 +10,16 @@ enum { kRawSums = -1 };   // the type of parts: the sums themselves, 32 bits eac
 
 // What becomes of a sum of row m of a and row n of b
 struct Finish {
-  const int* expo = nullptr;     // 2^(expo[n] - 15), 0 where it is kDeadRow (gradient of features)
+  const int* dead = nullptr;     // 0 where it is kDeadRow (gradient of features)
+  const int* expo = nullptr;     // 2^(expo[n] - 15) (gradient of features)
   const int* most = nullptr;     // 2^(the largest of most - 15) (gradient of weights)
   ScaleRef scale{nullptr, nullptr};
   BiasRef bias{nullptr, 0};      // of m
 };
 struct OutTask {
   Operand a, b;
+  FloatOperand fa, fb;           // ... of float, of fk entries
+  int64_t fk;
   int64_t m, n;
   Steps steps;
   void* out;                     // [n][pitch], entries of `type`; kRawSums: [part][n][pitch]
@@ -27,11 +30,11 @@ struct OutTask {
 };
 
 // launches of any size
-void product_out(int operands, const OutTask& t, hipStream_t stream);   // operands: PCM_BF16, PCM_F16, PCM_U8 (whole numbers)
+void product_out(int operands, const OutTask& t, hipStream_t stream);   // operands: PCM_F32, PCM_BF16, PCM_F16, PCM_U8 (whole numbers)
 // out = the finished sums of parts [parts][n][m] floats (or whole numbers)
 void join_parts(const void* parts, int count, bool whole, int64_t m, int64_t n, const Finish& finish, void* out, int type, int64_t pitch, hipStream_t stream);
 // how many parts the summed axis of a product is best cut into
-int parts_for(int64_t m, int64_t n, int64_t steps);
+int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float = false);
 
 #ifdef __HIPCC__
 struct FinishAt {                // of one n
@@ -40,7 +43,7 @@ struct FinishAt {                // of one n
   bool dead;
   __device__ __forceinline__ FinishAt(const Finish& f, int64_t n, int most) {
     expo = f.most ? most - 15 : f.expo ? f.expo[n] - 15 : 0;
-    dead = f.expo && f.expo[n] == kDeadRow;
+    dead = f.dead && f.dead[n] == kDeadRow;
     scale = f.scale.n ? f.scale.n[n] : 1.f;
   }
   // scale_m, bias_m: of m
@@ -54,10 +57,6 @@ __device__ __forceinline__ void store_as(void* out, int type, int64_t at, float 
   if (type == PCM_F32) static_cast<float*>(out)[at] = v;
   else if (type == PCM_BF16) static_cast<bf16*>(out)[at] = (bf16)v;
   else static_cast<f16*>(out)[at] = (f16)v;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pair_of(float a, float b) {
-  return (uint32_t)__builtin_bit_cast(uint16_t, (T)a) | (uint32_t)__builtin_bit_cast(uint16_t, (T)b) << 16;
 }
 // four neighbours, the address a multiple of their size
 __device__ __forceinline__ void store_four(void* out, int type, int64_t at, const float (&v)[4]) {

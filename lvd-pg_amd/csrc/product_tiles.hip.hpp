@@ -14,7 +14,6 @@ struct PlanePairs {
   uint32_t a, b;
 };
 constexpr PlanePairs kOnePlane{1, 0, 0}, kTwoOfB{2, 0, 0x1};   // b in two parts: the smaller one first
-constexpr PlanePairs kSixOfThree{6, 0x118, 0x52};              // h m l (0 1 2): hl lh mm hm mh hh
 // What a product sums over: `count` steps of 128 bytes for each pair of planes.  With parts > 1 part blockIdx.y takes its share of the steps.
 struct Steps {
   int count;
@@ -197,46 +196,6 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
     }
   }
   done(sums, tile.m0 + wm, tile.n0 + wn, s0);
-}
-
-// ---- scores of categories (a) under rows of features (b) -------------------------------------------------------
-struct ScoreInputs {
-  Operand w, f;
-  int64_t cats, rows;
-  Steps steps;
-  BiasRef bias;
-  ScaleRef scale;
-  GivenRef given;
-};
-// bias and scales of a tile's categories into LDS; barriers before and after
-template <typename S>
-__device__ __forceinline__ void tile_constants(const ScoreInputs& t, int64_t m0, float* bias, float* scale) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < S::BM; i += S::threads) {
-    bias[i] = bias_at(t.bias, m0 + i, t.cats);
-    scale[i] = t.scale.m && m0 + i < t.cats ? t.scale.m[m0 + i] : 1.f;
-  }
-  __syncthreads();
-}
-// The scores of the wave's j-th rows of features
-template <typename S, typename Sums>
-__device__ __forceinline__ void scores_of(const Sums (&sums)[S::FM][S::FN], int j, float scale_n, const float* bias, const float* scale, int half,
-                                          float (&x)[S::FM][16]) {
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = 32 * i + 8 * q + 4 * half;
-      const float4 b = *reinterpret_cast<const float4*>(bias + at);
-      if constexpr (__is_same(Sums, v16i)) {
-        const float4 s = *reinterpret_cast<const float4*>(scale + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][4 * q + e] = score_of((float)sums[i][j][4 * q + e] * scale_n * (&s.x)[e], (&b.x)[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][4 * q + e] = score_of(sums[i][j][4 * q + e], (&b.x)[e]);
-      }
-    }
 }
 #endif
 

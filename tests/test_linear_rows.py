@@ -204,7 +204,8 @@ def test_workspaces_follow_the_arguments():
 
     least = scores()
     assert least > 0 and scores(k=128) == least                          # nothing laid out
-    for other in (scores(type=0), scores(k=65), scores(at=p + 2), scores(stride=65), scores(inner=2, stride=128)):
+    assert scores(type=0, k=65, inner=2, stride=130, at=p + 4) == scores(type=0)   # float is read whatever its strides
+    for other in (scores(k=65), scores(at=p + 2), scores(stride=65), scores(inner=2, stride=128)):
         assert other > least
     assert scores(n=0) == 0 and scores(k=0) == 0 and scores(c=0) == 0 and scores(n=(1 << 22) + 1) == 0
     back = lambda of, n=100: lib.pcm_linear_scores_backward_workspace(p, p, 1, 64, 0, 1, 64, 1, n, 1, 64, 1000, of)
