@@ -25,122 +25,213 @@ FloatOperand float_operand(const Matrix2& x, bool turned, const int* skip = null
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef v4f v4f_by4 __attribute__((aligned(4)));
 typedef TileSizes<128, 128, 64, 64> FloatTile;
-constexpr int kFloatSteps = 32;              // entries of the summed axis in a stage
-constexpr int kFloatPitch = 80;              // bytes of a row of a plane: 64 and a gap that spreads rows over the banks
+constexpr int kFloatSteps = 16;              // entries of the summed axis in a stage
+constexpr int kFloatPitch = 48;              // bytes of a row of a plane: 32 and a gap that spreads rows over the banks
 constexpr int kFloatPlane = (FloatTile::BM + FloatTile::BN) * kFloatPitch;
 
-// A thread's part of an operand's stage: 4 x 4 floats.  Summed over entries: four neighbours of four rows 32 apart; over rows: a block of
-// four rows and four neighbours, turned on the way to LDS.
+// A thread's part of an operand's stage: eight floats.  Summed over entries: four neighbours of two rows 64 apart; over rows (kTurned): a
+// block of two rows and four neighbours, turned on the way to LDS.
+template <bool kTurned>
 struct FloatLoader {
   FloatOperand x;
-  const float* at[4];                        // summed over entries: the thread's rows
+  const float* at[2];                        // summed over entries: the thread's rows; over rows: its entries of row 0, and of row 1
   int64_t first;                             // the tile's first row (or entry)
   int64_t count;                             // rows (or entries) of the operand
   int row, step;                             // thread's place in the tile
+  v4f v[2];
+  int mark[2];                               // turned: of the rows
   __device__ __forceinline__ const float* row_at(int64_t r) const {
     return x.p + (x.vars == 1 ? r * x.stride_ex : r / x.vars * x.stride_ex + r % x.vars * x.stride_var);
   }
   __device__ __forceinline__ FloatLoader(const FloatOperand& o, int64_t first_, int64_t count_) : x(o), first(first_), count(count_) {
-    step = threadIdx.x % 8 * 4;
-    row = threadIdx.x / 8;
-    if (x.turned) row *= 4;
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i) at[i] = row_at(min(first + row + 32 * i, count - 1));
-  }
-  // steps [k, k + 32) of those below end
-  __device__ __forceinline__ void load(v4f (&v)[4], int64_t k, int64_t end) const {
-    const int64_t s = k + step;
-    if (!x.turned) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* const p = at[i] + s * x.stride;
-        if (x.stride == 1 && s + 4 <= end) v[i] = *reinterpret_cast<const v4f_by4*>(p);
-        else
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[i][e] = s + e < end ? p[e * x.stride] : 0.f;
-      }
+    if constexpr (kTurned) {
+      step = threadIdx.x % 8 * 2;
+      row = threadIdx.x / 8 * 4;
+      at[0] = x.p + min(first + row, count - 4) * x.stride;      // (plain(): four entries at least)
     } else {
-      const int64_t m = first + row;
+      step = threadIdx.x % 4 * 4;
+      row = threadIdx.x / 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool some = s + i < end && !(x.skip && x.skip[s + i] == kDeadRow);
-        v[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        if (!some) continue;
-        const float* const p = row_at(s + i) + m * x.stride;
-        if (x.stride == 1 && m + 4 <= count) v[i] = *reinterpret_cast<const v4f_by4*>(p);
-        else
+      for (int i = 0; i < 2; ++i) at[i] = row_at(min(first + row + 64 * i, count - 1));
+    }
+  }
+  // whether all of the tile's requests are of four neighbours
+  __device__ __forceinline__ bool plain() const {
+    return x.stride == 1 && (!kTurned || (x.vars == 1 && count >= 4 && (count % 4 == 0 || first + FloatTile::BM <= count)));
+  }
+  // steps [k, k + 16), all of them there
+  __device__ __forceinline__ void load_plain(int64_t k) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (m + e < count) v[i][e] = p[e * x.stride];
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (kTurned) {
+        const int64_t r = k + step + i;
+        // (without marks any word of the row is read, and not looked at)
+        mark[i] = *(x.skip ? x.skip + r : reinterpret_cast<const int*>(x.p + r * x.stride_ex));
+        v[i] = *reinterpret_cast<const v4f_by4*>(at[0] + r * x.stride_ex);
+      } else {
+        v[i] = *reinterpret_cast<const v4f_by4*>(at[i] + k + step);
       }
     }
   }
-  __device__ __forceinline__ void store(const v4f (&v)[4], char* planes_of) const {
+  // steps [k, k + 16) of those below end, any strides
+  __device__ __forceinline__ void load_any(int64_t k, int64_t end) {
+    const int64_t s = k + step;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v4f w;
-      if (x.turned) w = v4f{v[0][i], v[1][i], v[2][i], v[3][i]};
-      else w = v[i];
-      char* const to = planes_of + (row + (x.turned ? i : 32 * i)) * kFloatPitch + step * 2;
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (kTurned) {
+        const bool some = s + i < end && !(x.skip && x.skip[s + i] == kDeadRow);
+        mark[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = some && first + row + e < count ? row_at(s + i)[(first + row + e) * x.stride] : 0.f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = s + e < end ? at[i][(s + e) * x.stride] : 0.f;
+      }
+    }
+  }
+  // one half of the thread's floats to LDS, in three parts each
+  template <int kHalf>
+  __device__ __forceinline__ void store(char* planes_of) const {
+    if constexpr (!kTurned) {
+      v4f w = v[kHalf];
+      char* const to = planes_of + (row + 64 * kHalf) * kFloatPitch + step * 2;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         const uint32_t a = pair_of<bf16>(w[0], w[1]), b = pair_of<bf16>(w[2], w[3]);
         *reinterpret_cast<uint2*>(to + p * kFloatPlane) = make_uint2(a, b);
-        w -= v4f{as_float(a << 16), as_float(a & 0xffff0000u), as_float(b << 16), as_float(b & 0xffff0000u)};
+        if (p < 2) w -= v4f{as_float(a << 16), as_float(a & 0xffff0000u), as_float(b << 16), as_float(b & 0xffff0000u)};
+      }
+    } else {
+      const bool none[2] = {x.skip && mark[0] == kDeadRow, x.skip && mark[1] == kDeadRow};
+#pragma unroll
+      for (int e = 2 * kHalf; e < 2 * kHalf + 2; ++e) {
+        float u = none[0] ? 0.f : v[0][e], w = none[1] ? 0.f : v[1][e];
+        char* const to = planes_of + (row + e) * kFloatPitch + step * 2;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const uint32_t a = pair_of<bf16>(u, w);
+          *reinterpret_cast<uint32_t*>(to + p * kFloatPlane) = a;
+          if (p < 2) {
+            u -= as_float(a << 16);
+            w -= as_float(a & 0xffff0000u);
+          }
+        }
       }
     }
   }
 };
 
+// The tile loop.  Two stages in LDS: while one is multiplied the next is taken apart, instruction by instruction between the products,
+// and the one after it is on its way to registers; one barrier a stage.
+template <bool kTurnedA, bool kTurnedB>
+__device__ __forceinline__ void float_stages(const FloatOperand& a, const FloatOperand& b, const TileAt& tile, int64_t m, int64_t n, int64_t k, int64_t first,
+                                             int64_t last, char* lds, v16f (&sums)[FloatTile::FM][FloatTile::FN]) {
+  typedef FloatTile S;
+  FloatLoader<kTurnedA> from_a(a, tile.m0, m);
+  FloatLoader<kTurnedB> from_b(b, tile.n0, n);
+  const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5, wave = threadIdx.x / 64;
+  const int wm = wave % S::waves_m * S::WM, wn = wave / S::waves_m * S::WN;
+  const int at_a = (wm + row) * kFloatPitch + half * 16, at_b = (S::BM + wn + row) * kFloatPitch + half * 16;
+  auto load_any = [&](int64_t s) {
+    from_a.load_any(s * kFloatSteps, k);
+    from_b.load_any(s * kFloatSteps, k);
+  };
+  auto load_plain = [&](int64_t s) {
+    from_a.load_plain(s * kFloatSteps);
+    from_b.load_plain(s * kFloatSteps);
+  };
+  auto store = [&](char* to) {
+    from_a.template store<0>(to);
+    from_a.template store<1>(to);
+    from_b.template store<0>(to + S::BM * kFloatPitch);
+    from_b.template store<1>(to + S::BM * kFloatPitch);
+  };
+  v4i fa[3][S::FM], fb[3][S::FN];
+  auto read = [&](const char* from) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i) fa[p][i] = *reinterpret_cast<const v4i*>(from + at_a + p * kFloatPlane + i * 32 * kFloatPitch);
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) fb[p][j] = *reinterpret_cast<const v4i*>(from + at_b + p * kFloatPlane + j * 32 * kFloatPitch);
+    }
+  };
+  auto multiply = [&](int p) {               // hl lh mm hm mh hh
+    constexpr int of_a[6] = {0, 2, 1, 0, 1, 0}, of_b[6] = {2, 0, 1, 1, 0, 0};
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) sums[i][j] = Cores<bf16>::mma(fa[of_a[p]][i], fb[of_b[p]][j], sums[i][j]);
+  };
+  char *mine = lds, *next = lds + 3 * kFloatPlane;
+  auto swap = [&] {
+    char* const was = mine;
+    mine = next;
+    next = was;
+  };
+  // stages that are there in whole, in requests of four neighbours
+  const int64_t whole = from_a.plain() && from_b.plain() ? min(last, k / kFloatSteps) : first;
+  int64_t s = first;
+  if (first + 1 < whole) {
+    load_plain(first);
+    store(mine);
+    load_plain(first + 1);
+    __syncthreads();
+    for (; s + 1 < whole; ++s) {
+      read(mine);
+      char* const to_b = next + S::BM * kFloatPitch;
+      multiply(0);
+      from_a.template store<0>(next);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+      from_a.template store<1>(next);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(2);
+      from_b.template store<0>(to_b);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(3);
+      from_b.template store<1>(to_b);
+      __builtin_amdgcn_sched_barrier(0);
+      load_plain(min(s + 2, whole - 1));   // (at the end the last one once more, not used)
+      multiply(4);
+      multiply(5);
+      __syncthreads();
+      swap();
+    }
+  } else if (first < last) {
+    load_any(first);
+    store(mine);
+    __syncthreads();
+  }
+  for (; s < last; ++s) {                  // stage s is in LDS
+    if (s + 1 < last) load_any(s + 1);
+    read(mine);
+    if (s + 1 < last) store(next);
+#pragma unroll
+    for (int p = 0; p < 6; ++p) multiply(p);
+    __syncthreads();
+    swap();
+  }
+}
+
 // Sums over steps [0, k) of a's rows (m) and b's (n), as product_tile; parts of the steps by blockIdx.y
 template <typename Done>
 __device__ __forceinline__ void float_tile(const FloatOperand& a, const FloatOperand& b, int64_t m, int64_t n, int64_t k, int parts, Done done) {
   typedef FloatTile S;
-  __shared__ __attribute__((aligned(16))) char lds[3 * kFloatPlane];
+  __shared__ __attribute__((aligned(16))) char lds[6 * kFloatPlane];
   const TileAt tile = tile_at<S>(m, n);
   const int64_t stages = (k + kFloatSteps - 1) / kFloatSteps;
   const int64_t first = stages * blockIdx.y / parts, last = stages * (blockIdx.y + 1) / parts;
-  const FloatLoader from_a(a, tile.m0, m), from_b(b, tile.n0, n);
-  const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5, wave = threadIdx.x / 64;
-  const int wm = wave % S::waves_m * S::WM, wn = wave / S::waves_m * S::WN;
-  const char* const at_a = lds + (wm + row) * kFloatPitch + half * 16;
-  const char* const at_b = lds + (S::BM + wn + row) * kFloatPitch + half * 16;
   v16f sums[S::FM][S::FN] = {};
-  v4f va[4], vb[4];
-  if (first < last) {
-    from_a.load(va, first * kFloatSteps, k);
-    from_b.load(vb, first * kFloatSteps, k);
+  if (a.turned) {
+    if (b.turned) float_stages<true, true>(a, b, tile, m, n, k, first, last, lds, sums);
+    else float_stages<true, false>(a, b, tile, m, n, k, first, last, lds, sums);
+  } else {
+    if (b.turned) float_stages<false, true>(a, b, tile, m, n, k, first, last, lds, sums);
+    else float_stages<false, false>(a, b, tile, m, n, k, first, last, lds, sums);
   }
-  for (int64_t s = first; s < last; ++s) {
-    from_a.store(va, lds);
-    from_b.store(vb, lds + S::BM * kFloatPitch);
-    __syncthreads();
-    if (s + 1 < last) {
-      from_a.load(va, (s + 1) * kFloatSteps, k);
-      from_b.load(vb, (s + 1) * kFloatSteps, k);
-    }
-#pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      v4i fa[3][S::FM], fb[3][S::FN];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i) fa[p][i] = *reinterpret_cast<const v4i*>(at_a + p * kFloatPlane + i * 32 * kFloatPitch + step * 32);
-#pragma unroll
-        for (int j = 0; j < S::FN; ++j) fb[p][j] = *reinterpret_cast<const v4i*>(at_b + p * kFloatPlane + j * 32 * kFloatPitch + step * 32);
-      }
-      constexpr int of_a[6] = {0, 2, 1, 0, 1, 0}, of_b[6] = {2, 0, 1, 1, 0, 0};   // hl lh mm hm mh hh
-#pragma unroll
-      for (int p = 0; p < 6; ++p)
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-          for (int j = 0; j < S::FN; ++j) sums[i][j] = Cores<bf16>::mma(fa[of_a[p]][i], fb[of_b[p]][j], sums[i][j]);
-    }
-    __syncthreads();
-  }
-  done(sums, tile.m0 + wm, tile.n0 + wn, lds);
+  const int wave = threadIdx.x / 64;
+  done(sums, tile.m0 + wave % S::waves_m * S::WM, tile.n0 + wave / S::waves_m * S::WN, lds);
 }
 
 // ---- scores of categories (a) under rows of features (b) -------------------------------------------------------

@@ -67,10 +67,9 @@ struct Coded {
   __device__ __forceinline__ Coded(float u, float v) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const T a = (T)u, b = (T)v;
-      p[i] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
-      u -= (float)a;
-      v -= (float)b;
+      p[i] = pair_of<T>(u, v);
+      u -= (float)__builtin_bit_cast(T, (uint16_t)(p[i] & 0xffffu));
+      v -= (float)__builtin_bit_cast(T, (uint16_t)(p[i] >> 16));
     }
   }
 };

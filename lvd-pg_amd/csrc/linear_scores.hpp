@@ -100,7 +100,9 @@ __device__ __forceinline__ int largest_exponent(const int* most) {   // by every
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pair_of(float a, float b) {   // two of 16 bits
-  return (uint32_t)__builtin_bit_cast(uint16_t, (T)a) | (uint32_t)__builtin_bit_cast(uint16_t, (T)b) << 16;
+  typedef float two __attribute__((ext_vector_type(2)));
+  typedef T pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((two{a, b}), pair));
 }
 #endif
 
