@@ -7,6 +7,8 @@
 // time, 2.4 TFLOP/s a compute unit at most against 0.6 of the cores' own float products.
 #pragma once
 
+#include <type_traits>
+
 #include "product_tiles.hip.hpp"
 
 namespace pcm {
@@ -38,8 +40,8 @@ struct FloatLoader {
   int64_t first;                             // the tile's first row (or entry)
   int64_t count;                             // rows (or entries) of the operand
   int row, step;                             // thread's place in the tile
-  v4f v[2];
-  int mark[2];                               // turned: of the rows
+  v4f v[2][2];                               // two stages
+  int mark[2][2];                            // turned: of the rows
   __device__ __forceinline__ const float* row_at(int64_t r) const {
     return x.p + (x.vars == 1 ? r * x.stride_ex : r / x.vars * x.stride_ex + r % x.vars * x.stride_var);
   }
@@ -60,40 +62,41 @@ struct FloatLoader {
     return x.stride == 1 && (!kTurned || (x.vars == 1 && count >= 4 && (count % 4 == 0 || first + FloatTile::BM <= count)));
   }
   // steps [k, k + 16), all of them there
+  template <int kSet>
   __device__ __forceinline__ void load_plain(int64_t k) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if constexpr (kTurned) {
         const int64_t r = k + step + i;
         // (without marks any word of the row is read, and not looked at)
-        mark[i] = *(x.skip ? x.skip + r : reinterpret_cast<const int*>(x.p + r * x.stride_ex));
-        v[i] = *reinterpret_cast<const v4f_by4*>(at[0] + r * x.stride_ex);
+        mark[kSet][i] = *(x.skip ? x.skip + r : reinterpret_cast<const int*>(x.p + r * x.stride_ex));
+        v[kSet][i] = *reinterpret_cast<const v4f_by4*>(at[0] + r * x.stride_ex);
       } else {
-        v[i] = *reinterpret_cast<const v4f_by4*>(at[i] + k + step);
+        v[kSet][i] = *reinterpret_cast<const v4f_by4*>(at[i] + k + step);
       }
     }
   }
-  // steps [k, k + 16) of those below end, any strides
+  // steps [k, k + 16) of those below end, any strides; into the first set
   __device__ __forceinline__ void load_any(int64_t k, int64_t end) {
     const int64_t s = k + step;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if constexpr (kTurned) {
         const bool some = s + i < end && !(x.skip && x.skip[s + i] == kDeadRow);
-        mark[i] = 0;
+        mark[0][i] = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = some && first + row + e < count ? row_at(s + i)[(first + row + e) * x.stride] : 0.f;
+        for (int e = 0; e < 4; ++e) v[0][i][e] = some && first + row + e < count ? row_at(s + i)[(first + row + e) * x.stride] : 0.f;
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = s + e < end ? at[i][(s + e) * x.stride] : 0.f;
+        for (int e = 0; e < 4; ++e) v[0][i][e] = s + e < end ? at[i][(s + e) * x.stride] : 0.f;
       }
     }
   }
-  // one half of the thread's floats to LDS, in three parts each
-  template <int kHalf>
+  // one half of a set's floats to LDS, in three parts each
+  template <int kSet, int kHalf>
   __device__ __forceinline__ void store(char* planes_of) const {
     if constexpr (!kTurned) {
-      v4f w = v[kHalf];
+      v4f w = v[kSet][kHalf];
       char* const to = planes_of + (row + 64 * kHalf) * kFloatPitch + step * 2;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
@@ -102,10 +105,10 @@ struct FloatLoader {
         if (p < 2) w -= v4f{as_float(a << 16), as_float(a & 0xffff0000u), as_float(b << 16), as_float(b & 0xffff0000u)};
       }
     } else {
-      const bool none[2] = {x.skip && mark[0] == kDeadRow, x.skip && mark[1] == kDeadRow};
+      const bool none[2] = {x.skip && mark[kSet][0] == kDeadRow, x.skip && mark[kSet][1] == kDeadRow};
 #pragma unroll
       for (int e = 2 * kHalf; e < 2 * kHalf + 2; ++e) {
-        float u = none[0] ? 0.f : v[0][e], w = none[1] ? 0.f : v[1][e];
+        float u = none[0] ? 0.f : v[kSet][0][e], w = none[1] ? 0.f : v[kSet][1][e];
         char* const to = planes_of + (row + e) * kFloatPitch + step * 2;
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
@@ -136,15 +139,11 @@ __device__ __forceinline__ void float_stages(const FloatOperand& a, const FloatO
     from_a.load_any(s * kFloatSteps, k);
     from_b.load_any(s * kFloatSteps, k);
   };
-  auto load_plain = [&](int64_t s) {
-    from_a.load_plain(s * kFloatSteps);
-    from_b.load_plain(s * kFloatSteps);
-  };
   auto store = [&](char* to) {
-    from_a.template store<0>(to);
-    from_a.template store<1>(to);
-    from_b.template store<0>(to + S::BM * kFloatPitch);
-    from_b.template store<1>(to + S::BM * kFloatPitch);
+    from_a.template store<0, 0>(to);
+    from_a.template store<0, 1>(to);
+    from_b.template store<0, 0>(to + S::BM * kFloatPitch);
+    from_b.template store<0, 1>(to + S::BM * kFloatPitch);
   };
   v4i fa[3][S::FM], fb[3][S::FN];
   auto read = [&](const char* from) {
@@ -171,32 +170,49 @@ __device__ __forceinline__ void float_stages(const FloatOperand& a, const FloatO
   };
   // stages that are there in whole, in requests of four neighbours
   const int64_t whole = from_a.plain() && from_b.plain() ? min(last, k / kFloatSteps) : first;
+  auto load_plain = [&](auto set, int64_t s) {   // (past the end the last one once more, not used)
+    const int64_t at = min(s, whole - 1) * kFloatSteps;
+    from_a.template load_plain<set.value>(at);
+    from_b.template load_plain<set.value>(at);
+  };
+  // stage s is in LDS, s + 1 in the other set of registers; s + 2 goes into `set`
+  auto stage = [&](auto set, int64_t s) {
+    constexpr int kOther = 1 - set.value;
+    char* const to_b = next + S::BM * kFloatPitch;
+    load_plain(set, s + 2);
+    read(mine);
+    multiply(0);
+    from_a.template store<kOther, 0>(next);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1);
+    from_a.template store<kOther, 1>(next);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(2);
+    from_b.template store<kOther, 0>(to_b);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(3);
+    from_b.template store<kOther, 1>(to_b);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(4);
+    multiply(5);
+    __syncthreads();
+    swap();
+  };
+  constexpr std::integral_constant<int, 0> kSet0{};
+  constexpr std::integral_constant<int, 1> kSet1{};
   int64_t s = first;
   if (first + 1 < whole) {
-    load_plain(first);
+    load_plain(kSet0, first);
+    load_plain(kSet1, first + 1);
     store(mine);
-    load_plain(first + 1);
     __syncthreads();
-    for (; s + 1 < whole; ++s) {
-      read(mine);
-      char* const to_b = next + S::BM * kFloatPitch;
-      multiply(0);
-      from_a.template store<0>(next);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(1);
-      from_a.template store<1>(next);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(2);
-      from_b.template store<0>(to_b);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(3);
-      from_b.template store<1>(to_b);
-      __builtin_amdgcn_sched_barrier(0);
-      load_plain(min(s + 2, whole - 1));   // (at the end the last one once more, not used)
-      multiply(4);
-      multiply(5);
-      __syncthreads();
-      swap();
+    for (; s + 2 < whole; s += 2) {
+      stage(kSet0, s);
+      stage(kSet1, s + 1);
+    }
+    if (s + 1 < whole) {
+      stage(kSet0, s);
+      ++s;
     }
   } else if (first < last) {
     load_any(first);

@@ -206,7 +206,7 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
   });
 }
 template <typename T, typename S, int kParts>
-__global__ __launch_bounds__(S::threads) void gradient_kernel(GradientTask t) {
+__global__ __launch_bounds__(S::threads, 2) void gradient_kernel(GradientTask t) {
   gradient_tile<T, S, kParts>(t);
 }
 

@@ -81,7 +81,7 @@ __device__ __forceinline__ void score_tile(const ScoreTask& t) {
   });
 }
 template <typename T, typename S>
-__global__ __launch_bounds__(S::threads) void score_kernel(ScoreTask t) {
+__global__ __launch_bounds__(S::threads, 2) void score_kernel(ScoreTask t) {
   score_tile<T, S>(t);
 }
 

@@ -62,7 +62,7 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
   else product_tile<T, S>(t.a, t.b, t.m, t.n, t.steps, done);
 }
 template <typename T, typename S>
-__global__ __launch_bounds__(S::threads) void out_kernel(OutTask t, bool fours) {
+__global__ __launch_bounds__(S::threads, 2) void out_kernel(OutTask t, bool fours) {
   out_tile<T, S>(t, fours);
 }
 
