@@ -4,7 +4,7 @@
 // Categories are the rows of a, so that a lane's sums are of one row of features: it takes their maximum and the sum of
 // exponentials in registers, the tile's waves join theirs in LDS, and a pair of numbers per row and tile of categories is all that
 // is written; a second launch joins those.  The score of a given category is written by the lane that has it.
-#include "float_tiles.hip.hpp"
+#include "few_rows.hip.hpp"
 
 namespace pcm {
 
@@ -85,6 +85,46 @@ __global__ __launch_bounds__(S::threads, 2) void score_kernel(ScoreTask t) {
   score_tile<T, S>(t);
 }
 
+// Few rows: a thread has one of the tile's categories (kGroups 1) or up to four of one row
+template <typename T, int kGroups>
+__global__ __launch_bounds__(512) void score_few_kernel(ScoreTask t, FewOperand w, FewOperand f, int length) {
+  __shared__ float lds[8][kFewTile][kFewPitch<kGroups>];
+  __shared__ Part joined[512];
+  few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds);
+  constexpr int kRows = 16 * kGroups, kLanes = 512 / kRows;   // lanes to a row
+  const int n = threadIdx.x % kRows, lane = threadIdx.x / kRows;
+  const int64_t c0 = (int64_t)blockIdx.x * kFewTile;
+  const float sn = t.scale.n && n < t.rows ? t.scale.n[n] : 1.f;
+  float x[kFewTile / kLanes], base = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewTile / kLanes; ++i) {
+    const int at = lane + i * kLanes;
+    const int64_t c = c0 + at;
+    float v = lds[0][at][n];
+    if constexpr (sizeof(T) == 1) v = (float)__builtin_bit_cast(int, v) * sn * (c < t.cats ? t.scale.m[c] : 1.f);
+    x[i] = score_of(v, bias_at(t.bias, c, t.cats));
+    base = fmaxf(base, x[i]);
+  }
+  const float to = base == -INFINITY ? 0.f : base;
+#pragma unroll
+  for (int i = 0; i < kFewTile / kLanes; ++i) sum += __builtin_amdgcn_exp2f((x[i] - to) * kLog2e);
+  joined[threadIdx.x] = {sum == 0.f ? base : to, sum};
+  if (n < t.rows)
+    for (int s = 0; s < t.given.slots; ++s) {
+      const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - c0;
+#pragma unroll
+      for (int i = 0; i < kFewTile / kLanes; ++i)
+        if (g == lane + i * kLanes) t.logp[n * t.given.slots + s] = x[i];
+    }
+  __syncthreads();
+#pragma unroll
+  for (int s = kLanes / 2; s; s /= 2) {
+    if (lane < s) joined[threadIdx.x] = join(joined[threadIdx.x], joined[threadIdx.x + s * kRows]);
+    __syncthreads();
+  }
+  if (lane == 0 && n < t.rows) t.parts[blockIdx.x * t.rows + n] = joined[n];
+}
+
 // Joins the tiles' parts: `per` rows a workgroup, 256 / per lanes to each
 __global__ __launch_bounds__(256) void join_scores_kernel(const Part* parts, int64_t tiles, int64_t rows, int per, GivenRef given, int64_t cats,
                                                           float* logp, float* log_sum) {
@@ -122,12 +162,10 @@ __global__ __launch_bounds__(256) void join_scores_kernel(const Part* parts, int
 
 typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
-typedef TileSizes<128, 32, 32, 32> Narrow;
-enum { kWide, kMiddle, kNarrow };
+enum { kWide, kMiddle };
 
 int tiles_for(int64_t m, int64_t n, bool of_float) {
   if (of_float) return kMiddle;
-  if (n <= 32) return kNarrow;
   const int64_t wide = ((m + 255) / 256) * ((n + 255) / 256);
   return wide >= 192 ? kWide : kMiddle;
 }
@@ -139,22 +177,27 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch(const ScoreTask& t, hipStream_t stream) {
-  const int size = tiles_for(t.cats, t.rows, false);
-  if (size == kWide) launch<T, Wide>(t, stream);
-  else if (size == kMiddle) launch<T, Middle>(t, stream);
-  else launch<T, Narrow>(t, stream);
+  if (tiles_for(t.cats, t.rows, false) == kWide) launch<T, Wide>(t, stream);
+  else launch<T, Middle>(t, stream);
 }
-int64_t tiles_of_cats(int64_t cats, int64_t rows, bool of_float) {
-  const int64_t each = tiles_for(cats, rows, of_float) == kWide ? 256 : 128;
+template <typename T>
+void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
+  const dim3 grid((unsigned)((t.cats + kFewTile - 1) / kFewTile)), block(512);
+  if (t.rows <= 16) hipLaunchKernelGGL((score_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
+  else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
+  else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
+}
+int64_t tiles_of_cats(int64_t cats, int64_t rows, bool of_float, bool few) {
+  const int64_t each = few ? kFewTile : tiles_for(cats, rows, of_float) == kWide ? 256 : 128;
   return (cats + each - 1) / each;
 }
-int64_t parts_bytes(int64_t cats, int64_t rows, bool of_float) { return round_up(tiles_of_cats(cats, rows, of_float) * rows * (int64_t)sizeof(Part), 256); }
+int64_t parts_bytes(int64_t cats, int64_t rows, bool of_float, bool few) { return round_up(tiles_of_cats(cats, rows, of_float, few) * rows * (int64_t)sizeof(Part), 256); }
 
-void join_launch(const ScoreTask& t, float* d_log_sum, hipStream_t stream) {
+void join_launch(const ScoreTask& t, bool few, float* d_log_sum, hipStream_t stream) {
   // few rows: all lanes of a workgroup to one, many: neighbouring rows side by side
   const int per = t.rows >= 4096 ? 16 : t.rows >= 512 ? 4 : 1;
   hipLaunchKernelGGL(join_scores_kernel, dim3((unsigned)((t.rows + per - 1) / per)), dim3(256), 0, stream, t.parts,
-                     tiles_of_cats(t.cats, t.rows, t.fw.p),                     t.rows, per, t.given, t.cats, t.logp, d_log_sum);
+                     tiles_of_cats(t.cats, t.rows, t.fw.p, few),                     t.rows, per, t.given, t.cats, t.logp, d_log_sum);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of linear_scores failed: %s", hipGetErrorString(e));
 }
@@ -170,9 +213,13 @@ void check_linear(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const
   check_given(given);
 }
 
+bool few_rows(const Matrix2& f, const Matrix2& w) { return f.rows() <= kFewRowsMost && f.stride == 1 && w.stride == 1; }
+FewOperand few_operand(const Matrix2& x) { return {x.p, x.stride_ex, x.stride_var, x.vars}; }
+
 int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w) {
+  if (few_rows(f, w)) return parts_bytes(w.examples, f.rows(), false, true);
   return (readable(f) ? 0 : laid_bytes(f.rows(), f.length, 1)) + (readable(w) ? 0 : laid_bytes(w.rows(), w.length, 1)) +
-         parts_bytes(w.examples, f.rows(), f.type == PCM_F32);
+         parts_bytes(w.examples, f.rows(), f.type == PCM_F32, false);
 }
 
 void check_workspace(const void* d_work, int64_t work_bytes, int64_t need, const char* what) {
@@ -210,7 +257,9 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   check_workspace(d_work, work_bytes, linear_scores_workspace(f, w), "linear scores");
   ScoreTask t{};
   char* work = static_cast<char*>(d_work);
-  if (f.type == PCM_F32) {
+  const bool few = few_rows(f, w);
+  if (few) {
+  } else if (f.type == PCM_F32) {
     t.ff = float_operand(f, false);
     t.fw = float_operand(w, false);
     t.fk = f.length;
@@ -226,13 +275,22 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   t.given.vars = f.vars;
   t.logp = d_logp;
   t.parts = reinterpret_cast<Part*>(work);
-  if (f.type == PCM_F32) launch<float, FloatTile>(t, stream);
-  else if (f.type == PCM_F16) launch<f16>(t, stream);
-  else launch<bf16>(t, stream);
-  join_launch(t, d_log_sum, stream);
+  if (few) {
+    const FewOperand fw = few_operand(w), ff = few_operand(f);
+    if (f.type == PCM_F32) launch_few<float>(t, fw, ff, f.length, stream);
+    else if (f.type == PCM_F16) launch_few<f16>(t, fw, ff, f.length, stream);
+    else launch_few<bf16>(t, fw, ff, f.length, stream);
+  } else if (f.type == PCM_F32) {
+    launch<float, FloatTile>(t, stream);
+  } else if (f.type == PCM_F16) {
+    launch<f16>(t, stream);
+  } else {
+    launch<bf16>(t, stream);
+  }
+  join_launch(t, few, d_log_sum, stream);
 }
 
-int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, false); }
+int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, false, rows <= kFewRowsMost); }
 
 void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
                     int32_t length, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
@@ -257,8 +315,10 @@ void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, in
   t.given.vars = vars;
   t.logp = d_logp;
   t.parts = static_cast<Part*>(d_work);
-  launch<int8_t>(t, stream);
-  join_launch(t, d_log_sum, stream);
+  const bool few = t.rows <= kFewRowsMost;
+  if (few) launch_few<int8_t>(t, FewOperand{w, pitch, 0, 1}, FewOperand{f, pitch, 0, 1}, (int)pitch, stream);
+  else launch<int8_t>(t, stream);
+  join_launch(t, few, d_log_sum, stream);
 }
 
 }  // namespace pcm

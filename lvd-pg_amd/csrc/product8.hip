@@ -57,7 +57,8 @@ void rows8(const Matrix2& x, int8_t* d_codes, float* d_scales, hipStream_t strea
 
 int64_t product8_workspace(int64_t rows, int64_t cats, int32_t length) {
   if (rows < 1 || cats < 1 || length < 1 || length > kMaxLength8 || rows > 0x7fffffff || cats > 0x7fffffff) return 0;
-  const int parts = parts_for(cats, rows, round_up(length, kKBytes) / kKBytes);
+  const int steps = (int)(round_up(length, kKBytes) / kKBytes);
+  const int parts = rows <= kFewRowsMost ? parts_for_few(cats, steps) : parts_for(cats, rows, steps);
   return parts > 1 ? round_up(parts * rows * cats * 4, 256) : 0;
 }
 
@@ -73,7 +74,9 @@ void product8(const int8_t* a, const float* a_scales, int64_t rows, const int8_t
   if (((uintptr_t)a | (uintptr_t)b) & 15) fail(PCM_ERR_ARG, "8-bit product: codes must be 16-byte aligned");
   check_workspace(d_work, work_bytes, product8_workspace(rows, cats, length), "8-bit product");
   const int64_t codes = round_up(length, kKBytes);
-  const int steps = (int)(codes / kKBytes), parts = parts_for(cats, rows, steps);
+  const int steps = (int)(codes / kKBytes);
+  const bool few = rows <= kFewRowsMost;
+  const int parts = few ? parts_for_few(cats, steps) : parts_for(cats, rows, steps);
   OutTask t{};
   t.a = {b, codes, 0};
   t.b = {a, codes, 0};
@@ -86,13 +89,13 @@ void product8(const int8_t* a, const float* a_scales, int64_t rows, const int8_t
     t.out = d_out;
     t.type = type;
     t.pitch = pitch;
-    product_out(PCM_U8, t, stream);
+    few ? product_few(t, stream) : product_out(PCM_U8, t, stream);
     return;
   }
   t.out = d_work;
   t.type = kRawSums;
   t.pitch = cats;
-  product_out(PCM_U8, t, stream);
+  few ? product_few(t, stream) : product_out(PCM_U8, t, stream);
   join_parts(d_work, parts, true, cats, rows, t.finish, d_out, type, pitch, stream);
 }
 

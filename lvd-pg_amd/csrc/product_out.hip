@@ -66,6 +66,21 @@ __global__ __launch_bounds__(S::threads, 2) void out_kernel(OutTask t, bool four
   out_tile<T, S>(t, fours);
 }
 
+template <int kGroups>
+__global__ __launch_bounds__(512) void out_few_kernel(OutTask t) {
+  __shared__ float lds[8][kFewTile][kFewPitch<kGroups>];
+  few_sums<int8_t, kGroups>(FewOperand{t.a.p, t.a.pitch, 0, 1}, FewOperand{t.b.p, t.b.pitch, 0, 1}, t.m, t.n, t.steps.count * kKBytes, t.steps.parts, lds);
+  const int at = threadIdx.x % kFewTile;
+  const int64_t m = (int64_t)blockIdx.x * kFewTile + at;
+  if (m >= t.m) return;
+  const float scale = t.finish.scale.m[m], bias = bias_of(t.finish.bias, m);
+  for (int n = threadIdx.x / kFewTile; n < t.n; n += 512 / kFewTile) {
+    const int sum = __builtin_bit_cast(int, lds[0][at][n]);
+    if (t.type == kRawSums) static_cast<int*>(t.out)[((int64_t)blockIdx.y * t.n + n) * t.pitch + m] = sum;
+    else store_as(t.out, t.type, n * t.pitch + m, FinishAt(t.finish, n, 0)((float)sum, scale, bias));
+  }
+}
+
 __global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, int count, bool whole, int64_t m, int64_t n, Finish finish, void* out,
                                                          int type, int64_t pitch) {
   const int most = finish.most ? largest_exponent(finish.most) : 0;
@@ -87,7 +102,6 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, 
 
 typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
-typedef TileSizes<128, 32, 32, 32> Narrow;
 
 template <typename T, typename S>
 void launch(const OutTask& t, hipStream_t stream) {
@@ -100,18 +114,28 @@ void launch(const OutTask& t, hipStream_t stream) {
 bool wide(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
 template <typename T>
 void launch(const OutTask& t, hipStream_t stream) {
-  if (t.n <= 32) launch<T, Narrow>(t, stream);
-  else if (wide(t.m, t.n)) launch<T, Wide>(t, stream);
+  if (wide(t.m, t.n)) launch<T, Wide>(t, stream);
   else launch<T, Middle>(t, stream);
 }
 }  // namespace
 
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
-  if (of_float) n = std::max<int64_t>(n, 33);          // (one size of tiles)
-  else if (wide(m, n) && n > 32) return 1;
-  const int64_t tiles = ((m + 127) / 128) * ((n + (n <= 32 ? 31 : 127)) / (n <= 32 ? 32 : 128));
+  if (!of_float && wide(m, n)) return 1;
+  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
   // as many parts as fill the device twice over, each of eight steps or more
   return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 8, 64}));
+}
+int parts_for_few(int64_t m, int64_t steps) {
+  // a workgroup's waves take a step each at a time: parts of four rounds or more, as many as give every compute unit two workgroups
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 * kFewTile + m - 1) / m, steps / 32, 16}));
+}
+void product_few(const OutTask& t, hipStream_t stream) {
+  const dim3 grid((unsigned)((t.m + kFewTile - 1) / kFewTile), (unsigned)t.steps.parts), block(512);
+  if (t.n <= 16) hipLaunchKernelGGL(out_few_kernel<1>, grid, block, 0, stream, t);
+  else if (t.n <= 32) hipLaunchKernelGGL(out_few_kernel<2>, grid, block, 0, stream, t);
+  else hipLaunchKernelGGL(out_few_kernel<4>, grid, block, 0, stream, t);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of a product failed: %s", hipGetErrorString(e));
 }
 
 void product_out(int operands, const OutTask& t, hipStream_t stream) {

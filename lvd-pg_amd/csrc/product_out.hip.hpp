@@ -2,7 +2,7 @@
 // second launch joins.
 #pragma once
 
-#include "float_tiles.hip.hpp"
+#include "few_rows.hip.hpp"
 
 namespace pcm {
 
@@ -31,10 +31,13 @@ struct OutTask {
 
 // launches of any size
 void product_out(int operands, const OutTask& t, hipStream_t stream);   // operands: PCM_F32, PCM_BF16, PCM_F16, PCM_U8 (whole numbers)
+// ... of 8-bit rows, a few of b (kFewRowsMost): t.a, t.b and t.steps as for product_out
+void product_few(const OutTask& t, hipStream_t stream);
 // out = the finished sums of parts [parts][n][m] floats (or whole numbers)
 void join_parts(const void* parts, int count, bool whole, int64_t m, int64_t n, const Finish& finish, void* out, int type, int64_t pitch, hipStream_t stream);
 // how many parts the summed axis of a product is best cut into
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float = false);
+int parts_for_few(int64_t m, int64_t steps);   // ... of product_few
 
 #ifdef __HIPCC__
 struct FinishAt {                // of one n
