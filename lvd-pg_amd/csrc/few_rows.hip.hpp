@@ -1,7 +1,7 @@
 // Products of a long matrix (weights: categories or channels) with a few rows: bound by reading the long one once.
 //
-// A workgroup takes 32 rows of the long matrix, its eight waves every eighth piece of 128 bytes of them each, straight from memory into the
-// cores' operands: whatever the rows' length and alignment, nothing is laid out.  The waves' sums meet in LDS.
+// A workgroup takes 32 rows of the long matrix (64 with more than 32 others), its eight waves every eighth piece of 128 bytes of them each, whatever
+// the rows' length and alignment: nothing is laid out.  The waves' sums meet in LDS.
 #pragma once
 
 #include "float_tiles.hip.hpp"
@@ -9,7 +9,8 @@
 namespace pcm {
 
 constexpr int kFewRowsMost = 64;             // rows that are few
-constexpr int kFewTile = 32;                 // rows of the long matrix of a workgroup
+// rows of the long matrix of a workgroup
+inline int few_tile(int64_t rows) { return rows <= 32 ? 32 : 64; }
 struct FewOperand {                          // rows of neighbouring entries
   const void* p;
   int64_t stride_ex, stride_var;             // in entries
@@ -42,43 +43,53 @@ struct FewCores<int8_t> {
   static __device__ __forceinline__ v4i mma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
-// A lane's 32 bytes of a row's piece, 64 apart: of 16-bit and 8-bit types a step's operand each, of float one step's
+// A lane's 16 bytes of a piece of 128 bytes of a row, of which eight neighbouring lanes take one each
 template <typename T>
-struct FewPiece {
-  static constexpr int entries = 128 / sizeof(T);
-  raw4 v[2];
-  __device__ __forceinline__ void load(const T* row) {
-    const int quarter = (threadIdx.x & 63) / 16;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (sizeof(T) == 1) v[i] = *reinterpret_cast<const raw4*>(row + i * 64 + quarter * 16);
-      else v[i] = load16(row + (i * 64 + quarter * 16) / sizeof(T));
+struct FewChunk {
+  raw4 v;
+  uint32_t next;                             // 16-bit types: the word behind
+  __device__ __forceinline__ void load(const T* at) {
+    if constexpr (sizeof(T) == 1) {
+      v = *reinterpret_cast<const raw4*>(at);
+    } else if constexpr (sizeof(T) == 4) {
+      v = load16(at);
+    } else {                                 // whole words, of which the first and the last may hold a neighbour's entry
+      const uint32_t* const p = reinterpret_cast<const uint32_t*>((uintptr_t)at & ~(uintptr_t)3);
+      v = *reinterpret_cast<const raw4_by4*>(p);
+      next = p[(uintptr_t)at & 2 ? 4 : 3];
     }
   }
-  // with `left` entries left in the row
-  __device__ __forceinline__ void load_end(const T* row, int left) {
-    const int quarter = (threadIdx.x & 63) / 16;
+  // of the `left` entries that are left there
+  __device__ __forceinline__ void load_end(const T* at, int left) {
     constexpr int each = 16 / sizeof(T);
+    T e[each];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      T e[each];
+    for (int k = 0; k < each; ++k) e[k] = k < left ? at[k] : (T)0;
+    v = __builtin_bit_cast(raw4, e);
+  }
+  __device__ __forceinline__ raw4 get(const T* at) const {
+    if constexpr (sizeof(T) != 2) return v;
+    const uint32_t shift = ((uint32_t)(uintptr_t)at & 2) * 8;
+    raw4 w;
 #pragma unroll
-      for (int k = 0; k < each; ++k) {
-        const int at = (i * 64 + quarter * 16) / (int)sizeof(T) + k;
-        e[k] = at < left ? row[at] : (T)0;
-      }
-      v[i] = __builtin_bit_cast(raw4, e);
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t hi = k < 3 ? v[k < 3 ? k + 1 : 3] : next, lo = v[k];
+      w[k] = __builtin_amdgcn_alignbit(hi, lo, shift);
     }
+    return w;
   }
 };
 template <typename T>
-struct FewParts {                            // ... as operands of the cores
+struct FewParts {                            // two chunks of a row, 64 bytes apart, as operands of the cores
   v4i p[sizeof(T) == 4 ? 3 : 2];
-  __device__ __forceinline__ explicit FewParts(const FewPiece<T>& x) {
+  __device__ __forceinline__ FewParts(raw4 x, raw4 y) {
     if constexpr (sizeof(T) == 4) {          // three parts of eight floats
       float w[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = as_float(x.v[k / 4][k % 4]);
+      for (int k = 0; k < 4; ++k) {
+        w[k] = as_float(x[k]);
+        w[4 + k] = as_float(y[k]);
+      }
 #pragma unroll
       for (int q = 0; q < 3; ++q)
 #pragma unroll
@@ -91,105 +102,142 @@ struct FewParts {                            // ... as operands of the cores
           }
         }
     } else {
-      p[0] = __builtin_bit_cast(v4i, x.v[0]);
-      p[1] = __builtin_bit_cast(v4i, x.v[1]);
+      p[0] = __builtin_bit_cast(v4i, x);
+      p[1] = __builtin_bit_cast(v4i, y);
     }
   }
 };
 
-// Sums of rows [32 blockIdx.x, + 32) of a with all (16 kGroups at most) rows of b over `length` entries: sum of rows m and n of the tile at
-// lds[m][n], 32 bits (whole numbers: their bits), after a barrier.  Parts of the pieces by blockIdx.y.
 template <int kGroups>
-constexpr int kFewPitch = 16 * kGroups + 1;
+struct FewTile {                             // kGroups: of 16 rows of b
+  static constexpr int rows = 16 * kGroups;
+  static constexpr int longs = kGroups == 4 ? 64 : 32;        // rows of a: as many as of b, or more
+  static constexpr int wave_bytes = (longs + rows) * 128;     // a piece of each
+  static constexpr int pitch = rows + 1;                      // of the sums
+  static constexpr int sums_bytes = 8 * longs * pitch * 4;
+  static constexpr int lds = sums_bytes > 8 * wave_bytes ? sums_bytes : 8 * wave_bytes;
+};
+// Sums of rows [longs blockIdx.x, + longs) of a with all (16 kGroups at most) rows of b over `length` entries: sum of rows m and n of the tile
+// at m * pitch + n of what is returned (LDS), 32 bits (whole numbers: their bits), after a barrier.  Parts of the pieces by blockIdx.y.
+//
+// A wave's piece goes through its own share of LDS: requested by eight lanes a row, read back as the cores' operands.  No barrier until the
+// waves' sums meet; the next piece is requested before one is multiplied.
 template <typename T, int kGroups>
-__device__ __forceinline__ void few_sums(const FewOperand& a, const FewOperand& b, int64_t m, int64_t n, int length, int parts,
-                                         float (&lds)[8][kFewTile][kFewPitch<kGroups>]) {
+__device__ __forceinline__ const float* few_sums(const FewOperand& a, const FewOperand& b, int64_t m, int64_t n, int length, int parts, char* lds) {
   typedef typename std::conditional<sizeof(T) == 4, bf16, T>::type Core;
-  constexpr int kPiece = FewPiece<T>::entries;
+  typedef FewTile<kGroups> S;
+  constexpr int kPiece = 128 / sizeof(T), kEach = 16 / sizeof(T), kLongs = S::longs / 8, kRows = S::rows / 8, kCats = S::longs / 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const T *at_a[2], *at_b[kGroups];
+  char* const mine = lds + wave * S::wave_bytes;
+  const T *at_a[kLongs], *at_b[kRows];
 #pragma unroll
-  for (int g = 0; g < 2; ++g) at_a[g] = static_cast<const T*>(a.p) + min((int64_t)blockIdx.x * kFewTile + 16 * g + (lane & 15), m - 1) * a.stride_ex;
+  for (int g = 0; g < kLongs; ++g)
+    at_a[g] = static_cast<const T*>(a.p) + min((int64_t)blockIdx.x * S::longs + 8 * g + lane / 8, m - 1) * a.stride_ex + lane % 8 * kEach;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    const int64_t r = min((int64_t)(16 * g + (lane & 15)), n - 1);
-    at_b[g] = static_cast<const T*>(b.p) + r / b.vars * b.stride_ex + r % b.vars * b.stride_var;
+  for (int g = 0; g < kRows; ++g) {
+    const int64_t r = min((int64_t)(8 * g + lane / 8), n - 1);
+    at_b[g] = static_cast<const T*>(b.p) + r / b.vars * b.stride_ex + r % b.vars * b.stride_var + lane % 8 * kEach;
   }
-  typename FewCores<Core>::Sums sums[2][kGroups] = {};
-  auto multiply = [&](const FewPiece<T> (&pa)[2], const FewPiece<T> (&pb)[kGroups]) {
-    const FewParts<T> fa[2] = {FewParts<T>(pa[0]), FewParts<T>(pa[1])};
+  typename FewCores<Core>::Sums sums[kCats][kGroups] = {};
+  FewChunk<T> ca[kLongs], cb[kRows];
+  auto load = [&](int piece) {
+#pragma unroll
+    for (int g = 0; g < kLongs; ++g) ca[g].load(at_a[g] + (int64_t)piece * kPiece);
+#pragma unroll
+    for (int g = 0; g < kRows; ++g) cb[g].load(at_b[g] + (int64_t)piece * kPiece);
+  };
+  // chunk c of row r lies at c ^ (r / 2) % 8 of the row
+  const int to = lane / 8 * 128 + ((lane & 7) ^ (lane >> 4 & 3)) * 16;     // (row r + 8 g: bits of g join below)
+  auto put = [&](int g, raw4 v) { *reinterpret_cast<raw4*>(mine + g * 1024 + (to ^ (g & 1) * 64)) = v; };
+  auto operand = [&](int group) {
+    const int r = lane & 15, swap = r >> 1 & 7, quarter = lane / 16;
+    const char* const row = mine + (16 * group + r) * 128;
+    return FewParts<T>(*reinterpret_cast<const raw4*>(row + (quarter ^ swap) * 16), *reinterpret_cast<const raw4*>(row + ((quarter + 4) ^ swap) * 16));
+  };
+  auto multiply = [&] {
+    constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
+    v4i fa[kCats][kParts];
+#pragma unroll
+    for (int i = 0; i < kCats; ++i) {
+      const FewParts<T> x = operand(i);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) fa[i][q] = x.p[q];
+    }
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const FewParts<T> fb(pb[g]);
+      const FewParts<T> fb = operand(kCats + g);
       if constexpr (sizeof(T) == 4) {
         constexpr int of_a[6] = {0, 2, 1, 0, 1, 0}, of_b[6] = {2, 0, 1, 1, 0, 0};   // hl lh mm hm mh hh
 #pragma unroll
         for (int q = 0; q < 6; ++q)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) sums[i][g] = FewCores<Core>::mma(fa[i].p[of_a[q]], fb.p[of_b[q]], sums[i][g]);
+          for (int i = 0; i < kCats; ++i) sums[i][g] = FewCores<Core>::mma(fa[i][of_a[q]], fb.p[of_b[q]], sums[i][g]);
       } else {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) sums[i][g] = FewCores<Core>::mma(fa[i].p[q], fb.p[q], sums[i][g]);
+          for (int i = 0; i < kCats; ++i) sums[i][g] = FewCores<Core>::mma(fa[i][q], fb.p[q], sums[i][g]);
       }
     }
   };
-  // whole pieces first, the wave's next one on its way while one is multiplied; then what is left
+  // whole pieces first, then what is left
   const int whole = length / kPiece, pieces = (length + kPiece - 1) / kPiece;
   const int first = (int)((int64_t)pieces * blockIdx.y / parts), last = (int)((int64_t)pieces * (blockIdx.y + 1) / parts);
   const int end = min(last, whole);
-  FewPiece<T> pa[2][2], pb[2][kGroups];
-  auto load = [&](int set, int piece) {
+  if (first + wave < end) {
+    load(first + wave);
+    for (int piece = first + wave; piece < end; piece += 8) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) pa[set][g].load(at_a[g] + (int64_t)piece * kPiece);
+      for (int g = 0; g < kLongs; ++g) put(g, ca[g].get(at_a[g]));
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) pb[set][g].load(at_b[g] + (int64_t)piece * kPiece);
-  };
-  int piece = first + wave;
-  if (piece < end) {
-    load(0, piece);
-    for (; piece < end; piece += 16) {
-      load(1, min(piece + 8, end - 1));      // (past the end the last one once more, not used)
-      multiply(pa[0], pb[0]);
-      if (piece + 8 >= end) break;
-      load(0, min(piece + 16, end - 1));
-      multiply(pa[1], pb[1]);
+      for (int g = 0; g < kRows; ++g) put(kLongs + g, cb[g].get(at_b[g]));
+      load(min(piece + 8, end - 1));         // (past the end the last one once more, not used)
+      multiply();
     }
   }
-  if (last > end && wave == 7) {
-    const int left = length - whole * kPiece;
+  if constexpr (sizeof(T) > 1) {             // (8-bit rows are whole pieces)
+    if (last > end && wave == 7) {
+      const int left = length - whole * kPiece - lane % 8 * kEach;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) pa[0][g].load_end(at_a[g] + (int64_t)whole * kPiece, left);
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) pb[0][g].load_end(at_b[g] + (int64_t)whole * kPiece, left);
-    multiply(pa[0], pb[0]);
+      for (int g = 0; g < kLongs + kRows; ++g) {
+        __builtin_amdgcn_sched_barrier(0);   // one at a time: registers
+        ca[0].load_end((g < kLongs ? at_a[g < kLongs ? g : 0] : at_b[g < kLongs ? 0 : g - kLongs]) + (int64_t)whole * kPiece, left);
+        put(g, ca[0].v);
+      }
+      multiply();
+    }
   }
+  float* const out = reinterpret_cast<float*>(lds);
+  __syncthreads();
 #pragma unroll
   for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kCats; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const auto sum = sums[i][g][r];        // (a bit cast of a vector's element takes the vector's first one)
-        lds[wave][16 * i + 4 * (lane / 16) + r][16 * g + (lane & 15)] = __builtin_bit_cast(float, sum);
+        out[(wave * S::longs + 16 * i + 4 * (lane / 16) + r) * S::pitch + 16 * g + (lane & 15)] = __builtin_bit_cast(float, sum);
       }
   __syncthreads();
-  for (int i = threadIdx.x; i < kFewTile * 16 * kGroups; i += 512) {
-    const int r = i / (16 * kGroups), c = i % (16 * kGroups);
+  for (int i = threadIdx.x; i < S::longs * S::rows; i += 512) {
+    const int at = i / S::rows * S::pitch + i % S::rows;
     if constexpr (sizeof(T) == 1) {
       int s = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += __builtin_bit_cast(int, lds[w][r][c]);
-      lds[0][r][c] = __builtin_bit_cast(float, s);
+      for (int w = 0; w < 8; ++w) {
+        const float x = out[w * S::longs * S::pitch + at];
+        s += __builtin_bit_cast(int, x);
+      }
+      out[at] = __builtin_bit_cast(float, s);
     } else {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += lds[w][r][c];
-      lds[0][r][c] = s;
+      for (int w = 0; w < 8; ++w) s += out[w * S::longs * S::pitch + at];
+      out[at] = s;
     }
   }
   __syncthreads();
+  return out;
 }
 #endif
 

@@ -85,41 +85,42 @@ __global__ __launch_bounds__(S::threads, 2) void score_kernel(ScoreTask t) {
   score_tile<T, S>(t);
 }
 
-// Few rows: a thread has one of the tile's categories (kGroups 1) or up to four of one row
+// Few rows: a thread has some of the tile's categories, of one row
 template <typename T, int kGroups>
 __global__ __launch_bounds__(512) void score_few_kernel(ScoreTask t, FewOperand w, FewOperand f, int length) {
-  __shared__ float lds[8][kFewTile][kFewPitch<kGroups>];
+  typedef FewTile<kGroups> S;
+  __shared__ __attribute__((aligned(16))) char lds[S::lds];
   __shared__ Part joined[512];
-  few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds);
-  constexpr int kRows = 16 * kGroups, kLanes = 512 / kRows;   // lanes to a row
-  const int n = threadIdx.x % kRows, lane = threadIdx.x / kRows;
-  const int64_t c0 = (int64_t)blockIdx.x * kFewTile;
+  const float* const sums = few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds);
+  constexpr int kLanes = 512 / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
+  const int n = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
+  const int64_t c0 = (int64_t)blockIdx.x * S::longs;
   const float sn = t.scale.n && n < t.rows ? t.scale.n[n] : 1.f;
-  float x[kFewTile / kLanes], base = -INFINITY, sum = 0.f;
+  float x[kOwn], base = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kFewTile / kLanes; ++i) {
+  for (int i = 0; i < kOwn; ++i) {
     const int at = lane + i * kLanes;
     const int64_t c = c0 + at;
-    float v = lds[0][at][n];
+    float v = sums[at * S::pitch + n];
     if constexpr (sizeof(T) == 1) v = (float)__builtin_bit_cast(int, v) * sn * (c < t.cats ? t.scale.m[c] : 1.f);
     x[i] = score_of(v, bias_at(t.bias, c, t.cats));
     base = fmaxf(base, x[i]);
   }
   const float to = base == -INFINITY ? 0.f : base;
 #pragma unroll
-  for (int i = 0; i < kFewTile / kLanes; ++i) sum += __builtin_amdgcn_exp2f((x[i] - to) * kLog2e);
+  for (int i = 0; i < kOwn; ++i) sum += __builtin_amdgcn_exp2f((x[i] - to) * kLog2e);
   joined[threadIdx.x] = {sum == 0.f ? base : to, sum};
   if (n < t.rows)
     for (int s = 0; s < t.given.slots; ++s) {
       const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - c0;
 #pragma unroll
-      for (int i = 0; i < kFewTile / kLanes; ++i)
+      for (int i = 0; i < kOwn; ++i)
         if (g == lane + i * kLanes) t.logp[n * t.given.slots + s] = x[i];
     }
   __syncthreads();
 #pragma unroll
   for (int s = kLanes / 2; s; s /= 2) {
-    if (lane < s) joined[threadIdx.x] = join(joined[threadIdx.x], joined[threadIdx.x + s * kRows]);
+    if (lane < s) joined[threadIdx.x] = join(joined[threadIdx.x], joined[threadIdx.x + s * S::rows]);
     __syncthreads();
   }
   if (lane == 0 && n < t.rows) t.parts[blockIdx.x * t.rows + n] = joined[n];
@@ -182,13 +183,14 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
-  const dim3 grid((unsigned)((t.cats + kFewTile - 1) / kFewTile)), block(512);
+  const int each = few_tile(t.rows);
+  const dim3 grid((unsigned)((t.cats + each - 1) / each)), block(512);
   if (t.rows <= 16) hipLaunchKernelGGL((score_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
   else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
   else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
 }
 int64_t tiles_of_cats(int64_t cats, int64_t rows, bool of_float, bool few) {
-  const int64_t each = few ? kFewTile : tiles_for(cats, rows, of_float) == kWide ? 256 : 128;
+  const int64_t each = few ? few_tile(rows) : tiles_for(cats, rows, of_float) == kWide ? 256 : 128;
   return (cats + each - 1) / each;
 }
 int64_t parts_bytes(int64_t cats, int64_t rows, bool of_float, bool few) { return round_up(tiles_of_cats(cats, rows, of_float, few) * rows * (int64_t)sizeof(Part), 256); }
