@@ -11,11 +11,16 @@ namespace pcm {
 constexpr int kFewRowsMost = 64;             // rows that are few
 // rows of the long matrix of a workgroup
 inline int few_tile(int64_t rows) { return rows <= 32 ? 32 : 64; }
+constexpr int64_t kManyCats = 32768;         // categories that are many: 256 tiles of 128
 struct FewOperand {                          // rows of neighbouring entries
   const void* p;
   int64_t stride_ex, stride_var;             // in entries
   int32_t vars;
 };
+
+bool takes_few(const Matrix2& f, const Matrix2& w);
+bool takes_few8(int64_t rows, int64_t cats);
+FewOperand few_operand(const Matrix2& x);
 
 #ifdef __HIPCC__
 typedef float v4sums __attribute__((ext_vector_type(4)));

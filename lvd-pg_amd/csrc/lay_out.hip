@@ -1,6 +1,7 @@
 // Rows of 16-bit types laid out for the products: in rows of multiples of 128 bytes, as they lie or turned.
 //
-// Bound by the bytes moved: 64 x 64 tiles by way of LDS, read along whichever axis has neighbours.
+// Bound by the bytes moved.  Rows of neighbours are copied 16 bytes a lane, or turned in tiles of 64 x 64: 4 x 4 entries in a lane's registers, the
+// tile's rows put together in LDS (50000 x 4096 bf16: @@ us, 430 entry by entry); other strides go entry by entry.
 #include <algorithm>
 
 #include "linear_scores.hpp"
@@ -13,6 +14,90 @@ constexpr int kTile = 64;
 template <typename T>
 __device__ __forceinline__ T scaled(T v, int by) { return by == 0 ? v : (T)ldexpf((float)v, by); }
 
+// what a row is multiplied by: a power of two, or kDeadRow
+__device__ __forceinline__ int row_scale(const LayOut& with, const Matrix2& x, int64_t row, int largest) {
+  if (with.mask.p && bias_at(with.mask, row, x.examples) == -INFINITY) return kDeadRow;
+  if (!with.expo) return 0;
+  const int e = with.expo[row];
+  return e == kDeadRow ? e : max(e - largest, -300);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t v, int by) {
+  if (by == 0) return v;
+  if (by == kDeadRow) return 0;
+  const T a = __builtin_bit_cast(T, (uint16_t)(v & 0xffffu)), b = __builtin_bit_cast(T, (uint16_t)(v >> 16));
+  return pair_of<T>(ldexpf((float)a, by), ldexpf((float)b, by));
+}
+
+// rows of neighbours, as they lie: eight entries a lane
+template <typename T>
+__global__ __launch_bounds__(256) void copy_rows_kernel(Matrix2 x, int64_t first, int64_t count, uint16_t* to, int64_t pitch) {
+  const int c = (blockIdx.y * 8 + threadIdx.x % 8) * 8;
+  if (c >= pitch) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = (int64_t)blockIdx.x * 64 + i * 32 + threadIdx.x / 8;
+    if (r >= count) return;
+    const int64_t row = first + r;
+    const T* const from = static_cast<const T*>(x.p) + row / x.vars * x.stride_ex + row % x.vars * x.stride_var + c;
+    raw4 v = {0, 0, 0, 0};
+    if (c + 8 <= x.length) {
+      v = load16(from);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = c + k < x.length ? from[k] : (T)0.f;
+      v = __builtin_bit_cast(raw4, e);
+    }
+    *reinterpret_cast<raw4*>(to + r * pitch + c) = v;
+  }
+}
+
+// ... turned
+template <typename T>
+__global__ __launch_bounds__(256) void turn_rows_kernel(Matrix2 x, int64_t first, int64_t count, LayOut with, uint16_t* to, int64_t pitch) {
+  typedef uint32_t two __attribute__((ext_vector_type(2)));
+  typedef two two_by2 __attribute__((aligned(2)));
+  constexpr int kPitch = 136;                           // bytes: rows of LDS 34 banks apart
+  __shared__ __attribute__((aligned(8))) char tile[kTile * kPitch];   // [entry][row]
+  const int64_t r0 = (int64_t)blockIdx.x * kTile;
+  const int c0 = blockIdx.y * kTile, block = threadIdx.x / 16 * 4, c = c0 + threadIdx.x % 16 * 4;
+  const int largest = with.expo ? largest_exponent(with.most) : 0;
+  uint32_t a[4], b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + block + i, row = first + min(r, count - 1);
+    const T* const from = static_cast<const T*>(x.p) + row / x.vars * x.stride_ex + row % x.vars * x.stride_var + c;
+    two v = {0, 0};
+    if (c + 4 <= x.length) {
+      v = *reinterpret_cast<const two_by2*>(from);
+    } else {
+      T e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) e[k] = c + k < x.length ? from[k] : (T)0.f;
+      v = __builtin_bit_cast(two, e);
+    }
+    const int by = r < count ? row_scale(with, x, row, largest) : kDeadRow;
+    a[i] = scaled_pair<T>(v[0], by);
+    b[i] = scaled_pair<T>(v[1], by);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t* const v = e < 2 ? a : b;
+    const uint32_t order = e & 1 ? 0x07060302u : 0x05040100u;
+    *reinterpret_cast<uint2*>(tile + (c - c0 + e) * kPitch + block * 2) =
+        make_uint2(__builtin_amdgcn_perm(v[1], v[0], order), __builtin_amdgcn_perm(v[3], v[2], order));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = i * 32 + threadIdx.x / 8, k = threadIdx.x % 8;
+    if (c0 + at >= x.length) return;
+    const uint2 lo = *reinterpret_cast<const uint2*>(tile + at * kPitch + k * 16), hi = *reinterpret_cast<const uint2*>(tile + at * kPitch + k * 16 + 8);
+    *reinterpret_cast<uint4*>(to + (int64_t)(c0 + at) * pitch + r0 + k * 8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void lay_out_kernel(Matrix2 x, int64_t first, int64_t count, bool turned, bool along_rows, LayOut with, uint16_t* to,
                                                       int64_t pitch) {
@@ -22,17 +107,7 @@ __global__ __launch_bounds__(256) void lay_out_kernel(Matrix2 x, int64_t first, 
   const int c0 = blockIdx.y * kTile;
   const int t = threadIdx.x;
   const int largest = with.expo ? largest_exponent(with.most) : 0;
-  if (t < kTile) {
-    int e = 0;
-    if (r0 + t < count) {
-      if (with.expo) {
-        e = with.expo[first + r0 + t];
-        if (e != kDeadRow) e = max(e - largest, -300);
-      }
-      if (with.mask.p && bias_at(with.mask, first + r0 + t, x.examples) == -INFINITY) e = kDeadRow;
-    }
-    by[t] = e;
-  }
+  if (t < kTile) by[t] = r0 + t < count ? row_scale(with, x, first + r0 + t, largest) : 0;
   const T* const from = static_cast<const T*>(x.p);
 #pragma unroll
   for (int i = 0; i < kTile * kTile / 256; ++i) {
@@ -75,13 +150,26 @@ bool readable(const Matrix2& x) {
          (x.rows() <= 1 || (one_axis && pitch % 8 == 0 && pitch > 0 && pitch <= kMaxLength * 4));
 }
 
-void lay_out(const Matrix2& x, int64_t first, int64_t count, bool turned, const LayOut& with, void* d_to, hipStream_t stream) {
+namespace {
+template <typename T>
+void launch(const Matrix2& x, int64_t first, int64_t count, bool turned, const LayOut& with, void* d_to, hipStream_t stream) {
   const int64_t pitch = laid_length(turned ? count : x.length);
   const dim3 grid((unsigned)((count + kTile - 1) / kTile), (unsigned)((x.length + kTile - 1) / kTile));
-  const bool along_rows = x.vars == 1 && x.stride != 1 && (x.stride_ex == 1 || x.stride_ex == -1);
   uint16_t* const to = static_cast<uint16_t*>(d_to);
-  if (x.type == PCM_BF16) hipLaunchKernelGGL((lay_out_kernel<bf16>), grid, dim3(256), 0, stream, x, first, count, turned, along_rows, with, to, pitch);
-  else hipLaunchKernelGGL((lay_out_kernel<f16>), grid, dim3(256), 0, stream, x, first, count, turned, along_rows, with, to, pitch);
+  if (x.stride == 1 && turned) {
+    hipLaunchKernelGGL((turn_rows_kernel<T>), grid, dim3(256), 0, stream, x, first, count, with, to, pitch);
+  } else if (x.stride == 1) {
+    hipLaunchKernelGGL((copy_rows_kernel<T>), grid, dim3(256), 0, stream, x, first, count, to, pitch);
+  } else {
+    const bool along_rows = x.vars == 1 && (x.stride_ex == 1 || x.stride_ex == -1);
+    hipLaunchKernelGGL((lay_out_kernel<T>), grid, dim3(256), 0, stream, x, first, count, turned, along_rows, with, to, pitch);
+  }
+}
+}  // namespace
+
+void lay_out(const Matrix2& x, int64_t first, int64_t count, bool turned, const LayOut& with, void* d_to, hipStream_t stream) {
+  if (x.type == PCM_BF16) launch<bf16>(x, first, count, turned, with, d_to, stream);
+  else launch<f16>(x, first, count, turned, with, d_to, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of lay_out failed: %s", hipGetErrorString(e));
 }

@@ -210,6 +210,73 @@ __global__ __launch_bounds__(S::threads, 2) void gradient_kernel(GradientTask t)
   gradient_tile<T, S, kParts>(t);
 }
 
+// Few rows: dx of a tile of categories in LDS, then out in whichever orders are needed
+template <typename T, int kGroups>
+__global__ __launch_bounds__(512) void gradient_few_kernel(GradientTask t, FewOperand w, FewOperand f, int length) {
+  typedef FewTile<kGroups> S;
+  __shared__ __attribute__((aligned(16))) char lds[S::lds];
+  float* const dx = const_cast<float*>(few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds));
+  constexpr int kLanes = 512 / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
+  const int n = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
+  const int64_t c0 = (int64_t)blockIdx.x * S::longs, at_n = min((int64_t)n, t.rows - 1);
+  const float z = t.log_sum[at_n], of_p = t.of_p[at_n];
+  const int e = n < t.rows ? t.expo[at_n] : kDeadRow;
+  float own[kOwn];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int at = lane + i * kLanes;
+    const float x = score_of(dx[at * S::pitch + n], bias_at(t.bias, c0 + at, t.cats));
+    own[i] = e == kDeadRow ? 0.f : -of_p * __builtin_amdgcn_exp2f((x - z) * kLog2e);
+  }
+  if (e != kDeadRow)
+    for (int s = 0; s < t.given.slots; ++s) {
+      const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - t.first - c0;
+      const float add = t.grad_logp[n * t.given.slots + s];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) own[i] += g == lane + i * kLanes ? add : 0.f;
+    }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) dx[(lane + i * kLanes) * S::pitch + n] = own[i];
+  __syncthreads();
+  if (t.bias_parts && threadIdx.x < S::longs && c0 + threadIdx.x < t.cats) {
+    float s = 0.f;
+    for (int r = 0; r < S::rows; ++r) s += dx[threadIdx.x * S::pitch + r];
+    t.bias_parts[c0 + threadIdx.x] = s;
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (!t.dx) return;
+    for (int i = threadIdx.x; i < S::longs * S::rows; i += 512) {
+      const int c = i % S::longs, r = i / S::longs;
+      if (r < t.rows && c0 + c < t.pitch_row) t.dx[r * t.pitch_row + c0 + c] = dx[c * S::pitch + r];
+    }
+  } else {                             // two at a time, in two parts; the turned rows up to a whole step
+    if (t.by_row)
+      for (int i = threadIdx.x; i < S::longs / 2 * S::rows; i += 512) {
+        const int c = i % (S::longs / 2) * 2, r = i / (S::longs / 2);
+        if (r >= t.rows || c0 + c >= t.pitch_row) continue;
+        const int er = t.expo[r];
+        const float by = er == kDeadRow ? 0.f : ldexpf(1.f, 15 - er);
+        const Coded<T, 2> two(dx[c * S::pitch + r] * by, dx[(c + 1) * S::pitch + r] * by);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_row + part * t.plane_row + r * t.pitch_row + c0 + c) = two.p[part];
+      }
+    if (t.by_cat)
+      for (int i = threadIdx.x; i < S::longs * 32; i += 512) {
+        const int r = i % 32 * 2, c = i / 32;
+        if (c0 + c >= t.cats || r >= t.pitch_cat) continue;
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int er = r + k < t.rows ? t.expo[r + k] : kDeadRow;
+          v[k] = er == kDeadRow ? 0.f : dx[c * S::pitch + (r + k < S::rows ? r + k : 0)] * ldexpf(1.f, 15 - er);
+        }
+        const Coded<T, 2> two(v[0], v[1]);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_cat + part * t.plane_cat + (c0 + c) * t.pitch_cat + r) = two.p[part];
+      }
+  }
+}
+
 // float: categories that the bias masks, whose weights have no part in the features' gradients
 __global__ __launch_bounds__(256) void masked_kernel(BiasRef bias, int64_t cats, int* skip) {
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -233,8 +300,9 @@ __global__ __launch_bounds__(256) void join_bias_kernel(const float* parts, int6
 
 typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
+typedef TileSizes<128, 64, 64, 32> Slim;
 typedef TileSizes<128, 32, 32, 32> Narrow;
-int tile_rows(int64_t cats, int64_t rows, bool of_float) { return of_float ? 128 : rows <= 32 ? 32 : ((cats + 255) / 256) * ((rows + 255) / 256) >= 192 ? 256 : 128; }
+int tile_rows(int64_t cats, int64_t rows, bool of_float) { return of_float ? 128 : rows <= 64 ? (rows <= 32 ? 32 : 64) : ((cats + 255) / 256) * ((rows + 255) / 256) >= 192 ? 256 : 128; }
 
 template <typename T, typename S, int kParts>
 void launch(const GradientTask& t, hipStream_t stream) {
@@ -246,12 +314,22 @@ void launch(const GradientTask& t, hipStream_t stream) {
   const int size = tile_rows(t.cats, t.rows, false);
   if (size == 256) launch<T, Wide, kParts>(t, stream);
   else if (size == 128) launch<T, Middle, kParts>(t, stream);
+  else if (size == 64) launch<T, Slim, kParts>(t, stream);
   else launch<T, Narrow, kParts>(t, stream);
+}
+
+template <typename T>
+void launch_few(const GradientTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
+  const int64_t each = few_tile(t.rows), cols = sizeof(T) == 4 ? t.cats : laid_length(t.cats);   // (what is behind the last category is written too)
+  const dim3 grid((unsigned)((cols + each - 1) / each)), block(512);
+  if (t.rows <= 16) hipLaunchKernelGGL((gradient_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
+  else if (t.rows <= 32) hipLaunchKernelGGL((gradient_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
+  else hipLaunchKernelGGL((gradient_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
 }
 
 // What the workspace holds, and how the categories are cut into pieces
 struct Plan {
-  bool of_float, lay_f, lay_w;
+  bool of_float, few, lay_f, lay_w;
   int dx_planes;
   PlanePairs dx_pairs;
   int64_t rows, cats, length, piece, pieces;
@@ -263,8 +341,9 @@ struct Plan {
     rows = fm.rows();
     cats = wm.examples;
     length = fm.length;
-    lay_f = !readable(fm);
-    lay_w = !readable(wm);
+    few = takes_few(fm, wm);
+    lay_f = !few && !readable(fm);
+    lay_w = !few && !readable(wm);
     // The rounding of dx is the larger part of the error where sums have few terms that count, as the gradient of a given category's weights
     // has with few rows; over many rows it is what rounding the results costs.  In two parts: 20 rows of 64 bf16, 25000
     // categories, 2.3e-3 -> 1.6e-3 of the result (as rounding alone); the two products take twice the steps.
@@ -333,7 +412,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
   int* const skip = of_float && out.features && bias.p ? reinterpret_cast<int*>(work + plan.skip) : nullptr;
   if (skip) hipLaunchKernelGGL(masked_kernel, dim3((unsigned)((cats + 255) / 256)), dim3(256), 0, stream, bias, cats, skip);
   char* at = work + plan.f;
-  const Operand features = of_float ? Operand{} : operand_of(f, at, stream);
+  const Operand features = of_float || plan.few ? Operand{} : operand_of(f, at, stream);
   LayOut scaled;
   scaled.expo = expo;
   scaled.most = most;
@@ -348,7 +427,8 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     of_piece.p = static_cast<const char*>(w.p) + first * w.stride_ex * size;
     of_piece.examples = count;
     GradientTask t{};
-    if (of_float) {
+    if (plan.few) {
+    } else if (of_float) {
       t.fw = float_operand(of_piece, false);
       t.ff = float_operand(f, false);
       t.fk = f.length;
@@ -378,11 +458,16 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     else t.by_row = out.features ? reinterpret_cast<uint16_t*>(work + plan.by_row) : nullptr;
     t.by_cat = out.weight && !of_float ? reinterpret_cast<uint16_t*>(work + plan.by_cat) : nullptr;
     t.bias_parts = out.bias ? reinterpret_cast<float*>(work + plan.bias) : nullptr;
-    if (of_float) launch<float, FloatTile, 1>(t, stream);
+    if (plan.few) {
+      const FewOperand fw = few_operand(of_piece), ff = few_operand(f);
+      if (of_float) launch_few<float>(t, fw, ff, f.length, stream);
+      else if (f.type == PCM_BF16) launch_few<bf16>(t, fw, ff, f.length, stream);
+      else launch_few<f16>(t, fw, ff, f.length, stream);
+    } else if (of_float) launch<float, FloatTile, 1>(t, stream);
     else if (f.type == PCM_BF16) plan.dx_planes == 2 ? launch<bf16, 2>(t, stream) : launch<bf16, 1>(t, stream);
     else plan.dx_planes == 2 ? launch<f16, 2>(t, stream) : launch<f16, 1>(t, stream);
     if (out.bias) {
-      const int64_t each = tile_rows(count, rows, of_float);
+      const int64_t each = plan.few ? kFewRowsMost : tile_rows(count, rows, of_float);
       hipLaunchKernelGGL(join_bias_kernel, dim3((unsigned)((count + 31) / 32)), dim3(256), 0, stream, t.bias_parts, (rows + each - 1) / each, count,
                          out.bias, bias.type, first);
     }

@@ -163,10 +163,13 @@ __global__ __launch_bounds__(256) void join_scores_kernel(const Part* parts, int
 
 typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
-enum { kWide, kMiddle };
+typedef TileSizes<128, 64, 64, 32> Slim;
+typedef TileSizes<128, 32, 32, 32> Narrow;
+enum { kWide, kMiddle, kSlim, kNarrow };
 
 int tiles_for(int64_t m, int64_t n, bool of_float) {
   if (of_float) return kMiddle;
+  if (n <= 64) return n <= 32 ? kNarrow : kSlim;
   const int64_t wide = ((m + 255) / 256) * ((n + 255) / 256);
   return wide >= 192 ? kWide : kMiddle;
 }
@@ -178,8 +181,11 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch(const ScoreTask& t, hipStream_t stream) {
-  if (tiles_for(t.cats, t.rows, false) == kWide) launch<T, Wide>(t, stream);
-  else launch<T, Middle>(t, stream);
+  const int size = tiles_for(t.cats, t.rows, false);
+  if (size == kWide) launch<T, Wide>(t, stream);
+  else if (size == kMiddle) launch<T, Middle>(t, stream);
+  else if (size == kSlim) launch<T, Slim>(t, stream);
+  else launch<T, Narrow>(t, stream);
 }
 template <typename T>
 void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
@@ -215,11 +221,17 @@ void check_linear(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const
   check_given(given);
 }
 
-bool few_rows(const Matrix2& f, const Matrix2& w) { return f.rows() <= kFewRowsMost && f.stride == 1 && w.stride == 1; }
+// Few rows by way of few_rows.hip.hpp?  Where rows are read where they are, tiles of 128 categories stream faster once there are enough of them
+// (8 x 4096 x 50000 bf16: 80 us, 124 here); fewer leave compute units idle, and their long sums are what takes the time.
+bool takes_few(const Matrix2& f, const Matrix2& w) {
+  return f.rows() <= kFewRowsMost && f.stride == 1 && w.stride == 1 &&
+         (f.type == PCM_F32 || !readable(f) || !readable(w) || w.examples < kManyCats);
+}
+bool takes_few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cats < kManyCats; }
 FewOperand few_operand(const Matrix2& x) { return {x.p, x.stride_ex, x.stride_var, x.vars}; }
 
 int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w) {
-  if (few_rows(f, w)) return parts_bytes(w.examples, f.rows(), false, true);
+  if (takes_few(f, w)) return parts_bytes(w.examples, f.rows(), false, true);
   return (readable(f) ? 0 : laid_bytes(f.rows(), f.length, 1)) + (readable(w) ? 0 : laid_bytes(w.rows(), w.length, 1)) +
          parts_bytes(w.examples, f.rows(), f.type == PCM_F32, false);
 }
@@ -259,7 +271,7 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   check_workspace(d_work, work_bytes, linear_scores_workspace(f, w), "linear scores");
   ScoreTask t{};
   char* work = static_cast<char*>(d_work);
-  const bool few = few_rows(f, w);
+  const bool few = takes_few(f, w);
   if (few) {
   } else if (f.type == PCM_F32) {
     t.ff = float_operand(f, false);
@@ -292,7 +304,7 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   join_launch(t, few, d_log_sum, stream);
 }
 
-int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, false, rows <= kFewRowsMost); }
+int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, false, takes_few8(rows, cats)); }
 
 void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
                     int32_t length, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
@@ -317,7 +329,7 @@ void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, in
   t.given.vars = vars;
   t.logp = d_logp;
   t.parts = static_cast<Part*>(d_work);
-  const bool few = t.rows <= kFewRowsMost;
+  const bool few = takes_few8(t.rows, cats);
   if (few) launch_few<int8_t>(t, FewOperand{w, pitch, 0, 1}, FewOperand{f, pitch, 0, 1}, (int)pitch, stream);
   else launch<int8_t>(t, stream);
   join_launch(t, few, d_log_sum, stream);

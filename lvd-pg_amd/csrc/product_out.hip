@@ -19,20 +19,16 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
       scale[i] = t.finish.scale.m && m0 + i < t.m ? t.finish.scale.m[m0 + i] : 1.f;
     }
     __syncthreads();
+    if (raw) {
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-      __builtin_amdgcn_sched_barrier(0);
-      const int64_t row = n + 32 * j + (lane & 31);
-      if (row >= t.n) continue;
-      const FinishAt finish(t.finish, row, most);
+      for (int j = 0; j < S::FN; ++j) {
+        const int64_t row = n + 32 * j + (lane & 31);
+        if (row >= t.n) continue;
 #pragma unroll
-      for (int i = 0; i < S::FM; ++i)
+        for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int in = 32 * i + 8 * q + 4 * half;
-          const int64_t col = m + in;
-          if (col >= t.m) continue;
-          if (raw) {
+          for (int q = 0; q < 4; ++q) {
+            const int64_t col = m + 32 * i + 8 * q + 4 * half;
             uint32_t* const to = static_cast<uint32_t*>(t.out) + ((int64_t)blockIdx.y * t.n + row) * t.pitch + col;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -43,19 +39,54 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
                 }
                 to[e] = __builtin_bit_cast(uint32_t, v);
               }
-            continue;
           }
-          const float4 b = *reinterpret_cast<const float4*>(bias + wm + in), s = *reinterpret_cast<const float4*>(scale + wm + in);
-          float v[4];
+      }
+      return;
+    }
+    // eight rows of a wave's result at a time by way of its own LDS, so that they go out in whole lines
+    constexpr int kPitch = S::WM + 4;                                              // floats
+    float* const mine = scale + S::BM + threadIdx.x / 64 * 8 * kPitch;
+    static_assert((2 * S::BM + S::waves * 8 * kPitch) * sizeof(float) <= S::stage);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = finish((float)sums[i][j][4 * q + e], (&s.x)[e], (&b.x)[e]);
-          const int64_t at = row * t.pitch + col;
-          if (fours && col + 4 <= t.m) store_four(t.out, t.type, at, v);
-          else
+    for (int j = 0; j < S::FN; ++j) {
+      const int64_t row = n + 32 * j + (lane & 31);
+      const FinishAt finish(t.finish, row < t.n ? row : t.n - 1, most);
+      __builtin_amdgcn_sched_barrier(0);
+      float4 v[S::FM][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + e < t.m) store_as(t.out, t.type, at + e, v[e]);
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int in = wm + 32 * i + 8 * q + 4 * half;
+          const float4 b = *reinterpret_cast<const float4*>(bias + in), s = *reinterpret_cast<const float4*>(scale + in);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) (&v[i][q].x)[e] = finish((float)sums[i][j][4 * q + e], (&s.x)[e], (&b.x)[e]);
         }
+#pragma unroll
+      for (int eight = 0; eight < 4; ++eight) {
+        if ((lane & 31) / 8 == eight)
+#pragma unroll
+          for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(mine + lane % 8 * kPitch + 32 * i + 8 * q + 4 * half) = v[i][q];
+        __builtin_amdgcn_wave_barrier();
+        constexpr int kLanes = S::WM / 4;                                          // of four columns to a row
+#pragma unroll
+        for (int r = 0; r < 8; r += 64 / kLanes) {
+          const int in = r + lane / kLanes, at = lane % kLanes * 4;
+          const int64_t to = n + 32 * j + 8 * eight + in, col = m + at;
+          if (in < 8 && to < t.n) {
+            const float4 w = *reinterpret_cast<const float4*>(mine + in * kPitch + at);
+            const float v[4] = {w.x, w.y, w.z, w.w};
+            if (fours && col + 4 <= t.m) store_four(t.out, t.type, to * t.pitch + col, v);
+            else
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (col + e < t.m) store_as(t.out, t.type, to * t.pitch + col + e, v[e]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
     }
   };
   if constexpr (__is_same(T, float)) float_tile(t.fa, t.fb, t.m, t.n, t.fk, t.steps.parts, done);
@@ -105,6 +136,8 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, 
 
 typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
+typedef TileSizes<128, 64, 64, 32> Slim;
+typedef TileSizes<128, 32, 32, 32> Narrow;
 
 template <typename T, typename S>
 void launch(const OutTask& t, hipStream_t stream) {
@@ -117,14 +150,16 @@ void launch(const OutTask& t, hipStream_t stream) {
 bool wide(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
 template <typename T>
 void launch(const OutTask& t, hipStream_t stream) {
-  if (wide(t.m, t.n)) launch<T, Wide>(t, stream);
+  if (t.n <= 32) launch<T, Narrow>(t, stream);
+  else if (t.n <= 64) launch<T, Slim>(t, stream);
+  else if (wide(t.m, t.n)) launch<T, Wide>(t, stream);
   else launch<T, Middle>(t, stream);
 }
 }  // namespace
 
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
-  if (!of_float && wide(m, n)) return 1;
-  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
+  if (!of_float && n > 64 && wide(m, n)) return 1;
+  const int64_t each = of_float || n > 64 ? 128 : n > 32 ? 64 : 32, tiles = ((m + 127) / 128) * ((n + each - 1) / each);
   // as many parts as fill the device twice over, each of eight steps or more
   return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 8, 64}));
 }
