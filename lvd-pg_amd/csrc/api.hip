@@ -505,7 +505,7 @@ int pcm_product8(const int8_t* d_rows, const float* d_row_scales, int64_t num_ro
 }
 
 int64_t pcm_linear_scores8_workspace(int64_t num_examples, int32_t num_vars, int32_t length, int32_t num_cats) {
-  return linear_sizes(num_examples, num_vars, length, num_cats) ? pcm::linear_scores8_workspace(num_examples * num_vars, num_cats) : 0;
+  return linear_sizes(num_examples, num_vars, length, num_cats) ? pcm::linear_scores8_workspace(num_examples * num_vars, num_cats, length) : 0;
 }
 
 int pcm_linear_scores8(const int8_t* d_features, const float* d_feature_scales, const int8_t* d_weight, const float* d_weight_scales,

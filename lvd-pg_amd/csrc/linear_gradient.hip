@@ -302,7 +302,9 @@ typedef TileSizes<256, 256, 128, 64> Wide;
 typedef TileSizes<128, 128, 64, 64> Middle;
 typedef TileSizes<128, 64, 64, 32> Slim;
 typedef TileSizes<128, 32, 32, 32> Narrow;
-int tile_rows(int64_t cats, int64_t rows, bool of_float) { return of_float ? 128 : rows <= 64 ? (rows <= 32 ? 32 : 64) : ((cats + 255) / 256) * ((rows + 255) / 256) >= 192 ? 256 : 128; }
+int tile_rows(int64_t cats, int64_t rows, int64_t steps, bool of_float) {
+  return of_float ? 128 : rows <= 64 ? (rows <= 32 ? 32 : 64) : wide_tiles(cats, rows, steps) ? 256 : 128;
+}
 
 template <typename T, typename S, int kParts>
 void launch(const GradientTask& t, hipStream_t stream) {
@@ -311,7 +313,7 @@ void launch(const GradientTask& t, hipStream_t stream) {
 }
 template <typename T, int kParts>
 void launch(const GradientTask& t, hipStream_t stream) {
-  const int size = tile_rows(t.cats, t.rows, false);
+  const int size = tile_rows(t.cats, t.rows, t.steps.count, false);
   if (size == 256) launch<T, Wide, kParts>(t, stream);
   else if (size == 128) launch<T, Middle, kParts>(t, stream);
   else if (size == 64) launch<T, Slim, kParts>(t, stream);
@@ -467,7 +469,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     else if (f.type == PCM_BF16) plan.dx_planes == 2 ? launch<bf16, 2>(t, stream) : launch<bf16, 1>(t, stream);
     else plan.dx_planes == 2 ? launch<f16, 2>(t, stream) : launch<f16, 1>(t, stream);
     if (out.bias) {
-      const int64_t each = plan.few ? kFewRowsMost : tile_rows(count, rows, of_float);
+      const int64_t each = plan.few ? kFewRowsMost : tile_rows(count, rows, t.steps.count, of_float);
       hipLaunchKernelGGL(join_bias_kernel, dim3((unsigned)((count + 31) / 32)), dim3(256), 0, stream, t.bias_parts, (rows + each - 1) / each, count,
                          out.bias, bias.type, first);
     }

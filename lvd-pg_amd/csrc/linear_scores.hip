@@ -167,11 +167,10 @@ typedef TileSizes<128, 64, 64, 32> Slim;
 typedef TileSizes<128, 32, 32, 32> Narrow;
 enum { kWide, kMiddle, kSlim, kNarrow };
 
-int tiles_for(int64_t m, int64_t n, bool of_float) {
+int tiles_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
   if (of_float) return kMiddle;
   if (n <= 64) return n <= 32 ? kNarrow : kSlim;
-  const int64_t wide = ((m + 255) / 256) * ((n + 255) / 256);
-  return wide >= 192 ? kWide : kMiddle;
+  return wide_tiles(m, n, steps) ? kWide : kMiddle;
 }
 template <typename T, typename S>
 void launch(const ScoreTask& t, hipStream_t stream) {
@@ -181,7 +180,7 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch(const ScoreTask& t, hipStream_t stream) {
-  const int size = tiles_for(t.cats, t.rows, false);
+  const int size = tiles_for(t.cats, t.rows, t.steps.count, false);
   if (size == kWide) launch<T, Wide>(t, stream);
   else if (size == kMiddle) launch<T, Middle>(t, stream);
   else if (size == kSlim) launch<T, Slim>(t, stream);
@@ -195,17 +194,19 @@ void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, in
   else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
   else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
 }
-int64_t tiles_of_cats(int64_t cats, int64_t rows, bool of_float, bool few) {
-  const int64_t each = few ? few_tile(rows) : tiles_for(cats, rows, of_float) == kWide ? 256 : 128;
+int64_t tiles_of_cats(int64_t cats, int64_t rows, int64_t steps, bool of_float, bool few) {
+  const int64_t each = few ? few_tile(rows) : tiles_for(cats, rows, steps, of_float) == kWide ? 256 : 128;
   return (cats + each - 1) / each;
 }
-int64_t parts_bytes(int64_t cats, int64_t rows, bool of_float, bool few) { return round_up(tiles_of_cats(cats, rows, of_float, few) * rows * (int64_t)sizeof(Part), 256); }
+int64_t parts_bytes(int64_t cats, int64_t rows, int64_t steps, bool of_float, bool few) {
+  return round_up(tiles_of_cats(cats, rows, steps, of_float, few) * rows * (int64_t)sizeof(Part), 256);
+}
 
 void join_launch(const ScoreTask& t, bool few, float* d_log_sum, hipStream_t stream) {
   // few rows: all lanes of a workgroup to one, many: neighbouring rows side by side
   const int per = t.rows >= 4096 ? 16 : t.rows >= 512 ? 4 : 1;
   hipLaunchKernelGGL(join_scores_kernel, dim3((unsigned)((t.rows + per - 1) / per)), dim3(256), 0, stream, t.parts,
-                     tiles_of_cats(t.cats, t.rows, t.fw.p, few),                     t.rows, per, t.given, t.cats, t.logp, d_log_sum);
+                     tiles_of_cats(t.cats, t.rows, t.steps.count, t.fw.p, few),                     t.rows, per, t.given, t.cats, t.logp, d_log_sum);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of linear_scores failed: %s", hipGetErrorString(e));
 }
@@ -231,9 +232,9 @@ bool takes_few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cat
 FewOperand few_operand(const Matrix2& x) { return {x.p, x.stride_ex, x.stride_var, x.vars}; }
 
 int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w) {
-  if (takes_few(f, w)) return parts_bytes(w.examples, f.rows(), false, true);
+  if (takes_few(f, w)) return parts_bytes(w.examples, f.rows(), 0, false, true);
   return (readable(f) ? 0 : laid_bytes(f.rows(), f.length, 1)) + (readable(w) ? 0 : laid_bytes(w.rows(), w.length, 1)) +
-         parts_bytes(w.examples, f.rows(), f.type == PCM_F32, false);
+         parts_bytes(w.examples, f.rows(), laid_length(f.length) * 2 / kKBytes, f.type == PCM_F32, false);
 }
 
 void check_workspace(const void* d_work, int64_t work_bytes, int64_t need, const char* what) {
@@ -304,7 +305,9 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
   join_launch(t, few, d_log_sum, stream);
 }
 
-int64_t linear_scores8_workspace(int64_t rows, int64_t cats) { return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, false, takes_few8(rows, cats)); }
+int64_t linear_scores8_workspace(int64_t rows, int64_t cats, int32_t length) {
+  return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, round_up(length, kKBytes) / kKBytes, false, takes_few8(rows, cats));
+}
 
 void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
                     int32_t length, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
@@ -315,7 +318,7 @@ void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, in
   if (!shape.rows()) return;
   if (!f || !f_scales || !w || !w_scales || (given.slots && (!given.p || !d_logp))) fail(PCM_ERR_ARG, "linear scores of 8-bit rows: a pointer is null");
   if (((uintptr_t)f | (uintptr_t)w) & 15) fail(PCM_ERR_ARG, "linear scores of 8-bit rows: codes must be 16-byte aligned");
-  check_workspace(d_work, work_bytes, linear_scores8_workspace(shape.rows(), cats), "linear scores of 8-bit rows");
+  check_workspace(d_work, work_bytes, linear_scores8_workspace(shape.rows(), cats, length), "linear scores of 8-bit rows");
   ScoreTask t{};
   const int64_t pitch = round_up(length, kKBytes);
   t.f = {f, pitch, 0};

@@ -61,7 +61,7 @@ Operand operand_of(const Matrix2& x, char*& work, hipStream_t stream);
 int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w);
 void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum,
                    void* d_work, int64_t work_bytes, hipStream_t stream);
-int64_t linear_scores8_workspace(int64_t rows, int64_t cats);
+int64_t linear_scores8_workspace(int64_t rows, int64_t cats, int32_t length);
 void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
                     int32_t length, const BiasRef& bias, const GivenRef& given, float* d_logp, float* d_log_sum, void* d_work, int64_t work_bytes,
                     hipStream_t stream);

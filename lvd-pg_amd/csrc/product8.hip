@@ -4,35 +4,85 @@
 namespace pcm {
 
 namespace {
-// A workgroup per row: the largest |x| first, then code = rint(x (127 / largest)), scale = largest / 127.  The row is read twice, the second time from
-// the cache.  A row with NaN or an infinity gets scale NaN; one whose largest |x| is below 2^-119 counts as zeros (127 / largest
-// would pass the range).
-template <typename T>
-__global__ __launch_bounds__(256) void rows8_kernel(Matrix2 x, int64_t pitch, int8_t* codes, float* scales) {
-  __shared__ float sub[4];
-  for (int64_t r = blockIdx.x; r < x.rows(); r += gridDim.x) {
-    const T* const from = static_cast<const T*>(x.p) + r / x.vars * x.stride_ex + r % x.vars * x.stride_var;
-    float largest = 0.f;
-    for (int i = threadIdx.x; i < x.length; i += 256) {
-      const float v = fabsf((float)from[i * x.stride]);
-      largest = __builtin_elementwise_maximum(largest, v);
-    }
+// A workgroup per row: the largest |x| first, then code = rint(x (127 / largest)), scale = largest / 127.  A row with NaN or an infinity gets scale
+// NaN; one whose largest |x| is below 2^-119 counts as zeros (127 / largest would pass the range).
+struct RowScale {
+  float by, scale;
+  bool bad;
+  __device__ __forceinline__ RowScale(float largest, float (&sub)[4]) {
     largest = over_lanes<64>(largest, LargerOrNan());
     __syncthreads();
     if (threadIdx.x % 64 == 0) sub[threadIdx.x / 64] = largest;
     __syncthreads();
     largest = __builtin_elementwise_maximum(__builtin_elementwise_maximum(sub[0], sub[1]), __builtin_elementwise_maximum(sub[2], sub[3]));
-    const bool bad = !(largest < INFINITY), none = largest < 0x1p-119f;
-    const float by = bad || none ? 0.f : 127.f / largest;
-    if (threadIdx.x == 0) scales[r] = bad ? __builtin_nanf("") : none ? 0.f : largest / 127.f;
+    bad = !(largest < INFINITY);
+    const bool none = largest < 0x1p-119f;
+    by = bad || none ? 0.f : 127.f / largest;
+    scale = bad ? __builtin_nanf("") : none ? 0.f : largest / 127.f;
+  }
+  __device__ __forceinline__ uint32_t code(float x) const { return bad ? 0u : (uint32_t)(uint8_t)(int8_t)(int)rintf(x * by); }
+};
+// Rows of neighbours of up to 8192 entries stay in registers, eight to a lane at a time; any others are read twice, entry by entry
+template <typename T>
+__global__ __launch_bounds__(256) void rows8_kernel(Matrix2 x, int64_t pitch, int8_t* codes, float* scales) {
+  __shared__ float sub[4];
+  for (int64_t r = blockIdx.x; r < x.rows(); r += gridDim.x) {
+    const T* const from = static_cast<const T*>(x.p) + r / x.vars * x.stride_ex + r % x.vars * x.stride_var;
+    int8_t* const to = codes + r * pitch;
+    float largest = 0.f;
+    if (x.stride == 1 && x.length <= 8192) {
+      float v[4][8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = (i * 256 + threadIdx.x) * 8;
+        if (c + 8 <= x.length) {
+          if constexpr (sizeof(T) == 4) {
+            const raw4 a = load16(from + c), b = load16(from + c + 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[i][k] = as_float(a[k]);
+              v[i][4 + k] = as_float(b[k]);
+            }
+          } else {
+            const raw4 a = load16(from + c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t w = a[k];
+              v[i][2 * k] = (float)__builtin_bit_cast(T, (uint16_t)(w & 0xffffu));
+              v[i][2 * k + 1] = (float)__builtin_bit_cast(T, (uint16_t)(w >> 16));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[i][k] = c + k < x.length ? (float)from[c + k] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) largest = __builtin_elementwise_maximum(largest, fabsf(v[i][k]));
+      const RowScale s(largest, sub);
+      if (threadIdx.x == 0) scales[r] = s.scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = (i * 256 + threadIdx.x) * 8;
+        if (c >= pitch) break;
+        uint32_t w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          w[h] = s.code(v[i][4 * h]) | s.code(v[i][4 * h + 1]) << 8 | s.code(v[i][4 * h + 2]) << 16 | s.code(v[i][4 * h + 3]) << 24;
+        *reinterpret_cast<uint2*>(to + c) = make_uint2(w[0], w[1]);
+      }
+      continue;
+    }
+    for (int i = threadIdx.x; i < x.length; i += 256) largest = __builtin_elementwise_maximum(largest, fabsf((float)from[i * x.stride]));
+    const RowScale s(largest, sub);
+    if (threadIdx.x == 0) scales[r] = s.scale;
     for (int i = threadIdx.x * 4; i < pitch; i += 1024) {
       uint32_t w = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = i + e < x.length && !bad ? rintf((float)from[(i + e) * x.stride] * by) : 0.f;
-        w |= (uint32_t)(uint8_t)(int8_t)(int)v << 8 * e;
-      }
-      *reinterpret_cast<uint32_t*>(codes + r * pitch + i) = w;
+      for (int e = 0; e < 4; ++e) w |= (i + e < x.length ? s.code((float)from[(i + e) * x.stride]) : 0u) << 8 * e;
+      *reinterpret_cast<uint32_t*>(to + i) = w;
     }
   }
 }

@@ -147,21 +147,20 @@ void launch(const OutTask& t, hipStream_t stream) {
   const bool fours = t.type != kRawSums && t.pitch % 4 == 0 && (uintptr_t)t.out % (4 * size) == 0;
   hipLaunchKernelGGL((out_kernel<T, S>), dim3((unsigned)tiles, (unsigned)t.steps.parts), dim3(S::threads), 0, stream, t, fours);
 }
-bool wide(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
 template <typename T>
 void launch(const OutTask& t, hipStream_t stream) {
   if (t.n <= 32) launch<T, Narrow>(t, stream);
   else if (t.n <= 64) launch<T, Slim>(t, stream);
-  else if (wide(t.m, t.n)) launch<T, Wide>(t, stream);
+  else if (wide_tiles(t.m, t.n, t.steps.count * t.steps.pairs.count / t.steps.parts)) launch<T, Wide>(t, stream);
   else launch<T, Middle>(t, stream);
 }
 }  // namespace
 
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
-  if (!of_float && n > 64 && wide(m, n)) return 1;
+  if (!of_float && wide_tiles(m, n, steps)) return 1;
   const int64_t each = of_float || n > 64 ? 128 : n > 32 ? 64 : 32, tiles = ((m + 127) / 128) * ((n + each - 1) / each);
-  // as many parts as fill the device twice over, each of eight steps or more
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 8, 64}));
+  // as many parts as fill the device twice over, each of four steps or more
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 4, 64}));
 }
 int parts_for_few(int64_t m, int64_t n, int64_t steps) {
   // a workgroup's waves take a step each at a time: parts of four rounds or more, as many as give every compute unit two workgroups

@@ -21,6 +21,12 @@ struct Steps {
   int parts;
 };
 
+// Whether a product is best cut into tiles of 256 x 256, a workgroup's work a compute unit: enough of them, and long enough sums.  Short ones wait for
+// their first fragments and for their stores one after the other, which two workgroups of 128 x 128 do in turns (@@).
+inline bool wide_tiles(int64_t m, int64_t n, int64_t steps) {
+  return n > 64 && steps >= 12 && ((m + 255) / 256) * ((n + 255) / 256) >= 192;
+}
+
 #ifdef __HIPCC__
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
