@@ -266,15 +266,14 @@ __device__ __forceinline__ void score_sums(const ScoreInputs& t, Done done) {
   if constexpr (__is_same(T, float)) float_tile(t.fw, t.ff, t.cats, t.rows, t.fk, 1, done);
   else product_tile<T, S>(t.w, t.f, t.cats, t.rows, t.steps, done);
 }
-// bias and scales of a tile's categories into LDS; barriers before and after
+// bias and scales of the tile's categories into LDS, while its sums are on their way; a barrier before they are read
 template <typename S>
-__device__ __forceinline__ void tile_constants(const ScoreInputs& t, int64_t m0, float* bias, float* scale) {
-  __syncthreads();
+__device__ __forceinline__ void tile_constants(const ScoreInputs& t, float* bias, float* scale) {
+  const int64_t m0 = tile_at<S>(t.cats, t.rows).m0;
   for (int i = threadIdx.x; i < S::BM; i += S::threads) {
     bias[i] = bias_at(t.bias, m0 + i, t.cats);
     scale[i] = t.scale.m && m0 + i < t.cats ? t.scale.m[m0 + i] : 1.f;
   }
-  __syncthreads();
 }
 // The scores of the wave's j-th rows of features
 template <typename S, typename Sums>

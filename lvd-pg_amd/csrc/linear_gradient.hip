@@ -90,12 +90,12 @@ __device__ __forceinline__ void turn(uint32_t& a, uint32_t& b) {
 
 template <typename T, typename S, int kParts>
 __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
+  __shared__ __attribute__((aligned(16))) float bias[S::BM], scale[S::BM];
+  tile_constants<S>(t, bias, scale);
   score_sums<T, S>(t, [&](auto& sums, int64_t m, int64_t n, char* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x / 64, wm = wave % S::waves_m * S::WM;
-    float* const bias = reinterpret_cast<float*>(lds);                      // [BM]
-    float* const scale = bias + S::BM;                                      // [BM]
-    float* const of_bias = scale + S::BM;                                   // [waves_n][BM]
-    tile_constants<S>(t, m - wm, bias, scale);
+    float* const of_bias = reinterpret_cast<float*>(lds);                   // [waves_n][BM]
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
       __builtin_amdgcn_sched_barrier(0);

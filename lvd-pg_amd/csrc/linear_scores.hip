@@ -25,13 +25,13 @@ struct ScoreTask : ScoreInputs {
 
 template <typename T, typename S>
 __device__ __forceinline__ void score_tile(const ScoreTask& t) {
+  __shared__ __attribute__((aligned(16))) float bias[S::BM], scale[S::BM];
+  tile_constants<S>(t, bias, scale);
   score_sums<T, S>(t, [&](auto& sums, int64_t m, int64_t n, char* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x / 64, wm = wave % S::waves_m * S::WM;
-    float* const bias = reinterpret_cast<float*>(lds);                      // [BM]
-    float* const scale = bias + S::BM;                                      // [BM]
-    Part* const joined = reinterpret_cast<Part*>(scale + S::BM);            // [waves_m][BN]
-    static_assert(2 * S::BM * sizeof(float) + S::waves_m * S::BN * sizeof(Part) <= S::stage);
-    tile_constants<S>(t, m - wm, bias, scale);
+    Part* const joined = reinterpret_cast<Part*>(lds);                      // [waves_m][BN]
+    static_assert(S::waves_m * S::BN * sizeof(Part) <= S::stage);
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
       __builtin_amdgcn_sched_barrier(0);   // one j at a time: registers are full

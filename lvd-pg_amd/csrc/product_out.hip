@@ -6,18 +6,16 @@ namespace pcm {
 namespace {
 template <typename T, typename S>
 __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
+  __shared__ __attribute__((aligned(16))) float bias[S::BM], scale[S::BM];
+  const bool raw = t.type == kRawSums;
+  const int most = t.finish.most ? largest_exponent(t.finish.most) : 0;
+  const int64_t m0 = tile_at<S>(t.m, t.n).m0;
+  for (int i = threadIdx.x; i < S::BM; i += S::threads) {
+    bias[i] = m0 + i < t.m ? bias_of(t.finish.bias, m0 + i) : 0.f;
+    scale[i] = t.finish.scale.m && m0 + i < t.m ? t.finish.scale.m[m0 + i] : 1.f;
+  }
   auto done = [&](auto& sums, int64_t m, int64_t n, char* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = threadIdx.x / 64 % S::waves_m * S::WM;
-    const bool raw = t.type == kRawSums;
-    const int most = t.finish.most ? largest_exponent(t.finish.most) : 0;
-    float* const bias = reinterpret_cast<float*>(lds);   // [BM]
-    float* const scale = bias + S::BM;                   // [BM]
-    const int64_t m0 = m - wm;
-    __syncthreads();
-    for (int i = threadIdx.x; i < S::BM; i += S::threads) {
-      bias[i] = m0 + i < t.m ? bias_of(t.finish.bias, m0 + i) : 0.f;
-      scale[i] = t.finish.scale.m && m0 + i < t.m ? t.finish.scale.m[m0 + i] : 1.f;
-    }
     __syncthreads();
     if (raw) {
 #pragma unroll
@@ -45,8 +43,8 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
     }
     // eight rows of a wave's result at a time by way of its own LDS, so that they go out in whole lines
     constexpr int kPitch = S::WM + 4;                                              // floats
-    float* const mine = scale + S::BM + threadIdx.x / 64 * 8 * kPitch;
-    static_assert((2 * S::BM + S::waves * 8 * kPitch) * sizeof(float) <= S::stage);
+    float* const mine = reinterpret_cast<float*>(lds) + threadIdx.x / 64 * 8 * kPitch;
+    static_assert(S::waves * 8 * kPitch * sizeof(float) <= S::stage);
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
       const int64_t row = n + 32 * j + (lane & 31);
@@ -159,8 +157,8 @@ void launch(const OutTask& t, hipStream_t stream) {
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
   if (!of_float && wide_tiles(m, n, steps)) return 1;
   const int64_t each = of_float || n > 64 ? 128 : n > 32 ? 64 : 32, tiles = ((m + 127) / 128) * ((n + each - 1) / each);
-  // as many parts as fill the device twice over, each of four steps or more
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, steps / 4, 64}));
+  // as many parts as leave two workgroups a compute unit at most, each of four steps or more
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 4, 64}));
 }
 int parts_for_few(int64_t m, int64_t n, int64_t steps) {
   // a workgroup's waves take a step each at a time: parts of four rounds or more, as many as give every compute unit two workgroups

@@ -58,7 +58,29 @@ struct Cores<int8_t> {
   static __device__ __forceinline__ v16i mma(v4i a, v4i b, v16i c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
 };
 
-typedef __attribute__((address_space(3))) void LdsVoid;
+typedef __attribute__((address_space(3))) const void LdsVoid;
+
+// Sixteen bytes a lane from memory straight into LDS: lane l's from `base` (the first 48 bits of the descriptor) + at + k to lds + 16 l.
+// Written out so that the compiler does not wait for it at the next read of LDS, whichever stage that is of: stage_barrier says when what
+// is there.  It has no register to return to, and its address is taken when it is issued.
+__device__ __forceinline__ void request_into_lds(const char* lds, v4i base, uint32_t at, uint32_t k) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(LdsVoid*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(base), "s"(k) : "m0");
+}
+// the descriptor of memory from p on; p is the same in all lanes
+__device__ __forceinline__ v4i memory_at(const char* p) {
+  const uint64_t v = (uint64_t)p;
+  return v4i{(int)__builtin_amdgcn_readfirstlane((uint32_t)v), (int)(__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) & 0xffffu), -1, 0x00020000};
+}
+// A barrier after which what the workgroup's waves have requested into LDS is there, but for the last `kOpen` requests of each wave: a barrier
+// by itself says nothing of requests on their way.
+template <int kOpen>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((kOpen & 15) | kOpen >> 4 << 14 | 7 << 4);   // vmcnt(kOpen) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 template <int kBM, int kBN, int kWM, int kWN>
 struct TileSizes {
@@ -77,7 +99,7 @@ struct TileLoader {
   static_assert(each * 1024 * S::waves == S::stage && S::BM % 8 == 0 && S::BN % 8 == 0);
   const char *a0, *b0;
   int64_t plane_a, plane_b;
-  __amdgpu_buffer_rsrc_t a, b;
+  v4i a, b;
   uint32_t at[each];
   uint32_t k, begin, end;      // the bytes of a row that come next, and between which
   PlanePairs pairs;
@@ -85,8 +107,8 @@ struct TileLoader {
 
   __device__ __forceinline__ void choose_planes() {
     const int64_t pa = pairs.a >> 2 * product & 3, pb = pairs.b >> 2 * product & 3;
-    a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a0 + pa * plane_a), 0, 0xffffffffu, 0x00020000);
-    b = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b0 + pb * plane_b), 0, 0xffffffffu, 0x00020000);
+    a = memory_at(a0 + pa * plane_a);
+    b = memory_at(b0 + pb * plane_b);
   }
   __device__ __forceinline__ TileLoader(const Operand& oa, const Operand& ob, int64_t m0, int64_t n0, int64_t m, int64_t n, int first, int count,
                                         const PlanePairs& of) : pairs(of) {
@@ -95,8 +117,8 @@ struct TileLoader {
     b0 = static_cast<const char*>(ob.p) + n0 * ob.pitch;
     plane_a = oa.plane;
     plane_b = ob.plane;
-    k = begin = (uint32_t)first * kKBytes;
-    end = begin + (uint32_t)count * kKBytes;
+    k = begin = __builtin_amdgcn_readfirstlane((uint32_t)first * kKBytes);
+    end = begin + __builtin_amdgcn_readfirstlane((uint32_t)count * kKBytes);
     choose_planes();
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -108,11 +130,11 @@ struct TileLoader {
       at[i] = (uint32_t)((row < last ? row : last) * (of_a ? oa.pitch : ob.pitch)) + ((lane & 7) ^ (row >> 1 & 7)) * 16;
     }
   }
-  __device__ __forceinline__ void load(char* lds) {
+  __device__ __forceinline__ void load(const char* lds) {
 #pragma unroll
     for (int i = 0; i < each; ++i) {
       const int q = i * S::waves + wave;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(q < S::BM / 8 ? a : b, (LdsVoid*)(lds + q * 1024), 16, at[i], k, 0, 0);
+      request_into_lds(lds + q * 1024, q < S::BM / 8 ? a : b, at[i], k);
     }
     k += kKBytes;
     if (k == end && product + 1 < pairs.count) {
@@ -186,15 +208,19 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
       multiply(~step & 1);
       mix();
     }
-    __syncthreads();
+    stage_barrier<0>();
     if (t + 1 < stages) read(next, 0, 0);
     if (t + 2 < stages) from.load(mine);
     multiply(1);
   };
   if (stages > 0) {
     from.load(s0);
-    __syncthreads();
-    if (stages > 1) from.load(s1);
+    if (stages > 1) {
+      from.load(s1);
+      stage_barrier<TileLoader<S>::each>();
+    } else {
+      stage_barrier<0>();
+    }
     read(s0, 0, 0);
     for (int t = 0; t < stages; t += 2) {
       stage(s0, s1, t);
