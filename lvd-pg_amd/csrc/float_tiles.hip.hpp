@@ -49,7 +49,9 @@ struct FloatLoader {
     if constexpr (kTurned) {
       step = threadIdx.x % 8 * 2;
       row = threadIdx.x / 8 * 4;
-      at[0] = x.p + min(first + row, count - 4) * x.stride;      // (plain(): four entries at least)
+      // (blocks past the end take the last four entries, to where those belong)
+      if (plain()) row = (int)min((int64_t)row, count - 4 - first);
+      at[0] = x.p + (first + row) * x.stride;
     } else {
       step = threadIdx.x % 4 * 4;
       row = threadIdx.x / 4;
@@ -59,7 +61,7 @@ struct FloatLoader {
   }
   // whether all of the tile's requests are of four neighbours
   __device__ __forceinline__ bool plain() const {
-    return x.stride == 1 && (!kTurned || (x.vars == 1 && count >= 4 && (count % 4 == 0 || first + FloatTile::BM <= count)));
+    return x.stride == 1 && (!kTurned || (x.vars == 1 && count - first >= 4));
   }
   // steps [k, k + 16), all of them there
   template <int kSet>
@@ -79,13 +81,20 @@ struct FloatLoader {
   // steps [k, k + 16) of those below end, any strides; into the first set
   __device__ __forceinline__ void load_any(int64_t k, int64_t end) {
     const int64_t s = k + step;
+    const bool fours = plain();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if constexpr (kTurned) {
         const bool some = s + i < end && !(x.skip && x.skip[s + i] == kDeadRow);
         mark[0][i] = 0;
+        v[0][i] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (!some) continue;
+        if (fours) v[0][i] = *reinterpret_cast<const v4f_by4*>(at[0] + (s + i) * x.stride_ex);
+        else
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[0][i][e] = some && first + row + e < count ? row_at(s + i)[(first + row + e) * x.stride] : 0.f;
+          for (int e = 0; e < 4; ++e) v[0][i][e] = first + row + e < count ? row_at(s + i)[(first + row + e) * x.stride] : 0.f;
+      } else if (fours && s + 4 <= end) {
+        v[0][i] = *reinterpret_cast<const v4f_by4*>(at[i] + s);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[0][i][e] = s + e < end ? at[i][(s + e) * x.stride] : 0.f;

@@ -122,9 +122,11 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, 
     float sum = 0.f;
     if (whole) {
       int s = 0;
+#pragma unroll 8
       for (int p = 0; p < count; ++p) s += (int)parts[p * all + i];
       sum = (float)s;
     } else {
+#pragma unroll 8
       for (int p = 0; p < count; ++p) sum += __builtin_bit_cast(float, parts[p * all + i]);
     }
     const FinishAt f(finish, row, most);
@@ -157,8 +159,9 @@ void launch(const OutTask& t, hipStream_t stream) {
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
   if (!of_float && wide_tiles(m, n, steps)) return 1;
   const int64_t each = of_float || n > 64 ? 128 : n > 32 ? 64 : 32, tiles = ((m + 127) / 128) * ((n + each - 1) / each);
-  // as many parts as leave two workgroups a compute unit at most, each of four steps or more
-  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 4, 64}));
+  // as many parts as leave two workgroups a compute unit at most (one, where the sums are short and joining them would cost more), each of four
+  // steps or more
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(steps < 64 ? 256 : 512) / tiles, steps / 4, 64}));
 }
 int parts_for_few(int64_t m, int64_t n, int64_t steps) {
   // a workgroup's waves take a step each at a time: parts of four rounds or more, as many as give every compute unit two workgroups
