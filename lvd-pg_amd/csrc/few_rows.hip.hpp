@@ -8,7 +8,7 @@
 
 namespace pcm {
 
-constexpr int kFewRowsMost = 64;             // rows that are few
+constexpr int kFewRowsMost = 64;             // rows that are few: those of a workgroup
 // rows of the long matrix of a workgroup
 inline int few_tile(int64_t rows) { return rows <= 32 ? 32 : 64; }
 constexpr int64_t kManyCats = 32768;         // categories that are many: 256 tiles of 128
@@ -18,8 +18,11 @@ struct FewOperand {                          // rows of neighbouring entries
   int32_t vars;
 };
 
+// Whether a product of scores goes this way: few rows, or so few tiles of 128 x 128 that long sums are best cut among the waves of a workgroup (100 x
+// 3000 x 500 f32: 111 us by tiles, @@ here).  Where rows can be read where they are, tiles of 128 categories stream faster once there
+// are enough of them (8 x 4096 x 50000 bf16: 80 us, 124 here).
 bool takes_few(const Matrix2& f, const Matrix2& w);
-bool takes_few8(int64_t rows, int64_t cats);
+bool takes_few8(int64_t rows, int64_t cats, int64_t length);
 FewOperand few_operand(const Matrix2& x);
 
 #ifdef __HIPCC__
@@ -122,7 +125,7 @@ struct FewTile {                             // kGroups: of 16 rows of b
   static constexpr int sums_bytes = 8 * longs * pitch * 4;
   static constexpr int lds = sums_bytes > 8 * wave_bytes ? sums_bytes : 8 * wave_bytes;
 };
-// Sums of rows [longs blockIdx.x, + longs) of a with all (16 kGroups at most) rows of b over `length` entries: sum of rows m and n of the tile
+// Sums of rows [longs blockIdx.x, + longs) of a with rows [rows blockIdx.z, + rows) of b over `length` entries: sum of rows m and n of the tile
 // at m * pitch + n of what is returned (LDS), 32 bits (whole numbers: their bits), after a barrier.  Parts of the pieces by blockIdx.y.
 //
 // A wave's piece goes through its own share of LDS: requested by eight lanes a row, read back as the cores' operands.  No barrier until the
@@ -140,7 +143,7 @@ __device__ __forceinline__ const float* few_sums(const FewOperand& a, const FewO
     at_a[g] = static_cast<const T*>(a.p) + min((int64_t)blockIdx.x * S::longs + 8 * g + lane / 8, m - 1) * a.stride_ex + lane % 8 * kEach;
 #pragma unroll
   for (int g = 0; g < kRows; ++g) {
-    const int64_t r = min((int64_t)(8 * g + lane / 8), n - 1);
+    const int64_t r = min((int64_t)blockIdx.z * S::rows + 8 * g + lane / 8, n - 1);
     at_b[g] = static_cast<const T*>(b.p) + r / b.vars * b.stride_ex + r % b.vars * b.stride_var + lane % 8 * kEach;
   }
   typename FewCores<Core>::Sums sums[kCats][kGroups] = {};

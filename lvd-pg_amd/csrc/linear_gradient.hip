@@ -217,15 +217,15 @@ __global__ __launch_bounds__(512) void gradient_few_kernel(GradientTask t, FewOp
   __shared__ __attribute__((aligned(16))) char lds[S::lds];
   float* const dx = const_cast<float*>(few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds));
   constexpr int kLanes = 512 / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
-  const int n = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
-  const int64_t c0 = (int64_t)blockIdx.x * S::longs, at_n = min((int64_t)n, t.rows - 1);
+  const int in = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
+  const int64_t c0 = (int64_t)blockIdx.x * S::longs, n0 = (int64_t)blockIdx.z * S::rows, n = n0 + in, at_n = min(n, t.rows - 1);
   const float z = t.log_sum[at_n], of_p = t.of_p[at_n];
   const int e = n < t.rows ? t.expo[at_n] : kDeadRow;
   float own[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     const int at = lane + i * kLanes;
-    const float x = score_of(dx[at * S::pitch + n], bias_at(t.bias, c0 + at, t.cats));
+    const float x = score_of(dx[at * S::pitch + in], bias_at(t.bias, c0 + at, t.cats));
     own[i] = e == kDeadRow ? 0.f : -of_p * __builtin_amdgcn_exp2f((x - z) * kLog2e);
   }
   if (e != kDeadRow)
@@ -236,43 +236,43 @@ __global__ __launch_bounds__(512) void gradient_few_kernel(GradientTask t, FewOp
       for (int i = 0; i < kOwn; ++i) own[i] += g == lane + i * kLanes ? add : 0.f;
     }
 #pragma unroll
-  for (int i = 0; i < kOwn; ++i) dx[(lane + i * kLanes) * S::pitch + n] = own[i];
+  for (int i = 0; i < kOwn; ++i) dx[(lane + i * kLanes) * S::pitch + in] = own[i];
   __syncthreads();
   if (t.bias_parts && threadIdx.x < S::longs && c0 + threadIdx.x < t.cats) {
     float s = 0.f;
     for (int r = 0; r < S::rows; ++r) s += dx[threadIdx.x * S::pitch + r];
-    t.bias_parts[c0 + threadIdx.x] = s;
+    t.bias_parts[blockIdx.z * t.cats + c0 + threadIdx.x] = s;
   }
   if constexpr (sizeof(T) == 4) {
     if (!t.dx) return;
     for (int i = threadIdx.x; i < S::longs * S::rows; i += 512) {
       const int c = i % S::longs, r = i / S::longs;
-      if (r < t.rows && c0 + c < t.pitch_row) t.dx[r * t.pitch_row + c0 + c] = dx[c * S::pitch + r];
+      if (n0 + r < t.rows && c0 + c < t.pitch_row) t.dx[(n0 + r) * t.pitch_row + c0 + c] = dx[c * S::pitch + r];
     }
   } else {                             // two at a time, in two parts; the turned rows up to a whole step
     if (t.by_row)
       for (int i = threadIdx.x; i < S::longs / 2 * S::rows; i += 512) {
         const int c = i % (S::longs / 2) * 2, r = i / (S::longs / 2);
-        if (r >= t.rows || c0 + c >= t.pitch_row) continue;
-        const int er = t.expo[r];
+        if (n0 + r >= t.rows || c0 + c >= t.pitch_row) continue;
+        const int er = t.expo[n0 + r];
         const float by = er == kDeadRow ? 0.f : ldexpf(1.f, 15 - er);
         const Coded<T, 2> two(dx[c * S::pitch + r] * by, dx[(c + 1) * S::pitch + r] * by);
 #pragma unroll
-        for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_row + part * t.plane_row + r * t.pitch_row + c0 + c) = two.p[part];
+        for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_row + part * t.plane_row + (n0 + r) * t.pitch_row + c0 + c) = two.p[part];
       }
     if (t.by_cat)
       for (int i = threadIdx.x; i < S::longs * 32; i += 512) {
         const int r = i % 32 * 2, c = i / 32;
-        if (c0 + c >= t.cats || r >= t.pitch_cat) continue;
+        if (c0 + c >= t.cats || n0 + r >= t.pitch_cat) continue;
         float v[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int er = r + k < t.rows ? t.expo[r + k] : kDeadRow;
+          const int er = n0 + r + k < t.rows ? t.expo[n0 + r + k] : kDeadRow;
           v[k] = er == kDeadRow ? 0.f : dx[c * S::pitch + (r + k < S::rows ? r + k : 0)] * ldexpf(1.f, 15 - er);
         }
         const Coded<T, 2> two(v[0], v[1]);
 #pragma unroll
-        for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_cat + part * t.plane_cat + (c0 + c) * t.pitch_cat + r) = two.p[part];
+        for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_cat + part * t.plane_cat + (c0 + c) * t.pitch_cat + n0 + r) = two.p[part];
       }
   }
 }
@@ -323,7 +323,7 @@ void launch(const GradientTask& t, hipStream_t stream) {
 template <typename T>
 void launch_few(const GradientTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
   const int64_t each = few_tile(t.rows), cols = sizeof(T) == 4 ? t.cats : laid_length(t.cats);   // (what is behind the last category is written too)
-  const dim3 grid((unsigned)((cols + each - 1) / each)), block(512);
+  const dim3 grid((unsigned)((cols + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(512);
   if (t.rows <= 16) hipLaunchKernelGGL((gradient_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
   else if (t.rows <= 32) hipLaunchKernelGGL((gradient_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
   else hipLaunchKernelGGL((gradient_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);

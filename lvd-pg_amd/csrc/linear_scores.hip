@@ -93,15 +93,15 @@ __global__ __launch_bounds__(512) void score_few_kernel(ScoreTask t, FewOperand 
   __shared__ Part joined[512];
   const float* const sums = few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds);
   constexpr int kLanes = 512 / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
-  const int n = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
-  const int64_t c0 = (int64_t)blockIdx.x * S::longs;
+  const int in = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
+  const int64_t c0 = (int64_t)blockIdx.x * S::longs, n = (int64_t)blockIdx.z * S::rows + in;
   const float sn = t.scale.n && n < t.rows ? t.scale.n[n] : 1.f;
   float x[kOwn], base = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     const int at = lane + i * kLanes;
     const int64_t c = c0 + at;
-    float v = sums[at * S::pitch + n];
+    float v = sums[at * S::pitch + in];
     if constexpr (sizeof(T) == 1) v = (float)__builtin_bit_cast(int, v) * sn * (c < t.cats ? t.scale.m[c] : 1.f);
     x[i] = score_of(v, bias_at(t.bias, c, t.cats));
     base = fmaxf(base, x[i]);
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(512) void score_few_kernel(ScoreTask t, FewOperand 
     if (lane < s) joined[threadIdx.x] = join(joined[threadIdx.x], joined[threadIdx.x + s * S::rows]);
     __syncthreads();
   }
-  if (lane == 0 && n < t.rows) t.parts[blockIdx.x * t.rows + n] = joined[n];
+  if (lane == 0 && n < t.rows) t.parts[blockIdx.x * t.rows + n] = joined[in];
 }
 
 // Joins the tiles' parts: `per` rows a workgroup, 256 / per lanes to each
@@ -189,7 +189,7 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 template <typename T>
 void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
   const int each = few_tile(t.rows);
-  const dim3 grid((unsigned)((t.cats + each - 1) / each)), block(512);
+  const dim3 grid((unsigned)((t.cats + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(512);
   if (t.rows <= 16) hipLaunchKernelGGL((score_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
   else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
   else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
@@ -222,13 +222,19 @@ void check_linear(const Matrix2& f, const Matrix2& w, const BiasRef& bias, const
   check_given(given);
 }
 
-// Few rows by way of few_rows.hip.hpp?  Where rows are read where they are, tiles of 128 categories stream faster once there are enough of them
-// (8 x 4096 x 50000 bf16: 80 us, 124 here); fewer leave compute units idle, and their long sums are what takes the time.
-bool takes_few(const Matrix2& f, const Matrix2& w) {
-  return f.rows() <= kFewRowsMost && f.stride == 1 && w.stride == 1 &&
-         (f.type == PCM_F32 || !readable(f) || !readable(w) || w.examples < kManyCats);
+namespace {
+bool few_tiles(int64_t rows, int64_t cats, int64_t length) {
+  return rows <= 512 && length >= 512 && ((rows + 127) / 128) * ((cats + 127) / 128) <= 32;
 }
-bool takes_few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cats < kManyCats; }
+}  // namespace
+bool takes_few(const Matrix2& f, const Matrix2& w) {
+  if (f.stride != 1 || w.stride != 1) return false;
+  return (f.rows() <= kFewRowsMost && (f.type == PCM_F32 || !readable(f) || !readable(w) || w.examples < kManyCats)) ||
+         few_tiles(f.rows(), w.examples, f.length);
+}
+bool takes_few8(int64_t rows, int64_t cats, int64_t length) {
+  return (rows <= kFewRowsMost && cats < kManyCats) || few_tiles(rows, cats, length);
+}
 FewOperand few_operand(const Matrix2& x) { return {x.p, x.stride_ex, x.stride_var, x.vars}; }
 
 int64_t linear_scores_workspace(const Matrix2& f, const Matrix2& w) {
@@ -306,7 +312,7 @@ void linear_scores(const Matrix2& f, const Matrix2& w, const BiasRef& bias, cons
 }
 
 int64_t linear_scores8_workspace(int64_t rows, int64_t cats, int32_t length) {
-  return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, round_up(length, kKBytes) / kKBytes, false, takes_few8(rows, cats));
+  return rows < 1 || cats < 1 ? 0 : parts_bytes(cats, rows, round_up(length, kKBytes) / kKBytes, false, takes_few8(rows, cats, length));
 }
 
 void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, int32_t vars, const int8_t* w, const float* w_scales, int32_t cats,
@@ -332,7 +338,7 @@ void linear_scores8(const int8_t* f, const float* f_scales, int64_t examples, in
   t.given.vars = vars;
   t.logp = d_logp;
   t.parts = static_cast<Part*>(d_work);
-  const bool few = takes_few8(t.rows, cats);
+  const bool few = takes_few8(t.rows, cats, length);
   if (few) launch_few<int8_t>(t, FewOperand{w, pitch, 0, 1}, FewOperand{f, pitch, 0, 1}, (int)pitch, stream);
   else launch<int8_t>(t, stream);
   join_launch(t, few, d_log_sum, stream);

@@ -105,10 +105,14 @@ void rows8(const Matrix2& x, int8_t* d_codes, float* d_scales, hipStream_t strea
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of rows8 failed: %s", hipGetErrorString(e));
 }
 
+namespace {
+bool few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cats < kManyCats; }   // (as takes_few8; tiles are cut into parts)
+}  // namespace
+
 int64_t product8_workspace(int64_t rows, int64_t cats, int32_t length) {
   if (rows < 1 || cats < 1 || length < 1 || length > kMaxLength8 || rows > 0x7fffffff || cats > 0x7fffffff) return 0;
   const int steps = (int)(round_up(length, kKBytes) / kKBytes);
-  const int parts = takes_few8(rows, cats) ? parts_for_few(cats, rows, steps) : parts_for(cats, rows, steps);
+  const int parts = few8(rows, cats) ? parts_for_few(cats, rows, steps) : parts_for(cats, rows, steps);
   return parts > 1 ? round_up(parts * rows * cats * 4, 256) : 0;
 }
 
@@ -125,7 +129,7 @@ void product8(const int8_t* a, const float* a_scales, int64_t rows, const int8_t
   check_workspace(d_work, work_bytes, product8_workspace(rows, cats, length), "8-bit product");
   const int64_t codes = round_up(length, kKBytes);
   const int steps = (int)(codes / kKBytes);
-  const bool few = takes_few8(rows, cats);
+  const bool few = few8(rows, cats);
   const int parts = few ? parts_for_few(cats, rows, steps) : parts_for(cats, rows, steps);
   OutTask t{};
   t.a = {b, codes, 0};
