@@ -1,6 +1,6 @@
 // Products of a long matrix (weights: categories or channels) with a few rows: bound by reading the long one once.
 //
-// A workgroup takes 32 rows of the long matrix (64 with more than 32 others), its eight waves every eighth piece of 128 bytes of them each, whatever
+// A workgroup takes 32 rows of the long matrix, its waves (eight, or four with more than 32 others) a piece of 128 bytes of them each in turns, whatever
 // the rows' length and alignment: nothing is laid out.  The waves' sums meet in LDS.
 #pragma once
 
@@ -9,8 +9,7 @@
 namespace pcm {
 
 constexpr int kFewRowsMost = 64;             // rows that are few: those of a workgroup
-// rows of the long matrix of a workgroup
-inline int few_tile(int64_t rows) { return rows <= 32 ? 32 : 64; }
+constexpr int kFewTile = 32;                 // rows of the long matrix of a workgroup
 constexpr int64_t kManyCats = 32768;         // categories that are many: 256 tiles of 128
 struct FewOperand {                          // rows of neighbouring entries
   const void* p;
@@ -119,11 +118,12 @@ struct FewParts {                            // two chunks of a row, 64 bytes ap
 template <int kGroups>
 struct FewTile {                             // kGroups: of 16 rows of b
   static constexpr int rows = 16 * kGroups;
-  static constexpr int longs = kGroups == 4 ? 64 : 32;        // rows of a: as many as of b, or more
+  static constexpr int longs = kFewTile;                      // rows of a
+  static constexpr int waves = kGroups == 4 ? 4 : 8, threads = 64 * waves;   // (so that three workgroups fit a compute unit's LDS either way)
   static constexpr int wave_bytes = (longs + rows) * 128;     // a piece of each
   static constexpr int pitch = rows + 1;                      // of the sums
-  static constexpr int sums_bytes = 8 * longs * pitch * 4;
-  static constexpr int lds = sums_bytes > 8 * wave_bytes ? sums_bytes : 8 * wave_bytes;
+  static constexpr int sums_bytes = waves * longs * pitch * 4;
+  static constexpr int lds = sums_bytes > waves * wave_bytes ? sums_bytes : waves * wave_bytes;
 };
 // Sums of rows [longs blockIdx.x, + longs) of a with rows [rows blockIdx.z, + rows) of b over `length` entries: sum of rows m and n of the tile
 // at m * pitch + n of what is returned (LDS), 32 bits (whole numbers: their bits), after a barrier.  Parts of the pieces by blockIdx.y.
@@ -194,17 +194,17 @@ __device__ __forceinline__ const float* few_sums(const FewOperand& a, const FewO
   const int end = min(last, whole);
   if (first + wave < end) {
     load(first + wave);
-    for (int piece = first + wave; piece < end; piece += 8) {
+    for (int piece = first + wave; piece < end; piece += S::waves) {
 #pragma unroll
       for (int g = 0; g < kLongs; ++g) put(g, ca[g].get(at_a[g]));
 #pragma unroll
       for (int g = 0; g < kRows; ++g) put(kLongs + g, cb[g].get(at_b[g]));
-      load(min(piece + 8, end - 1));         // (past the end the last one once more, not used)
+      load(min(piece + S::waves, end - 1));         // (past the end the last one once more, not used)
       multiply();
     }
   }
   if constexpr (sizeof(T) > 1) {             // (8-bit rows are whole pieces)
-    if (last > end && wave == 7) {
+    if (last > end && wave == S::waves - 1) {
       const int left = length - whole * kPiece - lane % 8 * kEach;
 #pragma unroll
       for (int g = 0; g < kLongs + kRows; ++g) {
@@ -227,12 +227,12 @@ __device__ __forceinline__ const float* few_sums(const FewOperand& a, const FewO
         out[(wave * S::longs + 16 * i + 4 * (lane / 16) + r) * S::pitch + 16 * g + (lane & 15)] = __builtin_bit_cast(float, sum);
       }
   __syncthreads();
-  for (int i = threadIdx.x; i < S::longs * S::rows; i += 512) {
+  for (int i = threadIdx.x; i < S::longs * S::rows; i += S::threads) {
     const int at = i / S::rows * S::pitch + i % S::rows;
     if constexpr (sizeof(T) == 1) {
       int s = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
+      for (int w = 0; w < S::waves; ++w) {
         const float x = out[w * S::longs * S::pitch + at];
         s += __builtin_bit_cast(int, x);
       }
@@ -240,7 +240,7 @@ __device__ __forceinline__ const float* few_sums(const FewOperand& a, const FewO
     } else {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += out[w * S::longs * S::pitch + at];
+      for (int w = 0; w < S::waves; ++w) s += out[w * S::longs * S::pitch + at];
       out[at] = s;
     }
   }

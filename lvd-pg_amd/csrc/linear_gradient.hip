@@ -212,11 +212,11 @@ __global__ __launch_bounds__(S::threads, 2) void gradient_kernel(GradientTask t)
 
 // Few rows: dx of a tile of categories in LDS, then out in whichever orders are needed
 template <typename T, int kGroups>
-__global__ __launch_bounds__(512) void gradient_few_kernel(GradientTask t, FewOperand w, FewOperand f, int length) {
+__global__ __launch_bounds__(FewTile<kGroups>::threads) void gradient_few_kernel(GradientTask t, FewOperand w, FewOperand f, int length) {
   typedef FewTile<kGroups> S;
   __shared__ __attribute__((aligned(16))) char lds[S::lds];
   float* const dx = const_cast<float*>(few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds));
-  constexpr int kLanes = 512 / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
+  constexpr int kLanes = S::threads / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
   const int in = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
   const int64_t c0 = (int64_t)blockIdx.x * S::longs, n0 = (int64_t)blockIdx.z * S::rows, n = n0 + in, at_n = min(n, t.rows - 1);
   const float z = t.log_sum[at_n], of_p = t.of_p[at_n];
@@ -245,13 +245,13 @@ __global__ __launch_bounds__(512) void gradient_few_kernel(GradientTask t, FewOp
   }
   if constexpr (sizeof(T) == 4) {
     if (!t.dx) return;
-    for (int i = threadIdx.x; i < S::longs * S::rows; i += 512) {
+    for (int i = threadIdx.x; i < S::longs * S::rows; i += S::threads) {
       const int c = i % S::longs, r = i / S::longs;
       if (n0 + r < t.rows && c0 + c < t.pitch_row) t.dx[(n0 + r) * t.pitch_row + c0 + c] = dx[c * S::pitch + r];
     }
   } else {                             // two at a time, in two parts; the turned rows up to a whole step
     if (t.by_row)
-      for (int i = threadIdx.x; i < S::longs / 2 * S::rows; i += 512) {
+      for (int i = threadIdx.x; i < S::longs / 2 * S::rows; i += S::threads) {
         const int c = i % (S::longs / 2) * 2, r = i / (S::longs / 2);
         if (n0 + r >= t.rows || c0 + c >= t.pitch_row) continue;
         const int er = t.expo[n0 + r];
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(512) void gradient_few_kernel(GradientTask t, FewOp
         for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_row + part * t.plane_row + (n0 + r) * t.pitch_row + c0 + c) = two.p[part];
       }
     if (t.by_cat)
-      for (int i = threadIdx.x; i < S::longs * 32; i += 512) {
+      for (int i = threadIdx.x; i < S::longs * 32; i += S::threads) {
         const int r = i % 32 * 2, c = i / 32;
         if (c0 + c >= t.cats || n0 + r >= t.pitch_cat) continue;
         float v[2];
@@ -322,8 +322,8 @@ void launch(const GradientTask& t, hipStream_t stream) {
 
 template <typename T>
 void launch_few(const GradientTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
-  const int64_t each = few_tile(t.rows), cols = sizeof(T) == 4 ? t.cats : laid_length(t.cats);   // (what is behind the last category is written too)
-  const dim3 grid((unsigned)((cols + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(512);
+  const int64_t each = kFewTile, cols = sizeof(T) == 4 ? t.cats : laid_length(t.cats);   // (what is behind the last category is written too)
+  const dim3 grid((unsigned)((cols + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(t.rows > 32 ? 256 : 512);
   if (t.rows <= 16) hipLaunchKernelGGL((gradient_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
   else if (t.rows <= 32) hipLaunchKernelGGL((gradient_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
   else hipLaunchKernelGGL((gradient_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);

@@ -87,12 +87,12 @@ __global__ __launch_bounds__(S::threads, 2) void score_kernel(ScoreTask t) {
 
 // Few rows: a thread has some of the tile's categories, of one row
 template <typename T, int kGroups>
-__global__ __launch_bounds__(512) void score_few_kernel(ScoreTask t, FewOperand w, FewOperand f, int length) {
+__global__ __launch_bounds__(FewTile<kGroups>::threads) void score_few_kernel(ScoreTask t, FewOperand w, FewOperand f, int length) {
   typedef FewTile<kGroups> S;
   __shared__ __attribute__((aligned(16))) char lds[S::lds];
-  __shared__ Part joined[512];
+  __shared__ Part joined[S::threads];
   const float* const sums = few_sums<T, kGroups>(w, f, t.cats, t.rows, length, 1, lds);
-  constexpr int kLanes = 512 / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
+  constexpr int kLanes = S::threads / S::rows, kOwn = S::longs / kLanes;   // lanes to a row, and categories of each
   const int in = threadIdx.x % S::rows, lane = threadIdx.x / S::rows;
   const int64_t c0 = (int64_t)blockIdx.x * S::longs, n = (int64_t)blockIdx.z * S::rows + in;
   const float sn = t.scale.n && n < t.rows ? t.scale.n[n] : 1.f;
@@ -188,14 +188,14 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
-  const int each = few_tile(t.rows);
-  const dim3 grid((unsigned)((t.cats + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(512);
+  const int each = kFewTile;
+  const dim3 grid((unsigned)((t.cats + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(t.rows > 32 ? 256 : 512);
   if (t.rows <= 16) hipLaunchKernelGGL((score_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
   else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
   else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
 }
 int64_t tiles_of_cats(int64_t cats, int64_t rows, int64_t steps, bool of_float, bool few) {
-  const int64_t each = few ? few_tile(rows) : tiles_for(cats, rows, steps, of_float) == kWide ? 256 : 128;
+  const int64_t each = few ? kFewTile : tiles_for(cats, rows, steps, of_float) == kWide ? 256 : 128;
   return (cats + each - 1) / each;
 }
 int64_t parts_bytes(int64_t cats, int64_t rows, int64_t steps, bool of_float, bool few) {

@@ -112,7 +112,7 @@ bool few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cats < kM
 int64_t product8_workspace(int64_t rows, int64_t cats, int32_t length) {
   if (rows < 1 || cats < 1 || length < 1 || length > kMaxLength8 || rows > 0x7fffffff || cats > 0x7fffffff) return 0;
   const int steps = (int)(round_up(length, kKBytes) / kKBytes);
-  const int parts = few8(rows, cats) ? parts_for_few(cats, rows, steps) : parts_for(cats, rows, steps);
+  const int parts = few8(rows, cats) ? parts_for_few(cats, steps) : parts_for(cats, rows, steps);
   return parts > 1 ? round_up(parts * rows * cats * 4, 256) : 0;
 }
 
@@ -130,7 +130,7 @@ void product8(const int8_t* a, const float* a_scales, int64_t rows, const int8_t
   const int64_t codes = round_up(length, kKBytes);
   const int steps = (int)(codes / kKBytes);
   const bool few = few8(rows, cats);
-  const int parts = few ? parts_for_few(cats, rows, steps) : parts_for(cats, rows, steps);
+  const int parts = few ? parts_for_few(cats, steps) : parts_for(cats, rows, steps);
   OutTask t{};
   t.a = {b, codes, 0};
   t.b = {a, codes, 0};

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(S::threads, 2) void out_kernel(OutTask t, bool four
 }
 
 template <int kGroups>
-__global__ __launch_bounds__(512) void out_few_kernel(OutTask t) {
+__global__ __launch_bounds__(FewTile<kGroups>::threads) void out_few_kernel(OutTask t) {
   typedef FewTile<kGroups> S;
   __shared__ __attribute__((aligned(16))) char lds[S::lds];
   const float* const sums = few_sums<int8_t, kGroups>(FewOperand{t.a.p, t.a.pitch, 0, 1}, FewOperand{t.b.p, t.b.pitch, 0, 1}, t.m, t.n,
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(512) void out_few_kernel(OutTask t) {
   const int64_t m = (int64_t)blockIdx.x * S::longs + at;
   if (m >= t.m) return;
   const float scale = t.finish.scale.m[m], bias = bias_of(t.finish.bias, m);
-  for (int n = threadIdx.x / S::longs; n < t.n; n += 512 / S::longs) {
+  for (int n = threadIdx.x / S::longs; n < t.n; n += S::threads / S::longs) {
     const float bits = sums[at * S::pitch + n];
     const int sum = __builtin_bit_cast(int, bits);
     if (t.type == kRawSums) static_cast<int*>(t.out)[((int64_t)blockIdx.y * t.n + n) * t.pitch + m] = sum;
@@ -163,13 +163,13 @@ int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
   // steps or more
   return (int)std::max<int64_t>(1, std::min<int64_t>({(steps < 64 ? 256 : 512) / tiles, steps / 4, 64}));
 }
-int parts_for_few(int64_t m, int64_t n, int64_t steps) {
+int parts_for_few(int64_t m, int64_t steps) {
   // a workgroup's waves take a step each at a time: parts of four rounds or more, as many as give every compute unit two workgroups
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 * few_tile(n) + m - 1) / m, steps / 32, 16}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 * kFewTile + m - 1) / m, steps / 32, 16}));
 }
 void product_few(const OutTask& t, hipStream_t stream) {
-  const int each = few_tile(t.n);
-  const dim3 grid((unsigned)((t.m + each - 1) / each), (unsigned)t.steps.parts), block(512);
+  const int each = kFewTile;
+  const dim3 grid((unsigned)((t.m + each - 1) / each), (unsigned)t.steps.parts), block(t.n > 32 ? 256 : 512);
   if (t.n <= 16) hipLaunchKernelGGL(out_few_kernel<1>, grid, block, 0, stream, t);
   else if (t.n <= 32) hipLaunchKernelGGL(out_few_kernel<2>, grid, block, 0, stream, t);
   else hipLaunchKernelGGL(out_few_kernel<4>, grid, block, 0, stream, t);

@@ -37,7 +37,7 @@ void product_few(const OutTask& t, hipStream_t stream);
 void join_parts(const void* parts, int count, bool whole, int64_t m, int64_t n, const Finish& finish, void* out, int type, int64_t pitch, hipStream_t stream);
 // how many parts the summed axis of a product is best cut into
 int parts_for(int64_t m, int64_t n, int64_t steps, bool of_float = false);
-int parts_for_few(int64_t m, int64_t n, int64_t steps);   // ... of product_few
+int parts_for_few(int64_t m, int64_t steps);   // ... of product_few
 
 #ifdef __HIPCC__
 struct FinishAt {                // of one n
