@@ -18,7 +18,7 @@ struct FewOperand {                          // rows of neighbouring entries
 };
 
 // Whether a product of scores goes this way: few rows, or so few tiles of 128 x 128 that long sums are best cut among the waves of a workgroup (100 x
-// 3000 x 500 f32: 111 us by tiles, @@ here).  Where rows can be read where they are, tiles of 128 categories stream faster once there
+// 3000 x 500 f32: 111 us by tiles, 43 here).  Where rows can be read where they are, tiles of 128 categories stream faster once there
 // are enough of them (8 x 4096 x 50000 bf16: 80 us, 124 here).
 bool takes_few(const Matrix2& f, const Matrix2& w);
 bool takes_few8(int64_t rows, int64_t cats, int64_t length);

