@@ -568,8 +568,9 @@ int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t nu
  *   have no part in the features' gradients.  A row of nothing but masks: log Z and logp -inf.  NaN in a row's features or in an
  *   unmasked category's weights, and scores of +inf: NaN.
  * Products of 16-bit types are exact and summed in 32 bits; float is taken as three bfloat16 parts whose six largest products are summed
- *   (what is left out lies 2^-26 below a product).  dx is rounded to the features' type, relative to a power of two a row (float:
- *   three parts again).  Sums have a fixed order: the same bits every time.
+ *   (what is left out is less than 2^-24 of a product).  dx is rounded to the features' type, relative to a power of two a row (float:
+ *   three parts again; fewer than 1024 rows of 16 bits: two).  Features of half count in the weights' gradients down to 2^-25 of the largest
+ *   |dx| of any row, as their type has no smaller numbers.  Sums have a fixed order: the same bits every time.
  * At most 2^22 rows, 2^30 categories, length 2^20.  d_work: so many bytes of device memory as the _workspace function of the same arguments says, 16-byte
  * aligned, which belong to the call until its work is done; `of`: 1 features, 2 weight, 4 bias, added.
  *
@@ -580,7 +581,8 @@ int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t nu
  *   (lengths up to 131071), rounded to `type` once at the end; rows of d_out are out_stride >= num_channels entries apart.
  * pcm_linear_scores8: pcm_linear_scores of x = such a product.
  *
- * All queue their work on `stream` (of the current device), wait for nothing and allocate nothing: they can be captured.
+ * Results and d_work lie apart from each other and from everything that is read.  All queue their work on `stream` (of the current device), wait for
+ * nothing and allocate nothing: they can be captured.
  */
 int64_t pcm_linear_scores_workspace(const void* d_features, const void* d_weight, int32_t type, int64_t stride_ex, int64_t stride_var,
                                     int64_t stride, int64_t weight_stride_cat, int64_t weight_stride, int64_t num_examples, int32_t num_vars,

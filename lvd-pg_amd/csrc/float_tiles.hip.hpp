@@ -1,5 +1,5 @@
-// Products of float matrices on the matrix cores: each float as three bfloat16 parts, h + m + l, and the six largest of the nine
-// products of parts; what is left out lies 2^-26 below a product.
+// Products of float matrices on the matrix cores: each float as three bfloat16 parts, h + m + l, which hold all of its 24 bits, and the
+// six largest of the nine products of parts; what is left out (m l, l m, l l) is less than 2^-24 of the product.
 //
 // A tile's floats come through registers, are taken apart there (some six instructions an entry) and lie in LDS as three planes, from which all
 // six products are read: 12 fragments for 24 products of 32 x 32, so LDS is no bound, and the floats are read once, whatever

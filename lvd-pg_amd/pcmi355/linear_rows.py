@@ -105,8 +105,9 @@ def linear_scores(features, weight, given=None, *, bias=None):
     keeping the scores: `category_scores(features @ weight.T + bias, given)` in one pass over features and weights.
 
     features: float32, bfloat16 or float16 GPU tensor [rows, length] or [examples, variables, length]; weight: the same type,
-    [categories, length]; any strides.  Rows that are neighbours, of a multiple of 64 entries in two bytes at multiples of 16
-    bytes, are read where they are; others (odd lengths, float32, transposed weights) are laid out in a workspace in each call.  Or both as `rows8` returned them.
+    [categories, length]; any strides.  Both are read where they are, but for 16-bit types in some layouts (with more than 64 rows: lengths that
+    are no multiple of 64, rows not at multiples of 16 bytes; entries that are not neighbours), which are laid out in a workspace in each
+    call.  Or both as `rows8` returned them.
     given: uint8, int32 or int64, one category per row or [rows..., slots] with up to 64; a negative one was not observed and has
     log-probability 0, one past the categories NaN.  bias: [categories], any of the three types; at or below half of its type's lowest
     value it masks its category, whatever the weights hold.  A row of nothing but masks has log-sum and log-probabilities -inf, one with NaN or +inf
@@ -146,7 +147,8 @@ def linear_scores_backward(features, weight, log_sum, given=None, *, bias=None, 
     arguments and `log_sum` as for and from `linear_scores`, 8-bit rows excepted.
 
     The scores are computed once more, in pieces of the categories; their derivatives are rounded to the features' type, relative to a
-    power of two a row, which no scale of the loss overflows (float32: three bfloat16 parts).  The same category in several slots adds up, a negative one
+    power of two a row, which no scale of the loss overflows (float32: three bfloat16 parts; fewer than 1024 rows of 16 bits: two parts).
+    float16 features count in the weights' gradient down to 2^-25 of the largest derivative of any row.  The same category in several slots adds up, a negative one
     adds nothing, one past the categories makes its row's derivatives NaN.  A row whose derivatives are all 0 (a batch's padding,
     whose categories are all negative) has no part in any gradient, whatever its features hold; nor have a masked category's weights in the features' gradient.
     Returns `LinearGradients`: tensors of the shapes and types of features, weight and bias; the same bits every time."""

@@ -483,7 +483,7 @@ def _exact_product(torch, R, a, c, k):
 
 
 SHAPES8 = [(1, 1, 1), (1, 4096, 3001), (3, 5, 7), (31, 127, 33), (32, 128, 128), (33, 129, 130), (64, 1000, 256), (65, 200, 257), (300, 4000, 50), (2, 131071, 3),
-           (520, 128, 70), (3600, 100, 4000), (17, 33, 20000), (4096, 8192, 64)]
+           (520, 128, 70), (3600, 100, 4000), (17, 33, 20000), (4096, 8192, 64), (20, 200, 33000), (50, 129, 32800)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -554,7 +554,7 @@ def test_products_into_what_is_given(gpu):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", [(1, 64, 3), (1, 4096, 3001), (40, 200, 500), (300, 129, 1000), (3600, 128, 4000)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape", [(1, 64, 3), (1, 4096, 3001), (40, 200, 500), (300, 129, 1000), (3600, 128, 4000), (20, 200, 33000), (50, 129, 32800), (200, 600, 700)], ids=lambda s: "x".join(map(str, s)))
 def test_scores_of_eight_bits(gpu, dtype, shape):
     torch, P, R = gpu
     n, k, C = shape
