@@ -10,7 +10,6 @@ namespace pcm {
 
 constexpr int kFewRowsMost = 64;             // rows that are few: those of a workgroup
 constexpr int kFewTile = 32;                 // rows of the long matrix of a workgroup
-constexpr int64_t kManyCats = 32768;         // categories that are many: 256 tiles of 128
 struct FewOperand {                          // rows of neighbouring entries
   const void* p;
   int64_t stride_ex, stride_var;             // in entries
@@ -19,7 +18,12 @@ struct FewOperand {                          // rows of neighbouring entries
 
 // Whether a product of scores goes this way: few rows, or so few tiles of 128 x 128 that long sums are best cut among the waves of a workgroup (100 x
 // 3000 x 500 f32: 111 us by tiles, 43 here).  Where rows can be read where they are, tiles of 128 categories stream faster once there
-// are enough of them (8 x 4096 x 50000 bf16: 80 us, 124 here).
+// are enough of them for the compute units, fewer the shorter the rows and the more of them there are, since a workgroup here takes its time to
+// join sums (f16, tiles and here: 16 x 4096 x 15000 57 us, 38; 8 x 4096 x 50000 80, 124; 16 x 256 x 20000 11.4, 15.4; 64 x 1024 x 30000 26,
+// 38; 64 x 4096 x 10000 56, 49; either way within some percent near the rule).
+inline int64_t many_cats(int64_t rows, int64_t row_bytes) {
+  return rows <= 32 ? 36000 * row_bytes / (row_bytes + 1200) : 24000 * row_bytes / (row_bytes + 2200);
+}
 bool takes_few(const Matrix2& f, const Matrix2& w);
 bool takes_few8(int64_t rows, int64_t cats, int64_t length);
 FewOperand few_operand(const Matrix2& x);

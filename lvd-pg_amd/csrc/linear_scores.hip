@@ -232,11 +232,11 @@ bool few_tiles(int64_t rows, int64_t cats, int64_t length) {
 }  // namespace
 bool takes_few(const Matrix2& f, const Matrix2& w) {
   if (f.stride != 1 || w.stride != 1) return false;
-  return (f.rows() <= kFewRowsMost && (f.type == PCM_F32 || !readable(f) || !readable(w) || w.examples < kManyCats)) ||
+  return (f.rows() <= kFewRowsMost && (f.type == PCM_F32 || !readable(f) || !readable(w) || w.examples < many_cats(f.rows(), 2 * f.length))) ||
          few_tiles(f.rows(), w.examples, f.length);
 }
 bool takes_few8(int64_t rows, int64_t cats, int64_t length) {
-  return (rows <= kFewRowsMost && cats < kManyCats) || few_tiles(rows, cats, length);
+  return (rows <= kFewRowsMost && cats < many_cats(rows, length)) || few_tiles(rows, cats, length);
 }
 FewOperand few_operand(const Matrix2& x) { return {x.p, x.stride_ex, x.stride_var, x.vars}; }
 

@@ -106,7 +106,9 @@ void rows8(const Matrix2& x, int8_t* d_codes, float* d_scales, hipStream_t strea
 }
 
 namespace {
-bool few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cats < kManyCats; }   // (as takes_few8; tiles are cut into parts)
+// Few rows, unless tiles of 128 channels fill the compute units (16 and 64 rows of 4096, 25000 channels: 22.3 us by tiles, 21.2 by few rows; 27.7,
+// 29.9.  15000: 19.2, 13.5; 26.8, 18.3)
+bool few8(int64_t rows, int64_t cats) { return rows <= kFewRowsMost && cats < (rows <= 32 ? 32768 : 20000); }
 }  // namespace
 
 int64_t product8_workspace(int64_t rows, int64_t cats, int32_t length) {
