@@ -113,6 +113,93 @@ __global__ __launch_bounds__(FewTile<kGroups>::threads) void out_few_kernel(OutT
   }
 }
 
+// Short sums (kSteps of 128 bytes), b in two parts: bound by writing the result.  A wave keeps the operands of 32 rows of b in registers and goes over
+// the columns, 64 at a time, whose operands come from the caches; nothing waits in LDS or at a barrier, as a tile's one or two steps
+// do (30000 x 4096 bf16 from 64 rows: 148 us by tiles, 93 so, 130 with every wave at the same columns and straight from registers; 30001 x 1001
+// from 50: 61, 38).
+template <typename T, int kSteps>
+__device__ __forceinline__ void short_rows(const OutTask& t, int chunks) {
+  constexpr int kPitch = 144;                // bytes: 64 columns of a row and a gap
+  __shared__ __attribute__((aligned(16))) char lds[4 * 32 * kPitch];
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x / 64;
+  const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * 32, n = n0 + (lane & 31);
+  if (n0 >= t.n) return;
+  char* const mine = lds + wave * 32 * kPitch;
+  const int expo = largest_exponent(t.finish.most) - 15;
+  const char* const b = static_cast<const char*>(t.b.p) + min(n, t.n - 1) * t.b.pitch + half * 16;
+  v4i fb[2][4 * kSteps];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int s = 0; s < 4 * kSteps; ++s) fb[p][s] = *reinterpret_cast<const v4i*>(b + p * t.b.plane + s * 32);
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    // (each wave begins elsewhere: rows of a power of two bytes would otherwise keep all waves at a few of the memory's channels)
+    const int64_t m = ((int64_t)blockIdx.y * chunks + (chunk + blockIdx.x * 4 + wave) % chunks) * 64;
+    if (m >= t.m) continue;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* const a = static_cast<const char*>(t.a.p) + min(m + 32 * i + (lane & 31), t.m - 1) * t.a.pitch + half * 16;
+      v4i fa[4 * kSteps];
+#pragma unroll
+      for (int s = 0; s < 4 * kSteps; ++s) fa[s] = *reinterpret_cast<const v4i*>(a + s * 32);
+      v16f sums = {};
+#pragma unroll
+      for (int p = 1; p >= 0; --p)           // the smaller part first
+#pragma unroll
+        for (int s = 0; s < 4 * kSteps; ++s) sums = Cores<T>::mma(fa[s], fb[p][s], sums);
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {       // eight neighbouring columns a lane, from both halves' four
+        uint32_t code[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float u = sums[4 * q + 2 * k], v = sums[4 * q + 2 * k + 1];
+          code[k] = pair_of<T>(ldexpf(u, expo), ldexpf(v, expo));
+        }
+        const auto lo = __builtin_amdgcn_permlane32_swap(code[0], code[2], false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap(code[1], code[3], false, false);
+        *reinterpret_cast<uint4*>(mine + (lane & 31) * kPitch + (32 * i + 8 * q + 8 * half) * 2) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 32; r += 8) {        // eight rows' 128 bytes at a time
+      const int in = r + lane / 8;
+      const int64_t to_n = n0 + in, col = m + lane % 8 * 8;
+      if (to_n >= t.n) continue;
+      const char* const from = mine + in * kPitch + lane % 8 * 16;
+      const raw4 v = *reinterpret_cast<const raw4*>(from);
+      uint16_t* const to = static_cast<uint16_t*>(t.out) + to_n * t.pitch + col;
+      // rows that begin inside a word: a lane's seven last entries and the next lane's first one, whole words
+      const bool odd = (uintptr_t)to & 2;
+      if (!odd && col + 8 <= t.m) {
+        *reinterpret_cast<raw4_by4*>(to) = v;
+      } else if (odd && lane % 8 < 7 && col + 9 <= t.m) {
+        const uint32_t next = *reinterpret_cast<const uint32_t*>(from + 16);
+        raw4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t hi = k < 3 ? v[k < 3 ? k + 1 : 3] : next, lo = v[k];
+          w[k] = __builtin_amdgcn_alignbit(hi, lo, 16);
+        }
+        *reinterpret_cast<raw4_by4*>(to + 1) = w;
+        if (lane % 8 == 0) to[0] = (uint16_t)v[0];
+      } else {
+        const int e0 = odd && lane % 8 ? 1 : 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t w = v[e / 2];
+          if (e >= e0 && col + e < t.m) to[e] = (uint16_t)(w >> 16 * (e % 2));
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+template <typename T, int kSteps>
+__global__ __launch_bounds__(256) void out_short_kernel(OutTask t, int chunks) {   // chunks of 64 columns
+  short_rows<T, kSteps>(t, chunks);
+}
+
 __global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, int count, bool whole, int64_t m, int64_t n, Finish finish, void* out,
                                                          int type, int64_t pitch) {
   const int most = finish.most ? largest_exponent(finish.most) : 0;
@@ -173,6 +260,24 @@ void product_few(const OutTask& t, hipStream_t stream) {
   if (t.n <= 16) hipLaunchKernelGGL(out_few_kernel<1>, grid, block, 0, stream, t);
   else if (t.n <= 32) hipLaunchKernelGGL(out_few_kernel<2>, grid, block, 0, stream, t);
   else hipLaunchKernelGGL(out_few_kernel<4>, grid, block, 0, stream, t);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of a product failed: %s", hipGetErrorString(e));
+}
+
+namespace {
+template <typename T>
+void launch_short(const OutTask& t, hipStream_t stream) {
+  // up to 16 chunks of columns a workgroup, as many as leave two workgroups a compute unit
+  const int64_t rows = (t.n + 127) / 128, all = (t.m + 63) / 64;
+  const int chunks = (int)std::max<int64_t>(1, std::min<int64_t>(16, all * rows / 512));
+  const dim3 grid((unsigned)rows, (unsigned)((all + chunks - 1) / chunks));
+  if (t.steps.count == 1) hipLaunchKernelGGL((out_short_kernel<T, 1>), grid, dim3(256), 0, stream, t, chunks);
+  else hipLaunchKernelGGL((out_short_kernel<T, 2>), grid, dim3(256), 0, stream, t, chunks);
+}
+}  // namespace
+void product_short(int operands, const OutTask& t, hipStream_t stream) {
+  if (operands == PCM_BF16) launch_short<bf16>(t, stream);
+  else launch_short<f16>(t, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of a product failed: %s", hipGetErrorString(e));
 }
