@@ -512,7 +512,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
       o.pitch = f.length;
       o.add = first > 0;
       o.finish.dead = expo;
-      product_out(f.type, o, stream);
+      short_sums(f.type, o) ? product_short(f.type, o, stream) : product_out(f.type, o, stream);
     }
     if (out.weight) {
       OutTask o{};
@@ -532,9 +532,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
       char* const to = static_cast<char*>(out.weight) + first * f.length * size;
       o.out = plan.weight_parts > 1 ? work + plan.weight : to;
       o.type = plan.weight_parts > 1 ? kRawSums : f.type;
-      // (rows in two parts are few, and so the sums short)
-      if (plan.dx_planes == 2 && o.steps.count <= 2) product_short(f.type, o, stream);
-      else product_out(f.type, o, stream);
+      short_sums(f.type, o) ? product_short(f.type, o, stream) : product_out(f.type, o, stream);
       if (plan.weight_parts > 1) join_parts(o.out, plan.weight_parts, false, o.m, o.n, o.finish, to, f.type, f.length, stream);
     }
   }

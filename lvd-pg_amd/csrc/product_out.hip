@@ -113,11 +113,11 @@ __global__ __launch_bounds__(FewTile<kGroups>::threads) void out_few_kernel(OutT
   }
 }
 
-// Short sums (kSteps of 128 bytes), b in two parts: bound by writing the result.  A wave keeps the operands of 32 rows of b in registers and goes over
-// the columns, 64 at a time, whose operands come from the caches; nothing waits in LDS or at a barrier, as a tile's one or two steps
-// do (30000 x 4096 bf16 from 64 rows: 148 us by tiles, 93 so, 130 with every wave at the same columns and straight from registers; 30001 x 1001
-// from 50: 61, 38).
-template <typename T, int kSteps>
+// Short sums (kSteps of 128 bytes), b in one part or two: bound by writing the result.  A wave keeps the operands of 32 rows of b in registers and
+// goes over the columns, 64 at a time, whose operands come from the caches; nothing waits in LDS or at a barrier, as a tile's one or two steps
+// do.  30000 x 4096 bf16 from 64 rows: 148 us by tiles, 90 so (2.7 TB/s; 130 with every wave at the same columns and straight from
+// registers); 30001 x 1001 f16 from 50: 61, 38; 40000 x 1001 bf16 from 60 categories: 75, 46; 32768 x 768 f16 from 128: 34, 32.
+template <typename T, int kSteps, int kPlanes>
 __device__ __forceinline__ void short_rows(const OutTask& t, int chunks) {
   constexpr int kPitch = 144;                // bytes: 64 columns of a row and a gap
   __shared__ __attribute__((aligned(16))) char lds[4 * 32 * kPitch];
@@ -125,16 +125,17 @@ __device__ __forceinline__ void short_rows(const OutTask& t, int chunks) {
   const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * 32, n = n0 + (lane & 31);
   if (n0 >= t.n) return;
   char* const mine = lds + wave * 32 * kPitch;
-  const int expo = largest_exponent(t.finish.most) - 15;
+  const FinishAt finish(t.finish, min(n, t.n - 1), t.finish.most ? largest_exponent(t.finish.most) : 0);
+  const float by = ldexpf(1.f, finish.expo);   // (exponents lie within float's)
   const char* const b = static_cast<const char*>(t.b.p) + min(n, t.n - 1) * t.b.pitch + half * 16;
-  v4i fb[2][4 * kSteps];
+  v4i fb[kPlanes][4 * kSteps];
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
     for (int s = 0; s < 4 * kSteps; ++s) fb[p][s] = *reinterpret_cast<const v4i*>(b + p * t.b.plane + s * 32);
   for (int chunk = 0; chunk < chunks; ++chunk) {
-    // (each wave begins elsewhere: rows of a power of two bytes would otherwise keep all waves at a few of the memory's channels)
-    const int64_t m = ((int64_t)blockIdx.y * chunks + (chunk + blockIdx.x * 4 + wave) % chunks) * 64;
+    // (each workgroup begins elsewhere: rows of a power of two bytes would otherwise keep all at a few of the memory's channels)
+    const int64_t m = ((int64_t)blockIdx.y * chunks + (chunk + blockIdx.x) % chunks) * 64;
     if (m >= t.m) continue;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -144,7 +145,7 @@ __device__ __forceinline__ void short_rows(const OutTask& t, int chunks) {
       for (int s = 0; s < 4 * kSteps; ++s) fa[s] = *reinterpret_cast<const v4i*>(a + s * 32);
       v16f sums = {};
 #pragma unroll
-      for (int p = 1; p >= 0; --p)           // the smaller part first
+      for (int p = kPlanes - 1; p >= 0; --p)   // the smaller part first
 #pragma unroll
         for (int s = 0; s < 4 * kSteps; ++s) sums = Cores<T>::mma(fa[s], fb[p][s], sums);
 #pragma unroll
@@ -153,7 +154,7 @@ __device__ __forceinline__ void short_rows(const OutTask& t, int chunks) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float u = sums[4 * q + 2 * k], v = sums[4 * q + 2 * k + 1];
-          code[k] = pair_of<T>(ldexpf(u, expo), ldexpf(v, expo));
+          code[k] = finish.dead ? 0u : pair_of<T>(u * by, v * by);
         }
         const auto lo = __builtin_amdgcn_permlane32_swap(code[0], code[2], false, false);
         const auto hi = __builtin_amdgcn_permlane32_swap(code[1], code[3], false, false);
@@ -195,9 +196,9 @@ __device__ __forceinline__ void short_rows(const OutTask& t, int chunks) {
     __builtin_amdgcn_wave_barrier();
   }
 }
-template <typename T, int kSteps>
+template <typename T, int kSteps, int kPlanes>
 __global__ __launch_bounds__(256) void out_short_kernel(OutTask t, int chunks) {   // chunks of 64 columns
-  short_rows<T, kSteps>(t, chunks);
+  short_rows<T, kSteps, kPlanes>(t, chunks);
 }
 
 __global__ __launch_bounds__(256) void join_parts_kernel(const uint32_t* parts, int count, bool whole, int64_t m, int64_t n, Finish finish, void* out,
@@ -271,8 +272,11 @@ void launch_short(const OutTask& t, hipStream_t stream) {
   const int64_t rows = (t.n + 127) / 128, all = (t.m + 63) / 64;
   const int chunks = (int)std::max<int64_t>(1, std::min<int64_t>(16, all * rows / 512));
   const dim3 grid((unsigned)rows, (unsigned)((all + chunks - 1) / chunks));
-  if (t.steps.count == 1) hipLaunchKernelGGL((out_short_kernel<T, 1>), grid, dim3(256), 0, stream, t, chunks);
-  else hipLaunchKernelGGL((out_short_kernel<T, 2>), grid, dim3(256), 0, stream, t, chunks);
+  const bool one = t.steps.pairs.count == 1;
+  if (t.steps.count == 1 && one) hipLaunchKernelGGL((out_short_kernel<T, 1, 1>), grid, dim3(256), 0, stream, t, chunks);
+  else if (t.steps.count == 1) hipLaunchKernelGGL((out_short_kernel<T, 1, 2>), grid, dim3(256), 0, stream, t, chunks);
+  else if (one) hipLaunchKernelGGL((out_short_kernel<T, 2, 1>), grid, dim3(256), 0, stream, t, chunks);
+  else hipLaunchKernelGGL((out_short_kernel<T, 2, 2>), grid, dim3(256), 0, stream, t, chunks);
 }
 }  // namespace
 void product_short(int operands, const OutTask& t, hipStream_t stream) {
@@ -282,6 +286,9 @@ void product_short(int operands, const OutTask& t, hipStream_t stream) {
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of a product failed: %s", hipGetErrorString(e));
 }
 
+bool short_sums(int operands, const OutTask& t) {
+  return operands != PCM_F32 && t.type == operands && t.steps.count <= 2 && t.steps.parts == 1 && !t.add;
+}
 void product_out(int operands, const OutTask& t, hipStream_t stream) {
   if (operands == PCM_F32) launch<float, FloatTile>(t, stream);
   else if (operands == PCM_BF16) launch<bf16>(t, stream);

@@ -33,7 +33,8 @@ struct OutTask {
 void product_out(int operands, const OutTask& t, hipStream_t stream);   // operands: PCM_F32, PCM_BF16, PCM_F16, PCM_U8 (whole numbers)
 // ... of 8-bit rows, a few of b (kFewRowsMost): t.a, t.b and t.steps as for product_out
 void product_few(const OutTask& t, hipStream_t stream);
-// ... of 16-bit types over one or two steps, b in two parts, in that type, finished by finish.most alone
+// ... of 16-bit types over one or two steps, in that type (short_sums), finished without scales and bias
+bool short_sums(int operands, const OutTask& t);
 void product_short(int operands, const OutTask& t, hipStream_t stream);
 // out = the finished sums of parts [parts][n][m] floats (or whole numbers)
 void join_parts(const void* parts, int count, bool whole, int64_t m, int64_t n, const Finish& finish, void* out, int type, int64_t pitch, hipStream_t stream);
