@@ -5,8 +5,9 @@
 // exponentials in registers, the tile's waves join theirs in LDS, and a pair of numbers per row and tile of categories is all that
 // is written; a second launch joins those.  The score of a given category is written by the lane that has it.
 //
-// Bound by the matrix cores (4096 x 50304 of length 4096 bf16: 1.42 ms, 1.19 PFLOP/s at the clock that the card's power leaves; 8-bit rows 0.94 ms),
-// few rows by reading the weights.  Kept scores would be 824 MB there, written once and read once.
+// Bound by the matrix cores (4096 x 50304 of length 4096 bf16: 1.37 ms, 1.23 PFLOP/s at the clock that the card's power leaves; 2048 x 131072 in 8
+// bits: 0.95 ms, 2.3 POP/s), few rows by reading the weights (1 x 131072 of length 4096 bf16: 193 us, 5.6 TB/s).  Kept scores would
+// be 824 MB in the first, written once and read once.
 #include "few_rows.hip.hpp"
 
 namespace pcm {

@@ -1,4 +1,7 @@
 // Products that are written out: gradients of features and weights, and products of 8-bit rows.
+//
+// Long sums are bound by the matrix cores: 8192 x 16384 over 4096 in 8 bits 550 us (2.0 POP/s), 4096 x 4096 over 16384 bf16 460 us (1.19
+// PFLOP/s).  Results go out by way of LDS, since a lane's four neighbours alone fill an eighth of a line.
 #include "product_out.hip.hpp"
 
 namespace pcm {
