@@ -91,6 +91,36 @@ def test_gradients_in_pieces_of_the_categories(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(16500, 40, 7681), (2, 3, (1 << 20) + 5), (70, 8, (1 << 20) + 3)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_in_pieces_of_unlike_sizes(gpu, dtype, shape):
+    torch, P, R = gpu
+    f, w, b, g, gl, gz = _inputs(torch, dtype, *shape, 31, bias="masked", slots=2)
+    g[:, 0] = shape[2] - 1 - torch.arange(shape[0], device="cuda") % 3      # categories of the last piece
+    b[-3:] = 0.5
+    s, got = _check_scores(R, P, f, w, b, g)
+    _check_grads(R, P, f, w, b, s, got, g, gl, gz)
+
+
+# sums of one and of two steps that are written as they are: gradients of features under few categories, of weights from few rows
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("shape", [(1500, 33, 20), (1024, 64, 64), (2000, 130, 65), (1100, 1001, 128), (64, 515, 1000), (65, 64, 3000), (128, 1000, 257),
+                                   (5, 4099, 130)], ids=lambda s: "x".join(map(str, s)))
+def test_short_sums(gpu, dtype, shape):
+    torch, P, R = gpu
+    f, w, b, g, gl, gz = _inputs(torch, dtype, *shape, 32, bias="masked", slots=2)
+    g[3:5], gz[3:5] = -1, 0.0                                               # rows without derivatives, whatever they hold
+    s, got = _check_scores(R, P, f, w, b, g)
+    f[3:5] = float("nan")
+    clean = f.clone()
+    clean[3:5] = 0.0
+    s = R.Scores(clean, w, b)
+    want = R.gradients(clean, w, b, s, g, gl, gz)
+    d = P.linear_scores_backward(f, w, got.log_sum, g, bias=b, grad_logp=gl, grad_log_sum=gz)
+    for name, (v, off) in want.items():
+        R.within(getattr(d, name), v, off, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bias", ["masked", "lowest", None])
 @pytest.mark.parametrize("slots", [1, 16, 64])
 def test_masks_and_many_slots(gpu, dtype, bias, slots):
