@@ -1,5 +1,5 @@
 // Products of a long matrix (weights: categories or channels) with a few rows: bound by reading the long one once, and, with more than 16 rows, by
-// each workgroup's reading the others from the caches: 50021 x 1001 f16 with 16 rows 34 us (3 TB/s), with 48 62 us.
+// each workgroup's reading the others from the caches: 50021 x 1001 f16 with 16 rows 34 us (3 TB/s), with 48 50 us.
 //
 // A workgroup takes 32 rows of the long matrix, its waves (eight, or four with more than 32 others) a piece of 128 bytes of them each in turns, whatever
 // the rows' length and alignment: nothing is laid out.  The waves' sums meet in LDS.
