@@ -8,12 +8,12 @@
 
 namespace pcm {
 
-// Which planes of a and of b are multiplied, one after the other: two bits each, the first product lowest
+// Which planes of b are multiplied with a, one after the other: two bits each, the first product lowest
 struct PlanePairs {
   int count;
-  uint32_t a, b;
+  uint32_t b;
 };
-constexpr PlanePairs kOnePlane{1, 0, 0}, kTwoOfB{2, 0, 0x1};   // b in two parts: the smaller one first
+constexpr PlanePairs kOnePlane{1, 0}, kTwoOfB{2, 0x1};   // b in two parts: the smaller one first
 // What a product sums over: `count` steps of 128 bytes for each pair of planes.  With parts > 1 part blockIdx.y takes its share of the steps.
 struct Steps {
   int count;
@@ -98,16 +98,15 @@ struct TileLoader {
   static constexpr int each = S::stage / 1024 / S::waves;
   static_assert(each * 1024 * S::waves == S::stage && S::BM % 8 == 0 && S::BN % 8 == 0);
   const char *a0, *b0;
-  int64_t plane_a, plane_b;
+  int64_t plane_b;
   v4i a, b;
   uint32_t at[each];
   uint32_t k, begin, end;      // the bytes of a row that come next, and between which
   PlanePairs pairs;
   int wave, product = 0;
 
-  __device__ __forceinline__ void choose_planes() {
-    const int64_t pa = pairs.a >> 2 * product & 3, pb = pairs.b >> 2 * product & 3;
-    a = memory_at(a0 + pa * plane_a);
+  __device__ __forceinline__ void choose_plane() {
+    const int64_t pb = pairs.b >> 2 * product & 3;
     b = memory_at(b0 + pb * plane_b);
   }
   __device__ __forceinline__ TileLoader(const Operand& oa, const Operand& ob, int64_t m0, int64_t n0, int64_t m, int64_t n, int first, int count,
@@ -115,11 +114,11 @@ struct TileLoader {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     a0 = static_cast<const char*>(oa.p) + m0 * oa.pitch;
     b0 = static_cast<const char*>(ob.p) + n0 * ob.pitch;
-    plane_a = oa.plane;
     plane_b = ob.plane;
     k = begin = __builtin_amdgcn_readfirstlane((uint32_t)first * kKBytes);
     end = begin + __builtin_amdgcn_readfirstlane((uint32_t)count * kKBytes);
-    choose_planes();
+    a = memory_at(a0);
+    choose_plane();
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < each; ++i) {
@@ -140,7 +139,7 @@ struct TileLoader {
     if (k == end && product + 1 < pairs.count) {
       k = begin;
       ++product;
-      choose_planes();
+      choose_plane();
     }
   }
 };
