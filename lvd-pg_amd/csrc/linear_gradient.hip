@@ -413,8 +413,13 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
                             hipStream_t stream) {
   check_linear(f, w, bias, given_in, "gradient of linear scores");
   const int64_t rows = f.rows(), cats = w.examples;
+  if (!rows) {   // sums of nothing, which need no workspace
+    if (out.weight) join_parts(nullptr, 0, false, f.length, cats, Finish(), out.weight, f.type, f.length, stream);
+    if (out.bias) join_parts(nullptr, 0, false, cats, 1, Finish(), out.bias, bias.type, cats, stream);
+    return;
+  }
   if (given_in.slots && (!given_in.p || !d_grad_logp)) fail(PCM_ERR_ARG, "gradient of linear scores: given categories and their derivatives go together");
-  if (!w.p || (rows && (!f.p || !d_log_sum))) fail(PCM_ERR_ARG, "gradient of linear scores: a pointer is null");
+  if (!w.p || !f.p || !d_log_sum) fail(PCM_ERR_ARG, "gradient of linear scores: a pointer is null");
   const Plan plan(f, w, out.features, out.weight, out.bias);
   check_workspace(d_work, work_bytes, plan.bytes, "gradient of linear scores");
   char* const work = static_cast<char*>(d_work);
@@ -422,11 +427,6 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
   given.vars = f.vars;
   float* const of_p = reinterpret_cast<float*>(work + plan.of_p);
   int *const expo = reinterpret_cast<int*>(work + plan.expo), *const most = reinterpret_cast<int*>(work + plan.most);
-  if (!rows) {   // sums of nothing
-    if (out.weight) join_parts(nullptr, 0, false, f.length, cats, Finish(), out.weight, f.type, f.length, stream);
-    if (out.bias) join_parts(nullptr, 0, false, cats, 1, Finish(), out.bias, bias.type, cats, stream);
-    return;
-  }
   hipLaunchKernelGGL(row_terms_kernel, dim3(kMostBlocks), dim3(256), 0, stream, given, d_grad_logp, d_grad_log_sum, d_log_sum, rows, cats, of_p, expo, most);
   const bool of_float = plan.of_float;
   const int size = of_float ? 4 : 2;

@@ -212,3 +212,15 @@ def test_workspaces_follow_the_arguments():
     assert 0 < back(4) < back(1) < back(7) and back(2) < back(7) and back(7, 0) == 0
     assert lib.pcm_product8_workspace(0, 10, 100) == 0 and lib.pcm_product8_workspace(10, 10, 131072) == 0
     assert lib.pcm_linear_scores8_workspace(0, 1, 10, 10) == 0 and lib.pcm_linear_scores8_workspace(5, 1, 10, 10) > 0
+
+
+@pytest.mark.parametrize("type_", [0, 1, 2])
+def test_a_gradient_of_no_rows_needs_nothing(type_):
+    from pcmi355._lib import lib
+    p = 4096                                                             # (nothing is read there)
+    assert lib.pcm_linear_scores_backward_workspace(p, p, type_, 8, 0, 1, 8, 1, 0, 1, 8, 10, 7) == 0
+    for at in (p, None):
+        assert lib.pcm_linear_scores_backward(at, at, type_, 8, 0, 1, 8, 1, 0, 1, 8, 10, None, 0, None, 5, 0, 0, 0, 0, None, None, None, None, None,
+                                              None, None, 0, None) == 0
+    assert lib.pcm_linear_scores_backward(p, p, type_, 8, 0, 1, 8, 1, 0, 1, 0, 10, None, 0, None, 5, 0, 0, 0, 0, None, None, None, None, None, None,
+                                          None, 0, None) == -2           # (what is refused with rows is refused without)

@@ -657,3 +657,18 @@ def test_a_network_taught_the_clusters_of_a_circuit(gpu):
     exact = P.linear_scores(f, w, clusters, bias=b)
     step = float((w.abs().max(1).values / 127).max())
     assert float((exact.log_sum - direct.log_sum).abs().max()) <= V * step / 2 * 1.01 + 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_no_rows_through_the_c_entry(gpu, dtype):
+    """Weights' and bias's gradients are sums of nothing; no workspace, no features, no log-sums"""
+    torch, P, R = gpu
+    from pcmi355._lib import lib, check
+    code = {"float32": 0, "bfloat16": 1, "float16": 2}[dtype]
+    k, C = 70, 301
+    w = torch.ones(C, k, dtype=getattr(torch, dtype), device="cuda")
+    dw, db = torch.full((C + 1, k), 7.0, dtype=w.dtype, device="cuda"), torch.full((C + 1,), 7.0, device="cuda")
+    check(lib.pcm_linear_scores_backward(None, w.data_ptr(), code, k, 0, 1, k, 1, 0, 1, k, C, None, 0, None, 5, 0, 0, 0, 0, None, None, None, None,
+                                         dw.data_ptr(), db.data_ptr(), None, 0, None))
+    torch.cuda.synchronize()
+    assert (dw[:C] == 0).all() and (db[:C] == 0).all() and (dw[C] == 7).all() and db[C] == 7
