@@ -242,10 +242,10 @@ __device__ __forceinline__ void float_stages(const FloatOperand& a, const FloatO
 
 // Sums over steps [0, k) of a's rows (m) and b's (n), as product_tile; parts of the steps by blockIdx.y
 template <typename Done>
-__device__ __forceinline__ void float_tile(const FloatOperand& a, const FloatOperand& b, int64_t m, int64_t n, int64_t k, int parts, Done done) {
+__device__ __forceinline__ void float_tile(const FloatOperand& a, const FloatOperand& b, int64_t m, int64_t n, int64_t first_n, int64_t k, int parts, Done done) {
   typedef FloatTile S;
   __shared__ __attribute__((aligned(16))) char lds[6 * kFloatPlane];
-  const TileAt tile = tile_at<S>(m, n);
+  const TileAt tile = tile_at<S>(m, first_n);
   const int64_t stages = (k + kFloatSteps - 1) / kFloatSteps;
   const int64_t first = stages * blockIdx.y / parts, last = stages * (blockIdx.y + 1) / parts;
   v16f sums[S::FM][S::FN] = {};
@@ -266,6 +266,8 @@ struct ScoreInputs {
   FloatOperand fw, ff;       // ... of float, of fk entries
   int64_t fk;
   int64_t cats, rows;
+  int64_t first_cat;         // the category that is row 0 of w (category 0 of bias and scale)
+  int64_t first_row;         // the launch's first row of features, by tiles
   Steps steps;
   BiasRef bias;
   ScaleRef scale;
@@ -273,13 +275,13 @@ struct ScoreInputs {
 };
 template <typename T, typename S, typename Done>
 __device__ __forceinline__ void score_sums(const ScoreInputs& t, Done done) {
-  if constexpr (__is_same(T, float)) float_tile(t.fw, t.ff, t.cats, t.rows, t.fk, 1, done);
-  else product_tile<T, S>(t.w, t.f, t.cats, t.rows, t.steps, done);
+  if constexpr (__is_same(T, float)) float_tile(t.fw, t.ff, t.cats, t.rows, t.first_row, t.fk, 1, done);
+  else product_tile<T, S>(t.w, t.f, t.cats, t.rows, t.first_row, t.steps, done);
 }
 // bias and scales of the tile's categories into LDS, while its sums are on their way; a barrier before they are read
 template <typename S>
 __device__ __forceinline__ void tile_constants(const ScoreInputs& t, float* bias, float* scale) {
-  const int64_t m0 = tile_at<S>(t.cats, t.rows).m0;
+  const int64_t m0 = tile_at<S>(t.cats, 0).m0;
   for (int i = threadIdx.x; i < S::BM; i += S::threads) {
     bias[i] = bias_at(t.bias, m0 + i, t.cats);
     scale[i] = t.scale.m && m0 + i < t.cats ? t.scale.m[m0 + i] : 1.f;

@@ -2,8 +2,7 @@
 //
 // Bound by the bytes moved.  Rows of neighbours are copied 16 bytes a lane, or turned in tiles of 64 x 64: 4 x 4 entries in a lane's registers, the
 // tile's rows put together in LDS (50000 x 4096 bf16: 170 us, 430 entry by entry); other strides go entry by entry.
-#include <algorithm>
-
+#include "linear_plan.hpp"
 #include "linear_scores.hpp"
 
 namespace pcm {
@@ -168,8 +167,14 @@ void launch(const Matrix2& x, int64_t first, int64_t count, bool turned, const L
 }  // namespace
 
 void lay_out(const Matrix2& x, int64_t first, int64_t count, bool turned, const LayOut& with, void* d_to, hipStream_t stream) {
-  if (x.type == PCM_BF16) launch<bf16>(x, first, count, turned, with, d_to, stream);
-  else launch<f16>(x, first, count, turned, with, d_to, stream);
+  // (turned rows are those of features or of a piece of the categories, which a launch takes at once)
+  const int64_t most = units_a_launch(1, 256) * kTile, pitch = laid_length(x.length);
+  for (int64_t at = 0; at < count; at += most) {
+    uint16_t* const to = static_cast<uint16_t*>(d_to) + at * pitch;
+    const int64_t n = std::min(most, count - at);
+    if (x.type == PCM_BF16) launch<bf16>(x, first + at, n, turned, with, to, stream);
+    else launch<f16>(x, first + at, n, turned, with, to, stream);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of lay_out failed: %s", hipGetErrorString(e));
 }

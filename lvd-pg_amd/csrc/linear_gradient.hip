@@ -53,8 +53,7 @@ __global__ __launch_bounds__(256) void row_terms_kernel(GivenRef given, const fl
   if (threadIdx.x == 0) most[blockIdx.x] = sub[0];
 }
 
-struct GradientTask : ScoreInputs {
-  int64_t first;                     // the piece's first category, which is row 0 of w; cats is the piece's size
+struct GradientTask : ScoreInputs {   // of a piece of the categories
   const float *grad_logp, *log_sum, *of_p;
   const int* expo;
   float* dx;                         // float: dx [row][pitch_row]
@@ -121,7 +120,7 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
       if (t.given.slots && by != 0.f) {
         const int64_t ex = row / t.given.vars, v = row % t.given.vars;
         for (int s = 0; s < t.given.slots; ++s) {
-          const int64_t g = given_at(t.given, ex, v, s) - t.first - m;
+          const int64_t g = given_at(t.given, ex, v, s) - t.first_cat - m;
           if (g < 0 || g >= S::WM || (g >> 2 & 1) != half) continue;
           const float add = t.grad_logp[row * t.given.slots + s];
 #pragma unroll
@@ -234,7 +233,7 @@ __global__ __launch_bounds__(FewTile<kGroups>::threads) void gradient_few_kernel
   }
   if (e != kDeadRow)
     for (int s = 0; s < t.given.slots; ++s) {
-      const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - t.first - c0;
+      const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - t.first_cat - c0;
       const float add = t.grad_logp[n * t.given.slots + s];
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) own[i] += g == lane + i * kLanes ? add : 0.f;
@@ -465,7 +464,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     t.bias = bias;
     if (t.bias.p) t.bias.p = static_cast<const char*>(bias.p) + first * (bias.type == PCM_F32 ? 4 : 2);
     t.given = given;
-    t.first = first;
+    t.first_cat = first;
     t.grad_logp = d_grad_logp;
     t.log_sum = d_log_sum;
     t.of_p = of_p;

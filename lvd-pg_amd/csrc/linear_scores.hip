@@ -117,7 +117,7 @@ __global__ __launch_bounds__(FewTile<kGroups>::threads, kGroups == 4 ? 3 : 4) vo
   joined[threadIdx.x] = {sum == 0.f ? base : to, sum};
   if (n < t.rows)
     for (int s = 0; s < t.given.slots; ++s) {
-      const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - c0;
+      const int64_t g = given_at(t.given, n / t.given.vars, n % t.given.vars, s) - t.first_cat - c0;
 #pragma unroll
       for (int i = 0; i < kOwn; ++i)
         if (g == lane + i * kLanes) t.logp[n * t.given.slots + s] = x[i];
@@ -179,9 +179,12 @@ int tiles_for(int64_t m, int64_t n, int64_t steps, bool of_float) {
 }
 template <typename T, typename S>
 void launch(const ScoreTask& t, hipStream_t stream) {
-  const int64_t tiles = ((t.cats + S::BM - 1) / S::BM) * ((t.rows + S::BN - 1) / S::BN);
-  if (tiles > 0x7fffffff) fail(PCM_ERR_UNSUPPORTED, "linear scores: %lld tiles", (long long)tiles);
-  hipLaunchKernelGGL((score_kernel<T, S>), dim3((unsigned)tiles), dim3(S::threads), 0, stream, t);
+  const int64_t tiles_m = (t.cats + S::BM - 1) / S::BM, tiles_n = (t.rows + S::BN - 1) / S::BN, most = units_a_launch(tiles_m, S::threads);
+  ScoreTask of_launch = t;
+  for (int64_t first = 0; first < tiles_n; first += most) {
+    of_launch.first_row = first * S::BN;
+    hipLaunchKernelGGL((score_kernel<T, S>), dim3((unsigned)(tiles_m * std::min(most, tiles_n - first))), dim3(S::threads), 0, stream, of_launch);
+  }
 }
 template <typename T>
 void launch(const ScoreTask& t, hipStream_t stream) {
@@ -193,11 +196,24 @@ void launch(const ScoreTask& t, hipStream_t stream) {
 }
 template <typename T>
 void launch_few(const ScoreTask& t, const FewOperand& w, const FewOperand& f, int length, hipStream_t stream) {
-  const int each = kFewTile;
-  const dim3 grid((unsigned)((t.cats + each - 1) / each), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(t.rows > 32 ? 256 : 512);
-  if (t.rows <= 16) hipLaunchKernelGGL((score_few_kernel<T, 1>), grid, block, 0, stream, t, w, f, length);
-  else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, t, w, f, length);
-  else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, t, w, f, length);
+  const int64_t tiles = (t.cats + kFewTile - 1) / kFewTile;
+  const int threads = t.rows > 32 ? 256 : 512;
+  const int64_t most = units_a_launch(1, threads);
+  ScoreTask of_launch = t;
+  FewOperand of_w = w;
+  for (int64_t first = 0; first < tiles; first += most) {
+    const int64_t cat = first * kFewTile;
+    of_launch.first_cat = cat;
+    of_launch.cats = std::min(most * kFewTile, t.cats - cat);
+    of_w.p = static_cast<const char*>(w.p) + cat * w.stride_ex * (int64_t)sizeof(T);
+    if (t.bias.p) of_launch.bias.p = static_cast<const char*>(t.bias.p) + cat * (t.bias.type == PCM_F32 ? 4 : 2);
+    if (t.scale.m) of_launch.scale.m = t.scale.m + cat;
+    of_launch.parts = t.parts + first * t.rows;
+    const dim3 grid((unsigned)std::min(most, tiles - first), 1, (unsigned)((t.rows + kFewRowsMost - 1) / kFewRowsMost)), block(threads);
+    if (t.rows <= 16) hipLaunchKernelGGL((score_few_kernel<T, 1>), grid, block, 0, stream, of_launch, of_w, f, length);
+    else if (t.rows <= 32) hipLaunchKernelGGL((score_few_kernel<T, 2>), grid, block, 0, stream, of_launch, of_w, f, length);
+    else hipLaunchKernelGGL((score_few_kernel<T, 4>), grid, block, 0, stream, of_launch, of_w, f, length);
+  }
 }
 int64_t tiles_of_cats(int64_t cats, int64_t rows, int64_t steps, bool of_float, bool few) {
   const int64_t each = few ? kFewTile : tiles_for(cats, rows, steps, of_float) == kWide ? 256 : 128;

@@ -12,7 +12,7 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
   __shared__ __attribute__((aligned(16))) float bias[S::BM], scale[S::BM];
   const bool raw = t.type == kRawSums;
   const int most = t.finish.most ? largest_exponent(t.finish.most) : 0;
-  const int64_t m0 = tile_at<S>(t.m, t.n).m0;
+  const int64_t m0 = tile_at<S>(t.m, 0).m0;
   for (int i = threadIdx.x; i < S::BM; i += S::threads) {
     bias[i] = m0 + i < t.m ? bias_of(t.finish.bias, m0 + i) : 0.f;
     scale[i] = t.finish.scale.m && m0 + i < t.m ? t.finish.scale.m[m0 + i] : 1.f;
@@ -90,8 +90,8 @@ __device__ __forceinline__ void out_tile(const OutTask& t, bool fours) {
       }
     }
   };
-  if constexpr (__is_same(T, float)) float_tile(t.fa, t.fb, t.m, t.n, t.fk, t.steps.parts, done);
-  else product_tile<T, S>(t.a, t.b, t.m, t.n, t.steps, done);
+  if constexpr (__is_same(T, float)) float_tile(t.fa, t.fb, t.m, t.n, 0, t.fk, t.steps.parts, done);
+  else product_tile<T, S>(t.a, t.b, t.m, t.n, 0, t.steps, done);
 }
 template <typename T, typename S>
 __global__ __launch_bounds__(S::threads, 2) void out_kernel(OutTask t, bool fours) {
@@ -233,7 +233,7 @@ typedef TileSizes<128, 32, 32, 32> Narrow;
 template <typename T, typename S>
 void launch(const OutTask& t, hipStream_t stream) {
   const int64_t tiles = ((t.m + S::BM - 1) / S::BM) * ((t.n + S::BN - 1) / S::BN);
-  if (tiles > 0x7fffffff) fail(PCM_ERR_UNSUPPORTED, "product: %lld tiles", (long long)tiles);
+  if (tiles > most_blocks(S::threads)) fail(PCM_ERR_UNSUPPORTED, "product: %lld tiles", (long long)tiles);
   const int size = t.type == PCM_F32 ? 4 : 2;
   const bool fours = t.type != kRawSums && t.pitch % 4 == 0 && (uintptr_t)t.out % (4 * size) == 0;
   hipLaunchKernelGGL((out_kernel<T, S>), dim3((unsigned)tiles, (unsigned)t.steps.parts), dim3(S::threads), 0, stream, t, fours);

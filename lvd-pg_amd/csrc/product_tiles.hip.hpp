@@ -2,8 +2,7 @@
 // loop that the kernels of linear_scores.hip, linear_gradient.hip and product8.hip share, each with what it does with the sums.
 #pragma once
 
-#include <algorithm>
-
+#include "linear_plan.hpp"
 #include "linear_scores.hpp"
 
 namespace pcm {
@@ -20,12 +19,6 @@ struct Steps {
   PlanePairs pairs;
   int parts;
 };
-
-// Whether a product is best cut into tiles of 256 x 256, a workgroup's work a compute unit: enough of them, and long enough sums.  Short ones wait for
-// their first fragments and for their stores one after the other, which two workgroups of 128 x 128 do in turns (32768 x 768 over 128 f16: 42 us, 35).
-inline bool wide_tiles(int64_t m, int64_t n, int64_t steps) {
-  return n > 64 && steps >= 12 && ((m + 255) / 256) * ((n + 255) / 256) >= 192;
-}
 
 #ifdef __HIPCC__
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -58,13 +51,11 @@ struct Cores<int8_t> {
   static __device__ __forceinline__ v16i mma(v4i a, v4i b, v16i c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
 };
 
-typedef __attribute__((address_space(3))) const void LdsVoid;
-
 // Sixteen bytes a lane from memory straight into LDS: lane l's from `base` (the first 48 bits of the descriptor) + at + k to lds + 16 l.
 // Written out so that the compiler does not wait for it at the next read of LDS, whichever stage that is of: stage_barrier says when what
 // is there.  It has no register to return to, and its address is taken when it is issued.
 __device__ __forceinline__ void request_into_lds(const char* lds, v4i base, uint32_t at, uint32_t k) {
-  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(LdsVoid*)lds);
+  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);   // (an address in LDS is the lower half of one in memory's space)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(base), "s"(k) : "m0");
 }
 // the descriptor of memory from p on; p is the same in all lanes
@@ -144,33 +135,33 @@ struct TileLoader {
   }
 };
 
-// The tile of workgroup blockIdx.x: each of the eight dies takes a run of tiles, four rows of b's tiles at a time, so that what its
-// workgroups read at one time meets in its cache
+// The tile of workgroup blockIdx.x, of a launch over whole rows of tiles from row `first` of b on: each of the eight dies takes a run of tiles,
+// four rows of b's tiles at a time, so that what its workgroups read at one time meets in its cache
 struct TileAt {
   int64_t m0, n0;
 };
 template <typename S>
-__device__ __forceinline__ TileAt tile_at(int64_t m, int64_t n) {
-  const int tiles_m = (int)((m + S::BM - 1) / S::BM), tiles_n = (int)((n + S::BN - 1) / S::BN);
+__device__ __forceinline__ TileAt tile_at(int64_t m, int64_t first) {
   const int all = gridDim.x, die = blockIdx.x % 8;
+  const int tiles_m = (int)((m + S::BM - 1) / S::BM), tiles_n = all / tiles_m;
   const int id = die * (all / 8) + min(die, all % 8) + blockIdx.x / 8;
   constexpr int kRows = 4;
   const int group = id / (kRows * tiles_m), in = id % (kRows * tiles_m);
   const int rows = min(kRows, tiles_n - group * kRows);
-  return {(int64_t)(in / rows) * S::BM, (int64_t)(group * kRows + in % rows) * S::BN};
+  return {(int64_t)(in / rows) * S::BM, first + (int64_t)(group * kRows + in % rows) * S::BN};
 }
 
-// Sums of the tile at (m0, n0), handed to done(sums, m, n, lds): sums[i][j] of the wave's rows m + 32 i of a and n + 32 j of b, and the
-// first stage's LDS for its own use (after a barrier).
+// Sums of the tile at (m0, n0), of a launch over rows of b from first_n on, handed to done(sums, m, n, lds): sums[i][j] of the wave's rows
+// m + 32 i of a and n + 32 j of b, and the first stage's LDS for its own use (after a barrier).
 //
 // Two stages of 128 bytes in LDS.  Fragments are read from LDS one step of 32 bytes ahead of their products, and the barrier at a stage's
 // end stands before its last products: they run while the next stage's first fragments are on their way.  A stage's memory
 // requests go out as soon as that barrier has freed its LDS, one stage ahead of their use.
 template <typename T, typename S, typename Done>
-__device__ __forceinline__ void product_tile(const Operand& a, const Operand& b, int64_t m, int64_t n, const Steps& steps, Done done) {
+__device__ __forceinline__ void product_tile(const Operand& a, const Operand& b, int64_t m, int64_t n, int64_t first_n, const Steps& steps, Done done) {
   __shared__ __attribute__((aligned(1024))) char s0[S::stage];
   __shared__ __attribute__((aligned(1024))) char s1[S::stage];
-  const TileAt tile = tile_at<S>(m, n);
+  const TileAt tile = tile_at<S>(m, first_n);
   const int part = blockIdx.y, first = (int)((int64_t)steps.count * part / steps.parts);
   const int count = (int)((int64_t)steps.count * (part + 1) / steps.parts) - first;
   TileLoader<S> from(a, b, tile.m0, tile.n0, m, n, first, count, steps.pairs);

@@ -672,3 +672,49 @@ def test_gradients_of_no_rows_through_the_c_entry(gpu, dtype):
                                          dw.data_ptr(), db.data_ptr(), None, 0, None))
     torch.cuda.synchronize()
     assert (dw[:C] == 0).all() and (db[:C] == 0).all() and (dw[C] == 7).all() and db[C] == 7
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_categories_than_a_launch_has_threads_for(gpu, dtype):
+    """2^28 categories in tiles of 32, a workgroup of 512 threads each, pass 2^32 threads; those behind weigh most"""
+    torch, P, R = gpu
+    C = (1 << 28) + 133
+    w = torch.empty(C, 1, dtype=getattr(torch, dtype), device="cuda").uniform_(-1, 0, generator=torch.Generator(device="cuda").manual_seed(41))
+    last = 300
+    w[C - last:] = torch.linspace(24, 30, last, device="cuda")[:, None].to(w.dtype)
+    f = torch.tensor([[1.0], [0.5], [-1.0]], device="cuda").to(w.dtype)
+    g = torch.tensor([[C - 1, C - 150], [C - last, 0], [1 << 28, C]], device="cuda")
+    got = P.linear_scores(f, w, g)
+    tail, z, chunk = w[C - last:], [], 1 << 24
+    for v in f:
+        part = [torch.logsumexp(w[i:i + chunk, 0].double() * v.double(), 0) for i in range(0, C, chunk)]
+        z.append(torch.logsumexp(torch.stack(part), 0))
+    z = torch.stack(z)
+    # of the sum: a lane adds (2^23 + 5) / 256 parts one after the other, and 32 exponentials of 2^-22 and some joins before and after
+    off = 2.0 ** -24 * ((1 << 15) + 200 + 4 * z.abs())
+    R.within(got.log_sum, z, off, "log_sum")
+    x = torch.cat([w[g.clamp(max=C - 1).reshape(-1), 0]]).double().view(3, 2) * f.double()
+    want = x - z[:, None]
+    want[2, 1] = float("nan")
+    R.within(got.logp, want, off[:, None] + 2.0 ** -22 * (x.abs() + z.abs()[:, None]), "logp")
+    assert float(torch.logsumexp(tail[:, 0].double(), 0) - z[0]) > -0.01     # (row 0: without them it would be another number)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_more_tiles_than_a_launch_has_threads_for(gpu, dtype):
+    """2^13 + 2 rows of tiles by 2^11 tiles of 256 threads: 64 rows of features again and again, every repetition the same"""
+    torch, P, R = gpu
+    n, k, C = (1 << 20) + 130, 64 if dtype == "bfloat16" else 8, 1 << 18
+    few, w, b, g, _, _ = _inputs(torch, dtype, 64, k, C, 42)
+    f = few.repeat(-(-n // 64), 1)[:n].contiguous()
+    given = g.repeat(-(-n // 64), 1)[:n].contiguous()
+    got = P.linear_scores(f, w, given, bias=b)
+    x = R.product(few, w) + b.double()
+    z = torch.logsumexp(x, 1)
+    size = R.product(few.abs(), w.abs()) + b.double().abs()
+    most = R.sum_bound(size, k, few.dtype).max(1).values + 2.0 ** -24 * (160 + 2048 / 16 + 4 * z.abs())
+    R.within(got.log_sum[:64], z, most, "log_sum")
+    lp = torch.where(g < 0, 0.0, x.gather(1, g.clamp(min=0)) - z[:, None])
+    R.within(got.logp[:64], lp, 2 * most[:, None] + 2.0 ** -22 * (lp.abs() + z.abs()[:, None]), "logp")
+    again = torch.arange(n, device="cuda") % 64
+    assert torch.equal(got.log_sum, got.log_sum[:64][again]) and torch.equal(got.logp, got.logp[:64][again])
