@@ -106,7 +106,7 @@ struct FewParts {                            // two chunks of a row, 64 bytes ap
       for (int q = 0; q < 3; ++q)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t two = pair_of<bf16>(w[2 * k], w[2 * k + 1]);
+          const uint32_t two = q ? pair_of<bf16>(w[2 * k], w[2 * k + 1]) : pair_of<bf16>(first_part(w[2 * k]), first_part(w[2 * k + 1]));
           p[q][k] = (int)two;
           if (q < 2) {
             w[2 * k] -= as_float(two << 16);

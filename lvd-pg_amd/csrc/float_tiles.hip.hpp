@@ -1,5 +1,6 @@
-// Products of float matrices on the matrix cores: each float as three bfloat16 parts, h + m + l, which hold all of its 24 bits, and the
-// six largest of the nine products of parts; what is left out (m l, l m, l l) is less than 2^-24 of the product.
+// Products of float matrices on the matrix cores: each float as three bfloat16 parts, h + m + l, which hold all of its 24 bits (from 2^-110 on;
+// smaller ones to 2^-134), and the six largest of the nine products of parts; what is left out (m l, l m, l l) is less than 2^-24 of the
+// product.  An infinity has no such parts: a product with one is NaN, as may be one that passes float's range.
 //
 // A tile's floats come through registers, are taken apart there (some six instructions an entry) and lie in LDS as three planes, from which all
 // six products are read: 12 fragments for 24 products of 32 x 32, so LDS is no bound, and the floats are read once, whatever
@@ -110,7 +111,8 @@ struct FloatLoader {
       char* const to = planes_of + (row + 64 * kHalf) * kFloatPitch + step * 2;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
-        const uint32_t a = pair_of<bf16>(w[0], w[1]), b = pair_of<bf16>(w[2], w[3]);
+        const uint32_t a = p ? pair_of<bf16>(w[0], w[1]) : pair_of<bf16>(first_part(w[0]), first_part(w[1]));
+        const uint32_t b = p ? pair_of<bf16>(w[2], w[3]) : pair_of<bf16>(first_part(w[2]), first_part(w[3]));
         *reinterpret_cast<uint2*>(to + p * kFloatPlane) = make_uint2(a, b);
         if (p < 2) w -= v4f{as_float(a << 16), as_float(a & 0xffff0000u), as_float(b << 16), as_float(b & 0xffff0000u)};
       }
@@ -122,7 +124,7 @@ struct FloatLoader {
         char* const to = planes_of + (row + e) * kFloatPitch + step * 2;
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
-          const uint32_t a = pair_of<bf16>(u, w);
+          const uint32_t a = p ? pair_of<bf16>(u, w) : pair_of<bf16>(first_part(u), first_part(w));
           *reinterpret_cast<uint32_t*>(to + p * kFloatPlane) = a;
           if (p < 2) {
             u -= as_float(a << 16);

@@ -21,6 +21,11 @@ struct Steps {
 };
 
 #ifdef __HIPCC__
+// The first of a float's three parts is its nearest bfloat16, but no infinity for a finite one: the second part has the rest (NaN comes back in it too)
+__device__ __forceinline__ float first_part(float x) {
+  constexpr float most = 0x1.fep127f;        // bfloat16's largest
+  return __builtin_amdgcn_fmed3f(x, -most, most);
+}
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));

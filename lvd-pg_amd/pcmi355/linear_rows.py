@@ -111,8 +111,8 @@ def linear_scores(features, weight, given=None, *, bias=None):
     given: uint8, int32 or int64, one category per row or [rows..., slots] with up to 64; a negative one was not observed and has
     log-probability 0, one past the categories NaN.  bias: [categories], any of the three types; at or below half of its type's lowest
     value it masks its category, whatever the weights hold.  A row of nothing but masks has log-sum and log-probabilities -inf, one with NaN or +inf
-    NaN.  float32 is taken as three bfloat16 parts whose six largest products are summed, which leaves out less than 2^-24 of a
-    product; all sums are held in 32 bits.  Returns `LinearScores`, numbers in float32."""
+    NaN (float32: with any infinity among its factors, or products past the type's range).  float32 is taken as three bfloat16 parts whose six largest
+    products are summed, which leaves out less than 2^-24 of a product, and what lies below 2^-134 of a factor; all sums are held in 32 bits.  Returns `LinearScores`, numbers in float32."""
     eight = _check_factors(features, weight)
     rows = tuple(features.shape[:-1])
     where = _check_given(given, rows)

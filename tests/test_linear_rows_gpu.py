@@ -718,3 +718,32 @@ def test_more_tiles_than_a_launch_has_threads_for(gpu, dtype):
     R.within(got.logp[:64], lp, 2 * most[:, None] + 2.0 ** -22 * (lp.abs() + z.abs()[:, None]), "logp")
     again = torch.arange(n, device="cuda") % 64
     assert torch.equal(got.log_sum, got.log_sum[:64][again]) and torch.equal(got.logp, got.logp[:64][again])
+
+
+@pytest.mark.parametrize("n", [3, 200])
+def test_floats_beyond_the_largest_of_16_bits(gpu, n):
+    """float32's finite entries past bfloat16's largest (3.39e38) are as good as any other: in scores, and in both gradients' sums"""
+    torch, P, R = gpu
+    big = torch.tensor([torch.finfo(torch.float32).max, 3.396e38, -3.4e38, 3.3895314e38, 1e38], device="cuda")
+    f = big.repeat(n)[:n, None] if n < 5 else big.repeat(n // 5)[:, None]
+    small = torch.tensor([[2.0 ** -100], [-1.7 * 2.0 ** -110], [1.3 * 2.0 ** -120]], device="cuda")
+    for w in small:                                    # one category: its score is the log-sum
+        for x, y in ((f, w[None]), (w[None].expand(n, 1), f[:1])):
+            got = P.linear_scores(x, y).log_sum.double()
+            want = x.double()[:, 0] * y.double()[0, 0]
+            # (and the small factor's third part ends at bfloat16's least number, 2^-133: up to half of it is left out, 2^-134 / |w| of the product)
+            assert float(((got - want) / want).abs().max()) < 2.0 ** -24 + 6 * 2.0 ** -23 + 2.0 ** -134 / float(w.abs())
+    # two categories of equal scores: dx is +-gl / 2
+    given, by = torch.zeros(n, dtype=torch.int64, device="cuda"), torch.full((n,), 2.0 ** -12, device="cuda")
+    zero, w = torch.zeros(n, 5, device="cuda"), torch.stack([big, big.flip(0)])
+    s = P.linear_scores(zero, w, given)
+    d = P.linear_scores_backward(zero, w, s.log_sum, given, grad_logp=by, of="features").features.double()
+    want = 2.0 ** -13 * (w[0].double() - w[1].double())
+    size = 2.0 ** -13 * w.double().abs().sum(0)
+    assert (((d - want).abs() - size * (2.0 ** -20 + 14 * 2.0 ** -23)) <= 0).all()     # (p: 2^-20 of it)
+    f, w = big.expand(n, 5).contiguous(), torch.zeros(2, 5, device="cuda")
+    s = P.linear_scores(f, w, given)
+    d = P.linear_scores_backward(f, w, s.log_sum, given, grad_logp=by / n, of="weight").weight.double()
+    want = 2.0 ** -13 * big.double()
+    size = want.abs() * (2.0 ** -20 + (6 * n + 8) * 2.0 ** -23)
+    assert ((d[0] - want).abs() <= size).all() and ((d[1] + want).abs() <= size).all()
