@@ -572,7 +572,8 @@ int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t nu
  *   relative to a power of two a row (float: three parts again; fewer than 1024 rows of 16 bits: two).  Features of half count in the weights' gradients down to 2^-25 of the largest
  *   |dx| of any row, as their type has no smaller numbers.  Sums have a fixed order: the same bits every time.
  * At most 2^22 rows, 2^30 categories, length 2^20.  d_work: so many bytes of device memory as the _workspace function of the same arguments says, 16-byte
- * aligned, which belong to the call until its work is done; `of`: 1 features, 2 weight, 4 bias, added.
+ * aligned, which belong to the call until its work is done; `of`: 1 features, 2 weight, 4 bias, added.  The gradient's: 5 GiB at most, beside 8 bytes for
+ * every entry of the features (their rows rounded up to 64 entries), 264 for a row and 4 for a category.
  *
  * Rows in 8-bit integers, for products of them (pcm_rows8): d_codes [rows][length rounded up to 128], zeros behind a row's end, 16-byte
  * aligned, and d_scales [rows].  Code rint(x (127 / a)) and scale a / 127, a the row's largest |x|, in 32 bits; a row whose a lies

@@ -337,7 +337,8 @@ struct Plan {
   bool of_float, few, lay_f, lay_w;
   int dx_planes;
   PlanePairs dx_pairs;
-  int64_t rows, cats, length, piece, pieces;
+  int64_t rows, cats, length, piece, pieces, part, parts;     // part: rows of one
+  bool features_direct, weight_direct;                        // whether a product gives them as they are
   int features_parts, weight_parts;
   int64_t of_p, expo, most, skip, f, f_turned, w, w_turned, by_row, by_cat, features, weight, bias, bytes;   // offsets
 
@@ -354,13 +355,17 @@ struct Plan {
     // categories, 2.3e-3 -> 1.6e-3 of the result (as rounding alone); the two products take twice the steps.
     dx_planes = !of_float && rows < kFewRows ? 2 : 1;
     dx_pairs = dx_planes == 2 ? kTwoOfB : kOnePlane;
-    // a piece's dx takes 2^26 entries or so, 4096 categories at least and 2^20 at most, in tiles of 256
-    const int64_t most_cats = std::min<int64_t>(kMaxLength, std::max<int64_t>(4096, ((int64_t)1 << 26) / std::max<int64_t>(rows, 1) / 256 * 256));
+    // (float's weights are read where they are)
+    const int64_t most_cats = most_piece(rows, length, !of_float);
     piece = cats <= most_cats ? cats : piece_for(most_cats);
     pieces = (cats + piece - 1) / piece;
-    const int64_t cat_steps = steps_of(piece), row_steps = steps_of(rows);
-    features_parts = (int)std::min<int64_t>(parts_for(length, rows, cat_steps * dx_pairs.count, of_float), cat_steps);
-    weight_parts = (int)std::min<int64_t>(parts_for(length, piece, row_steps * dx_pairs.count, of_float), std::max<int64_t>(1, row_steps));
+    part = part_rows(rows, fm.vars, piece);
+    parts = (rows + part - 1) / part;
+    const int64_t cat_steps = steps_of(piece), row_steps = steps_of(part);
+    features_parts = (int)std::min<int64_t>(parts_for(length, part, cat_steps * dx_pairs.count, of_float), cat_steps);
+    weight_parts = (int)std::min<int64_t>(parts_for(length, piece, row_steps * dx_pairs.count, of_float), row_steps);
+    features_direct = pieces == 1 && features_parts == 1;
+    weight_direct = parts == 1 && weight_parts == 1;
     int64_t at = 0;
     auto take = [&](bool needed, int64_t n) {
       const int64_t here = at;
@@ -375,11 +380,11 @@ struct Plan {
     f_turned = take(of_weight && !of_float, laid_bytes(length, rows, 1));
     w = take(lay_w, laid_bytes(piece, length, 1));
     w_turned = take(of_features && !of_float, laid_bytes(length, piece, 1));
-    by_row = take(of_float ? of_features || of_weight : of_features, of_float ? rows * round_up(piece, 4) * 4 : laid_bytes(rows, piece, dx_planes));
-    by_cat = take(of_weight && !of_float, laid_bytes(piece, rows, dx_planes));
-    features = take(of_features && (features_parts > 1 || pieces > 1), features_parts * rows * length * 4);
-    weight = take(of_weight && weight_parts > 1, weight_parts * piece * length * 4);
-    bias = take(of_bias, (rows + 31) / 32 * piece * 4);
+    by_row = take(of_float ? of_features || of_weight : of_features, of_float ? part * round_up(piece, 4) * 4 : laid_bytes(part, piece, dx_planes));
+    by_cat = take(of_weight && !of_float, laid_bytes(piece, part, dx_planes));
+    features = take(of_features && !features_direct, features_parts * rows * length * 4);
+    weight = take(of_weight && !weight_direct, weight_parts * piece * length * 4);
+    bias = take(of_bias, (rows + 63) / 64 * piece * 4);       // (tiles have 64 rows or more, if there are as many)
     bytes = at;
   }
   // The size of pieces, of at most `most` categories: the one whose tiles take the fewest turns of the compute units (256 tiles of 256 x 256, or 512 of
@@ -439,8 +444,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
   if (out.weight && !of_float) lay_out(f, 0, rows, true, scaled, work + plan.f_turned, stream);
   LayOut masked;
   masked.mask = bias;
-  const int64_t turned_f = laid_length(rows);
-  const bool features_direct = plan.pieces == 1 && plan.features_parts == 1;
+  const int64_t all_turned = laid_length(rows), index_bytes = given.type == PCM_U8 ? 1 : given.type == PCM_I32 ? 4 : 8;
   for (int64_t first = 0; first < cats; first += plan.piece) {
     const int64_t count = std::min(plan.piece, cats - first), laid = laid_length(count), pitch = of_float ? round_up(count, 4) : laid;
     Matrix2 of_piece = w;
@@ -449,7 +453,6 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     GradientTask t{};
     if (!plan.few && of_float) {
       t.fw = float_operand(of_piece, false);
-      t.ff = float_operand(f, false);
       t.fk = f.length;
     } else if (plan.lay_w) {
       lay_out(w, first, count, false, LayOut(), work + plan.w, stream);
@@ -457,91 +460,104 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     } else if (!plan.few) {
       t.w = {of_piece.p, w.stride_ex * 2, 0};
     }
-    t.f = features;
     t.cats = count;
-    t.rows = rows;
     t.steps = {(int)(laid_length(f.length) * 2 / kKBytes), kOnePlane, 1};
     t.bias = bias;
     if (t.bias.p) t.bias.p = static_cast<const char*>(bias.p) + first * (bias.type == PCM_F32 ? 4 : 2);
     t.given = given;
     t.first_cat = first;
-    t.grad_logp = d_grad_logp;
-    t.log_sum = d_log_sum;
-    t.of_p = of_p;
-    t.expo = expo;
     t.pitch_row = pitch;
-    t.pitch_cat = turned_f;
-    t.plane_row = rows * laid;
-    t.plane_cat = count * turned_f;
     if (of_float) t.dx = out.features || out.weight ? reinterpret_cast<float*>(work + plan.by_row) : nullptr;
     else t.by_row = out.features ? reinterpret_cast<uint16_t*>(work + plan.by_row) : nullptr;
     t.by_cat = out.weight && !of_float ? reinterpret_cast<uint16_t*>(work + plan.by_cat) : nullptr;
-    t.bias_parts = out.bias ? reinterpret_cast<float*>(work + plan.bias) : nullptr;
-    if (plan.few) {
-      const FewOperand fw = few_operand(of_piece), ff = few_operand(f);
-      if (of_float) launch_few<float>(t, fw, ff, f.length, stream);
-      else if (f.type == PCM_BF16) launch_few<bf16>(t, fw, ff, f.length, stream);
-      else launch_few<f16>(t, fw, ff, f.length, stream);
-    } else if (of_float) launch<float, FloatTile, 1>(t, stream);
-    else if (f.type == PCM_BF16) plan.dx_planes == 2 ? launch<bf16, 2>(t, stream) : launch<bf16, 1>(t, stream);
-    else plan.dx_planes == 2 ? launch<f16, 2>(t, stream) : launch<f16, 1>(t, stream);
-    if (out.bias) {
-      const int64_t each = plan.few ? kFewRowsMost : tile_rows(count, rows, t.steps.count, of_float);
-      hipLaunchKernelGGL(join_bias_kernel, dim3((unsigned)((count + 31) / 32)), dim3(256), 0, stream, t.bias_parts, (rows + each - 1) / each, count,
-                         out.bias, bias.type, first);
-    }
-    const Matrix2 dx{t.dx, PCM_F32, pitch, 0, 1, rows, 1, (int32_t)count};
-    if (out.features) {
-      OutTask o{};
-      if (of_float) {
-        o.fa = float_operand(of_piece, true, skip ? skip + first : nullptr);
-        o.fb = float_operand(dx, false);
-        o.fk = count;
-      } else {
-        lay_out(w, first, count, true, masked, work + plan.w_turned, stream);
-        o.a = {work + plan.w_turned, laid * 2, 0};
-        o.b = {t.by_row, laid * 2, t.plane_row * 2};
-        o.finish.expo = expo;
+    int64_t bias_tiles = 0;
+    for (int64_t row = 0; row < rows; row += plan.part) {
+      const int64_t n = std::min(plan.part, rows - row), example = row / f.vars, turned = laid_length(n);
+      Matrix2 of_rows = f;
+      of_rows.p = static_cast<const char*>(f.p) + example * f.stride_ex * size;
+      of_rows.examples = n / f.vars;
+      if (!plan.few && of_float) t.ff = float_operand(of_rows, false);
+      t.f = features;
+      if (features.p) t.f.p = static_cast<const char*>(features.p) + row * features.pitch;
+      t.rows = n;
+      if (given.p) t.given.p = static_cast<const char*>(given.p) + example * given.stride_ex * index_bytes;
+      t.grad_logp = d_grad_logp + row * given.slots;
+      t.log_sum = d_log_sum + row;
+      t.of_p = of_p + row;
+      t.expo = expo + row;
+      t.pitch_cat = turned;
+      t.plane_row = n * laid;
+      t.plane_cat = count * turned;
+      t.bias_parts = out.bias ? reinterpret_cast<float*>(work + plan.bias) + bias_tiles * count : nullptr;
+      if (plan.few) {
+        const FewOperand fw = few_operand(of_piece), ff = few_operand(of_rows);
+        if (of_float) launch_few<float>(t, fw, ff, f.length, stream);
+        else if (f.type == PCM_BF16) launch_few<bf16>(t, fw, ff, f.length, stream);
+        else launch_few<f16>(t, fw, ff, f.length, stream);
+      } else if (of_float) launch<float, FloatTile, 1>(t, stream);
+      else if (f.type == PCM_BF16) plan.dx_planes == 2 ? launch<bf16, 2>(t, stream) : launch<bf16, 1>(t, stream);
+      else plan.dx_planes == 2 ? launch<f16, 2>(t, stream) : launch<f16, 1>(t, stream);
+      const int64_t bias_rows = plan.few ? kFewRowsMost : tile_rows(count, n, t.steps.count, of_float);
+      bias_tiles += (n + bias_rows - 1) / bias_rows;
+      const Matrix2 dx{t.dx, PCM_F32, pitch, 0, 1, n, 1, (int32_t)count};
+      if (out.features) {
+        OutTask o{};
+        if (of_float) {
+          o.fa = float_operand(of_piece, true, skip ? skip + first : nullptr);
+          o.fb = float_operand(dx, false);
+          o.fk = count;
+        } else {
+          if (!row) lay_out(w, first, count, true, masked, work + plan.w_turned, stream);
+          o.a = {work + plan.w_turned, laid * 2, 0};
+          o.b = {t.by_row, laid * 2, t.plane_row * 2};
+          o.finish.expo = t.expo;
+        }
+        o.m = f.length;
+        o.n = n;
+        o.steps = {(int)(laid * 2 / kKBytes), plan.dx_pairs, (int)std::min(plan.steps_of(count), (int64_t)plan.features_parts)};
+        o.out = plan.features_direct ? static_cast<char*>(out.features) + row * f.length * size : work + plan.features + plan.features_parts * row * f.length * 4;
+        o.type = plan.features_direct ? f.type : kRawSums;
+        o.pitch = f.length;
+        o.add = first > 0;
+        o.finish.dead = t.expo;
+        short_sums(f.type, o) ? product_short(f.type, o, stream) : product_out(f.type, o, stream);
       }
-      o.m = f.length;
-      o.n = rows;
-      o.steps = {(int)(laid * 2 / kKBytes), plan.dx_pairs, (int)std::min(plan.steps_of(count), (int64_t)plan.features_parts)};
-      o.out = features_direct ? out.features : work + plan.features;
-      o.type = features_direct ? f.type : kRawSums;
-      o.pitch = f.length;
-      o.add = first > 0;
-      o.finish.dead = expo;
-      short_sums(f.type, o) ? product_short(f.type, o, stream) : product_out(f.type, o, stream);
-    }
-    if (out.weight) {
-      OutTask o{};
-      if (of_float) {
-        o.fa = float_operand(f, true, expo);
-        o.fb = float_operand(dx, true);
-        o.fk = rows;
-      } else {
-        o.a = {work + plan.f_turned, turned_f * 2, 0};
-        o.b = {t.by_cat, turned_f * 2, t.plane_cat * 2};
-        o.finish.most = most;
+      if (out.weight) {
+        OutTask o{};
+        if (of_float) {
+          o.fa = float_operand(of_rows, true, t.expo);
+          o.fb = float_operand(dx, true);
+          o.fk = n;
+        } else {
+          o.a = {work + plan.f_turned + row * 2, all_turned * 2, 0};
+          o.b = {t.by_cat, turned * 2, t.plane_cat * 2};
+          o.finish.most = most;
+        }
+        o.m = f.length;
+        o.n = count;
+        o.steps = {(int)(turned * 2 / kKBytes), plan.dx_pairs, (int)std::min(plan.steps_of(n), (int64_t)plan.weight_parts)};
+        o.pitch = f.length;
+        char* const to = static_cast<char*>(out.weight) + first * f.length * size;
+        o.out = plan.weight_direct ? to : work + plan.weight;
+        o.type = plan.weight_direct ? f.type : kRawSums;
+        o.add = row > 0;
+        short_sums(f.type, o) ? product_short(f.type, o, stream) : product_out(f.type, o, stream);
+        // (a last part of fewer steps than parts of the sum leaves some of them as the rows before it did; so does a last piece below)
+        if (!plan.weight_direct && row + n == rows) join_parts(o.out, plan.weight_parts, false, o.m, o.n, o.finish, to, f.type, f.length, stream);
       }
-      o.m = f.length;
-      o.n = count;
-      o.steps = {(int)(turned_f * 2 / kKBytes), plan.dx_pairs, plan.weight_parts};
-      o.pitch = f.length;
-      char* const to = static_cast<char*>(out.weight) + first * f.length * size;
-      o.out = plan.weight_parts > 1 ? work + plan.weight : to;
-      o.type = plan.weight_parts > 1 ? kRawSums : f.type;
-      short_sums(f.type, o) ? product_short(f.type, o, stream) : product_out(f.type, o, stream);
-      if (plan.weight_parts > 1) join_parts(o.out, plan.weight_parts, false, o.m, o.n, o.finish, to, f.type, f.length, stream);
     }
+    if (out.bias)
+      hipLaunchKernelGGL(join_bias_kernel, dim3((unsigned)((count + 31) / 32)), dim3(256), 0, stream, reinterpret_cast<float*>(work + plan.bias), bias_tiles,
+                         count, out.bias, bias.type, first);
   }
-  if (out.features && !features_direct) {
-    Finish finish;
-    finish.dead = expo;
-    if (!of_float) finish.expo = expo;
-    // (a last piece of fewer steps than parts leaves some of them as the pieces before it did)
-    join_parts(work + plan.features, plan.features_parts, false, f.length, rows, finish, out.features, f.type, f.length, stream);
-  }
+  if (out.features && !plan.features_direct)
+    for (int64_t row = 0; row < rows; row += plan.part) {
+      Finish finish;
+      finish.dead = expo + row;
+      if (!of_float) finish.expo = expo + row;
+      join_parts(work + plan.features + plan.features_parts * row * f.length * 4, plan.features_parts, false, f.length, std::min(plan.part, rows - row), finish,
+                 static_cast<char*>(out.features) + row * f.length * size, f.type, f.length, stream);
+    }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) fail(PCM_ERR_HIP, "launch of linear_scores_backward failed: %s", hipGetErrorString(e));
 }

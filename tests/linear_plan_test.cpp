@@ -19,5 +19,20 @@ int main() {
       }
   std::printf("tiles_none %d\ntiles_past %d\ntiles_several %d\n", none, past, several);
   std::printf("few_512 %lld\nfew_256 %lld\n", (long long)units_a_launch(1, 512), (long long)units_a_launch(1, 256));
+  // pieces of the categories and parts of the rows
+  int uneven = 0, large = 0, many = 0;
+  for (int64_t rows = 1; rows <= (int64_t)1 << 22; rows += rows < 100 ? 1 : rows / 3)
+    for (int64_t vars : {1, 3, 64, 100, 1000})
+      for (int64_t length = 1; length <= (int64_t)1 << 20; length *= 4)
+        for (bool laid : {false, true}) {
+          if (rows % vars) continue;
+          const int64_t piece = most_piece(rows, length, laid), part = part_rows(rows, vars, piece);
+          uneven += piece < 256 || piece % 256 || part < 1 || part > rows || part % vars || (part < rows && part % 64);
+          large += part * piece > kMostDerivatives && part > 64 * vars;
+          large += laid && piece * length > (int64_t)1 << 30 && piece > 256;
+          large += part < rows && piece * length > (int64_t)1 << 28 && piece > 256;
+          many += part < rows;
+        }
+  std::printf("pieces_uneven %d\npieces_large %d\npieces_parts %d\n", uneven, large, many);
   std::printf("few_past %d\n", units_a_launch(1, 512) * 512 >= (int64_t)1 << 32 || units_a_launch(1, 256) * 256 >= (int64_t)1 << 32);
 }

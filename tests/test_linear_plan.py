@@ -20,3 +20,7 @@ def test_no_launch_has_two_to_the_32_threads(got):
     assert got["tiles_none"] == 0 and got["tiles_past"] == 0 and got["few_past"] == 0
     assert got["tiles_several"] > 0                    # (there are sizes that take several)
     assert got["few_512"] == 2 ** 23 - 1 and got["few_256"] == 2 ** 24 - 1
+
+
+def test_pieces_and_parts_have_bounds(got):
+    assert got["pieces_uneven"] == 0 and got["pieces_large"] == 0 and got["pieces_parts"] > 0

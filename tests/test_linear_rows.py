@@ -224,3 +224,17 @@ def test_a_gradient_of_no_rows_needs_nothing(type_):
                                               None, None, 0, None) == 0
     assert lib.pcm_linear_scores_backward(p, p, type_, 8, 0, 1, 8, 1, 0, 1, 0, 10, None, 0, None, 5, 0, 0, 0, 0, None, None, None, None, None, None,
                                           None, 0, None) == -2           # (what is refused with rows is refused without)
+
+
+@pytest.mark.parametrize("type_", [0, 1, 2])
+def test_the_gradients_workspace_has_a_bound(type_):
+    """5 GiB beside the features turned and summed, whatever the number of categories, of rows and of entries"""
+    from pcmi355._lib import lib
+    p = 1 << 20
+    for n in (1, 2, 40, 64, 65, 1000, 1023, 1024, 4096, 16500, 65536, 65537, 100000, 1 << 18, 1 << 20, 1 << 22):
+        for k in (1, 3, 64, 65, 768, 4096, 8192, 16384, 100000, 1 << 20):
+            for c in (2, 300, 4096, 4097, 50304, 140000, 1 << 20, 1 << 24, 1 << 30):
+                for inner in (1, 2):                                     # (2: both are laid out)
+                    for v in (1, 32) if n % 32 == 0 else (1,):
+                        need = lib.pcm_linear_scores_backward_workspace(p, p, type_, k * inner * v, k * inner, inner, k * inner, inner, n // v, v, k, c, 7)
+                        assert 0 < need <= (5 << 30) + n * (8 * (k + 63) + 264) + 4 * c, (n, k, c, inner, v, need)

@@ -747,3 +747,40 @@ def test_floats_beyond_the_largest_of_16_bits(gpu, n):
     want = 2.0 ** -13 * big.double()
     size = want.abs() * (2.0 ** -20 + (6 * n + 8) * 2.0 ** -23)
     assert ((d[0] - want).abs() <= size).all() and ((d[1] + want).abs() <= size).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,v", [((140001, 24, 4200), 1), ((140001, 40, 4097), 3), ((262200, 8, 2100), 1)], ids=lambda s: "x".join(map(str, s)) if isinstance(s, tuple) else str(s))
+def test_gradients_in_parts_of_the_rows(gpu, dtype, shape, v):
+    """So many rows that a piece's derivatives are taken in parts: 2^29 of them and what is left, or whole examples"""
+    torch, P, R = gpu
+    f, w, b, g, gl, gz = _inputs(torch, dtype, *shape, 43, bias="masked", slots=2)
+    n = shape[0]
+    g[n - 40:], gz[n - 40:] = -1, 0.0                                       # a padded end, in the last part
+    g[131000:131150, 0] = shape[2] - 1                                      # the same category on both sides of a border
+    b[-1] = 0.5
+    s = R.Scores(f, w, b)
+    rows = (n // v, v) if v > 1 else (n,)
+    if v > 1:
+        f = f.view(n // v, v, -1).transpose(0, 1).contiguous().transpose(0, 1)
+    shaped = lambda t: t.view(*rows, 2)
+    got = P.linear_scores(f, w, shaped(g).to(torch.int32), bias=b)
+    R.within(got.log_sum.reshape(-1), s.log_sum, s.log_sum_off, "log_sum")
+    flat = f.reshape(n, -1).clone()
+    f[-1] = float("nan")                                                    # (rows of the padded end)
+    d = P.linear_scores_backward(f, w, got.log_sum, shaped(g).to(torch.int32), bias=b, grad_logp=shaped(gl), grad_log_sum=gz.view(rows))
+    want = R.gradients(flat, w, b, s, g, gl, gz)
+    R.within(d.features.reshape(n, -1), *want["features"], "features")
+    R.within(d.weight, *want["weight"], "weight")
+    R.within(d.bias, *want["bias"], "bias")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_gradients_in_pieces_of_long_weights(gpu, dtype):
+    """Few rows, and weights of more than 2^30 entries: pieces of the categories"""
+    torch, P, R = gpu
+    f, w, b, g, gl, gz = _inputs(torch, dtype, 3, 8200, 131100, 44, bias="masked", slots=2)
+    g[:, 0] = 131099 - torch.arange(3, device="cuda")
+    b[-3:] = 0.5
+    s, got = _check_scores(R, P, f, w, b, g)
+    _check_grads(R, P, f, w, b, s, got, g, gl, gz)
