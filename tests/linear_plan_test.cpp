@@ -1,11 +1,15 @@
 // Host test of csrc/linear_plan.hpp: how the work of scores from features and weights is cut.  Prints one line per case: "<name> <value>".
+// With arguments m n steps: whether such a product goes by tiles of 256 x 256.  With rows length: the most categories of a piece.
 #include <cstdio>
+#include <cstdlib>
 
 #include "linear_plan.hpp"
 
 using namespace pcm;
 
-int main() {
+int main(int argc, char** argv) {
+  if (argc == 4) return std::printf("wide %d\n", wide_tiles(std::atoll(argv[1]), std::atoll(argv[2]), std::atoll(argv[3]))), 0;
+  if (argc == 3) return std::printf("piece %lld\n", (long long)most_piece(std::atoll(argv[1]), std::atoll(argv[2]), true)), 0;
   // launches over rows of tiles, and over tiles of 32 categories, at the largest sizes that the entry points take and at powers of two below
   const struct { int64_t bm, bn; int threads; } tiles[] = {{256, 256, 512}, {128, 128, 256}, {128, 64, 256}, {128, 32, 256}};
   int none = 0, past = 0, several = 0;

@@ -4,6 +4,12 @@ steps round or cut off, is off by K 2^-23 of the sum of the products' sizes; flo
 at most and sums six times as many."""
 import torch
 
+# (rows, length, categories) at which products of 16-bit types go by tiles of 256 x 256, and which do: scores and dx, the features' gradient and the
+# weights' (with pieces of the categories: of how many); fewer than 1024 rows have dx in two parts
+WIDE = [((3501, 800, 4001), ("scores",), 1), ((3501, 3590, 4001), ("scores", "features", "weight"), 1), ((16500, 770, 9100), ("scores", "features"), 3),
+        ((1001, 12500, 800), ("features", "weight"), 1), ((1001, 800, 12500), ("scores",), 1)]
+WIDE8 = [(3601, 1601, 4001), (3584, 1664, 4096)]      # of 8-bit rows
+
 LEAST = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
 
 

@@ -784,3 +784,43 @@ def test_gradients_in_pieces_of_long_weights(gpu, dtype):
     b[-3:] = 0.5
     s, got = _check_scores(R, P, f, w, b, g)
     _check_grads(R, P, f, w, b, s, got, g, gl, gz)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("at", range(5))
+def test_tiles_of_256(gpu, dtype, at):
+    """Sizes that the host test of the rule holds to be cut into tiles of 256 x 256: odd borders, masks, several slots, padded rows"""
+    torch, P, R = gpu
+    assert len(R.WIDE) == 5
+    shape = R.WIDE[at][0]
+    f, w, b, g, gl, gz = _inputs(torch, dtype, *shape, 45, bias="masked", slots=2)
+    g[:, 0] = shape[2] - 1 - torch.arange(shape[0], device="cuda") % 7      # categories of the last tile
+    b[-7:] = 0.5
+    g[-20:], gz[-20:] = -1, 0.0
+    s, got = _check_scores(R, P, f, w, b, g)
+    _check_grads(R, P, f, w, b, s, got, g, gl, gz)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("at", range(2))
+def test_tiles_of_256_of_eight_bits(gpu, dtype, at):
+    torch, P, R = gpu
+    assert len(R.WIDE8) == 2
+    n, k, C = R.WIDE8[at]
+    f, w, b, g, _, _ = _inputs(torch, dtype, n, k, C, 46, bias="masked", slots=3)
+    a, c = P.rows8(f), P.rows8(w)
+    whole = _exact_product(torch, R, a, c, k)
+    x = whole * a.scales.double()[:, None] * c.scales.double()
+    seen = torch.where(R.masked(b), torch.zeros_like(b), b)
+    v = x + seen.double()
+    R.within(P.product8(a, c, bias=seen), v, 4 * 2.0 ** -24 * (x.abs() + v.abs()) + R.half_step(f.dtype) * v.abs() * 1.001 + R.LEAST[f.dtype], "product")
+    assert torch.equal(P.product8(a, c, dtype=torch.float32), whole.float() * a.scales[:, None] * c.scales)
+    off = 4 * 2.0 ** -24 * x.abs() + 2.0 ** -24 * v.abs()
+    v[:, R.masked(b)] = -float("inf")
+    off[:, R.masked(b)] = 0.0
+    z = torch.logsumexp(v, 1)
+    most = off.max(1).values + 2.0 ** -24 * (160 + 4 * z.abs())
+    got = P.linear_scores(a, c, g, bias=b)
+    R.within(got.log_sum, z, most, "log_sum")
+    lp = torch.where(g < 0, 0.0, v.gather(1, g.clamp(min=0)) - z[:, None])
+    R.within(got.logp, lp, 2 * most[:, None] + 2.0 ** -22 * lp.abs().nan_to_num(posinf=0.0), "logp")
