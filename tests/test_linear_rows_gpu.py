@@ -824,3 +824,34 @@ def test_tiles_of_256_of_eight_bits(gpu, dtype, at):
     R.within(got.log_sum, z, most, "log_sum")
     lp = torch.where(g < 0, 0.0, v.gather(1, g.clamp(min=0)) - z[:, None])
     R.within(got.logp, lp, 2 * most[:, None] + 2.0 ** -22 * lp.abs().nan_to_num(posinf=0.0), "logp")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,cut", [((50, 96, 301), 100), ((1100, 64, 700), 256)], ids=["few", "many"])
+def test_shards_of_the_categories(gpu, dtype, shape, cut):
+    """Two shards' log-sums join by their log-sum, log-probabilities are the scores less the joined one, and each shard's gradients come from it: a slot
+    whose category the other shard has is negative, its derivative goes from grad_log_sum"""
+    torch, P, R = gpu
+    f, w, b, g, gl, gz = _inputs(torch, dtype, *shape, 47, bias="masked", slots=3)
+    s = R.Scores(f, w, b)
+    parts = ((0, cut), (cut, shape[2]))
+    own = [torch.where((g >= lo) & (g < hi), g - lo, -1) for lo, hi in parts]
+    each = [P.linear_scores(f, w[lo:hi], o, bias=b[lo:hi]) for (lo, hi), o in zip(parts, own)]
+    z = torch.logsumexp(torch.stack([e.log_sum.double() for e in each]), 0).float()
+    s.log_sum_off = s.log_sum_off + 2.0 ** -24 * s.log_sum.abs()            # (the joined one is rounded once more)
+    R.within(z, s.log_sum, s.log_sum_off, "log_sum")
+    lp = sum(torch.where(o < 0, 0.0, (e.logp.double() + e.log_sum.double()[:, None] - z.double()[:, None])) for o, e in zip(own, each))
+    v, off = s.logp(g)
+    R.within(lp, v, off + sum(e.log_sum.abs().double()[:, None] for e in each) * 2.0 ** -22, "logp")
+    want = R.gradients(f, w, b, s, g, gl, gz)
+    dx = R.dx_of(s, g, gl, gz)[0]
+    got, sizes = [], torch.zeros(shape[0], shape[1], dtype=torch.float64, device="cuda")
+    for (lo, hi), o in zip(parts, own):
+        other = torch.where((g >= 0) & (o < 0), gl, 0.0).sum(1)
+        got.append(P.linear_scores_backward(f, w[lo:hi], z, o, bias=b[lo:hi], grad_logp=gl, grad_log_sum=gz - other))
+        seen = torch.where(R.masked(b[lo:hi])[:, None], torch.zeros_like(w[lo:hi]), w[lo:hi])
+        sizes += R.product(dx[:, lo:hi], seen.t().contiguous()).abs()
+    # (gz less a slot's derivative is rounded once: 2^-24 of the row's size, of which p is a part at most)
+    R.within(sum(d.features.double() for d in got), want["features"][0], want["features"][1] * 1.01 + R.half_step(f.dtype) * sizes + R.LEAST[f.dtype], "features")
+    R.within(torch.cat([d.weight for d in got]), *want["weight"], "weight")
+    R.within(torch.cat([d.bias for d in got]), *want["bias"], "bias")
