@@ -18,7 +18,7 @@ __device__ __forceinline__ int row_scale(const LayOut& with, const Matrix2& x, i
   if (with.mask.p && bias_at(with.mask, row, x.examples) == -INFINITY) return kDeadRow;
   if (!with.expo) return 0;
   const int e = with.expo[row];
-  return e == kDeadRow ? e : max(e - largest, -300);
+  return e == kDeadRow ? e : with.most ? max(e - largest, -300) : 0;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t scaled_pair(uint32_t v, int by) {
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void turn_rows_kernel(Matrix2 x, int64_t first
   __shared__ __attribute__((aligned(8))) char tile[kTile * kPitch];   // [entry][row]
   const int64_t r0 = (int64_t)blockIdx.x * kTile;
   const int c0 = blockIdx.y * kTile, block = threadIdx.x / 16 * 4, c = c0 + threadIdx.x % 16 * 4;
-  const int largest = with.expo ? largest_exponent(with.most) : 0;
+  const int largest = with.most ? largest_exponent(with.most) : 0;
   uint32_t a[4], b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void lay_out_kernel(Matrix2 x, int64_t first, 
   const int64_t r0 = (int64_t)blockIdx.x * kTile;
   const int c0 = blockIdx.y * kTile;
   const int t = threadIdx.x;
-  const int largest = with.expo ? largest_exponent(with.most) : 0;
+  const int largest = with.most ? largest_exponent(with.most) : 0;
   if (t < kTile) by[t] = r0 + t < count ? row_scale(with, x, first + r0 + t, largest) : 0;
   const T* const from = static_cast<const T*>(x.p);
 #pragma unroll

@@ -3,10 +3,10 @@
 //   dx[n][c] = sum_j gl[n][j] [c = g_j] - (sum_j gl[n][j] - gz[n]) p[n][c],  p = exp(x - Z)
 //   features: dx w, weights: dx^T f, bias: sum_n dx
 // The categories are taken in pieces: the scores of a piece once more (gradient_kernel), whose dx goes into the workspace in both
-// orders, rounded to the operands' 16 bits (fewer than 1024 rows: in two parts; float: as it is, in one order), then the piece's two products.  dx is held as dx 2^(15 - e[n]),
-// 2^e[n] the next power of two above what |dx| of the row can be, so that half's range holds it whatever the loss's scale; features are
-// turned with 2^(e[n] - largest e) for the sum over rows, which is exact down to the type's least normal number (half: what lies below
-// 2^-14 after it is off by 2^-25 at most).
+// orders, rounded to the operands' 16 bits (fewer than 1024 rows: in two parts; float: as it is, in one order), then the piece's two products.
+// Half's dx is held as dx 2^(15 - e[n]), 2^e[n] the next power of two above what |dx| of the row can be, so that its range holds it whatever the
+// loss's scale; its features are turned with 2^(e[n] - largest e) for the sum over rows, which is exact down to the type's least normal
+// number (what lies below 2^-14 after it is off by 2^-25 at most).
 //
 // Bound by the matrix cores where sums are long: 4096 rows of 4096 bf16, a piece of 16384 categories: the scores and dx 500 us (1.10
 // PFLOP/s; the scores alone go at 1.23), either product 460 to 480.  Few rows are bound by reading the weights twice and writing their gradients.
@@ -63,6 +63,11 @@ struct GradientTask : ScoreInputs {   // of a piece of the categories
   float* bias_parts;                 // [tile of rows][category of the piece]; null: none
 };
 
+// What dx of a row with exponent e is multiplied by on its way to the operands, 0 for a row without a gradient: only half's range needs it (bfloat16 has
+// float's, and sums of scaled ones would leave that where weights or features are large)
+template <typename T>
+__device__ __forceinline__ float scale_of(int e) { return e == kDeadRow ? 0.f : __is_same(T, f16) ? ldexpf(1.f, 15 - e) : 1.f; }
+
 // Numbers as the operands hold them, two to a word: the nearest ones, and with kParts > 1 the nearest ones to what is left
 template <typename T, int kParts>
 struct Coded {
@@ -108,8 +113,7 @@ __device__ __forceinline__ void gradient_tile(const GradientTask& t) {
       float dx[S::FM][16];
       scores_of<S>(sums, j, 1.f, bias + wm, scale + wm, half, dx);
       const float z = t.log_sum[at], of_p = t.of_p[at];
-      const int e = valid ? t.expo[at] : kDeadRow;
-      const float by = e == kDeadRow ? 0.f : __is_same(T, float) ? 1.f : ldexpf(1.f, 15 - e);
+      const float by = scale_of<T>(valid ? t.expo[at] : kDeadRow);
 #pragma unroll
       for (int i = 0; i < S::FM; ++i)
 #pragma unroll
@@ -257,8 +261,7 @@ __global__ __launch_bounds__(FewTile<kGroups>::threads) void gradient_few_kernel
       for (int i = threadIdx.x; i < S::longs / 2 * S::rows; i += S::threads) {
         const int c = i % (S::longs / 2) * 2, r = i / (S::longs / 2);
         if (n0 + r >= t.rows || c0 + c >= t.pitch_row) continue;
-        const int er = t.expo[n0 + r];
-        const float by = er == kDeadRow ? 0.f : ldexpf(1.f, 15 - er);
+        const float by = scale_of<T>(t.expo[n0 + r]);
         const Coded<T, 2> two(dx[c * S::pitch + r] * by, dx[(c + 1) * S::pitch + r] * by);
 #pragma unroll
         for (int part = 0; part < 2; ++part) *reinterpret_cast<uint32_t*>(t.by_row + part * t.plane_row + (n0 + r) * t.pitch_row + c0 + c) = two.p[part];
@@ -270,8 +273,8 @@ __global__ __launch_bounds__(FewTile<kGroups>::threads) void gradient_few_kernel
         float v[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int er = n0 + r + k < t.rows ? t.expo[n0 + r + k] : kDeadRow;
-          v[k] = er == kDeadRow ? 0.f : dx[c * S::pitch + (r + k < S::rows ? r + k : 0)] * ldexpf(1.f, 15 - er);
+          const float by = scale_of<T>(n0 + r + k < t.rows ? t.expo[n0 + r + k] : kDeadRow);
+          v[k] = by == 0.f ? 0.f : dx[c * S::pitch + (r + k < S::rows ? r + k : 0)] * by;
         }
         const Coded<T, 2> two(v[0], v[1]);
 #pragma unroll
@@ -432,7 +435,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
   float* const of_p = reinterpret_cast<float*>(work + plan.of_p);
   int *const expo = reinterpret_cast<int*>(work + plan.expo), *const most = reinterpret_cast<int*>(work + plan.most);
   hipLaunchKernelGGL(row_terms_kernel, dim3(kMostBlocks), dim3(256), 0, stream, given, d_grad_logp, d_grad_log_sum, d_log_sum, rows, cats, of_p, expo, most);
-  const bool of_float = plan.of_float;
+  const bool of_float = plan.of_float, of_half = f.type == PCM_F16;
   const int size = of_float ? 4 : 2;
   int* const skip = of_float && out.features && bias.p ? reinterpret_cast<int*>(work + plan.skip) : nullptr;
   if (skip) hipLaunchKernelGGL(masked_kernel, dim3((unsigned)((cats + 255) / 256)), dim3(256), 0, stream, bias, cats, skip);
@@ -440,7 +443,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
   const Operand features = of_float || plan.few ? Operand{} : operand_of(f, at, stream);
   LayOut scaled;
   scaled.expo = expo;
-  scaled.most = most;
+  if (of_half) scaled.most = most;
   if (out.weight && !of_float) lay_out(f, 0, rows, true, scaled, work + plan.f_turned, stream);
   LayOut masked;
   masked.mask = bias;
@@ -510,7 +513,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
           if (!row) lay_out(w, first, count, true, masked, work + plan.w_turned, stream);
           o.a = {work + plan.w_turned, laid * 2, 0};
           o.b = {t.by_row, laid * 2, t.plane_row * 2};
-          o.finish.expo = t.expo;
+          if (of_half) o.finish.expo = t.expo;
         }
         o.m = f.length;
         o.n = n;
@@ -531,7 +534,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
         } else {
           o.a = {work + plan.f_turned + row * 2, all_turned * 2, 0};
           o.b = {t.by_cat, turned * 2, t.plane_cat * 2};
-          o.finish.most = most;
+          if (of_half) o.finish.most = most;
         }
         o.m = f.length;
         o.n = count;
@@ -554,7 +557,7 @@ void linear_scores_backward(const Matrix2& f, const Matrix2& w, const BiasRef& b
     for (int64_t row = 0; row < rows; row += plan.part) {
       Finish finish;
       finish.dead = expo + row;
-      if (!of_float) finish.expo = expo + row;
+      if (of_half) finish.expo = expo + row;
       join_parts(work + plan.features + plan.features_parts * row * f.length * 4, plan.features_parts, false, f.length, std::min(plan.part, rows - row), finish,
                  static_cast<char*>(out.features) + row * f.length * size, f.type, f.length, stream);
     }

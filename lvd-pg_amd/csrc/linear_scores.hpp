@@ -41,7 +41,7 @@ inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; 
 inline int64_t laid_length(int64_t length) { return round_up(length, kKBytes / 2); }
 inline int64_t laid_bytes(int64_t rows, int64_t length, int planes) { return round_up(rows * laid_length(length) * 2 * planes, 256); }
 
-// What laying out changes on the way: rows are scaled by powers of two (float exponents `expo` relative to the largest of `most`,
+// What laying out changes on the way: rows are scaled by powers of two (float exponents `expo` relative to the largest of `most`, if given;
 // nothing of a row at kDeadRow), categories that the bias masks become zeros.
 struct LayOut {
   const int* expo = nullptr;

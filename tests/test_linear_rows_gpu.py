@@ -855,3 +855,19 @@ def test_shards_of_the_categories(gpu, dtype, shape, cut):
     R.within(sum(d.features.double() for d in got), want["features"][0], want["features"][1] * 1.01 + R.half_step(f.dtype) * sizes + R.LEAST[f.dtype], "features")
     R.within(torch.cat([d.weight for d in got]), *want["weight"], "weight")
     R.within(torch.cat([d.bias for d in got]), *want["bias"], "bias")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(7, 70, 40), (300, 64, 200), (1100, 100, 300)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_with_large_factors(gpu, dtype, shape):
+    """Finite gradients where factors are as large as their types (float32, bfloat16) have them: weights against features of 0 and the other way round"""
+    torch, P, R = gpu
+    f, w, b, g, gl, gz = _inputs(torch, dtype, *shape, 48, slots=2)
+    n, k, C = shape
+    f[:, 0], f[:, 1], w[:, 0], w[:, 1] = 0.0, 0.0, 0.0, 0.0
+    w[g[0].clamp(min=0), 0] = 2.0 ** 120                                   # (one or two categories; derivatives are 1 / n at most)
+    f[1, 1] = 2.0 ** 120
+    s, got = _check_scores(R, P, f, w, b, g)
+    d = _check_grads(R, P, f, w, b, s, got, g, gl, gz)
+    assert torch.isfinite(d.features).all() and torch.isfinite(d.weight).all()
+    assert float(d.features[:, 0].float().abs().max()) > 2.0 ** 100 and float(d.weight[:, 1].float().abs().max()) > 2.0 ** 100
