@@ -569,7 +569,9 @@ int pcm_restore_rows(const uint8_t* d_codes, const int32_t* d_scales, int64_t nu
  *   unmasked category's weights, and scores of +inf: NaN (float: any infinity there, and products past the type's range).
  * Products of 16-bit types are exact and summed in 32 bits; float is taken as three bfloat16 parts whose six largest products are summed
  *   (what is left out is less than 2^-24 of a product, and what lies below 2^-134 of a factor).  dx is rounded to the features' type
- *   (float: three parts again; fewer than 1024 rows of 16 bits: two), half's relative to a power of two a row, which no scale of the loss overflows.  Features of half count in the weights' gradients down to 2^-25 of the largest
+ *   (float: three parts again; fewer than 1024 rows of 16 bits: two), half's relative to a power of two a row, which no scale of the loss overflows.
+ *   Rounded once, it is off by as much again as rounding the results is (bfloat16 gradients 2.3e-3 of their norm instead of 1.7e-3, half 2.8e-4 instead
+ *   of 2.1e-4).  Features of half count in the weights' gradients down to 2^-25 of the largest
  *   |dx| of any row, as their type has no smaller numbers.  Sums have a fixed order: the same bits every time.
  * At most 2^22 rows, 2^30 categories, length 2^20.  d_work: so many bytes of device memory as the _workspace function of the same arguments says, 16-byte
  * aligned, which belong to the call until its work is done; `of`: 1 features, 2 weight, 4 bias, added.  The gradient's: 5 GiB at most, beside 8 bytes for

@@ -129,7 +129,7 @@ template <int kGroups>
 struct FewTile {                             // kGroups: of 16 rows of b
   static constexpr int rows = 16 * kGroups;
   static constexpr int longs = kFewTile;                      // rows of a
-  static constexpr int waves = kGroups == 4 ? 4 : 8, threads = 64 * waves;   // (so that three workgroups fit a compute unit's LDS either way)
+  static constexpr int waves = kGroups == 4 ? 4 : 8, threads = 64 * waves;   // (three workgroups fit a compute unit's LDS, with 17 to 32 rows two)
   static constexpr int wave_bytes = (longs + rows) * 128;     // a piece of each
   static constexpr int pitch = rows + 1;                      // of the sums
   static constexpr int sums_bytes = waves * longs * pitch * 4;

@@ -5,8 +5,8 @@
 // A tile's floats come through registers, are taken apart there (some six instructions an entry) and lie in LDS as three planes, from which all
 // six products are read: 12 fragments for 24 products of 32 x 32, so LDS is no bound, and the floats are read once, whatever
 // their strides and alignment.  Either operand may be turned: summed over its rows.  The six products take six times a bfloat16 product's
-// time, 2.4 TFLOP/s a compute unit at most against 0.6 of the cores' own float products.  Scores of 2048 x 32003 over 1024: 730 us, 184
-// TFLOP/s (both operands turned: 850 us, where stores to LDS are of words; whole rows of four there, from requests of two, took 1000).
+// time, 2.4 TFLOP/s a compute unit at most against 0.6 of the cores' own float products.  Scores of 2048 x 32003 over 1024: 757 us, 177
+// TFLOP/s (both operands turned: 946 us, where stores to LDS are of words; whole rows of four there, from requests of two, took more).
 #pragma once
 
 #include <type_traits>

@@ -16,7 +16,7 @@ namespace pcm {
 
 namespace {
 constexpr int kMostBlocks = 256;     // candidates of the largest exponent
-constexpr int kFewRows = 1024;       // fewer: dx in two parts
+constexpr int kFewRows = 1024;       // fewer: dx in two parts (Plan)
 
 // Per row: the weight of p, and the exponent
 __global__ __launch_bounds__(256) void row_terms_kernel(GivenRef given, const float* grad_logp, const float* grad_log_sum, const float* log_sum,
@@ -353,9 +353,10 @@ struct Plan {
     few = takes_few(fm, wm);
     lay_f = !few && !readable(fm);
     lay_w = !few && !readable(wm);
-    // The rounding of dx is the larger part of the error where sums have few terms that count, as the gradient of a given category's weights
-    // has with few rows; over many rows it is what rounding the results costs.  In two parts: 20 rows of 64 bf16, 25000
-    // categories, 2.3e-3 -> 1.6e-3 of the result (as rounding alone); the two products take twice the steps.
+    // Rounded once, dx is off by as much as rounding the results is, however many terms a sum has: bf16 gradients by 2.2e-3 to 2.3e-3 of their norm, where
+    // the results' own rounding is 1.66e-3, half's by 2.8e-4 and 2.1e-4.  A second part takes that away, for twice the steps of two of the
+    // four products.  Rows x 4096 x 50304 bf16, one part and two: 16 rows 559 us, 636; 64 568, 653; 256 786, 1014; 1000 1668, 2506; 4096
+    // 4834, 7686; 32768 x 768 x 128 f16 124, 142.  So fewer than 1024 rows, where it is less than a millisecond, take two.
     dx_planes = !of_float && rows < kFewRows ? 2 : 1;
     dx_pairs = dx_planes == 2 ? kTwoOfB : kOnePlane;
     // (float's weights are read where they are)

@@ -89,8 +89,8 @@ __global__ __launch_bounds__(S::threads, 2) void score_kernel(ScoreTask t) {
   score_tile<T, S>(t);
 }
 
-// Few rows: a thread has some of the tile's categories, of one row.  Three workgroups of four waves a compute unit, or two of eight: as many as fit its
-// LDS (48 x 1001 x 50021 f16: 50 us, 57 with the registers of two; the gradient's kernel would not keep its sums in so few)
+// Few rows: a thread has some of the tile's categories, of one row.  Three workgroups of four waves a compute unit, or two of eight (LDS has
+// room for no more with 17 rows and more; 48 x 1001 x 50021 f16: 50 us, 57 with the registers of two; the gradient's kernel would not keep its sums in so few)
 template <typename T, int kGroups>
 __global__ __launch_bounds__(FewTile<kGroups>::threads, kGroups == 4 ? 3 : 4) void score_few_kernel(ScoreTask t, FewOperand w, FewOperand f, int length) {
   typedef FewTile<kGroups> S;
